@@ -514,6 +514,124 @@ int tfcc_rocm_gather_rows(void* stream, const void* params, unsigned batch, uint
 /* tfcc::data::cast: out[i] = static_cast<out type>(in[i]) for any pair of the ten element types above. */
 int tfcc_rocm_cast(void* stream, const void* in, int in_type, void* out, int out_type, uint64_t total);
 
+/* ---- generation: between the products of a model that answers token by token ---------------------------------------
+ * No counterpart in the reference, which runs a converted graph over whole sequences; these stand beside its softmax, top_k,
+ * quantize and gather (tfcc/core/operations/tfcc_nn.cpp, tfcc_math.cpp, tfcc_quantization.cpp).  float32 activations; all
+ * strides in elements, the values of one head contiguous.  Nothing here waits for the device, allocates, or depends on what an
+ * earlier call left: every call may be captured into a graph, and what the device arrays hold is read when it runs.
+ *
+ * Rotary positions: the pair (a, b) of values 2i and 2i + 1 (interleaved) or i and i + part / 2 (halves) of every head turns by
+ * angle = position * frequencies[i]: (a cos - b sin, b cos + a sin) * magnitude.  Values behind the first `part` of a head
+ * are copied.  Angles are formed and reduced in 64 bits, so that far positions keep the accuracy of near ones. */
+enum {
+  TFCC_ROCM_ROTARY_PLAIN = 0,  /* base^(-2i / part) */
+  TFCC_ROCM_ROTARY_LINEAR = 1, /* ... / factor: positions interpolated */
+  TFCC_ROCM_ROTARY_BASE = 2,   /* base * factor^(part / (part - 2)) in place of base: the slowest pair is divided by factor, the fastest kept */
+  /* each pair between its plain frequency and that divided by factor: plain * (r + (1 - r) / factor), where r grows from 0 to 1 */
+  TFCC_ROCM_ROTARY_TURNS = 3,  /* ... with the turns a pair makes over original_length, from `low` to `high` of them */
+  TFCC_ROCM_ROTARY_INDEX = 4   /* ... with the pair's index, from where it makes `high` turns down to 0 where it makes `low`, rounded
+                                * outwards to whole indices; *magnitude = 0.1 ln(factor) + 1 (elsewhere 1) */
+};
+/* frequencies: part / 2 doubles in HOST memory, to be copied to the device once; magnitude may be NULL.  original_length, low and
+ * high are read by TURNS and INDEX only (0 < low < high), factor (> 0) by all but PLAIN. */
+int tfcc_rocm_rotary_frequencies(unsigned part, double base, int scaling, double factor, unsigned original_length, double low,
+                                 double high, double* frequencies, float* magnitude);
+/* Up to two tensors [tokens, heads, size] (queries and keys) in one launch; in[1] NULL: one.  out[i] is in[i] with the same strides, or
+ * memory that overlaps neither input.  size <= 1024. */
+typedef struct tfcc_rocm_rotary_desc {
+  const float* in[2];
+  float* out[2];
+  unsigned heads[2];
+  uint64_t in_token_stride[2], in_head_stride[2], out_token_stride[2], out_head_stride[2];
+  unsigned tokens, size, part; /* part: even, 2 to size */
+  const void* positions;       /* [tokens] */
+  int position_type;           /* TFCC_ROCM_S32 or S64 */
+  const double* frequencies;   /* device, [part / 2], radians for each position */
+  float magnitude;
+  int interleaved;
+} tfcc_rocm_rotary_desc;
+int tfcc_rocm_rotary_f32(void* stream, const tfcc_rocm_rotary_desc* desc);
+
+/* Keys and values of many sequences in pages: row `slot % page_size` of page `slot / page_size` for each head.  type TFCC_ROCM_F32, or
+ * TFCC_ROCM_S8 with one scale for each slot and head, as cache_write makes them: scale = max |x| / 127 in float32, integers
+ * x / scale rounded to nearest, ties to even; a row of zeros has scale 0, and a row that holds an infinity or a NaN reads back as
+ * NaN.  keys and values have the same strides, and so have the scales; key and value arrays, scales, slots do not overlap.
+ * size: up to 256, a multiple of 4 (F32) or 8 (S8), with pointers and strides of keys and values multiples of 16 bytes (F32) or 8 (S8). */
+typedef struct tfcc_rocm_paged_cache {
+  void *keys, *values;
+  float *key_scales, *value_scales; /* S8 only */
+  int type;
+  unsigned pages, heads, page_size, size;
+  uint64_t page_stride, head_stride, row_stride;
+  uint64_t scale_page_stride, scale_head_stride, scale_row_stride;
+} tfcc_rocm_paged_cache;
+/* Token i's keys and values [tokens, heads, size] go to slot slots[i] (TFCC_ROCM_S32 or S64); a slot outside the cache (-1 for a
+ * padded token) is skipped.  Two tokens of one call must not name the same slot: its contents are then unspecified. */
+int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, const float* keys, uint64_t key_token_stride,
+                          uint64_t key_head_stride, const float* values, uint64_t value_token_stride,
+                          uint64_t value_head_stride, unsigned tokens, const void* slots, int slot_type);
+/* The first starts[i + 1] - starts[i] tokens of each sequence, back to back: rows starts[i] .. of dense keys and values [tokens, heads, size].
+ * table [batch, table_width], row stride table_stride: the pages of each sequence in order.  starts [batch + 1], ascending from 0.
+ * Rows from starts[batch] on are left as they were; rows on a page outside the cache or behind the table are zeros. */
+int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const int32_t* table, uint64_t table_stride,
+                         unsigned table_width, unsigned batch, const int32_t* starts, unsigned tokens, float* keys,
+                         float* values);
+
+/* out = softmax(scale * q k^T) v of a chunk of tokens of each sequence over what the cache holds of it, the chunk itself among that.
+ * q and out [tokens, heads, size]; sequence i's chunk is rows starts[i] .. starts[i + 1] - 1 and its last token the last of lengths[i]
+ * cached ones.  Query head h reads cache head h / (heads / cache heads).  causal: a token sees the keys up to its own position and,
+ * with window > 0, only the last `window` of those; causal 0: all lengths[i].  A token that sees no key gets zeros, rows from
+ * starts[batch] on are left as they were, and a key on a page outside the cache or behind the table is not seen.  max_length: an
+ * upper bound of lengths[] that the host knows (0: table_width * page_size): how the work is split follows it; keys behind it are not seen.
+ * workspace: tfcc_rocm_paged_attention_workspace() bytes, 16-byte aligned, of any contents, not in use by another call at the same time.
+ * Products are exact to float32 whatever the cache's type.  out overlaps no input. */
+typedef struct tfcc_rocm_paged_attention_desc {
+  tfcc_rocm_paged_cache cache;
+  const float* q;
+  float* out;
+  uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* multiples of 4, pointers 16-byte aligned */
+  unsigned tokens, heads, batch;
+  const int32_t* starts;  /* [batch + 1], ascending from 0 */
+  const int32_t* lengths; /* [batch] */
+  const int32_t* table;
+  uint64_t table_stride;
+  unsigned table_width, max_length;
+  float scale;
+  int causal;
+  unsigned window;
+  void* workspace;
+  size_t workspace_bytes;
+} tfcc_rocm_paged_attention_desc;
+size_t tfcc_rocm_paged_attention_workspace(const tfcc_rocm_paged_attention_desc* desc); /* 0 for a call that is refused, or needs none */
+int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_desc* desc);
+
+/* One token for each row of logits [rows, length], given a random number in [0, 1) for each.  Weights are exp((x - max) / temperature);
+ * tokens stand in the order of falling logits, equal ones by position.  Of these, the first top_k are kept; of those, the
+ * fewest whose weights reach top_p of theirs; of those, the ones with a weight of at least min_p times the largest; always the
+ * first.  The token is the first kept one, in order of position, at which the running sum of weights passes random times their sum.
+ * Each of temperature, top_k, top_p, min_p is [rows] in device memory or NULL (1, and no filter); temperature <= 0 takes the first in order;
+ * top_k <= 0, top_p >= 1 and min_p <= 0 keep all.  NaN logits and those of -infinity are never chosen unless nothing else is there: then
+ * token -1 with probability 0.  Where the largest is +infinity, those that are share the weight.  Weights are summed as integers of
+ * 2^-43 of the largest or finer: the result does not depend on the order of the sums.  length <= 2^20.
+ * tokens [rows]; probabilities [rows] (or NULL): the token's weight over the sum of the kept ones.
+ * workspace: tfcc_rocm_sample_workspace() bytes, 16-byte aligned, of any contents, not in use by another call at the same time. */
+typedef struct tfcc_rocm_sample_desc {
+  const float* logits;
+  uint64_t row_stride;
+  unsigned rows, length;
+  const float* random;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* tokens;
+  float* probabilities;
+  void* workspace;
+  size_t workspace_bytes;
+} tfcc_rocm_sample_desc;
+size_t tfcc_rocm_sample_workspace(unsigned rows, unsigned length);
+int tfcc_rocm_sample_f32(void* stream, const tfcc_rocm_sample_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif

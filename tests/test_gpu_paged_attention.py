@@ -1,0 +1,288 @@
+"""Attention over a paged cache against the definition in 64 bits, within what float32 sums may be off by."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import generation_reference as R
+from conftest import rel_fro
+
+
+def test_refused_without_a_device(pkg):
+    lib, d = pkg.lib(), pkg.PagedAttentionDesc()
+    call = lambda: lib.tfcc_rocm_paged_attention_f32(None, C.byref(d))
+    size = lambda: lib.tfcc_rocm_paged_attention_workspace(C.byref(d))
+    assert lib.tfcc_rocm_paged_attention_f32(None, None) == 1 and lib.tfcc_rocm_paged_attention_workspace(None) == 0
+    c = d.cache
+    c.keys = c.values = c.key_scales = c.value_scales = 4096
+    c.type, c.pages, c.heads, c.page_size, c.size = pkg.S8, 200, 2, 16, 64
+    d.heads, d.tokens, d.batch, d.table_width, d.causal = 8, 1, 1, 200, 1
+    assert call() == 1 and b"null" in lib.tfcc_rocm_last_error_string()
+    d.q = d.out = d.starts = d.lengths = d.table = 4096
+    needs = size()
+    assert needs > 0 and call() == 1 and b"workspace" in lib.tfcc_rocm_last_error_string()
+    d.workspace, d.workspace_bytes = 4096, needs - 1
+    assert call() == 1
+    d.workspace, d.workspace_bytes = 4097, needs
+    assert call() == 1
+    d.workspace = 4096
+    for name, value in (("heads", 0), ("heads", 7), ("tokens", 1 << 31), ("q", 4100), ("out", 4104), ("q_token_stride", 6), ("out_head_stride", 5),
+                        ("table_width", 1 << 30)):
+        before = getattr(d, name)
+        setattr(d, name, value)
+        assert call() == 1 and size() == 0, (name, value)
+        setattr(d, name, before)
+    d.causal, d.window = 0, 5
+    assert call() == 1 and size() == 0
+    d.window, d.tokens = 0, 0
+    assert call() == 0 and size() == 0
+
+
+class Made:
+    """A cache with the pages of its sequences mixed up, and a chunk of queries for each."""
+
+    def __init__(self, pkg, kind, lengths, chunks, heads, kv, size, page, seed, spare=2):
+        import torch
+        rng = self.rng = np.random.default_rng(seed)
+        each = [max(1, -(-n // page)) for n in lengths]
+        pages = sum(each) + spare
+        order = rng.permutation(pages).astype(np.int32)
+        self.table = rng.integers(-5, pages + 5, (len(lengths), max(each) + 1)).astype(np.int32)  # what lies behind is anything
+        at = 0
+        for i, n in enumerate(each):
+            self.table[i, :n] = order[at:at + n]
+            at += n
+        shape = (pages, kv, page, size)
+        if kind == "s8":
+            self.cache = [rng.integers(-127, 128, shape, dtype=np.int8) for _ in range(2)]
+            self.cache += [(rng.random(shape[:3]) * 0.02 + 0.01).astype(np.float32) for _ in range(2)]
+        else:
+            self.cache = [rng.normal(size=shape).astype(np.float32) for _ in range(2)]
+        self.lengths, self.page = np.array(lengths, np.int32), page
+        self.starts = np.concatenate([[0], np.cumsum(chunks)]).astype(np.int32)
+        self.q = rng.normal(size=(int(self.starts[-1]), heads, size)).astype(np.float32)
+        self.scale = float(size ** -0.5)
+        self.pkg = pkg
+
+    def on(self, T):
+        return tuple(T.t(c) for c in self.cache)
+
+    def run(self, T, cache=None, out=None, **kw):
+        return self.pkg.paged_attention(T.t(self.q), cache or self.on(T), T.t(self.table), T.t(self.starts), T.t(self.lengths), self.scale, out=out, **kw)
+
+    def check(self, T, got=None, cache=None, **kw):
+        got = T.n(self.run(T, cache, **kw) if got is None else got).astype(np.float64)
+        most = kw.pop("max_length", None)
+        want, off = R.attention(self.q, self.cache, self.table, self.starts, self.lengths, self.scale, most=most, **kw)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        fine = ~np.isnan(want)
+        same = got == want  # infinities among them
+        with np.errstate(invalid="ignore"):
+            assert (same | (np.abs(got - want) <= off))[fine].all(), np.nanmax((np.abs(got - want) / off)[fine & ~same])
+        finite = np.isfinite(want)
+        assert rel_fro(got[finite], want[finite]) <= 1e-5
+
+
+CASES = [
+    # kind, lengths, chunks, heads, kv heads, size, page, more
+    ("s8", [1], [1], 1, 1, 64, 16, {}),
+    ("f32", [1], [1], 1, 1, 64, 16, {}),
+    ("s8", [777], [1], 12, 12, 64, 16, {}),
+    ("s8", [33, 0, 200, 1, 517], [1, 1, 1, 1, 1], 8, 2, 128, 32, {}),         # one has nothing cached
+    ("f32", [33, 0, 200, 1, 517], [1, 1, 1, 1, 1], 8, 2, 128, 32, {}),
+    ("s8", [40, 300, 90], [40, 7, 0], 6, 2, 128, 16, {}),                      # a whole prompt, a chunk, a sequence without one
+    ("f32", [40, 300, 90], [40, 7, 0], 6, 2, 64, 16, {}),
+    ("s8", [3, 70], [5, 66], 4, 4, 64, 16, {}),                                # more tokens than cached: the first see nothing
+    ("f32", [3, 70], [5, 66], 4, 4, 64, 16, {}),
+    ("s8", [257, 65], [1, 3], 20, 5, 80, 24, {}),                              # pages that end inside a tile
+    ("f32", [257, 65], [1, 3], 20, 5, 80, 24, {}),
+    ("s8", [130, 61], [30, 2], 3, 1, 40, 7, {}),                               # rows of 8 bytes, odd pages, groups of three
+    ("f32", [130, 61], [30, 2], 3, 1, 36, 7, {}),
+    ("s8", [129], [9], 33, 1, 200, 1, {}),                                     # pages of one row, more heads than a tile has rows
+    ("f32", [129], [9], 33, 1, 252, 16, {}),
+    ("s8", [500, 90], [64, 1], 4, 2, 256, 64, {}),
+    ("f32", [500, 90], [64, 1], 4, 2, 192, 64, {}),
+    ("s8", [700, 100], [3, 100], 8, 8, 64, 16, {"window": 1}),
+    ("f32", [700, 100], [3, 100], 8, 8, 64, 16, {"window": 37}),
+    ("s8", [1500, 600], [1, 130], 8, 1, 128, 32, {"window": 300}),
+    ("s8", [90, 300], [20, 3], 4, 4, 96, 16, {"causal": False}),
+    ("f32", [90, 300], [20, 3], 4, 4, 96, 16, {"causal": False}),
+    ("s8", [900, 60], [2, 2], 4, 1, 64, 16, {"max_length": 512}),              # keys behind the bound are not seen
+    ("s8", [3000, 1, 2048, 129], [1, 1, 1, 1], 32, 8, 128, 128, {}),           # many pieces
+    ("f32", [3000, 1, 2048, 129], [1, 1, 1, 1], 32, 8, 128, 128, {}),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_against_the_definition(pkg, T, case):
+    kind, lengths, chunks, heads, kv, size, page, more = CASES[case]
+    Made(pkg, kind, lengths, chunks, heads, kv, size, page, case).check(T, **more)
+
+
+@pytest.mark.gpu
+def test_many_sequences(pkg, T):
+    """More sequences than a wavefront has lanes, some without tokens."""
+    rng = np.random.default_rng(9)
+    chunks = rng.integers(0, 4, 150)
+    chunks[:70] = 0
+    lengths = chunks + rng.integers(0, 60, 150)
+    for kind in ("s8", "f32"):
+        Made(pkg, kind, lengths, chunks, 4, 2, 64, 16, 3).check(T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["s8", "f32"])
+def test_pages_outside_the_cache(pkg, T, kind):
+    m = Made(pkg, kind, [200, 90, 64], [1, 30, 64], 4, 2, 64, 16, 4)
+    m.table[0, [0, 5]] = [-1, 10 ** 6]
+    m.table[1, 3] = len(m.cache[0])
+    m.table[2, :4] = -1  # nothing is there at all
+    m.check(T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["s8", "f32"])
+@pytest.mark.parametrize("chunks", [[1, 1], [40, 21]])
+def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks):
+    import torch
+    m = Made(pkg, kind, [150, 70], chunks, 6, 2, 64, 16, 5)
+    clean = T.n(m.run(T)).copy()
+    rows = np.ones((m.cache[0].shape[0], 16), bool)  # slots of no sequence
+    for i, n in enumerate(m.lengths):
+        at = np.arange(n)
+        rows[m.table[i][at // 16], at % 16] = False
+    for c in m.cache[:2] if kind == "f32" else m.cache[2:]:
+        c.swapaxes(1, 2)[rows] = np.nan
+    assert np.array_equal(T.n(m.run(T)), clean)
+    # the last token's own key and value are not finite: the rows before it do not see them
+    last = m.lengths[0] - 1
+    page, inside = m.table[0, last // 16], last % 16
+    if kind == "s8":
+        m.cache[3][page, 1, inside] = np.inf
+    else:
+        m.cache[1][page, 1, inside, 5] = np.inf
+        m.cache[1][page, 1, inside, 40] = np.nan
+    got = T.n(m.run(T))
+    mine = np.zeros(got.shape, bool)
+    mine[m.starts[1] - 1, 3:] = True
+    assert np.array_equal(got[~mine], clean[~mine])
+    if kind == "f32":
+        assert np.isposinf(got[m.starts[1] - 1, 3:, 5]).all() and np.isnan(got[m.starts[1] - 1, 3:, 40]).all()
+        m.check(T)
+
+
+@pytest.mark.gpu
+def test_scales_of_all_sizes(pkg, T):
+    """Rows of values from 10^-20 to 10^20, zeros among them, and queries likewise."""
+    m = Made(pkg, "s8", [300, 45], [2, 45], 4, 2, 128, 16, 6)
+    m.cache[3][:] = np.exp(m.rng.normal(size=m.cache[3].shape) * 15).astype(np.float32)
+    m.cache[3][m.rng.random(m.cache[3].shape) < 0.2] = 0
+    m.cache[2][m.rng.random(m.cache[2].shape) < 0.2] = 0
+    m.q[1] *= 1e-25
+    m.q[2] = 0
+    m.check(T)
+    for c in m.cache[3:]:
+        c[:] = 0
+    assert not T.n(m.run(T)).any()
+
+
+@pytest.mark.gpu
+def test_large_scores(pkg, T):
+    """Weights that all fall on one key or underflow."""
+    for kind in ("s8", "f32"):
+        m = Made(pkg, kind, [400, 30], [3, 30], 4, 2, 64, 16, 7)
+        m.scale *= 100
+        m.check(T)
+
+
+@pytest.mark.gpu
+def test_rows_whose_scores_rise_beside_rows_whose_do_not(pkg, T):
+    """The largest score of one row moves with every key, that of the other stays: neither loses what it has."""
+    m = Made(pkg, "s8", [5000], [1], 2, 1, 64, 16, 13)
+    m.cache[0][:] = m.cache[0][0, 0, 0]
+    at = np.arange(5000)
+    m.cache[2][m.table[0][at // 16], 0, at % 16] = np.linspace(0.001, 0.02, 5000, dtype=np.float32)
+    m.q[0, 0] = m.cache[0][0, 0, 0] / np.float32(100)
+    m.q[0, 1] = -m.q[0, 0]
+    got = m.run(T)
+    m.check(T, got)
+    want, _ = R.attention(m.q, m.cache, m.table, m.starts, m.lengths, m.scale)
+    assert rel_fro(T.n(got), want) <= 1.5e-6  # scores up to 20: 20 x 2^-24 each
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,size", [("s8", 64), ("f32", 64), ("s8", 72), ("f32", 100)])
+def test_strides(pkg, T, kind, size):
+    import torch
+    from test_gpu_paged_cache import strided
+    m = Made(pkg, kind, [300, 45], [1, 20], 4, 2, size, 16, 8)
+    plain = m.run(T)
+    assert torch.equal(m.run(T, cache=strided(m.on(T))), plain)
+    wide = torch.full((21, 3, 4, size + 4), 9.0, device="cuda")
+    q, out = wide[:, 0, :, 4:], wide[:, 2, :, 4:]
+    q.copy_(T.t(m.q))
+    before = wide.clone()
+    got = pkg.paged_attention(q, m.on(T), T.t(np.concatenate([m.table, m.table], 1))[:, :m.table.shape[1]], T.t(m.starts), T.t(m.lengths), m.scale, out=out)
+    assert got is out and torch.equal(out, plain)
+    before[:, 2, :, 4:] = plain
+    assert torch.equal(wide, before)
+    # a query that does not begin at 16 bytes
+    with pytest.raises(pkg.TfccRocmError):
+        pkg.paged_attention(torch.zeros((21, 4, size + 1), device="cuda")[..., 1:], m.on(T), T.t(m.table), T.t(m.starts), T.t(m.lengths), m.scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,chunks", [([2000, 1, 700], [1, 1, 1]), ([90, 200], [60, 3])])
+def test_rows_behind_the_last_sequence_stay(pkg, T, lengths, chunks):
+    import torch
+    m = Made(pkg, "s8", lengths, chunks, 8, 2, 64, 16, 10)
+    n = int(m.starts[-1])
+    want = m.run(T)
+    m.q = np.concatenate([m.q, m.q[:2], m.q[:1] * np.nan])
+    out = torch.full(m.q.shape, 3.25, device="cuda")
+    m.run(T, out=out)
+    assert torch.allclose(out[:n], want, rtol=1e-5, atol=1e-6) and bool((out[n:] == 3.25).all())
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(pkg, T):
+    """Pages that lie more than 2^32 elements into the cache."""
+    import torch
+    pages, page, size = 2 ** 20 + 64, 64, 72
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("not enough memory")
+    cache = pkg.paged_cache(pages, 1, page, size)
+    m = Made(pkg, "s8", [200, 77], [1, 20], 4, 1, size, page, 11)
+    there = pages - 1 - np.arange(m.cache[0].shape[0])
+    for big, small in zip(cache, m.cache):
+        big[torch.from_numpy(there).cuda()] = T.t(small)
+    small = m.on(T)
+    want = m.run(T, cache=small)
+    table = m.table
+    m.table = np.where((table >= 0) & (table < len(there)), there[np.clip(table, 0, len(there) - 1)], -1).astype(np.int32)
+    assert torch.equal(m.run(T, cache=cache), want)
+    back = pkg.cache_read(cache, T.t(m.table), T.t(np.array([0, 200, 277], np.int32)), 277)
+    near = pkg.cache_read(small, T.t(table), T.t(np.array([0, 200, 277], np.int32)), 277)
+    assert torch.equal(back[0], near[0]) and torch.equal(back[1], near[1])
+    x = T.t(m.rng.normal(size=(2, 1, size)).astype(np.float32))
+    slots = np.array([pages * page - 1, (pages - 3) * page + 5])
+    pkg.cache_write(cache, x, x, T.t(slots))
+    n, s = R.quantized(T.n(x))
+    assert np.array_equal(T.n(cache[0][-1, :, -1]), n[0]) and np.array_equal(T.n(cache[3][-3, :, 5]), s[1])
+
+
+@pytest.mark.gpu
+def test_refused(pkg, T):
+    import torch
+    m = Made(pkg, "s8", [30], [2], 4, 2, 64, 16, 12)
+    cache, q, table, starts, lengths = m.on(T), T.t(m.q), T.t(m.table), T.t(m.starts), T.t(m.lengths)
+    for args in ((q[:, :3], cache, table, starts, lengths), (q[..., :32], cache, table, starts, lengths), (q, cache, table.long(), starts, lengths),
+                 (q, cache, table, starts[:1], lengths), (q, cache, table, starts, lengths.long()), (q.double(), cache, table, starts, lengths),
+                 (q, cache[:2], table, starts, lengths), (q, cache, table.cpu(), starts, lengths), (q, cache, torch.cat([table, table]), starts, lengths)):
+        with pytest.raises(pkg.InvalidArgumentError):
+            pkg.paged_attention(*args, 0.125)
+    for kw in (dict(window=-1), dict(window=3, causal=False), dict(max_length=-1), dict(out=q[:1]), dict(out=q.double())):
+        with pytest.raises(pkg.InvalidArgumentError):
+            pkg.paged_attention(q, cache, table, starts, lengths, 0.125, **kw)
+    assert pkg.paged_attention(q[:0], cache, table, torch.zeros_like(starts), lengths, 0.125).shape == (0, 4, 64)

@@ -8,6 +8,10 @@ The functions mirror the reference's operator interface for this path:
   quantization_matmul    tfcc::mkl::quantization::matmul      (tfcc/mkl/operations/tfcc_mklquantization.h:39-42)
   reduce_sum             tfcc::mkl::quantization::reduce_sum  (tfcc/mkl/operations/tfcc_mklquantization.h:50-51)
   quantize / requantize / dequantize   tfcc::quantization::*  (tfcc/core/operations/tfcc_quantization.cpp:26-98)
+and, without a counterpart there, what a model that answers token by token needs between its products:
+  rotary, rotary_frequencies           positions on the heads of queries and keys
+  cache_write, cache_read, paged_attention   a paged cache of keys and values, float32 or int8, and attention over it
+  sample                               a token for each row of logits
 """
 import ctypes as C
 import os
@@ -76,6 +80,39 @@ class LstmSequenceDesc(C.Structure):
         [(n, C.c_void_p * 2) for n in ("x", "kernel", "bias", "h0", "c0", "out", "h", "c")] + \
         [("backward", C.c_int * 2), ("forget", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
          ("wait_us", C.c_uint)]
+
+
+class RotaryDesc(C.Structure):
+    """tfcc_rocm_rotary_desc"""
+    _fields_ = [("in_", C.c_void_p * 2), ("out", C.c_void_p * 2), ("heads", C.c_uint * 2)] + \
+        [(n, C.c_uint64 * 2) for n in ("in_token_stride", "in_head_stride", "out_token_stride", "out_head_stride")] + \
+        [("tokens", C.c_uint), ("size", C.c_uint), ("part", C.c_uint), ("positions", C.c_void_p), ("position_type", C.c_int),
+         ("frequencies", C.c_void_p), ("magnitude", C.c_float), ("interleaved", C.c_int)]
+
+
+class PagedCache(C.Structure):
+    """tfcc_rocm_paged_cache"""
+    _fields_ = [(n, C.c_void_p) for n in ("keys", "values", "key_scales", "value_scales")] + \
+        [("type", C.c_int)] + [(n, C.c_uint) for n in ("pages", "heads", "page_size", "size")] + \
+        [(n, C.c_uint64) for n in ("page_stride", "head_stride", "row_stride", "scale_page_stride", "scale_head_stride",
+                                   "scale_row_stride")]
+
+
+class PagedAttentionDesc(C.Structure):
+    """tfcc_rocm_paged_attention_desc"""
+    _fields_ = [("cache", PagedCache), ("q", C.c_void_p), ("out", C.c_void_p)] + \
+        [(n, C.c_uint64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")] + \
+        [("tokens", C.c_uint), ("heads", C.c_uint), ("batch", C.c_uint), ("starts", C.c_void_p), ("lengths", C.c_void_p),
+         ("table", C.c_void_p), ("table_stride", C.c_uint64), ("table_width", C.c_uint), ("max_length", C.c_uint),
+         ("scale", C.c_float), ("causal", C.c_int), ("window", C.c_uint), ("workspace", C.c_void_p),
+         ("workspace_bytes", C.c_size_t)]
+
+
+class SampleDesc(C.Structure):
+    """tfcc_rocm_sample_desc"""
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_uint64), ("rows", C.c_uint), ("length", C.c_uint)] + \
+        [(n, C.c_void_p) for n in ("random", "temperature", "top_k", "top_p", "min_p", "tokens", "probabilities", "workspace")] + \
+        [("workspace_bytes", C.c_size_t)]
 
 
 # name -> (restype, argtypes): every symbol include/tfcc_rocm.h declares
@@ -163,6 +200,14 @@ SYMBOLS = {
     "tfcc_rocm_gru_cell_gates_f32": (_I, [_VP, _U, _U, _U, _VP, _VP, _VP, _VP, _VP]),
     "tfcc_rocm_gru_cell_candidate_f32": (_I, [_VP, _U, _U, _VP, _VP, _VP, _VP, _VP, _VP]),
     "tfcc_rocm_pytorch_gru_cell_f32": (_I, [_VP, _U, _U, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "tfcc_rocm_rotary_frequencies": (_I, [_U, _D, _I, _D, _U, _D, _D, C.POINTER(C.c_double), C.POINTER(C.c_float)]),
+    "tfcc_rocm_rotary_f32": (_I, [_VP, C.POINTER(RotaryDesc)]),
+    "tfcc_rocm_cache_write": (_I, [_VP, C.POINTER(PagedCache), _VP, _U64, _U64, _VP, _U64, _U64, _U, _VP, _I]),
+    "tfcc_rocm_cache_read": (_I, [_VP, C.POINTER(PagedCache), _VP, _U64, _U, _U, _VP, _U, _VP, _VP]),
+    "tfcc_rocm_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedAttentionDesc)]),
+    "tfcc_rocm_paged_attention_f32": (_I, [_VP, C.POINTER(PagedAttentionDesc)]),
+    "tfcc_rocm_sample_workspace": (C.c_size_t, [_U, _U]),
+    "tfcc_rocm_sample_f32": (_I, [_VP, C.POINTER(SampleDesc)]),
 }
 
 _lib = None
@@ -1041,3 +1086,242 @@ def transpose(a, perm):
     out = torch.empty([a.shape[i] for i in perm], dtype=a.dtype, device=a.device)
     check(lib().tfcc_rocm_transpose_f32(_stream(), _ptr(a), shape, p, a.dim(), _ptr(out)))
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Generation: between the products of a model that answers token by token
+# ---------------------------------------------------------------------------------------------
+
+ROTARY_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "turns": 3, "index": 4}
+
+
+def rotary_frequencies(part, base=10000.0, scaling="plain", factor=1.0, original_length=0, low=1.0, high=4.0):
+    """tfcc_rocm_rotary_frequencies: (list of part / 2 radians for each position, magnitude).  A program makes a float64 device
+    tensor of the list once.  scaling: one of ROTARY_SCALINGS."""
+    if scaling not in ROTARY_SCALINGS:
+        raise InvalidArgumentError("invalid scaling")
+    f, magnitude = (C.c_double * max(1, part // 2))(), C.c_float()
+    if lib().tfcc_rocm_rotary_frequencies(part, base, ROTARY_SCALINGS[scaling], factor, original_length, low, high, f,
+                                          C.byref(magnitude)):
+        raise InvalidArgumentError(lib().tfcc_rocm_last_error_string().decode())
+    return list(f), magnitude.value
+
+
+def _on_device(device, *tensors):
+    """Device tensors of one device, which the current stream belongs to."""
+    import torch
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device != device):
+            raise InvalidArgumentError("tensors on different devices")
+    if device.index != torch.cuda.current_device():
+        raise InvalidArgumentError("tensors are not on the current device")
+
+
+def _heads_of(t, name):
+    """[tokens, heads, size] of float32 whose heads are contiguous."""
+    import torch
+    if t.dim() != 3 or t.dtype != torch.float32:
+        raise InvalidArgumentError("invalid " + name)
+    return t if t.shape[2] <= 1 or t.stride(2) == 1 else t.contiguous()
+
+
+def _integers(t, name, count, types):
+    if t.dtype not in types or t.dim() != 1 or t.shape[0] != count:
+        raise InvalidArgumentError("invalid " + name)
+    return t.contiguous()
+
+
+def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0, out=None):
+    """Heads of queries (and of keys; k may be None) [tokens, heads, size], each token turned by the angles of its position:
+    tfcc_rocm_rotary_f32.  positions: int32 or int64 [tokens]; frequencies: float64 [part / 2].  out: a pair like the result,
+    (q, k) itself to turn them in place.  Returns (q, k)."""
+    import torch
+    if out is None:
+        done = _native().rotary(q, k, positions, frequencies, interleaved, magnitude)
+        if done is not None:
+            return done
+    _on_device(q.device, k, positions, frequencies, *(out or ()))
+    inputs = [_heads_of(q, "q")] + ([] if k is None else [_heads_of(k, "k")])
+    tokens, _, size = q.shape
+    if k is not None and (k.shape[0] != tokens or k.shape[2] != size):
+        raise InvalidArgumentError("invalid k")
+    positions = _integers(positions, "positions", tokens, (torch.int32, torch.int64))
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1 or not 1 <= frequencies.shape[0] <= size // 2:
+        raise InvalidArgumentError("invalid frequencies")
+    frequencies = frequencies.contiguous()
+    if out is None:
+        outputs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in inputs]
+    else:
+        outputs = [t for t in out if t is not None]
+        if len(outputs) != len(inputs) or any(o.shape != t.shape or o.dtype != t.dtype or (size > 1 and o.stride(2) != 1)
+                                              for o, t in zip(outputs, inputs)):
+            raise InvalidArgumentError("invalid out")
+    d = RotaryDesc()
+    for i, (t, o) in enumerate(zip(inputs, outputs)):
+        d.in_[i], d.out[i], d.heads[i] = _ptr(t), _ptr(o), t.shape[1]
+        d.in_token_stride[i], d.in_head_stride[i] = t.stride(0), t.stride(1)
+        d.out_token_stride[i], d.out_head_stride[i] = o.stride(0), o.stride(1)
+    d.tokens, d.size, d.part = tokens, size, 2 * frequencies.shape[0]
+    d.positions, d.position_type, d.frequencies = _ptr(positions), _type_code(positions.dtype), _ptr(frequencies)
+    d.magnitude, d.interleaved = magnitude, 1 if interleaved else 0
+    if all(t.numel() for t in inputs):
+        check(lib().tfcc_rocm_rotary_f32(_stream(), C.byref(d)))
+    return outputs[0], outputs[1] if k is not None else None
+
+
+def _cache_desc(cache):
+    """A tfcc_rocm_paged_cache over (keys, values) of float32 or (keys, values, key scales, value scales) of int8."""
+    import torch
+    if len(cache) not in (2, 4):
+        raise InvalidArgumentError("invalid cache")
+    keys, values = cache[0], cache[1]
+    s8 = len(cache) == 4
+    if keys.dim() != 4 or keys.dtype != (torch.int8 if s8 else torch.float32) or keys.numel() == 0:
+        raise InvalidArgumentError("invalid cache keys")
+    if values.shape != keys.shape or values.dtype != keys.dtype or values.stride() != keys.stride() or keys.stride(3) != 1:
+        raise InvalidArgumentError("invalid cache values")
+    _on_device(keys.device, *cache)
+    d = PagedCache()
+    d.keys, d.values, d.type = _ptr(keys), _ptr(values), S8 if s8 else F32
+    d.pages, d.heads, d.page_size, d.size = keys.shape
+    d.page_stride, d.head_stride, d.row_stride = keys.stride()[:3]
+    if s8:
+        for t in cache[2:]:
+            if t.shape != keys.shape[:3] or t.dtype != torch.float32 or t.stride() != cache[2].stride():
+                raise InvalidArgumentError("invalid cache scales")
+        d.key_scales, d.value_scales = _ptr(cache[2]), _ptr(cache[3])
+        d.scale_page_stride, d.scale_head_stride, d.scale_row_stride = cache[2].stride()
+    return d
+
+
+def paged_cache(pages, heads, page_size, size, dtype=None, device="cuda"):
+    """Zeroed memory of a paged cache as the calls below take it: (keys, values), each [pages, heads, page_size, size], and for
+    int8 (the default) (..., key scales, value scales), each [pages, heads, page_size].  Any tensors of these shapes will do,
+    views of other strides among them."""
+    import torch
+    dtype = torch.int8 if dtype is None else dtype
+    if dtype not in (torch.int8, torch.float32):
+        raise InvalidArgumentError("a cache is int8 or float32")
+    held = tuple(torch.zeros((pages, heads, page_size, size), dtype=dtype, device=device) for _ in range(2))
+    if dtype == torch.float32:
+        return held
+    return held + tuple(torch.zeros((pages, heads, page_size), dtype=torch.float32, device=device) for _ in range(2))
+
+
+def cache_write(cache, keys, values, slots):
+    """Keys and values [tokens, heads, size] of new tokens into the cache's slots (page * page_size + row; int32 or int64 [tokens];
+    -1: the token is skipped), as int8 with a scale for each token and head or as they are: tfcc_rocm_cache_write."""
+    done = _native().cache_write(cache, keys, values, slots)
+    if done is not None:
+        return
+    import torch
+    d = _cache_desc(cache)
+    _on_device(cache[0].device, keys, values, slots)
+    keys, values = _heads_of(keys, "keys"), _heads_of(values, "values")
+    if tuple(keys.shape[1:]) != (d.heads, d.size):
+        raise InvalidArgumentError("invalid keys")
+    if values.shape != keys.shape:
+        raise InvalidArgumentError("invalid values")
+    slots = _integers(slots, "slots", keys.shape[0], (torch.int32, torch.int64))
+    check(lib().tfcc_rocm_cache_write(_stream(), C.byref(d), _ptr(keys), keys.stride(0), keys.stride(1), _ptr(values), values.stride(0),
+                                      values.stride(1), keys.shape[0], _ptr(slots), _type_code(slots.dtype)))
+
+
+def _table_of(table, batch, name):
+    import torch
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != batch:
+        raise InvalidArgumentError("invalid " + name)
+    return table if table.shape[1] <= 1 or table.stride(1) == 1 else table.contiguous()
+
+
+def cache_read(cache, table, starts, tokens):
+    """The sequences that the cache holds, back to back in float32: (keys, values), each [tokens, heads, size], where sequence i is
+    rows starts[i] to starts[i + 1] - 1 (int32 [batch + 1], from 0): tfcc_rocm_cache_read.  table: int32 [batch, pages], the pages
+    of each sequence in order.  Rows behind the last sequence are not written."""
+    done = _native().cache_read(cache, table, starts, tokens)
+    if done is not None:
+        return done
+    import torch
+    d = _cache_desc(cache)
+    _on_device(cache[0].device, table, starts)
+    table = _table_of(table, table.shape[0], "table")
+    starts = _integers(starts, "starts", table.shape[0] + 1, (torch.int32,))
+    if tokens < 0:
+        raise InvalidArgumentError("invalid tokens")
+    keys, values = (torch.empty((tokens, d.heads, d.size), dtype=torch.float32, device=table.device) for _ in range(2))
+    check(lib().tfcc_rocm_cache_read(_stream(), C.byref(d), _ptr(table), table.stride(0), table.shape[1], table.shape[0], _ptr(starts),
+                                     tokens, _ptr(keys), _ptr(values)))
+    return keys, values
+
+
+def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window=0, max_length=0, out=None):
+    """Attention of a chunk of new tokens of each sequence over what the cache holds of it: tfcc_rocm_paged_attention_f32.  q
+    [tokens, heads, size]: the chunks back to back, sequence i's rows starts[i] to starts[i + 1] - 1 (int32 [batch + 1]); lengths
+    (int32 [batch]): cached tokens, the chunk's own among them; table: int32 [batch, pages].  max_length: an upper bound of lengths
+    that the program knows, which the work is dealt out by.  Rows of out behind the last sequence are left as they were."""
+    if out is None:
+        done = _native().paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length)
+        if done is not None:
+            return done
+    import torch
+    d = PagedAttentionDesc()
+    d.cache = _cache_desc(cache)
+    _on_device(cache[0].device, q, table, starts, lengths, out)
+    q = _heads_of(q, "q")
+    if q.shape[2] != d.cache.size or q.shape[1] == 0 or q.shape[1] % d.cache.heads:
+        raise InvalidArgumentError("invalid q")
+    lengths = _integers(lengths, "lengths", lengths.numel(), (torch.int32,))
+    batch = lengths.shape[0]
+    table = _table_of(table, batch, "table")
+    starts = _integers(starts, "starts", batch + 1, (torch.int32,))
+    if window < 0 or max_length < 0 or (window and not causal):
+        raise InvalidArgumentError("invalid window")
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+    elif out.shape != q.shape or out.dtype != torch.float32 or out.stride(2) != 1:
+        raise InvalidArgumentError("invalid out")
+    d.q, d.out = _ptr(q), _ptr(out)
+    d.q_token_stride, d.q_head_stride, d.out_token_stride, d.out_head_stride = q.stride(0), q.stride(1), out.stride(0), out.stride(1)
+    d.tokens, d.heads, d.batch = q.shape[0], q.shape[1], batch
+    d.starts, d.lengths, d.table, d.table_stride, d.table_width = _ptr(starts), _ptr(lengths), _ptr(table), table.stride(0), table.shape[1]
+    d.max_length, d.scale, d.causal, d.window = max_length, scale, 1 if causal else 0, window
+    if q.shape[0] == 0 or batch == 0:
+        return out
+    needs = lib().tfcc_rocm_paged_attention_workspace(C.byref(d))
+    workspace = torch.empty(needs, dtype=torch.uint8, device=q.device) if needs else None
+    d.workspace, d.workspace_bytes = _ptr(workspace), needs
+    check(lib().tfcc_rocm_paged_attention_f32(_stream(), C.byref(d)))
+    return out
+
+
+def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None):
+    """A token for each row of logits [rows, length] from a given number in [0, 1) for each: tfcc_rocm_sample_f32.  random, temperature,
+    top_p, min_p: float32 [rows], top_k: int32 [rows]; None: temperature 1, no such filter.  Returns (int64 tokens, float32
+    probabilities among the kept ones), each [rows]."""
+    done = _native().sample(logits, random, temperature, top_k, top_p, min_p)
+    if done is not None:
+        return done
+    import torch
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[1] == 0:
+        raise InvalidArgumentError("invalid logits")
+    _on_device(logits.device, random, temperature, top_k, top_p, min_p)
+    rows, length = logits.shape
+    if length > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    given = {}
+    for name, t, dtype in (("random", random, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if t is None and name == "random":
+            raise InvalidArgumentError("invalid random")
+        given[name] = None if t is None else _integers(t, name, rows, (dtype,))
+    tokens = torch.empty((rows,), dtype=torch.int64, device=logits.device)
+    probabilities = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    d = SampleDesc()
+    d.logits, d.row_stride, d.rows, d.length = _ptr(logits), logits.stride(0), rows, length
+    d.random, d.temperature, d.top_k, d.top_p, d.min_p = (_ptr(given[n]) for n in ("random", "temperature", "top_k", "top_p", "min_p"))
+    d.tokens, d.probabilities = _ptr(tokens), _ptr(probabilities)
+    needs = lib().tfcc_rocm_sample_workspace(rows, length)
+    workspace = torch.empty(needs, dtype=torch.uint8, device=logits.device) if needs else None
+    d.workspace, d.workspace_bytes = _ptr(workspace), needs
+    check(lib().tfcc_rocm_sample_f32(_stream(), C.byref(d)))
+    return tokens, probabilities

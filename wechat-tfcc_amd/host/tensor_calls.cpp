@@ -362,10 +362,239 @@ PyObject* dequantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A tensor as above but for its strides, of which the last is one.
+const Tensor* rows_of(PyObject* o, at::ScalarType type, int64_t dims, c10::DeviceIndex device) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || !t.has_storage() || t.layout() != at::kStrided || t.scalar_type() != type || t.get_device() != device || t.is_neg()) return nullptr;
+  return t.dim() == dims && t.numel() > 0 && t.numel() <= INT32_MAX * int64_t{256} && t.stride(dims - 1) == 1 ? &t : nullptr;
+}
+
+// int32 or int64 [count]; the type's code, -1: neither
+int integers(PyObject* o, int64_t count, c10::DeviceIndex device, const Tensor** t) {
+  for (const auto& [type, code] : {std::pair{at::kInt, TFCC_ROCM_S32}, std::pair{at::kLong, TFCC_ROCM_S64}})
+    if ((*t = plain(o, type, device)) != nullptr) return (*t)->dim() == 1 && (*t)->numel() == count ? code : -1;
+  return -1;
+}
+
+bool number(PyObject* o, int64_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  const long long x = PyLong_AsLongLongAndOverflow(o, &overflow);
+  *v = x;
+  return !overflow && x >= 0 && x <= INT32_MAX;
+}
+
+// The memory of a paged cache: a tuple of two tensors of float32, or of two of int8 and two of scales.
+bool cache_of(PyObject* o, c10::DeviceIndex device, tfcc_rocm_paged_cache& c) {
+  if (!PyTuple_CheckExact(o)) return false;
+  const Py_ssize_t n = PyTuple_GET_SIZE(o);
+  if (n != 2 && n != 4) return false;
+  const at::ScalarType type = n == 4 ? at::kChar : at::kFloat;
+  const Tensor* keys = rows_of(PyTuple_GET_ITEM(o, 0), type, 4, device);
+  const Tensor* values = rows_of(PyTuple_GET_ITEM(o, 1), type, 4, device);
+  if (!keys || !values || keys->sizes() != values->sizes() || keys->strides() != values->strides()) return false;
+  if (!fits(keys->size(0)) || !fits(keys->size(1)) || !fits(keys->size(2)) || !fits(keys->size(3))) return false;
+  c.keys = data(keys);
+  c.values = data(values);
+  c.type = n == 4 ? TFCC_ROCM_S8 : TFCC_ROCM_F32;
+  c.pages = static_cast<unsigned>(keys->size(0));
+  c.heads = static_cast<unsigned>(keys->size(1));
+  c.page_size = static_cast<unsigned>(keys->size(2));
+  c.size = static_cast<unsigned>(keys->size(3));
+  c.page_stride = keys->stride(0);
+  c.head_stride = keys->stride(1);
+  c.row_stride = keys->stride(2);
+  if (n == 2) return true;
+  const Tensor* key_scales = plain(PyTuple_GET_ITEM(o, 2), at::kFloat, device);
+  const Tensor* value_scales = plain(PyTuple_GET_ITEM(o, 3), at::kFloat, device);
+  if (!key_scales || !value_scales || key_scales->dim() != 3 || value_scales->sizes() != key_scales->sizes() ||
+      key_scales->sizes() != keys->sizes().slice(0, 3) || key_scales->strides() != value_scales->strides())
+    return false;
+  c.key_scales = data<float>(key_scales);
+  c.value_scales = data<float>(value_scales);
+  c.scale_page_stride = key_scales->stride(0);
+  c.scale_head_stride = key_scales->stride(1);
+  c.scale_row_stride = key_scales->stride(2);
+  return true;
+}
+
+// rotary(q, k or None, positions, frequencies, interleaved, magnitude)
+PyObject* rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6 || !PyBool_Check(args[4]) || !PyFloat_CheckExact(args[5])) return none();
+  Here here(args[0]);
+  const Tensor* in[2] = {rows_of(args[0], at::kFloat, 3, here.device), nullptr};
+  const Tensor *positions, *frequencies = plain(args[3], at::kDouble, here.device);
+  if (!in[0] || !frequencies || frequencies->dim() != 1) return none();
+  const int64_t tokens = in[0]->size(0), size = in[0]->size(2), half = frequencies->size(0);
+  if (args[1] != Py_None) {
+    in[1] = rows_of(args[1], at::kFloat, 3, here.device);
+    if (!in[1] || in[1]->size(0) != tokens || in[1]->size(2) != size) return none();
+  }
+  tfcc_rocm_rotary_desc d{};
+  d.position_type = integers(args[2], tokens, here.device, &positions);
+  if (d.position_type < 0 || half < 1 || half > size / 2 || !fits(tokens) || !fits(size)) return none();
+  Tensor out[2];
+  for (int i = 0; i < 2 && in[i]; ++i) {
+    if (!fits(in[i]->size(1))) return none();
+    out[i] = empty(in[i]->sizes(), at::kFloat, here.device);
+    d.in[i] = data<float>(in[i]);
+    d.out[i] = data<float>(out[i]);
+    d.heads[i] = static_cast<unsigned>(in[i]->size(1));
+    d.in_token_stride[i] = in[i]->stride(0);
+    d.in_head_stride[i] = in[i]->stride(1);
+    d.out_token_stride[i] = static_cast<uint64_t>(in[i]->size(1)) * size;
+    d.out_head_stride[i] = size;
+  }
+  d.tokens = static_cast<unsigned>(tokens);
+  d.size = static_cast<unsigned>(size);
+  d.part = static_cast<unsigned>(2 * half);
+  d.positions = data(positions);
+  d.frequencies = data<double>(frequencies);
+  d.magnitude = static_cast<float>(PyFloat_AS_DOUBLE(args[5]));
+  d.interleaved = args[4] == Py_True ? 1 : 0;
+  void* stream = here.stream();
+  if (launch([&] { return tfcc_rocm_rotary_f32(stream, &d); }) != TFCC_ROCM_OK) return none();
+  PyObject* second = in[1] ? wrap(std::move(out[1])) : none();
+  return pack({wrap(std::move(out[0])), second});
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_write(cache, keys, values, slots): True where it was done
+PyObject* cache_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) return none();
+  Here here(args[1]);
+  tfcc_rocm_paged_cache c{};
+  const Tensor* keys = rows_of(args[1], at::kFloat, 3, here.device);
+  const Tensor* values = rows_of(args[2], at::kFloat, 3, here.device);
+  if (!keys || !values || keys->sizes() != values->sizes() || !cache_of(args[0], here.device, c)) return none();
+  if (keys->size(1) != c.heads || keys->size(2) != c.size || !fits(keys->size(0))) return none();
+  const Tensor* slots;
+  const int type = integers(args[3], keys->size(0), here.device, &slots);
+  if (type < 0) return none();
+  void* stream = here.stream();
+  if (launch([&] {
+        return tfcc_rocm_cache_write(stream, &c, data<float>(keys), keys->stride(0), keys->stride(1), data<float>(values), values->stride(0),
+                                     values->stride(1), static_cast<unsigned>(keys->size(0)), data(slots), type);
+      }) != TFCC_ROCM_OK)
+    return none();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_read(cache, table, starts, tokens)
+PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) return none();
+  Here here(args[1]);
+  tfcc_rocm_paged_cache c{};
+  const Tensor* table = rows_of(args[1], at::kInt, 2, here.device);
+  const Tensor* starts = plain(args[2], at::kInt, here.device);
+  int64_t tokens;
+  if (!table || !starts || !number(args[3], &tokens) || tokens == 0 || !cache_of(args[0], here.device, c)) return none();
+  if (starts->dim() != 1 || starts->size(0) != table->size(0) + 1 || !fits(table->size(0)) || !fits(table->size(1))) return none();
+  Tensor keys = empty({tokens, c.heads, c.size}, at::kFloat, here.device), values = empty({tokens, c.heads, c.size}, at::kFloat, here.device);
+  void* stream = here.stream();
+  if (launch([&] {
+        return tfcc_rocm_cache_read(stream, &c, data<int32_t>(table), table->stride(0), static_cast<unsigned>(table->size(1)),
+                                    static_cast<unsigned>(table->size(0)), data<int32_t>(starts), static_cast<unsigned>(tokens),
+                                    data<float>(keys), data<float>(values));
+      }) != TFCC_ROCM_OK)
+    return none();
+  return pack({wrap(std::move(keys)), wrap(std::move(values))});
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length)
+PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 9 || !PyFloat_CheckExact(args[5]) || !PyBool_Check(args[6])) return none();
+  Here here(args[0]);
+  tfcc_rocm_paged_attention_desc d{};
+  const Tensor* q = rows_of(args[0], at::kFloat, 3, here.device);
+  const Tensor* table = rows_of(args[2], at::kInt, 2, here.device);
+  const Tensor *starts = plain(args[3], at::kInt, here.device), *lengths = plain(args[4], at::kInt, here.device);
+  int64_t window, most;
+  if (!q || !table || !starts || !lengths || !number(args[7], &window) || !number(args[8], &most) || !cache_of(args[1], here.device, d.cache)) return none();
+  const int64_t batch = table->size(0);
+  if (lengths->dim() != 1 || lengths->size(0) != batch || starts->dim() != 1 || starts->size(0) != batch + 1) return none();
+  if (!fits(q->size(0)) || !fits(q->size(1)) || q->size(2) != d.cache.size || !fits(batch) || !fits(table->size(1))) return none();
+  Tensor out = empty(q->sizes(), at::kFloat, here.device);
+  d.q = data<float>(q);
+  d.out = data<float>(out);
+  d.q_token_stride = q->stride(0);
+  d.q_head_stride = q->stride(1);
+  d.out_token_stride = static_cast<uint64_t>(q->size(1)) * q->size(2);
+  d.out_head_stride = q->size(2);
+  d.tokens = static_cast<unsigned>(q->size(0));
+  d.heads = static_cast<unsigned>(q->size(1));
+  d.batch = static_cast<unsigned>(batch);
+  d.starts = data<int32_t>(starts);
+  d.lengths = data<int32_t>(lengths);
+  d.table = data<int32_t>(table);
+  d.table_stride = table->stride(0);
+  d.table_width = static_cast<unsigned>(table->size(1));
+  d.max_length = static_cast<unsigned>(most);
+  d.scale = static_cast<float>(PyFloat_AS_DOUBLE(args[5]));
+  d.causal = args[6] == Py_True ? 1 : 0;
+  d.window = static_cast<unsigned>(window);
+  Tensor workspace;
+  d.workspace_bytes = tfcc_rocm_paged_attention_workspace(&d);
+  if (d.workspace_bytes > 0) {
+    workspace = empty({static_cast<int64_t>(d.workspace_bytes)}, at::kByte, here.device);
+    d.workspace = data(workspace);
+  }
+  void* stream = here.stream();
+  if (launch([&] { return tfcc_rocm_paged_attention_f32(stream, &d); }) != TFCC_ROCM_OK) return none();
+  return wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, random, temperature, top_k, top_p, min_p), the last four or None
+PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) return none();
+  Here here(args[0]);
+  const Tensor* logits = rows_of(args[0], at::kFloat, 2, here.device);
+  if (!logits || !fits(logits->size(0)) || !fits(logits->size(1))) return none();
+  const int64_t rows = logits->size(0);
+  const Tensor* given[5] = {};
+  for (int i = 0; i < 5; ++i) {
+    if (args[1 + i] == Py_None && i > 0) continue;
+    given[i] = plain(args[1 + i], i == 2 ? at::kInt : at::kFloat, here.device);
+    if (!given[i] || given[i]->dim() != 1 || given[i]->size(0) != rows) return none();
+  }
+  tfcc_rocm_sample_desc d{};
+  Tensor tokens = empty({rows}, at::kLong, here.device), probabilities = empty({rows}, at::kFloat, here.device), workspace;
+  d.logits = data<float>(logits);
+  d.row_stride = logits->stride(0);
+  d.rows = static_cast<unsigned>(rows);
+  d.length = static_cast<unsigned>(logits->size(1));
+  d.random = data<float>(given[0]);
+  d.temperature = data<float>(given[1]);
+  d.top_k = data<int32_t>(given[2]);
+  d.top_p = data<float>(given[3]);
+  d.min_p = data<float>(given[4]);
+  d.tokens = data<int64_t>(tokens);
+  d.probabilities = data<float>(probabilities);
+  d.workspace_bytes = tfcc_rocm_sample_workspace(d.rows, d.length);
+  if (d.workspace_bytes > 0) {
+    workspace = empty({static_cast<int64_t>(d.workspace_bytes)}, at::kByte, here.device);
+    d.workspace = data(workspace);
+  }
+  void* stream = here.stream();
+  if (launch([&] { return tfcc_rocm_sample_f32(stream, &d); }) != TFCC_ROCM_OK) return none();
+  return pack({wrap(std::move(tokens)), wrap(std::move(probabilities))});
+  END_HANDLE_TH_ERRORS
+}
+
 #define TENSOR_CALL(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(NAME)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TENSOR_CALL(blas_matmul), TENSOR_CALL(reduce_sum), TENSOR_CALL(quantization_matmul),
                          TENSOR_CALL(quantization_matmul_requantize), TENSOR_CALL(gemv_dequant), TENSOR_CALL(gemv_dequant_packed),
-                         TENSOR_CALL(quantize), TENSOR_CALL(dequantize), {nullptr, nullptr, 0, nullptr}};
+                         TENSOR_CALL(quantize), TENSOR_CALL(dequantize), TENSOR_CALL(rotary),
+                         TENSOR_CALL(cache_write), TENSOR_CALL(cache_read), TENSOR_CALL(paged_attention), TENSOR_CALL(sample), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
