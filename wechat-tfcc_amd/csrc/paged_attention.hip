@@ -17,6 +17,7 @@
 //
 // The keys of a tile are dealt to the four wavefronts of a workgroup in turns, and in pieces to several workgroups where there are few
 // tiles; each wavefront keeps maximum, sum and output of its own, joined in LDS, the pieces by a second launch.
+#include "lds_dma.hpp"
 #include "paged_attention_plan.hpp"
 #include "paged_cache.hpp"
 
@@ -29,7 +30,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256;  // of the launch that joins pieces
 
 struct AttentionArgs {
   CacheView cache;
@@ -61,29 +62,41 @@ struct Tile {
   int row_low, row_high;
 };
 
+// The value of the lane that a data-parallel move names, 0 where there is none.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ unsigned moved(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xf, false);
+}
+// Sums of the lanes up to each: 1, 2, 4 and 8 lanes along the rows of 16, then on from row to row and from half to half.
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+
 // The chunks' tiles are counted off along the batch, 64 sequences at a time.
-__device__ Tile find_tile(const AttentionArgs& p, unsigned tile, unsigned rows_of_tile, unsigned row) {
+__device__ __forceinline__ Tile find_tile(const AttentionArgs& p, unsigned tile, unsigned rows_of_tile, unsigned row) {
   const unsigned lane = threadIdx.x & 63;
   Tile t;
   t.any = false;
   unsigned before = 0;
+  int length = 0;
+#pragma unroll 1
   for (unsigned base = 0; base < p.batch; base += 64) {
     const unsigned b = base + lane;
-    int first = 0, count = 0;
+    int first = 0, count = 0, held = 0;
     if (b < p.batch) {
       first = p.starts[b];
       int next = p.starts[b + 1];
+      held = p.lengths[b];
       next = next > (int)p.tokens ? (int)p.tokens : next;
       count = first >= 0 && next > first ? next - first : 0;
     }
-    const unsigned mine = ((unsigned)count * p.group.d + rows_of_tile - 1) / rows_of_tile;
-    unsigned upto = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const unsigned o = (unsigned)__shfl_up((int)upto, m, 64);
-      if (lane >= (unsigned)m) upto += o;
-    }
-    upto += before;
+    const unsigned mine = ((unsigned)count * p.group.d + rows_of_tile - 1) / rows_of_tile, upto = wave_scan(mine) + before;
     const unsigned long long past = __ballot(upto > tile);
     if (past != 0) {
       const int at = __builtin_ctzll(past);
@@ -91,13 +104,13 @@ __device__ Tile find_tile(const AttentionArgs& p, unsigned tile, unsigned rows_o
       t.sequence = base + at;
       t.first = __builtin_amdgcn_readlane(first, at);
       t.count = __builtin_amdgcn_readlane(count, at);
+      length = __builtin_amdgcn_readlane(held, at);
       t.row0 = (int)((tile - (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), at)) * rows_of_tile);
       break;
     }
     before = (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
   }
   if (!t.any) return t;
-  int length = p.lengths[t.sequence];
   length = length < 0 ? 0 : length;
   const int position0 = length - t.count;  // of the chunk's first token
   t.length = length < (int)p.max_length ? length : (int)p.max_length;
@@ -188,42 +201,45 @@ __device__ __forceinline__ void split_two(float a, float b, f16x2& hi, f16x2& lo
   lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a - (float)hi[0], b - (float)hi[1]));
 }
 
-// Joins the four wavefronts' outputs and writes them: to `out` where the keys are in one piece, else to the piece's part of the workspace.
+// Joins the wavefronts' outputs and writes them: to `out` where the keys are in one piece, else to the piece's part of the workspace.
 // o[] of a lane is its row's value `place(n)`; four neighbours in n are four neighbours in memory.
-template <int DPAD, class Place>
-__device__ void join_and_store(const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, float m, float l, const float* o, Place place) {
-  constexpr int LD = DPAD + 4;
-  __shared__ __align__(16) float outputs[kWaves][kAttentionRows][LD];
-  __shared__ float maxima[kWaves][kAttentionRows], sums[kWaves][kAttentionRows];
+template <int DPAD, int WAVES>
+struct Joining {
+  static constexpr int LD = DPAD + 4;
+  alignas(16) float outputs[WAVES][kAttentionRows][LD];
+  float maxima[WAVES][kAttentionRows], sums[WAVES][kAttentionRows];
+};
+template <int DPAD, int WAVES, class Place>
+__device__ __forceinline__ void join_and_store(Joining<DPAD, WAVES>& s, const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, float m, float l, const float* o, Place place) {
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, row = lane % 16;
   constexpr int N = DPAD / 4;  // of a lane: 16 rows of DPAD values over 64 lanes
   if (lane < 16) {
-    maxima[wave][row] = m;
-    sums[wave][row] = l;
+    s.maxima[wave][row] = m;
+    s.sums[wave][row] = l;
   }
 #pragma unroll
   for (int n = 0; n < N; n += 4) {
     const f32x4 v = {o[n], o[n + 1], o[n + 2], o[n + 3]};
-    *reinterpret_cast<f32x4*>(&outputs[wave][row][place(n)]) = v;
+    *reinterpret_cast<f32x4*>(&s.outputs[wave][row][place(n)]) = v;
   }
   __syncthreads();
   const unsigned size = p.cache.size, heads = p.cache.heads * p.group.d;
   const int rows = t.count * (int)p.group.d;
-  for (unsigned at = threadIdx.x; at < kAttentionRows * (DPAD / 4); at += kThreads) {
+  for (unsigned at = threadIdx.x; at < kAttentionRows * (DPAD / 4); at += (WAVES * 64)) {
     const unsigned r = at / (DPAD / 4), d = at % (DPAD / 4) * 4;
     const int in_chunk = t.row0 + (int)r;
     if (in_chunk >= rows || d >= size) continue;
-    float top = maxima[0][r];
+    float top = s.maxima[0][r];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, maxima[w][r]);
+    for (int w = 1; w < WAVES; ++w) top = fmaxf(top, s.maxima[w][r]);
     float total = 0;
     f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      if (sums[w][r] == 0.0f) continue;  // a wavefront that saw no key of this row
-      const float f = __builtin_amdgcn_exp2f(maxima[w][r] - top);
-      total += f * sums[w][r];
-      sum += f * *reinterpret_cast<const f32x4*>(&outputs[w][r][d]);
+    for (int w = 0; w < WAVES; ++w) {
+      if (s.sums[w][r] == 0.0f) continue;  // a wavefront that saw no key of this row
+      const float f = __builtin_amdgcn_exp2f(s.maxima[w][r] - top);
+      total += f * s.sums[w][r];
+      sum += f * *reinterpret_cast<const f32x4*>(&s.outputs[w][r][d]);
     }
     const unsigned token = p.group.quotient((unsigned)in_chunk), inner = (unsigned)in_chunk - token * p.group.d;
     const unsigned long long global = t.first + token, query_head = head * p.group.d + inner;
@@ -264,6 +280,22 @@ __device__ __forceinline__ bool take_work(const AttentionArgs& p, Tile& t, unsig
   return true;
 }
 
+// The page that holds a key, in two halves: what the table says of it, and, when that is wanted, whether there is such a page (-1: none).
+// What is loaded in one step is looked at in the next: a step does not wait for the table.
+// (Constant memory as far as a launch goes, so that entries come through the scalar cache: among the vector loads, which return in their order,
+// one would have to wait for all the rows that are on their way.)
+struct PageEntry {
+  int named;
+  bool listed;
+};
+typedef const __attribute__((address_space(4))) int* ConstantInts;
+__device__ __forceinline__ PageEntry entry_of(const AttentionArgs& p, const int* table, unsigned index) {  // a table that has a column
+  const bool listed = index < p.table_width;
+  return {((ConstantInts)table)[listed ? index : 0], listed};
+}
+__device__ __forceinline__ int page_of(const AttentionArgs& p, const PageEntry& e) {
+  return e.listed && (unsigned)e.named < p.cache.pages ? e.named : -1;
+}
 // The page that holds a key; -1: none.
 __device__ __forceinline__ int page_of(const AttentionArgs& p, const int* table, unsigned index) {
   if (index >= p.table_width) return -1;
@@ -271,26 +303,18 @@ __device__ __forceinline__ int page_of(const AttentionArgs& p, const int* table,
   return page >= 0 && (unsigned)page < p.cache.pages ? page : -1;
 }
 
-// int8: 32 keys in one step of a wavefront.  FAST: pages of a multiple of 16 rows, rows and scales that can be read 16 bytes at a time.
-template <int BLOCKS, bool FAST>
-__global__ __launch_bounds__(kThreads) void attention_s8_kernel(AttentionArgs p) {
-  constexpr int DPAD = 64 * BLOCKS;
-  Tile t;
-  unsigned head, split;
-  int begin, end;
-  if (!take_work(p, t, head, split, begin, end)) return;
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16, c = lane % 16;
-  const unsigned size = p.cache.size;
-  const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
-  const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
-  const float* const key_scales = p.cache.key_scales + head * p.cache.scale_head;
-  const float* const value_scales = p.cache.value_scales + head * p.cache.scale_head;
-  const int* const table = p.table + t.sequence * p.table_stride;
+// A tile's rows over an int8 cache: queries and running results of one wavefront.
+template <int BLOCKS>
+struct S8Rows {
+  static constexpr int N = 4 * BLOCKS;
+  f16x8 q_hi[2 * BLOCKS], q_lo[2 * BLOCKS];  // value 64 b + 16 g + 8 h + j of the head in [2 b + h][j], as two fp16 under a power of two
+  f32x4 o[N];                                // value N (4 g + i) + n in [n][i]
+  float row_scale;
+  // weights times value scales were at most w_most, which is at most w_limit = 2^w_e, and enter times w_up = 2^(14 - w_e)
+  float m = -INFINITY, l = 0.0f, w_most = 0.0f, w_limit = 0.0f, w_up = 0.0f;
+  int w_e = -100;
 
-  // the row's query: value 64 b + 16 g + 8 h + j of the head in q[2 b + h][j], as two fp16 under a power of two
-  f16x8 q_hi[2 * BLOCKS], q_lo[2 * BLOCKS];
-  float row_scale = 0.0f;
-  {
+  __device__ __forceinline__ void start(const AttentionArgs& p, const Tile& t, unsigned head, unsigned g) {
     f32x4 x[4 * BLOCKS];
     float top = 0.0f;
     const float* q = p.q + (unsigned long long)(t.first + (t.row_token < 0 ? 0 : t.row_token)) * p.q_token + (head * p.group.d + t.row_head) * p.q_head;
@@ -298,11 +322,13 @@ __global__ __launch_bounds__(kThreads) void attention_s8_kernel(AttentionArgs p)
     for (int b = 0; b < 4 * BLOCKS; ++b) {
       const unsigned d = 64 * (b / 4) + 16 * g + 4 * (b % 4);
       f32x4 v = {0, 0, 0, 0};
-      if (t.row_token >= 0 && d < size) v = *reinterpret_cast<const f32x4*>(q + d);
+      if (t.row_token >= 0 && d < p.cache.size) v = *reinterpret_cast<const f32x4*>(q + d);
       x[b] = v;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[j]));
     }
+#pragma unroll
+    for (int b = 0; b < 4 * BLOCKS; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[b][j]));
     top = across_groups_max(top);
     const int e = bound_of(top);
     const float up = power(14 - e);
@@ -315,100 +341,50 @@ __global__ __launch_bounds__(kThreads) void attention_s8_kernel(AttentionArgs p)
       q_hi[b] = hi.v;
       q_lo[b] = lo.v;
     }
+#pragma unroll
+    for (int n = 0; n < N; ++n) o[n] = f32x4{0, 0, 0, 0};
   }
 
-  // V: value (DPAD / 16) c + n of the head in tile n
-  constexpr int N = DPAD / 16;
-  f32x4 o[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) o[n] = f32x4{0, 0, 0, 0};
-  // weights times value scales were at most w_most, which is at most w_limit = 2^w_e, and enter times w_up = 2^(14 - w_e)
-  float m = -INFINITY, l = 0.0f, w_most = 0.0f, w_limit = 0.0f, w_up = 0.0f;
-  int w_e = -100;
-
-  for (int kb = begin + 32 * (int)wave; kb < end; kb += 32 * kWaves) {
-    unsigned long long key_at[2], value_at[8];
-    float ks[8], vs[8];
-    bool there[8];
-    if constexpr (FAST) {
-      const unsigned index0 = p.cache.page_size.quotient((unsigned)kb), index1 = p.cache.page_size.quotient((unsigned)kb + 16);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const unsigned index = h ? index1 : index0;
-        const unsigned inside = (unsigned)kb + 16 * h - index * p.cache.page_size.d;
-        const int page = page_of(p, table, index);
-        const unsigned long long base = page < 0 ? 0 : page * p.cache.page + inside * p.cache.row;
-        const unsigned long long scale_base = page < 0 ? 0 : page * p.cache.scale_page + inside;
-        const unsigned long long row = page < 0 ? 0 : p.cache.row;
-        key_at[h] = base + c * row;
-        const f32x4 a = *reinterpret_cast<const f32x4*>(key_scales + scale_base + 4 * g), b = *reinterpret_cast<const f32x4*>(value_scales + scale_base + 4 * g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          value_at[4 * h + i] = base + (4 * g + i) * row;
-          ks[4 * h + i] = a[i];
-          vs[4 * h + i] = b[i];
-          there[4 * h + i] = page >= 0;
-        }
-      }
-    } else {
-      const auto locate = [&](int key, unsigned long long& at, unsigned long long& scale_at) {
-        const unsigned index = p.cache.page_size.quotient((unsigned)key), inside = (unsigned)key - index * p.cache.page_size.d;
-        const int page = page_of(p, table, index);
-        at = page < 0 ? 0 : page * p.cache.page + inside * p.cache.row;
-        scale_at = page < 0 ? 0 : page * p.cache.scale_page + inside * p.cache.scale_row;
-        return page >= 0;
-      };
-      unsigned long long unused;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) locate(kb + 16 * h + (int)c, key_at[h], unused);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        unsigned long long scale_at;
-        there[i] = locate(kb + 16 * (i / 4) + 4 * (int)g + i % 4, value_at[i], scale_at);
-        ks[i] = key_scales[scale_at];
-        vs[i] = value_scales[scale_at];
-      }
-    }
-    float s[8];
+  // k: 16 bytes from value 64 b + 16 g of key 16 h + c in [h][b]; key_scale: of keys 16 h + 4 g + i, and so s[4 h + i]
+  __device__ __forceinline__ void score(const u32x4 (&k)[2][BLOCKS], const f32x4 (&key_scale)[2], float (&s)[8]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
-        const unsigned d = 64 * b + 16 * g;
-        u32x4 w;
-        if constexpr (FAST) {
-          w = *reinterpret_cast<const u32x4*>(keys + key_at[h] + (d < size ? d : 0));
-        } else {
-          const u32x2 w0 = *reinterpret_cast<const u32x2*>(keys + key_at[h] + (d < size ? d : 0));
-          const u32x2 w1 = *reinterpret_cast<const u32x2*>(keys + key_at[h] + (d + 8 < size ? d + 8 : 0));
-          w = u32x4{w0[0], w0[1], w1[0], w1[1]};
-        }
-        const f16x8 k0 = eight_int8(w[0], w[1]), k1 = eight_int8(w[2], w[3]);
+        const f16x8 k0 = eight_int8(k[h][b][0], k[h][b][1]), k1 = eight_int8(k[h][b][2], k[h][b][3]);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q_lo[2 * b], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_lo[2 * b + 1], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, q_hi[2 * b], acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_hi[2 * b + 1], acc, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * h + i] = acc[i] * (row_scale * ks[4 * h + i]);
+      for (int i = 0; i < 4; ++i) s[4 * h + i] = acc[i] * (row_scale * key_scale[h][i]);
     }
+  }
+
+  // `missing`: a bit for each of the lane's eight keys that no page holds
+  __device__ __forceinline__ static void hide(const Tile& t, int kb, unsigned g, unsigned missing, float (&s)[8]) {
+    if (__any(missing != 0) || kb < t.all_low || kb + 32 > t.all_high) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = kb + 16 * (i / 4) + 4 * (int)g + i % 4;
-      const bool seen = there[i] && key >= t.row_low && key < t.row_high;
-      s[i] = seen ? s[i] : -INFINITY;
+      for (int i = 0; i < 8; ++i) {
+        const int key = kb + 16 * (i / 4) + 4 * (int)g + i % 4;
+        s[i] = (missing >> i & 1) == 0 && key >= t.row_low && key < t.row_high ? s[i] : -INFINITY;
+      }
     }
+  }
+
+  // v: words from value N c of key 16 h + 4 g + i in [4 h + i]
+  __device__ __forceinline__ void add(float (&s)[8], const f32x4 (&value_scale)[2], const unsigned (&v)[8][BLOCKS]) {
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     top = across_groups_max(top);
     const float next = fmaxf(m, top), zero = next == -INFINITY ? 0.0f : next;
-    Half8 w_hi, w_lo;
     float w[8], w_top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float e = __builtin_amdgcn_exp2f(s[i] - zero);
       s[i] = e;
-      w[i] = e == 0.0f ? 0.0f : e * vs[i];
+      w[i] = e == 0.0f ? 0.0f : e * value_scale[i / 4][i % 4];
       w_top = fmaxf(w_top, fabsf(w[i]));
     }
     w_top = across_groups_max(w_top);
@@ -423,8 +399,9 @@ __global__ __launch_bounds__(kThreads) void attention_s8_kernel(AttentionArgs p)
       w_up = power(14 - e);
       const float both = f * power(step < -126 ? -126 : step > 127 ? 127 : step);
 #pragma unroll
-      for (int n = 0; n < N; ++n) o[n] *= both;
+      for (int i = 0; i < N; ++i) o[i] *= both;
     }
+    Half8 w_hi, w_lo;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       l += s[i];
@@ -432,13 +409,11 @@ __global__ __launch_bounds__(kThreads) void attention_s8_kernel(AttentionArgs p)
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_two(w[2 * i], w[2 * i + 1], w_hi.p[i], w_lo.p[i]);
-    // DPAD / 16 bytes of each of the lane's eight keys, four at a time
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) {
       unsigned word[8];
-      const unsigned d = 4 * BLOCKS * c + 4 * b;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) word[i] = *reinterpret_cast<const unsigned*>(values + value_at[i] + (d < size ? d : 0));
+      for (int i = 0; i < 8; ++i) word[i] = v[i][b];
       const f16x8 v0 = eight_of<0>(word), v1 = eight_of<1>(word), v2 = eight_of<2>(word), v3 = eight_of<3>(word);
       o[4 * b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, w_lo.v, o[4 * b], 0, 0, 0);
       o[4 * b + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, w_lo.v, o[4 * b + 1], 0, 0, 0);
@@ -450,21 +425,225 @@ __global__ __launch_bounds__(kThreads) void attention_s8_kernel(AttentionArgs p)
       o[4 * b + 3] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v3, w_hi.v, o[4 * b + 3], 0, 0, 0);
     }
   }
-  l = across_groups_sum(l);
-  const float down = power(w_e - 14);
-  // o[n][i] is value N (4 g + i) + n: rearranged so that neighbours of the list are neighbours of the head
-  float list[DPAD / 4];
+
+  template <int WAVES>
+  __device__ __forceinline__ void finish(Joining<64 * BLOCKS, WAVES>& joining, const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, unsigned g) {
+    l = across_groups_sum(l);
+    const float down = power(w_e - 14);
+    float list[4 * N];  // neighbours in the list are neighbours in the head
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int n = 0; n < N; ++n) list[i * N + n] = o[n][i] * down;
-  join_and_store<DPAD>(p, t, head, split, m, l, list, [&](int at) { return N * (4 * (int)g + at / N) + at % N; });
+      for (int n = 0; n < N; ++n) list[i * N + n] = o[n][i] * down;
+    join_and_store(joining, p, t, head, split, m, l, list, [&](int at) { return N * (4 * (int)g + at / N) + at % N; });
+  }
+};
+
+// int8 with pages of a multiple of 16 rows whose rows and scales can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
+// of 16.  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
+// straight into LDS, a ring of STAGES of its own (no barriers), and reads a step from there when it is due.
+template <int BLOCKS, int WAVES>
+struct S8Ring {
+  static constexpr int kRows = 4 * BLOCKS * 1024, kBytes = kRows + 256;  // keys and values, scales
+  static constexpr int kStages = BLOCKS == 1 ? 4 : 2;
+  static constexpr int kCopies = 4 * BLOCKS + 1;
+  union {
+    alignas(16) unsigned char ring[WAVES][kStages][kBytes];
+    Joining<64 * BLOCKS, WAVES> joining;
+  };
+};
+template <int BLOCKS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs p) {
+  typedef S8Ring<BLOCKS, WAVES> Ring;
+  constexpr int STEP = 32 * WAVES, CHUNKS = 4 * BLOCKS /* of 16 bytes in a row */, PER_COPY = 64 / CHUNKS /* rows */, FOURS = PER_COPY / 4;
+  __shared__ Ring shared;
+  Tile t;
+  unsigned head, split;
+  int begin, end;
+  if (!take_work(p, t, head, split, begin, end)) return;
+  const unsigned lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
+  const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
+  const unsigned size = p.cache.size, row_bytes = (unsigned)p.cache.row;
+  const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
+  const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
+  const float* const scales = (lane < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head;
+  const int* const table = p.table + (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)t.sequence) * p.table_stride;
+  int kb = __builtin_amdgcn_readfirstlane(begin + 32 * (int)wave);
+  end = __builtin_amdgcn_readfirstlane(end);
+
+  const auto exchange = [](unsigned row) { return BLOCKS == 1 ? row / 4 % 4 : row % CHUNKS; };
+  // A copy brings PER_COPY whole rows, CHUNKS lanes to a row: lanes side by side ask for memory side by side (with a lane for each row the copies
+  // take four times as long).  A lane puts its 16 bytes at its own place in LDS; which of the row's chunks that is, and which row, is free
+  // and chosen so that what is read together lies in different banks.  Keys are read 16 rows at a time, a chunk of each: chunks are
+  // exchanged within a row by its number.  Values are read a few bytes of rows 4 g + i at a time: those rows lie side by side.
+  unsigned key_at[BLOCKS], value_at[BLOCKS];
+  const unsigned slot = lane / CHUNKS, chunk = lane % CHUNKS;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) {
+    const unsigned row = b * PER_COPY + slot, from = (chunk ^ exchange(row)) * 16;
+    key_at[b] = row * row_bytes + (from < size ? from : 0);
+    value_at[b] = ((b * FOURS + slot % FOURS) * 4 + slot / FOURS) * row_bytes + (chunk * 16 < size ? chunk * 16 : 0);
+  }
+  const unsigned half_bytes = 15 * row_bytes + size;
+  unsigned char* const ring = shared.ring[wave][0];
+  const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)ring;
+
+  PageEntry entries[2] = {};
+  const auto ask_pages = [&](int at) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) entries[h] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 16 * h));
+  };
+  const auto copy = [&](unsigned stage, int at, const int (&page)[2]) {
+    const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(ring_at + stage * Ring::kBytes));
+    unsigned long long scale_at[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned key = (unsigned)at + 16 * h, inside = key - p.cache.page_size.quotient(key) * p.cache.page_size.d;
+      const unsigned long long held = page[h] < 0 ? 0 : (unsigned)page[h], base = held * p.cache.page + inside * p.cache.row;
+      scale_at[h] = held * p.cache.scale_page + inside;
+      const lds_dma_v4i k = make_rsrc(keys + base, half_bytes), v = make_rsrc(values + base, half_bytes);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) dma16(k, to + (h * BLOCKS + b) * 1024, key_at[b]);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) dma16(v, to + ((2 + h) * BLOCKS + b) * 1024, value_at[b]);
+    }
+    const float* const scale = scales + ((lane & 16) ? scale_at[1] : scale_at[0]) + c;
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to + Ring::kRows), "v"(scale) : "memory", "m0");
+  };
+  unsigned gone = 0;  // two bits a stage: halves that no page holds
+  if (kb < end) ask_pages(kb);
+  int ahead = kb;  // the first step that no copy is under way for
+  const auto send = [&](unsigned stage) {
+    if (ahead < end) {
+      const int pages[2] = {page_of(p, entries[0]), page_of(p, entries[1])};
+      copy(stage, ahead, pages);
+      gone = (gone & ~(3u << (2 * stage))) | ((pages[0] < 0 ? 1u : 0u) | (pages[1] < 0 ? 2u : 0u)) << (2 * stage);
+      ahead += STEP;
+      if (ahead < end) ask_pages(ahead);
+    }
+  };
+#pragma unroll 1
+  for (unsigned stage = 0; stage < Ring::kStages; ++stage) send(stage);
+
+  S8Rows<BLOCKS> rows;
+  rows.start(p, t, head, g);
+  unsigned stage = 0;
+#pragma unroll 1
+  for (; kb < end; kb += STEP) {
+    // the copies of the stages behind this one may still be under way
+    if (kb + (Ring::kStages - 1) * STEP < end) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((Ring::kStages - 1) * Ring::kCopies) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    const unsigned char* const from = ring + stage * Ring::kBytes;
+    u32x4 k[2][BLOCKS];
+    unsigned v[8][BLOCKS];
+    f32x4 key_scale[2], value_scale[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) k[h][b] = *reinterpret_cast<const u32x4*>(from + h * BLOCKS * 1024 + c * (CHUNKS * 16) + ((4 * b + g) ^ exchange(c)) * 16);
+      key_scale[h] = *reinterpret_cast<const f32x4*>(from + Ring::kRows + (16 * h + 4 * g) * 4);
+      value_scale[h] = *reinterpret_cast<const f32x4*>(from + Ring::kRows + 128 + (16 * h + 4 * g) * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned char* const at = from + (2 + i / 4) * BLOCKS * 1024 + (g / FOURS) * 1024 + ((i % 4) * FOURS + g % FOURS) * (CHUNKS * 16) + 4 * BLOCKS * c;
+      if constexpr (BLOCKS == 1) {
+        v[i][0] = *reinterpret_cast<const unsigned*>(at);
+      } else if constexpr (BLOCKS == 2) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+        v[i][0] = w[0];
+        v[i][1] = w[1];
+      } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(at);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[i][b] = w[b];
+      }
+    }
+    const unsigned none = gone >> (2 * stage) & 3;
+    const unsigned missing = (none & 1 ? 15u : 0u) | (none & 2 ? 240u : 0u);
+    // Read: the stage may be written again.  (By the builtin, which the compiler counts with: it would else wait for the reads once more, and
+    // with them for the page entries that send() has asked for.)
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    send(stage);
+    stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    float s[8];
+    rows.score(k, key_scale, s);
+    rows.hide(t, kb, g, missing, s);
+    rows.add(s, value_scale, v);
+  }
+  __syncthreads();  // the ring is done with
+  rows.template finish<WAVES>(shared.joining, p, t, head, split, g);
 }
 
-// float32: 16 keys in one step of a wavefront.  UNIFORM: pages of a multiple of 16 rows.
-template <int BLOCKS, bool UNIFORM>
-__global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p) {
-  constexpr int DPAD = 64 * BLOCKS;
+// int8 in any layout, a page for each key, loaded when it is due.
+template <int BLOCKS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attention_s8_any_kernel(AttentionArgs p) {
+  constexpr int STEP = 32 * WAVES;
+  __shared__ Joining<64 * BLOCKS, WAVES> joining;
+  Tile t;
+  unsigned head, split;
+  int begin, end;
+  if (!take_work(p, t, head, split, begin, end)) return;
+  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16, c = lane % 16;
+  const unsigned size = p.cache.size;
+  const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
+  const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
+  const float* const key_scales = p.cache.key_scales + head * p.cache.scale_head;
+  const float* const value_scales = p.cache.value_scales + head * p.cache.scale_head;
+  const int* const table = p.table + t.sequence * p.table_stride;
+  const auto locate = [&](int key, unsigned long long& row, unsigned long long& scale) {
+    const unsigned index = p.cache.page_size.quotient((unsigned)key), inside = (unsigned)key - index * p.cache.page_size.d;
+    const int page = page_of(p, table, index);
+    row = page < 0 ? 0 : page * p.cache.page + inside * p.cache.row;
+    scale = page < 0 ? 0 : page * p.cache.scale_page + inside * p.cache.scale_row;
+    return page >= 0;
+  };
+  S8Rows<BLOCKS> rows;
+  rows.start(p, t, head, g);
+#pragma unroll 1
+  for (int kb = begin + 32 * (int)wave; kb < end; kb += STEP) {
+    u32x4 k[2][BLOCKS];
+    unsigned v[8][BLOCKS], missing = 0;
+    f32x4 key_scale[2], value_scale[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unsigned long long row, scale;
+      locate(kb + 16 * h + (int)c, row, scale);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const unsigned d = 64 * b + 16 * g;  // rows are 8-byte aligned
+        const u32x2 w0 = *reinterpret_cast<const u32x2*>(keys + row + (d < size ? d : 0));
+        const u32x2 w1 = *reinterpret_cast<const u32x2*>(keys + row + (d + 8 < size ? d + 8 : 0));
+        k[h][b] = u32x4{w0[0], w0[1], w1[0], w1[1]};
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        missing |= locate(kb + 16 * h + 4 * (int)g + i, row, scale) ? 0u : 1u << (4 * h + i);
+        key_scale[h][i] = key_scales[scale];
+        value_scale[h][i] = value_scales[scale];
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+          const unsigned d = 4 * BLOCKS * c + 4 * b;
+          v[4 * h + i][b] = *reinterpret_cast<const unsigned*>(values + row + (d < size ? d : 0));
+        }
+      }
+    }
+    float s[8];
+    rows.score(k, key_scale, s);
+    rows.hide(t, kb, g, missing, s);
+    rows.add(s, value_scale, v);
+  }
+  rows.template finish<WAVES>(joining, p, t, head, split, g);
+}
+
+// float32: 16 keys in one step of a wavefront.  The next step's keys are loaded into the registers of this one's as soon as the
+// scores are formed, its values once the weights have met them.  UNIFORM: pages of a multiple of 16 rows; `missing`: a bit for each of the
+// lane's four keys that no page holds.
+template <int BLOCKS, int WAVES, bool UNIFORM>
+__global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs p) {
+  constexpr int DPAD = 64 * BLOCKS, STEP = 16 * WAVES;
+  __shared__ Joining<DPAD, WAVES> joining;
   Tile t;
   unsigned head, split;
   int begin, end;
@@ -475,6 +654,45 @@ __global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p
   const float* const values = static_cast<const float*>(p.cache.values) + head * p.cache.head;
   const int* const table = p.table + t.sequence * p.table_stride;
 
+  int kb = __builtin_amdgcn_readfirstlane(begin + 16 * (int)wave);
+  end = __builtin_amdgcn_readfirstlane(end);
+  f32x4 k[4 * BLOCKS], v[4][BLOCKS];
+  unsigned missing = 0;
+  const auto inside_page = [&](unsigned key) { return key - p.cache.page_size.quotient(key) * p.cache.page_size.d; };
+  const auto locate = [&](int key, unsigned long long& row) {
+    const int page = page_of(p, table, p.cache.page_size.quotient((unsigned)key));
+    row = page < 0 ? 0 : page * p.cache.page + inside_page((unsigned)key) * p.cache.row;
+    return page >= 0;
+  };
+  PageEntry entry = {};
+  const auto ask_page = [&](int at) {
+    if constexpr (UNIFORM) entry = entry_of(p, table, p.cache.page_size.quotient((unsigned)at));
+  };
+  const auto load_keys = [&](int at, int page) {
+    unsigned long long row;
+    if constexpr (UNIFORM) row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (inside_page((unsigned)at) + c) * p.cache.row;
+    else locate(at + (int)c, row);
+#pragma unroll
+    for (int b = 0; b < 4 * BLOCKS; ++b) k[b] = *reinterpret_cast<const f32x4*>(keys + row + (16 * b + 4 * g < size ? 16 * b + 4 * g : 0));
+  };
+  const auto load_values = [&](int at, int page) {
+    missing = UNIFORM && page < 0 ? 15u : 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned long long row;
+      if constexpr (UNIFORM) row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (inside_page((unsigned)at) + 4 * g + i) * p.cache.row;
+      else missing |= locate(at + 4 * (int)g + i, row) ? 0u : 1u << i;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) v[i][b] = *reinterpret_cast<const f32x4*>(values + row + (64 * b + 4 * c < size ? 64 * b + 4 * c : 0));
+    }
+  };
+  if (kb < end) {
+    ask_page(kb);
+    const int page = page_of(p, entry);
+    load_keys(kb, page);
+    load_values(kb, page);
+    if (kb + STEP < end) ask_page(kb + STEP);
+  }
   // value 16 b + 4 g + j of the row's query in q[b][j]
   f32x4 q[4 * BLOCKS];
   {
@@ -495,48 +713,7 @@ __global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p
     for (int j = 0; j < 4; ++j) o[b][j] = f32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
 
-  for (int kb = begin + 16 * (int)wave; kb < end; kb += 16 * kWaves) {
-    unsigned long long key_at, value_at[4];
-    bool there[4], every = true;
-    if constexpr (UNIFORM) {
-      const unsigned index = p.cache.page_size.quotient((unsigned)kb), inside = (unsigned)kb - index * p.cache.page_size.d;
-      const int page = page_of(p, table, index);
-      const unsigned long long base = page < 0 ? 0 : page * p.cache.page + inside * p.cache.row, row = page < 0 ? 0 : p.cache.row;
-      key_at = base + c * row;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        value_at[i] = base + (4 * g + i) * row;
-        there[i] = page >= 0;
-      }
-      every = page >= 0;
-    } else {
-      const auto locate = [&](int key, unsigned long long& at) {
-        const unsigned index = p.cache.page_size.quotient((unsigned)key), inside = (unsigned)key - index * p.cache.page_size.d;
-        const int page = page_of(p, table, index);
-        at = page < 0 ? 0 : page * p.cache.page + inside * p.cache.row;
-        return page >= 0;
-      };
-      locate(kb + (int)c, key_at);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        there[i] = locate(kb + 4 * (int)g + i, value_at[i]);
-        every = every && there[i];
-      }
-      every = __all(every);
-    }
-    f32x4 k[4 * BLOCKS], v[4][BLOCKS];
-#pragma unroll
-    for (int b = 0; b < 4 * BLOCKS; ++b) {
-      const unsigned d = 16 * b + 4 * g;
-      k[b] = *reinterpret_cast<const f32x4*>(keys + key_at + (d < size ? d : 0));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        const unsigned d = 64 * b + 4 * c;
-        v[i][b] = *reinterpret_cast<const f32x4*>(values + value_at[i] + (d < size ? d : 0));
-      }
+  for (; kb < end; kb += STEP) {
     f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
     for (int b = 0; b < 4 * BLOCKS; ++b) {
@@ -548,14 +725,18 @@ __global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p
       s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], q[b][3], s1, 0, 0, 0);
     }
     f32x4 s = s0 + s1;
-    const bool edge = !every || kb < t.all_low || kb + 16 > t.all_high;
+    const bool more = kb + STEP < end;
+    const int page = page_of(p, entry);
+    if (more) load_keys(kb + STEP, page);
+    const bool edge = __any(missing != 0) || kb < t.all_low || kb + 16 > t.all_high;
     unsigned foreign = 0;  // values that are not finite, of keys that some row does not see
     if (edge) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = kb + 4 * (int)g + i;
-        s[i] = there[i] && key >= t.row_low && key < t.row_high ? s[i] : -INFINITY;
-        const bool none = !there[i] || key < t.low || key >= t.high;
+        const bool there = (missing >> i & 1) == 0;
+        s[i] = there && key >= t.row_low && key < t.row_high ? s[i] : -INFINITY;
+        const bool none = !there || key < t.low || key >= t.high;
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -599,9 +780,9 @@ __global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p
         const float e0 = __shfl(e[0], (int)from, 64), e1 = __shfl(e[1], (int)from, 64), e2 = __shfl(e[2], (int)from, 64), e3 = __shfl(e[3], (int)from, 64);
         const float weight = at % 4 == 0 ? e0 : at % 4 == 1 ? e1 : at % 4 == 2 ? e2 : e3;
         const unsigned index = p.cache.page_size.quotient((unsigned)key), inside = (unsigned)key - index * p.cache.page_size.d;
-        const int page = page_of(p, table, index);
-        if (page < 0 || key < t.row_low || key >= t.row_high) continue;
-        const float* row = values + page * p.cache.page + inside * p.cache.row;
+        const int held = page_of(p, table, index);
+        if (held < 0 || key < t.row_low || key >= t.row_high) continue;
+        const float* row = values + held * p.cache.page + inside * p.cache.row;
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
@@ -614,6 +795,10 @@ __global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p
             }
       }
     }
+    if (more) {
+      load_values(kb + STEP, page);
+      if (kb + 2 * STEP < end) ask_page(kb + 2 * STEP);
+    }
   }
   l = across_groups_sum(l);
   float list[DPAD / 4];
@@ -623,41 +808,63 @@ __global__ __launch_bounds__(kThreads) void attention_f32_kernel(AttentionArgs p
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) list[(b * 4 + i) * 4 + j] = o[b][j][i];
-  join_and_store<DPAD>(p, t, head, split, m, l, list, [&](int at) { return 64 * (at / 16) + 4 * (4 * (int)g + at % 16 / 4); });
+  join_and_store(joining, p, t, head, split, m, l, list, [&](int at) { return 64 * (at / 16) + 4 * (4 * (int)g + at % 16 / 4); });
 }
 
-// The pieces of a row joined: one wavefront to a row.
+// The pieces of a row joined: a workgroup to a row, its threads four values each of one in every kThreads / (size / 4) pieces.
 __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) {
-  __shared__ float weights[kWaves][kAttentionMostSplits];
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, heads = p.cache.heads * p.group.d, size = p.cache.size;
-  const unsigned long long row = (unsigned long long)blockIdx.x * kWaves + wave, rows = (unsigned long long)p.tokens * heads;
-  if (row >= rows) return;
-  const unsigned token = (unsigned)(row / heads), head = (unsigned)(row - (unsigned long long)token * heads);
+  __shared__ float weights[kAttentionMostSplits];
+  __shared__ __align__(16) f32x4 sums[kThreads];
+  const unsigned lane = threadIdx.x & 63, heads = p.cache.heads * p.group.d, size = p.cache.size, quads = size / 4;
+  const unsigned long long row = blockIdx.x, rows = (unsigned long long)p.tokens * heads;
+  const unsigned token = blockIdx.x / heads, head = blockIdx.x - token * heads;
   if ((int)token >= p.starts[p.batch] || (int)token < p.starts[0]) return;
-  float top = -INFINITY;
+  float top = -INFINITY, total = 0.0f;
   for (unsigned i = lane; i < p.splits; i += 64) {
     const float* s = p.statistics + (i * rows + row) * 2;
     if (s[1] != 0.0f) top = fmaxf(top, s[0]);
   }
   top = wave_max(top);
-  float total = 0.0f;
   for (unsigned i = lane; i < p.splits; i += 64) {
     const float* s = p.statistics + (i * rows + row) * 2;
     const float w = s[1] != 0.0f ? __builtin_amdgcn_exp2f(s[0] - top) : 0.0f;
-    weights[wave][i] = s[1] != 0.0f ? w : -1.0f;  // below 0: the piece has no key of this row, and wrote no output
+    // below 0: the piece has no key of this row, and wrote no output.  (All wavefronts write the same.)
+    weights[i] = s[1] != 0.0f ? w : -1.0f;
     total += w * s[1];
   }
   total = wave_sum(total);
-  wave_lds_order();
-  for (unsigned d = lane * 4; d < size; d += 256) {
-    f32x4 sum = {0, 0, 0, 0};
-    for (unsigned i = 0; i < p.splits; ++i) {
-      const float w = weights[wave][i];
+  __syncthreads();
+  const unsigned shares = kThreads / quads, share = threadIdx.x / quads, d = threadIdx.x % quads * 4;
+  f32x4 sum = {0, 0, 0, 0};
+  if (share < shares) {
+#pragma unroll 8
+    for (unsigned i = share; i < p.splits; i += shares) {
+      const float w = weights[i];
       if (!(w < 0.0f)) sum += w * *reinterpret_cast<const f32x4*>(p.partial + (i * rows + row) * size + d);
     }
+  }
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  if (share == 0) {
+    for (unsigned i = 1; i < shares; ++i) sum += sums[threadIdx.x + i * quads];
     const f32x4 none = {0, 0, 0, 0};
     *reinterpret_cast<f32x4*>(p.out + token * p.out_token + head * p.out_head + d) = total == 0.0f ? none : sum / total;
   }
+}
+
+template <int BLOCKS>
+void launch_s8(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves, bool fast) {
+  const auto start = [&](auto kernel, unsigned width) { hipLaunchKernelGGL(kernel, grid, dim3(width * 64), 0, s, a); };
+  if constexpr (BLOCKS <= 2)
+    if (waves == 8) return start(fast ? attention_s8_kernel<BLOCKS, 8> : attention_s8_any_kernel<BLOCKS, 8>, 8);
+  start(fast ? attention_s8_kernel<BLOCKS, 4> : attention_s8_any_kernel<BLOCKS, 4>, 4);
+}
+template <int BLOCKS>
+void launch_f32(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves, bool uniform) {
+  const auto start = [&](auto kernel, unsigned width) { hipLaunchKernelGGL(kernel, grid, dim3(width * 64), 0, s, a); };
+  if constexpr (BLOCKS <= 2)
+    if (waves == 8) return start(uniform ? attention_f32_kernel<BLOCKS, 8, true> : attention_f32_kernel<BLOCKS, 8, false>, 8);
+  start(uniform ? attention_f32_kernel<BLOCKS, 4, true> : attention_f32_kernel<BLOCKS, 4, false>, 4);
 }
 
 int check_attention(const tfcc_rocm_paged_attention_desc& d) {
@@ -678,7 +885,7 @@ unsigned most_keys(const tfcc_rocm_paged_attention_desc& d) {
 }
 
 PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
-  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, most_keys(d), d.causal, d.window);
+  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window);
 }
 
 size_t workspace_of(const tfcc_rocm_paged_attention_desc& d, const PagedAttentionPlan& plan) {
@@ -708,7 +915,7 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
   TFCC_REQUIRE(needs == 0 || (d.workspace != nullptr && d.workspace_bytes >= needs), "paged_attention: a workspace of %zu bytes where %zu are needed",
                d.workspace == nullptr ? (size_t)0 : d.workspace_bytes, needs);
   const uint64_t groups = (uint64_t)plan.tiles * plan.splits * d.cache.heads;
-  TFCC_REQUIRE(groups <= 0x7fffffffu / kThreads, "paged_attention: %u tiles of rows", plan.tiles);
+  TFCC_REQUIRE(groups <= 0x7fffffffu / 512 && (uint64_t)d.tokens * d.heads <= 0x7fffffffu / kThreads, "paged_attention: %u tiles of rows", plan.tiles);
   AttentionArgs a{};
   a.cache = view_of(d.cache);
   a.q = d.q;
@@ -737,29 +944,27 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
   a.partial = static_cast<float*>(d.workspace);
   const hipStream_t s = as_stream(stream);
   const dim3 grid((unsigned)groups);
-  const auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a); };
   const tfcc_rocm_paged_cache& c = d.cache;
   const unsigned blocks = (c.size + 63) / 64;
+  const bool uniform = c.page_size % 16 == 0;
+  const bool fast = uniform && c.size % 16 == 0 && (c.page_stride | c.head_stride | c.row_stride) % 16 == 0 && c.scale_row_stride == 1 && c.row_stride < (1u << 26) &&
+                    (c.scale_page_stride | c.scale_head_stride) % 4 == 0 &&
+                    (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values) | reinterpret_cast<uintptr_t>(c.key_scales) |
+                     reinterpret_cast<uintptr_t>(c.value_scales)) % 16 == 0;
   if (c.type == TFCC_ROCM_S8) {
-    const bool fast = c.page_size % 16 == 0 && c.size % 16 == 0 && (c.page_stride | c.head_stride | c.row_stride) % 16 == 0 && c.scale_row_stride == 1 &&
-                      (c.scale_page_stride | c.scale_head_stride) % 4 == 0 &&
-                      (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values) | reinterpret_cast<uintptr_t>(c.key_scales) |
-                       reinterpret_cast<uintptr_t>(c.value_scales)) % 16 == 0;
-    if (blocks == 1) start(fast ? attention_s8_kernel<1, true> : attention_s8_kernel<1, false>);
-    else if (blocks == 2) start(fast ? attention_s8_kernel<2, true> : attention_s8_kernel<2, false>);
-    else if (blocks == 3) start(fast ? attention_s8_kernel<3, true> : attention_s8_kernel<3, false>);
-    else start(fast ? attention_s8_kernel<4, true> : attention_s8_kernel<4, false>);
+    if (blocks == 1) launch_s8<1>(a, grid, s, plan.waves, fast);
+    else if (blocks == 2) launch_s8<2>(a, grid, s, plan.waves, fast);
+    else launch_s8<4>(a, grid, s, plan.waves, fast);
   } else {
-    const bool uniform = c.page_size % 16 == 0;
-    if (blocks == 1) start(uniform ? attention_f32_kernel<1, true> : attention_f32_kernel<1, false>);
-    else if (blocks == 2) start(uniform ? attention_f32_kernel<2, true> : attention_f32_kernel<2, false>);
-    else if (blocks == 3) start(uniform ? attention_f32_kernel<3, true> : attention_f32_kernel<3, false>);
-    else start(uniform ? attention_f32_kernel<4, true> : attention_f32_kernel<4, false>);
+    if (blocks == 1) launch_f32<1>(a, grid, s, plan.waves, uniform);
+    else if (blocks == 2) launch_f32<2>(a, grid, s, plan.waves, uniform);
+    else if (blocks == 3) launch_f32<3>(a, grid, s, plan.waves, uniform);
+    else launch_f32<4>(a, grid, s, plan.waves, uniform);
   }
   if (int e = check_launch("paged_attention")) return e;
   if (plan.splits > 1) {
     const unsigned rows = d.tokens * d.heads;
-    hipLaunchKernelGGL(join_pieces_kernel, dim3((rows + kWaves - 1) / kWaves), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(join_pieces_kernel, dim3(rows), dim3(kThreads), 0, s, a);
     return check_launch("paged_attention join");
   }
   return TFCC_ROCM_OK;

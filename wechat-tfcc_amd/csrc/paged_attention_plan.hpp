@@ -7,12 +7,13 @@ namespace tfcc_rocm {
 
 struct PagedAttentionPlan {
   unsigned tiles;       // an upper bound of the tiles of rows that all chunks make
+  unsigned waves;       // of a workgroup, 4 or 8
   unsigned splits;      // pieces of the keys, each with a workgroup for every tile and cache head
-  unsigned split_keys;  // keys of a piece, a multiple of 128
+  unsigned split_keys;  // keys of a piece, a multiple of 256
 };
 
 constexpr unsigned kAttentionRows = 16;    // rows (a token's query heads of one cache head) of a tile
-constexpr unsigned kAttentionStep = 128;   // keys that the four wavefronts of a workgroup take in one step
+constexpr unsigned kAttentionStep = 256;   // keys that eight wavefronts take in one step
 constexpr unsigned kAttentionMostSplits = 256;
 
 // A chunk of n tokens makes ceil(n * group / rows) tiles; how the tokens are spread over the sequences only the device knows.
@@ -21,19 +22,31 @@ inline unsigned paged_attention_tiles(unsigned tokens, unsigned batch, unsigned 
   return (unsigned)(((uint64_t)tokens * group + (uint64_t)(rows - 1) * chunks) / rows);
 }
 
-inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, unsigned group, unsigned cache_heads, unsigned max_length,
+inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, unsigned group, unsigned cache_heads, unsigned size, unsigned max_length,
                                                int causal, unsigned window) {
   PagedAttentionPlan p;
   p.tiles = paged_attention_tiles(tokens, batch, group, kAttentionRows);
   // a tile spans at most `rows` tokens: the keys that one of them sees
   uint64_t keys = max_length;
   if (causal && window > 0 && (uint64_t)window + kAttentionRows + 32 < keys) keys = (uint64_t)window + kAttentionRows + 32;
-  const uint64_t groups = (uint64_t)p.tiles * cache_heads;
-  uint64_t splits = groups == 0 ? 1 : 1024 / groups;
-  const uint64_t most = (keys + 2 * kAttentionStep - 1) / (2 * kAttentionStep);
-  if (splits > most) splits = most;
-  if (splits > kAttentionMostSplits) splits = kAttentionMostSplits;
-  if (splits < 1) splits = 1;
+  // Workgroups to expect: chunks of about the same number of tokens.
+  const uint64_t chunks = tokens < batch ? tokens : batch, mean = chunks == 0 ? 0 : (tokens + chunks - 1) / chunks;
+  const uint64_t groups = chunks * ((mean * group + kAttentionRows - 1) / kAttentionRows) * cache_heads;
+  // One workgroup of eight wavefronts to a CU is best as long as there are no more than two for each CU: it has the CU's LDS for rows on
+  // their way, and little time goes into beginnings and ends (64 sequences of up to 4096 keys, 8 heads of 128 in int8: 88 us, with
+  // four wavefronts 97; 200 sequences of 700: 78 and 59).  Eight with heads wider than 128 do not have the registers.
+  uint64_t splits = 1;
+  p.waves = groups <= 512 && size <= 128 && keys > kAttentionStep / 2 ? 8 : 4;
+  if (groups > 0 && groups < 256) {
+    // Fewer than CUs: pieces of the keys, where they save more steps than the launch that joins them costs, three steps of 256 keys with
+    // heads of 128 and four with heads of 64 (16 sequences of 4096: two pieces 30 us, one 40; one sequence of 1024: four 12.4, one 14.4;
+    // 16 of 1024: two 16.6, one 15.6).
+    const uint64_t steps = (keys + kAttentionStep - 1) / kAttentionStep;
+    splits = 256 / groups;
+    splits = splits < steps ? splits : steps;
+    if (splits > 1 && (steps - (steps + splits - 1) / splits) * (size + 128) < 3 * 256) splits = 1;
+    if (splits < 1) splits = 1;
+  }
   uint64_t each = (keys + splits - 1) / splits;
   each = (each + kAttentionStep - 1) / kAttentionStep * kAttentionStep;
   if (each == 0) each = kAttentionStep;
