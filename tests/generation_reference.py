@@ -74,11 +74,11 @@ def attention(q, cache, table, starts, lengths, scale, causal=True, window=0, mo
                     a, top = (np.abs(kk) @ np.abs(x)).max() * abs(scale), np.abs(s).max()
                     ds = (size + 4) * EPS * a + 8 * EPS * a + 4 * EPS * top
                     if len(cache) == 4:
-                        # pieces are multiples of 2^-24 under a factor that brings the row's largest to 2^13 or above: each
-                        # value of the query and each weight times value scale may be off by 2^-37 of the largest as well,
-                        # also where a key or value beside it is zero
+                        # the pieces of a query are multiples of 2^-24 where its largest value is 2^13 or above, those of a weight times a
+                        # value's scale where the largest such product of the row is 2^8 or above, or lies 2^7 below one that is and
+                        # that a later step outgrew: each is off by 2^-37 and 2^-32 of the largest, also beside a key or value of zero
                         ds += size * 2.0 ** -37 * np.abs(x).max() * np.abs(kk).max() * abs(scale)
-                        rest = len(p) * 2.0 ** -37 * 127 * (p * value_scales[seen, h // group]).max()
+                        rest = len(p) * 2.0 ** -32 * 127 * (p * value_scales[seen, h // group]).max()
                     else:
                         rest = 0.0
                     off[row, h] = (2 * ds + 16 * EPS + (len(p) + 32) * EPS) * (p @ np.abs(vv)) + rest + 1e-37

@@ -110,6 +110,24 @@ CASES = [
     ("s8", [900, 60], [2, 2], 4, 1, 64, 16, {"max_length": 512}),              # keys behind the bound are not seen
     ("s8", [3000, 1, 2048, 129], [1, 1, 1, 1], 32, 8, 128, 128, {}),           # many pieces
     ("f32", [3000, 1, 2048, 129], [1, 1, 1, 1], 32, 8, 128, 128, {}),
+    # chunks of many tokens
+    ("s8", [64], [64], 1, 1, 64, 16, {}),
+    ("s8", [300, 129, 70], [300, 33, 70], 2, 2, 64, 16, {}),
+    ("s8", [1000, 257], [130, 257], 8, 2, 128, 32, {}),
+    ("s8", [513, 90], [200, 90], 5, 1, 80, 48, {}),
+    ("s8", [200, 40, 0, 77], [100, 60, 0, 77], 4, 4, 96, 16, {}),              # the second has more tokens than are cached
+    ("s8", [400, 300], [160, 1], 3, 1, 192, 16, {}),
+    ("s8", [333], [333], 2, 1, 144, 16, {}),
+    ("s8", [290, 100], [290, 100], 4, 2, 256, 16, {}),
+    ("s8", [1500, 600], [200, 600], 2, 2, 64, 32, {"window": 1}),
+    ("s8", [1500, 600], [200, 600], 4, 2, 128, 32, {"window": 150}),
+    ("s8", [300, 500], [100, 120], 4, 2, 128, 16, {"causal": False}),
+    ("s8", [6000], [70], 8, 2, 128, 64, {}),                                   # few tiles of a long context: pieces
+    ("s8", [2500, 700], [90, 90], 8, 2, 128, 16, {"max_length": 2100}),
+    ("f32", [300, 129, 70], [300, 33, 70], 2, 2, 64, 16, {}),
+    ("f32", [513, 90], [200, 90], 5, 1, 80, 48, {"window": 100}),
+    ("f32", [1000, 257], [130, 257], 8, 2, 128, 32, {}),
+    ("f32", [290, 100], [290, 100], 4, 2, 256, 16, {}),
 ]
 
 
@@ -133,8 +151,9 @@ def test_many_sequences(pkg, T):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s8", "f32"])
-def test_pages_outside_the_cache(pkg, T, kind):
-    m = Made(pkg, kind, [200, 90, 64], [1, 30, 64], 4, 2, 64, 16, 4)
+@pytest.mark.parametrize("chunks", [[1, 30, 64], [150, 90, 64]])
+def test_pages_outside_the_cache(pkg, T, kind, chunks):
+    m = Made(pkg, kind, [200, 90, 64], chunks, 4, 2, 64, 16, 4)
     m.table[0, [0, 5]] = [-1, 10 ** 6]
     m.table[1, 3] = len(m.cache[0])
     m.table[2, :4] = -1  # nothing is there at all
@@ -143,7 +162,7 @@ def test_pages_outside_the_cache(pkg, T, kind):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s8", "f32"])
-@pytest.mark.parametrize("chunks", [[1, 1], [40, 21]])
+@pytest.mark.parametrize("chunks", [[1, 1], [40, 21], [120, 70]])
 def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks):
     import torch
     m = Made(pkg, kind, [150, 70], chunks, 6, 2, 64, 16, 5)
@@ -173,9 +192,10 @@ def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks):
 
 
 @pytest.mark.gpu
-def test_scales_of_all_sizes(pkg, T):
+@pytest.mark.parametrize("chunks", [[2, 45], [200, 45]])
+def test_scales_of_all_sizes(pkg, T, chunks):
     """Rows of values from 10^-20 to 10^20, zeros among them, and queries likewise."""
-    m = Made(pkg, "s8", [300, 45], [2, 45], 4, 2, 128, 16, 6)
+    m = Made(pkg, "s8", [300, 45], chunks, 4, 2, 128, 16, 6)
     m.cache[3][:] = np.exp(m.rng.normal(size=m.cache[3].shape) * 15).astype(np.float32)
     m.cache[3][m.rng.random(m.cache[3].shape) < 0.2] = 0
     m.cache[2][m.rng.random(m.cache[2].shape) < 0.2] = 0
@@ -188,23 +208,25 @@ def test_scales_of_all_sizes(pkg, T):
 
 
 @pytest.mark.gpu
-def test_large_scores(pkg, T):
+@pytest.mark.parametrize("chunks", [[3, 30], [250, 30]])
+def test_large_scores(pkg, T, chunks):
     """Weights that all fall on one key or underflow."""
     for kind in ("s8", "f32"):
-        m = Made(pkg, kind, [400, 30], [3, 30], 4, 2, 64, 16, 7)
+        m = Made(pkg, kind, [400, 30], chunks, 4, 2, 64, 16, 7)
         m.scale *= 100
         m.check(T)
 
 
 @pytest.mark.gpu
-def test_rows_whose_scores_rise_beside_rows_whose_do_not(pkg, T):
+@pytest.mark.parametrize("chunk", [1, 64])
+def test_rows_whose_scores_rise_beside_rows_whose_do_not(pkg, T, chunk):
     """The largest score of one row moves with every key, that of the other stays: neither loses what it has."""
-    m = Made(pkg, "s8", [5000], [1], 2, 1, 64, 16, 13)
+    m = Made(pkg, "s8", [5000], [chunk], 2, 1, 64, 16, 13)
     m.cache[0][:] = m.cache[0][0, 0, 0]
     at = np.arange(5000)
     m.cache[2][m.table[0][at // 16], 0, at % 16] = np.linspace(0.001, 0.02, 5000, dtype=np.float32)
-    m.q[0, 0] = m.cache[0][0, 0, 0] / np.float32(100)
-    m.q[0, 1] = -m.q[0, 0]
+    m.q[:, 0] = m.cache[0][0, 0, 0] / np.float32(100)
+    m.q[:, 1] = -m.q[:, 0]
     got = m.run(T)
     m.check(T, got)
     want, _ = R.attention(m.q, m.cache, m.table, m.starts, m.lengths, m.scale)

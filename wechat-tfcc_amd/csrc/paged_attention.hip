@@ -10,13 +10,14 @@
 // exchanged between lanes but two steps of the row maximum.  V is loaded as it lies, row by row; which column of the
 // product stands for which value of a head is free as well and follows the loads.
 //
-// An int8 cache keeps float32 accuracy: an int8 is exact in fp16, a float32 is nearly the sum of two (22 bits), so each product is two
-// fp16 matrix operations.  Queries are scaled by a power of two per row, weights times value scales by one per row that follows
-// the largest such product, so that the largest are near 2^14 and what fp16 cannot hold is 2^-38 of it.  A float32 cache
-// goes through the fp32 matrix operations.
+// An int8 cache keeps float32 accuracy: an int8 is exact in fp16, a float32 is the sum of two but for 2^-24 of it, so each product is two
+// fp16 matrix operations.  Queries are scaled by a power of two for each row.  What meets the values is a weight times a value's scale, and
+// what has to stay in fp16's range is that product, not the weight: a row's weights are 2^(score - frame), and the frame moves where
+// score + log2(scale) exceeds it by 15, to 8 below.  Between moves nothing is rescaled, and what fp16 cannot hold is 2^-32 of
+// the largest product or less.  The sum of the weights is kept in the same frame.  A float32 cache goes through the fp32 matrix operations.
 //
-// The keys of a tile are dealt to the four wavefronts of a workgroup in turns, and in pieces to several workgroups where there are few
-// tiles; each wavefront keeps maximum, sum and output of its own, joined in LDS, the pieces by a second launch.
+// The keys of a tile are dealt to the wavefronts of a workgroup in turns, and in pieces to several workgroups where there are few tiles; each
+// wavefront keeps frame, sum and output of its own, joined in LDS, the pieces by a second launch.  A frame of -infinity: no key was seen.
 #include "lds_dma.hpp"
 #include "paged_attention_plan.hpp"
 #include "paged_cache.hpp"
@@ -24,7 +25,9 @@
 namespace tfcc_rocm {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -195,11 +198,24 @@ __device__ __forceinline__ f16x8 eight_of(const unsigned (&w)[8]) {
   return h.v;
 }
 
-// float32 as the sum of two fp16, both cut off: 22 bits, the error at most 2^-21 of the value
+// float32 as the sum of two fp16, both to the nearest: the error is at most 2^-24 of the value, or half of fp16's smallest number, 2^-25
 __device__ __forceinline__ void split_two(float a, float b, f16x2& hi, f16x2& lo) {
-  hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a, b));
-  lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a - (float)hi[0], b - (float)hi[1]));
+  hi = __builtin_convertvector(f32x2{a, b}, f16x2);
+  lo = __builtin_convertvector(f32x2{fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b)}, f16x2);
 }
+
+// Powers of two for a row of queries whose largest value is `top`: `up` brings it to 2^13 .. 2^14 under the sign of the scale (0 for a scale of 0),
+// `scale` undoes that and is the positive factor of the scores.
+struct QueryScale {
+  float up, scale;
+};
+__device__ __forceinline__ QueryScale query_scale(float top, float scale) {
+  const int e = bound_of(top);
+  const float up = power(14 - e);
+  return {scale > 0.0f ? up : scale < 0.0f ? -up : 0.0f * scale, scale != 0.0f ? fmaxf(power(e - 14) * fabsf(scale), 1.17549435e-38f) : 1.0f};
+}
+// log2 of a value's scale for the frame.  A row of zeros, whose scale is 0, counts like one of 2^-90: its weight is summed and may not overflow.
+__device__ __forceinline__ float frame_log(float value_scale) { return fmaxf(__builtin_amdgcn_logf(fabsf(value_scale)), -90.0f); }
 
 // Joins the wavefronts' outputs and writes them: to `out` where the keys are in one piece, else to the piece's part of the workspace.
 // o[] of a lane is its row's value `place(n)`; four neighbours in n are four neighbours in memory.
@@ -236,7 +252,7 @@ __device__ __forceinline__ void join_and_store(Joining<DPAD, WAVES>& s, const At
     f32x4 sum = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      if (s.sums[w][r] == 0.0f) continue;  // a wavefront that saw no key of this row
+      if (s.maxima[w][r] == -INFINITY) continue;  // a wavefront that saw no key of this row
       const float f = __builtin_amdgcn_exp2f(s.maxima[w][r] - top);
       total += f * s.sums[w][r];
       sum += f * *reinterpret_cast<const f32x4*>(&s.outputs[w][r][d]);
@@ -245,7 +261,7 @@ __device__ __forceinline__ void join_and_store(Joining<DPAD, WAVES>& s, const At
     const unsigned long long global = t.first + token, query_head = head * p.group.d + inner;
     if (p.splits == 1) {
       const f32x4 none = {0, 0, 0, 0};
-      *reinterpret_cast<f32x4*>(p.out + global * p.out_token + query_head * p.out_head + d) = total == 0.0f ? none : sum / total;
+      *reinterpret_cast<f32x4*>(p.out + global * p.out_token + query_head * p.out_head + d) = top == -INFINITY ? none : sum / total;
     } else {
       const unsigned long long place_of = ((unsigned long long)split * p.tokens + global) * heads + query_head;
       *reinterpret_cast<f32x4*>(p.partial + place_of * size + d) = sum;
@@ -259,18 +275,18 @@ __device__ __forceinline__ void join_and_store(Joining<DPAD, WAVES>& s, const At
 
 // The workgroup's tile, cache head and piece of the keys; false: nothing to do here.  A piece without keys still says so to the
 // launch that joins the pieces.
-__device__ __forceinline__ bool take_work(const AttentionArgs& p, Tile& t, unsigned& head, unsigned& split, int& begin, int& end) {
+__device__ __forceinline__ bool take_work(const AttentionArgs& p, unsigned rows_of_tile, unsigned row, Tile& t, unsigned& head, unsigned& split, int& begin, int& end) {
   // cache heads first, then pieces, then tiles
   const unsigned outer = p.cache_heads.quotient(blockIdx.x), tile = p.pieces.quotient(outer);
   head = blockIdx.x - outer * p.cache_heads.d;
   split = outer - tile * p.pieces.d;
-  t = find_tile(p, tile, kAttentionRows, threadIdx.x % 16);
+  t = find_tile(p, tile, rows_of_tile, row);
   if (!t.any) return false;
   const long long from = (t.low & ~31) + (long long)split * p.split_keys, upto = from + p.split_keys;
   end = upto < t.high ? (int)upto : t.high;
   begin = from < end ? (int)from : end;
   if (begin >= end && p.splits > 1) {
-    if (threadIdx.x < kAttentionRows && t.row_token >= 0) {
+    if (t.row_token >= 0) {  // several lanes write the same for a row
       const unsigned long long at = ((unsigned long long)split * p.tokens + t.first + t.row_token) * p.cache.heads * p.group.d + head * p.group.d + t.row_head;
       p.statistics[at * 2] = -INFINITY;
       p.statistics[at * 2 + 1] = 0.0f;
@@ -309,10 +325,7 @@ struct S8Rows {
   static constexpr int N = 4 * BLOCKS;
   f16x8 q_hi[2 * BLOCKS], q_lo[2 * BLOCKS];  // value 64 b + 16 g + 8 h + j of the head in [2 b + h][j], as two fp16 under a power of two
   f32x4 o[N];                                // value N (4 g + i) + n in [n][i]
-  float row_scale;
-  // weights times value scales were at most w_most, which is at most w_limit = 2^w_e, and enter times w_up = 2^(14 - w_e)
-  float m = -INFINITY, l = 0.0f, w_most = 0.0f, w_limit = 0.0f, w_up = 0.0f;
-  int w_e = -100;
+  float row_scale, frame = -INFINITY, l = 0.0f;
 
   __device__ __forceinline__ void start(const AttentionArgs& p, const Tile& t, unsigned head, unsigned g) {
     f32x4 x[4 * BLOCKS];
@@ -329,10 +342,9 @@ struct S8Rows {
     for (int b = 0; b < 4 * BLOCKS; ++b)
 #pragma unroll
       for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[b][j]));
-    top = across_groups_max(top);
-    const int e = bound_of(top);
-    const float up = power(14 - e);
-    row_scale = power(e - 14) * p.scale;
+    const QueryScale scale = query_scale(across_groups_max(top), p.scale);
+    const float up = scale.up;
+    row_scale = scale.scale;
 #pragma unroll
     for (int b = 0; b < 2 * BLOCKS; ++b) {
       Half8 hi, lo;
@@ -345,7 +357,7 @@ struct S8Rows {
     for (int n = 0; n < N; ++n) o[n] = f32x4{0, 0, 0, 0};
   }
 
-  // k: 16 bytes from value 64 b + 16 g of key 16 h + c in [h][b]; key_scale: of keys 16 h + 4 g + i, and so s[4 h + i]
+  // k: 16 bytes from value 64 b + 16 g of key 16 h + c in [h][b]; key_scale: of keys 16 h + 4 g + i, and so s[4 h + i], scores but for row_scale
   __device__ __forceinline__ void score(const u32x4 (&k)[2][BLOCKS], const f32x4 (&key_scale)[2], float (&s)[8]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -359,54 +371,45 @@ struct S8Rows {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, q_hi[2 * b + 1], acc, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * h + i] = acc[i] * (row_scale * key_scale[h][i]);
+      for (int i = 0; i < 4; ++i) s[4 * h + i] = acc[i] * key_scale[h][i];
     }
   }
 
   // `missing`: a bit for each of the lane's eight keys that no page holds
-  __device__ __forceinline__ static void hide(const Tile& t, int kb, unsigned g, unsigned missing, float (&s)[8]) {
+  __device__ __forceinline__ static void hide(const Tile& t, int kb, unsigned g, unsigned missing, float (&s)[8], f32x4 (&value_scale)[2]) {
     if (__any(missing != 0) || kb < t.all_low || kb + 32 > t.all_high) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int key = kb + 16 * (i / 4) + 4 * (int)g + i % 4;
-        s[i] = (missing >> i & 1) == 0 && key >= t.row_low && key < t.row_high ? s[i] : -INFINITY;
+        const bool seen = (missing >> i & 1) == 0 && key >= t.row_low && key < t.row_high;
+        s[i] = seen ? s[i] : -INFINITY;
+        value_scale[i / 4][i % 4] = seen ? value_scale[i / 4][i % 4] : 0.0f;
       }
     }
   }
 
   // v: words from value N c of key 16 h + 4 g + i in [4 h + i]
   __device__ __forceinline__ void add(float (&s)[8], const f32x4 (&value_scale)[2], const unsigned (&v)[8][BLOCKS]) {
-    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaf(s[i], row_scale, frame_log(value_scale[i / 4][i % 4])));
     top = across_groups_max(top);
-    const float next = fmaxf(m, top), zero = next == -INFINITY ? 0.0f : next;
-    float w[8], w_top = 0.0f;
+    if (__any(top - frame > 15.0f)) {
+      const float next = top - frame > 15.0f ? top - 8.0f : frame, f = next == frame ? 1.0f : __builtin_amdgcn_exp2f(frame - next);
+      frame = next;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] *= f;
+    }
+    const float zero = frame == -INFINITY ? 0.0f : frame;
+    float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float e = __builtin_amdgcn_exp2f(s[i] - zero);
-      s[i] = e;
-      w[i] = e == 0.0f ? 0.0f : e * value_scale[i / 4][i % 4];
-      w_top = fmaxf(w_top, fabsf(w[i]));
-    }
-    w_top = across_groups_max(w_top);
-    if (__any(next > m || w_top > w_limit)) {
-      const float f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-      m = next;
-      l *= f;
-      w_most = fmaxf(w_top, w_most * f);
-      const int e = bound_of(w_most), step = w_e - e;
-      w_e = e;
-      w_limit = power(e);
-      w_up = power(14 - e);
-      const float both = f * power(step < -126 ? -126 : step > 127 ? 127 : step);
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] *= both;
+      const float e = __builtin_amdgcn_exp2f(fmaf(s[i], row_scale, -zero));
+      l += e;
+      w[i] = e * value_scale[i / 4][i % 4];
     }
     Half8 w_hi, w_lo;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      l += s[i];
-      w[i] *= w_up;
-    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_two(w[2 * i], w[2 * i + 1], w_hi.p[i], w_lo.p[i]);
 #pragma unroll
@@ -429,13 +432,12 @@ struct S8Rows {
   template <int WAVES>
   __device__ __forceinline__ void finish(Joining<64 * BLOCKS, WAVES>& joining, const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, unsigned g) {
     l = across_groups_sum(l);
-    const float down = power(w_e - 14);
     float list[4 * N];  // neighbours in the list are neighbours in the head
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int n = 0; n < N; ++n) list[i * N + n] = o[n][i] * down;
-    join_and_store(joining, p, t, head, split, m, l, list, [&](int at) { return N * (4 * (int)g + at / N) + at % N; });
+      for (int n = 0; n < N; ++n) list[i * N + n] = o[n][i];
+    join_and_store(joining, p, t, head, split, frame, l, list, [&](int at) { return N * (4 * (int)g + at / N) + at % N; });
   }
 };
 
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
   Tile t;
   unsigned head, split;
   int begin, end;
-  if (!take_work(p, t, head, split, begin, end)) return;
+  if (!take_work(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
   const unsigned lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
   const unsigned size = p.cache.size, row_bytes = (unsigned)p.cache.row;
@@ -569,11 +571,281 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
     stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
     float s[8];
     rows.score(k, key_scale, s);
-    rows.hide(t, kb, g, missing, s);
+    rows.hide(t, kb, g, missing, s, value_scale);
     rows.add(s, value_scale, v);
   }
   __syncthreads();  // the ring is done with
   rows.template finish<WAVES>(shared.joining, p, t, head, split, g);
+}
+
+// Chunks of many tokens, int8 as above: a workgroup takes 128 rows, a wavefront 32 of them, and all go over the same keys, 32 in a step.  Bound: the
+// matrix cores and, with as much to do, the vector unit.  So the keys and values of a step are turned into fp16 once for the four wavefronts, in the
+// order in which the matrix cores take them, into one of two LDS buffers while the other is worked on; the next step's rows
+// are on their way to registers meanwhile.  Products of 32 x 32 as above, with
+//   S^T: lane l holds row l % 32 and keys 8 a + 4 (l / 32) + i in [4 a + i]
+//   O^T: likewise values place(8 a + 4 (l / 32) + i, n) of the head in tile n
+constexpr int kTileWaves = 4, kTileKeys = 32;
+
+// Which value of a head is row L of tile n of the second product: a word of four values goes to four tiles, or to two rows of two where
+// 64 values are left.
+template <int BLOCKS>
+__device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
+  return n / 4 * 4 + 4 <= 2 * BLOCKS ? n / 4 * 128 + 4 * L + n % 4 : n / 4 * 128 + 4 * (L % 16) + 2 * (L / 16) + n % 4;
+}
+
+template <int BLOCKS>
+__global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attention_s8_tile_kernel(AttentionArgs p) {
+  constexpr int KS = 4 * BLOCKS, N = 2 * BLOCKS;  // products over a head, tiles of 32 of its values
+  struct Stage {
+    u32x4 keys[KS][64];       // lane l: key l % 32, values 16 s + 8 (l / 32) + j
+    u32x4 values[N][2][64];   // lane l: value_of(l % 32, n), keys 16 m + 8 (j / 4) + 4 (l / 32) + j % 4
+    float key_scale[kTileKeys], value_scale[kTileKeys], value_log[kTileKeys];
+    unsigned gone[2];  // a bit of its own for a half that no page holds
+  };
+  __shared__ Stage stages[2];
+  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = lane / 32;
+  Tile t;
+  unsigned head, split;
+  int begin, end;
+  if (!take_work(p, kAttentionChunkRows, wave * 32 + lane % 32, t, head, split, begin, end)) return;
+  const unsigned size = p.cache.size;
+  const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
+  const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
+  const int* const table = p.table + (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)t.sequence) * p.table_stride;
+  begin = __builtin_amdgcn_readfirstlane(begin);
+  end = __builtin_amdgcn_readfirstlane(end);
+  // what this wavefront's rows see; rows that are there come first
+  const int there = __builtin_popcountll(__ballot(t.row_token >= 0) & 0xffffffffull), last = there > 0 ? there - 1 : 0;
+  const int low = __builtin_amdgcn_readfirstlane(t.row_low), high = there > 0 ? __builtin_amdgcn_readlane(t.row_high, last) : 0;
+  const int all_low = __builtin_amdgcn_readlane(t.row_low, last), all_high = __builtin_amdgcn_readfirstlane(t.row_high);
+
+  // A step's rows: threads of the first half fetch keys, 16 bytes of key (thread % 32) at a time; those of the second values, a word of eight keys
+  // at a time; the first wavefront the scales.
+  constexpr int WORDS = 16 * BLOCKS, TASKS = (4 * WORDS + 127) / 128;
+  const bool for_keys = threadIdx.x < 128;
+  const unsigned me = threadIdx.x % 128;
+  u32x4 raw[BLOCKS <= 2 ? 2 : 4];  // BLOCKS times 16 bytes of a key, or TASKS times eight words
+  // Each thread asks for the pages of its own rows, through the vector loads: they come back in order, after the rows that were asked for before.
+  // (Entries through the scalar cache would be waited for with the LDS reads.)
+  float scale = 0.0f;
+  bool gone = false;
+  int named[TASKS];
+  const auto half_of = [&](int k) { return for_keys ? me / 16 % 2 : (me + 128 * k) / WORDS / 2 % 2; };
+  const auto ask_pages = [&](int at) {
+#pragma unroll
+    for (int k = 0; k < TASKS; ++k) {
+      const unsigned index = p.cache.page_size.quotient((unsigned)at + 16 * half_of(k));
+      named[k] = index < p.table_width ? table[index] : -1;
+    }
+  };
+  const auto fetch = [&](int at) {
+    const unsigned inside[2] = {(unsigned)at - p.cache.page_size.quotient((unsigned)at) * p.cache.page_size.d,
+                                (unsigned)at + 16 - p.cache.page_size.quotient((unsigned)at + 16) * p.cache.page_size.d};
+    const auto page_row = [&](int k, unsigned long long& held) {
+      const bool none = (unsigned)named[k] >= p.cache.pages;
+      held = none ? 0 : (unsigned)named[k];
+      return none;
+    };
+    unsigned long long held;
+    if (for_keys) {
+      gone = page_row(0, held);
+      const unsigned first = half_of(0) ? inside[1] : inside[0];
+      const int8_t* const row = keys + held * p.cache.page + (first + (me & 15)) * p.cache.row;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const unsigned d = 16 * (me / 32 + 4 * b);
+        raw[b] = *reinterpret_cast<const u32x4*>(row + (d < size ? d : 0));
+      }
+      if (threadIdx.x < 64) {
+        const float* const s = (threadIdx.x < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head;
+        scale = s[held * p.cache.scale_page + first + (threadIdx.x & 15)];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < TASKS; ++k) {
+        const unsigned task = me + 128 * k, word = task % WORDS, group = task / WORDS;
+        if (4 * WORDS % 128 == 0 || group < 4) {
+          (void)page_row(k, held);
+          const unsigned first = (group / 2 ? inside[1] : inside[0]) + 4 * (group % 2);
+          const int8_t* const row = values + held * p.cache.page + first * p.cache.row + (4 * word < size ? 4 * word : 0);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) raw[2 * k + j / 4][j % 4] = *reinterpret_cast<const unsigned*>(row + (8 * (j / 4) + j % 4) * p.cache.row);
+        }
+      }
+    }
+  };
+  const auto store = [&](Stage& s) {
+    if (for_keys) {
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) {
+        const unsigned step = me / 32 + 4 * b;
+        s.keys[step][me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][0], raw[b][1]));
+        s.keys[step][32 + me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][2], raw[b][3]));
+      }
+      if (threadIdx.x < 32) {
+        s.key_scale[threadIdx.x] = scale;
+        if (threadIdx.x % 16 == 0) s.gone[threadIdx.x / 16] = gone ? 1u << (threadIdx.x / 16) : 0u;
+      } else if (threadIdx.x < 64) {
+        s.value_scale[threadIdx.x - 32] = scale;
+        s.value_log[threadIdx.x - 32] = frame_log(scale);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < TASKS; ++k) {
+        const unsigned task = me + 128 * k, word = task % WORDS, group = task / WORDS;
+        if (4 * WORDS % 128 == 0 || group < 4) {
+          unsigned w[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[j] = raw[2 * k + j / 4][j % 4];
+          const f16x8 v[4] = {eight_of<0>(w), eight_of<1>(w), eight_of<2>(w), eight_of<3>(w)};
+          const bool quarters = (word / 32 + 1) * 4 <= N;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const unsigned n = word / 32 * 4 + (quarters ? b : b % 2), L = quarters ? word % 32 : word % 16 + 16 * (b / 2);
+            s.values[n][group / 2][32 * (group % 2) + L] = __builtin_bit_cast(u32x4, v[b]);
+          }
+        }
+      }
+    }
+  };
+
+  if (begin < end) {
+    ask_pages(begin);
+    fetch(begin);
+    if (begin + kTileKeys < end) ask_pages(begin + kTileKeys);
+  }
+  // the row's query, as above: value 16 s + 8 (l / 32) + j in [s][j]
+  f16x8 q_hi[KS], q_lo[KS];
+  float row_scale;
+  {
+    const float* const q = p.q + (unsigned long long)(t.first + (t.row_token < 0 ? 0 : t.row_token)) * p.q_token + (head * p.group.d + t.row_head) * p.q_head;
+    f32x4 x[2 * KS];
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < 2 * KS; ++s) {
+      const unsigned d = 16 * (s / 2) + 8 * half + 4 * (s % 2);
+      x[s] = f32x4{0, 0, 0, 0};
+      if (t.row_token >= 0 && d < size) x[s] = *reinterpret_cast<const f32x4*>(q + d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(x[s][j]));
+    }
+    float a, b;
+    butterfly_pair<32>(top, a, b);
+    const QueryScale scale = query_scale(fmaxf(a, b), p.scale);
+    const float up = scale.up;
+    row_scale = scale.scale;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      Half8 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_two(x[2 * s + j / 2][j % 2 * 2] * up, x[2 * s + j / 2][j % 2 * 2 + 1] * up, hi.p[j], lo.p[j]);
+      q_hi[s] = hi.v;
+      q_lo[s] = lo.v;
+    }
+  }
+  f32x16 o[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) o[n] = f32x16{};
+  float frame = -INFINITY, l = 0.0f;
+
+  unsigned turn = 0;
+#pragma unroll 1
+  for (int kb = begin; kb < end; kb += kTileKeys, turn ^= 1) {
+    Stage& s = stages[turn];
+    store(s);
+    if (kb + kTileKeys < end) {
+      fetch(kb + kTileKeys);
+      if (kb + 2 * kTileKeys < end) ask_pages(kb + 2 * kTileKeys);
+    }
+    __syncthreads();
+    if (kb >= high || kb + kTileKeys <= low) continue;
+    f32x16 x = {};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const f16x8 a = __builtin_bit_cast(f16x8, s.keys[k][lane]);
+      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_lo[k], x, 0, 0, 0);
+      x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[k], x, 0, 0, 0);
+    }
+    f32x4 value_scale[4], value_log[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const f32x4 key_scale = *reinterpret_cast<const f32x4*>(s.key_scale + 8 * a + 4 * half);
+      value_scale[a] = *reinterpret_cast<const f32x4*>(s.value_scale + 8 * a + 4 * half);
+      value_log[a] = *reinterpret_cast<const f32x4*>(s.value_log + 8 * a + 4 * half);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * a + i] *= key_scale[i];
+    }
+    const unsigned none = s.gone[0] | s.gone[1];
+    if (none != 0 || kb < all_low || kb + kTileKeys > all_high) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = kb + 8 * (i / 4) + 4 * (int)half + i % 4;
+        const bool seen = (none >> (i / 8) & 1) == 0 && key >= t.row_low && key < t.row_high;
+        x[i] = seen ? x[i] : -INFINITY;
+        value_scale[i / 4][i % 4] = seen ? value_scale[i / 4][i % 4] : 0.0f;
+      }
+    }
+    float top = -INFINITY, a, b;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaf(x[i], row_scale, value_log[i / 4][i % 4]));
+    butterfly_pair<32>(top, a, b);
+    top = fmaxf(a, b);
+    if (__any(top - frame > 15.0f)) {
+      const float next = top - frame > 15.0f ? top - 8.0f : frame, f = next == frame ? 1.0f : __builtin_amdgcn_exp2f(frame - next);
+      frame = next;
+      l *= f;
+#pragma unroll
+      for (int n = 0; n < N; ++n) o[n] *= f;
+    }
+    const float zero = frame == -INFINITY ? 0.0f : frame;
+    Half8 w_hi[2], w_lo[2];
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(fmaf(x[i], row_scale, -zero));
+      l += e;
+      w[i] = e * value_scale[i / 4][i % 4];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split_two(w[2 * i], w[2 * i + 1], w_hi[i / 4].p[i % 4], w_lo[i / 4].p[i % 4]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const f16x8 v = __builtin_bit_cast(f16x8, s.values[n][h][lane]);
+        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w_lo[h].v, o[n], 0, 0, 0);
+        o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w_hi[h].v, o[n], 0, 0, 0);
+      }
+  }
+  float a, b;
+  butterfly_pair<32>(l, a, b);
+  l = a + b;
+  if (t.row_token < 0) return;
+  const unsigned long long token = t.first + t.row_token, query_head = head * p.group.d + t.row_head;
+  float* to = p.out + token * p.out_token + query_head * p.out_head;
+  float factor = 1.0f;
+  if (p.splits > 1) {
+    const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
+    to = p.partial + place * size;
+    if (half == 0) {
+      p.statistics[place * 2] = frame;
+      p.statistics[place * 2 + 1] = l;
+    }
+  } else {
+    factor = frame == -INFINITY ? 0.0f : 1.0f / l;
+  }
+#pragma unroll
+  for (int n = 0; n < N; n += n / 4 * 4 + 4 <= N ? 4 : 2)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const unsigned d = value_of<BLOCKS>(8 * (i / 4) + 4 * half + i % 4, n);
+      if (d >= size) continue;
+      if (n / 4 * 4 + 4 <= N) {
+        *reinterpret_cast<f32x4*>(to + d) = f32x4{o[n][i], o[n + 1][i], o[n + 2][i], o[n + 3][i]} * factor;
+      } else {
+        *reinterpret_cast<f32x2*>(to + d) = f32x2{o[n][i] * factor, o[n + 1][i] * factor};
+      }
+    }
 }
 
 // int8 in any layout, a page for each key, loaded when it is due.
@@ -584,7 +856,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_any_kernel(AttentionA
   Tile t;
   unsigned head, split;
   int begin, end;
-  if (!take_work(p, t, head, split, begin, end)) return;
+  if (!take_work(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16, c = lane % 16;
   const unsigned size = p.cache.size;
   const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
@@ -631,7 +903,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_any_kernel(AttentionA
     }
     float s[8];
     rows.score(k, key_scale, s);
-    rows.hide(t, kb, g, missing, s);
+    rows.hide(t, kb, g, missing, s, value_scale);
     rows.add(s, value_scale, v);
   }
   rows.template finish<WAVES>(joining, p, t, head, split, g);
@@ -647,7 +919,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
   Tile t;
   unsigned head, split;
   int begin, end;
-  if (!take_work(p, t, head, split, begin, end)) return;
+  if (!take_work(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16, c = lane % 16;
   const unsigned size = p.cache.size;
   const float* const keys = static_cast<const float*>(p.cache.keys) + head * p.cache.head;
@@ -821,16 +1093,15 @@ __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) 
   if ((int)token >= p.starts[p.batch] || (int)token < p.starts[0]) return;
   float top = -INFINITY, total = 0.0f;
   for (unsigned i = lane; i < p.splits; i += 64) {
-    const float* s = p.statistics + (i * rows + row) * 2;
-    if (s[1] != 0.0f) top = fmaxf(top, s[0]);
+    top = fmaxf(top, p.statistics[(i * rows + row) * 2]);
   }
   top = wave_max(top);
   for (unsigned i = lane; i < p.splits; i += 64) {
     const float* s = p.statistics + (i * rows + row) * 2;
-    const float w = s[1] != 0.0f ? __builtin_amdgcn_exp2f(s[0] - top) : 0.0f;
-    // below 0: the piece has no key of this row, and wrote no output.  (All wavefronts write the same.)
-    weights[i] = s[1] != 0.0f ? w : -1.0f;
-    total += w * s[1];
+    const bool none = s[0] == -INFINITY;  // the piece has no key of this row
+    const float w = none ? 0.0f : __builtin_amdgcn_exp2f(s[0] - top);
+    weights[i] = none ? -1.0f : w;  // (all wavefronts write the same)
+    total += none ? 0.0f : w * s[1];
   }
   total = wave_sum(total);
   __syncthreads();
@@ -848,7 +1119,7 @@ __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) 
   if (share == 0) {
     for (unsigned i = 1; i < shares; ++i) sum += sums[threadIdx.x + i * quads];
     const f32x4 none = {0, 0, 0, 0};
-    *reinterpret_cast<f32x4*>(p.out + token * p.out_token + head * p.out_head + d) = total == 0.0f ? none : sum / total;
+    *reinterpret_cast<f32x4*>(p.out + token * p.out_token + head * p.out_head + d) = top == -INFINITY ? none : sum / total;
   }
 }
 
@@ -884,8 +1155,16 @@ unsigned most_keys(const tfcc_rocm_paged_attention_desc& d) {
   return d.max_length > 0 && d.max_length < held ? d.max_length : held;
 }
 
+// An int8 cache with pages of a multiple of 16 rows whose rows and scales can be read 16 bytes at a time.
+bool wide_reads(const tfcc_rocm_paged_cache& c) {
+  return c.type == TFCC_ROCM_S8 && c.page_size % 16 == 0 && c.size % 16 == 0 && (c.page_stride | c.head_stride | c.row_stride) % 16 == 0 &&
+         c.scale_row_stride == 1 && c.row_stride < (1u << 26) && (c.scale_page_stride | c.scale_head_stride) % 4 == 0 &&
+         (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values) | reinterpret_cast<uintptr_t>(c.key_scales) |
+          reinterpret_cast<uintptr_t>(c.value_scales)) % 16 == 0;
+}
+
 PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
-  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window);
+  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, wide_reads(d.cache));
 }
 
 size_t workspace_of(const tfcc_rocm_paged_attention_desc& d, const PagedAttentionPlan& plan) {
@@ -946,12 +1225,14 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
   const dim3 grid((unsigned)groups);
   const tfcc_rocm_paged_cache& c = d.cache;
   const unsigned blocks = (c.size + 63) / 64;
-  const bool uniform = c.page_size % 16 == 0;
-  const bool fast = uniform && c.size % 16 == 0 && (c.page_stride | c.head_stride | c.row_stride) % 16 == 0 && c.scale_row_stride == 1 && c.row_stride < (1u << 26) &&
-                    (c.scale_page_stride | c.scale_head_stride) % 4 == 0 &&
-                    (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values) | reinterpret_cast<uintptr_t>(c.key_scales) |
-                     reinterpret_cast<uintptr_t>(c.value_scales)) % 16 == 0;
-  if (c.type == TFCC_ROCM_S8) {
+  const bool uniform = c.page_size % 16 == 0, fast = wide_reads(c);
+  if (plan.rows == kAttentionChunkRows) {
+    const auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kTileWaves * 64), 0, s, a); };
+    if (blocks == 1) start(attention_s8_tile_kernel<1>);
+    else if (blocks == 2) start(attention_s8_tile_kernel<2>);
+    else if (blocks == 3) start(attention_s8_tile_kernel<3>);
+    else start(attention_s8_tile_kernel<4>);
+  } else if (c.type == TFCC_ROCM_S8) {
     if (blocks == 1) launch_s8<1>(a, grid, s, plan.waves, fast);
     else if (blocks == 2) launch_s8<2>(a, grid, s, plan.waves, fast);
     else launch_s8<4>(a, grid, s, plan.waves, fast);

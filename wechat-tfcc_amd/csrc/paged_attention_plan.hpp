@@ -6,6 +6,7 @@
 namespace tfcc_rocm {
 
 struct PagedAttentionPlan {
+  unsigned rows;        // of a tile
   unsigned tiles;       // an upper bound of the tiles of rows that all chunks make
   unsigned waves;       // of a workgroup, 4 or 8
   unsigned splits;      // pieces of the keys, each with a workgroup for every tile and cache head
@@ -13,6 +14,7 @@ struct PagedAttentionPlan {
 };
 
 constexpr unsigned kAttentionRows = 16;    // rows (a token's query heads of one cache head) of a tile
+constexpr unsigned kAttentionChunkRows = 128;  // of a tile of a chunk of many tokens
 constexpr unsigned kAttentionStep = 256;   // keys that eight wavefronts take in one step
 constexpr unsigned kAttentionMostSplits = 256;
 
@@ -23,15 +25,16 @@ inline unsigned paged_attention_tiles(unsigned tokens, unsigned batch, unsigned 
 }
 
 inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, unsigned group, unsigned cache_heads, unsigned size, unsigned max_length,
-                                               int causal, unsigned window) {
+                                               int causal, unsigned window, bool chunk_tiles) {
   PagedAttentionPlan p;
-  p.tiles = paged_attention_tiles(tokens, batch, group, kAttentionRows);
+  // chunks of about the same number of tokens
+  const uint64_t chunks = tokens < batch ? tokens : batch, mean = chunks == 0 ? 0 : (tokens + chunks - 1) / chunks;
+  p.rows = chunk_tiles && mean * group >= 64 ? kAttentionChunkRows : kAttentionRows;
+  p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
   // a tile spans at most `rows` tokens: the keys that one of them sees
   uint64_t keys = max_length;
-  if (causal && window > 0 && (uint64_t)window + kAttentionRows + 32 < keys) keys = (uint64_t)window + kAttentionRows + 32;
-  // Workgroups to expect: chunks of about the same number of tokens.
-  const uint64_t chunks = tokens < batch ? tokens : batch, mean = chunks == 0 ? 0 : (tokens + chunks - 1) / chunks;
-  const uint64_t groups = chunks * ((mean * group + kAttentionRows - 1) / kAttentionRows) * cache_heads;
+  if (causal && window > 0 && (uint64_t)window + p.rows + 32 < keys) keys = (uint64_t)window + p.rows + 32;
+  const uint64_t groups = chunks * ((mean * group + p.rows - 1) / p.rows) * cache_heads;
   // One workgroup of eight wavefronts to a CU is best as long as there are no more than two for each CU: it has the CU's LDS for rows on
   // their way, and little time goes into beginnings and ends (64 sequences of up to 4096 keys, 8 heads of 128 in int8: 88 us, with
   // four wavefronts 97; 200 sequences of 700: 78 and 59).  Eight with heads wider than 128 do not have the registers.
