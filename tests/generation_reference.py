@@ -50,38 +50,43 @@ def attention(q, cache, table, starts, lengths, scale, causal=True, window=0, mo
         page = np.where(there, page, 0)
         ks, vs = k[page, :, at % page_size], v[page, :, at % page_size]  # [cached, heads, size]
         value_scales = cache[3][page, :, at % page_size].astype(np.float64) if len(cache) == 4 else None
-        for t in range(n):
-            position = length - n + t
-            seen = there.copy()
-            if causal:
-                seen &= at <= position
-                if window:
-                    seen &= at > position - window
-            for h in range(q.shape[1]):
-                row = starts[i] + t
-                x = q[row, h].astype(np.float64)
-                kk, vv = ks[seen, h // group], vs[seen, h // group]
-                if not len(kk):
-                    out[row, h] = 0
-                    continue
-                with np.errstate(invalid="ignore"):
-                    s = kk @ x * scale
-                    e = np.exp(s - s.max())
-                    p = e / e.sum()
-                    out[row, h] = p @ vv
-                    # float32 sums of `size` products, one of the factors in two pieces of 11 bits cut off (2^-21), a scale and the
-                    # maximum taken off; then a sum of len(p) products with weights in two such pieces
-                    a, top = (np.abs(kk) @ np.abs(x)).max() * abs(scale), np.abs(s).max()
-                    ds = (size + 4) * EPS * a + 8 * EPS * a + 4 * EPS * top
-                    if len(cache) == 4:
-                        # the pieces of a query are multiples of 2^-24 where its largest value is 2^13 or above, those of a weight times a
-                        # value's scale where the largest such product of the row is 2^8 or above, or lies 2^7 below one that is and
-                        # that a later step outgrew: each is off by 2^-37 and 2^-32 of the largest, also beside a key or value of zero
-                        ds += size * 2.0 ** -37 * np.abs(x).max() * np.abs(kk).max() * abs(scale)
-                        rest = len(p) * 2.0 ** -32 * 127 * (p * value_scales[seen, h // group]).max()
-                    else:
-                        rest = 0.0
-                    off[row, h] = (2 * ds + 16 * EPS + (len(p) + 32) * EPS) * (p @ np.abs(vv)) + rest + 1e-37
+        position = (int(length) - n + np.arange(n))[:, None]
+        seen = np.broadcast_to(there, (n, cached)).copy()
+        if causal:
+            seen &= at <= position
+            if window:
+                seen &= at > position - window
+        seen = np.repeat(seen, group, 0)  # a row for each token and query head of the cache head
+        for h in range(heads):
+            rows = q[starts[i]:starts[i + 1], h * group:(h + 1) * group].astype(np.float64)
+            if not rows.size:
+                continue
+            x, kk, vv = rows.reshape(-1, size), ks[:, h], vs[:, h]
+            with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
+                s = np.where(seen, x @ kk.T * scale, -np.inf)
+                top = s.max(-1, keepdims=True, initial=-np.inf)
+                e = np.where(seen, np.exp(s - np.where(np.isfinite(top), top, 0)), 0)
+                p = np.where(seen.any(-1, keepdims=True), e / e.sum(-1, keepdims=True), 0)
+                # values of keys that a row does not see are not its own, whatever they are
+                odd = ~np.isfinite(vv).all(-1)
+                y = p @ np.where(odd[:, None], 0, vv)
+                size_of = p @ np.where(odd[:, None], 0, np.abs(vv))
+                for j in np.flatnonzero(odd):
+                    y = np.where(seen[:, j:j + 1], y + p[:, j:j + 1] * vv[j], y)
+                # float32 sums of `size` products, one of the factors in two pieces that leave 2^-24 of it, a scale and the maximum taken
+                # off; then a sum of products with weights in two such pieces
+                a = np.where(seen, np.abs(x) @ np.abs(kk).T, 0).max(-1, keepdims=True, initial=0) * abs(scale)
+                ds = (size + 12) * EPS * a + 4 * EPS * np.abs(np.where(seen, s, 0)).max(-1, keepdims=True, initial=0)
+                rest = 0.0
+                if len(cache) == 4:
+                    # the pieces of a query are multiples of 2^-24 where its largest value is 2^13 or above, those of a weight times a
+                    # value's scale where the largest such product of the row is 2^8 or above, or lies 2^7 below one that is and
+                    # that a later step outgrew: each is off by 2^-37 and 2^-32 of the largest, also beside a key or value of zero
+                    ds = ds + size * 2.0 ** -37 * np.abs(x).max(-1, keepdims=True) * np.where(seen, np.abs(kk).max(-1), 0).max(-1, keepdims=True, initial=0) * abs(scale)
+                    rest = seen.sum(-1, keepdims=True) * 2.0 ** -32 * 127 * np.where(seen, p * value_scales[:, h], 0).max(-1, keepdims=True, initial=0)
+                bound = (2 * ds + 48 * EPS + seen.sum(-1, keepdims=True) * EPS) * size_of + rest + 1e-37
+            out[starts[i]:starts[i + 1], h * group:(h + 1) * group] = y.reshape(rows.shape)
+            off[starts[i]:starts[i + 1], h * group:(h + 1) * group] = bound.reshape(rows.shape)
     return out, off
 
 

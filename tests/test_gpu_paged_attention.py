@@ -110,7 +110,7 @@ CASES = [
     ("s8", [900, 60], [2, 2], 4, 1, 64, 16, {"max_length": 512}),              # keys behind the bound are not seen
     ("s8", [3000, 1, 2048, 129], [1, 1, 1, 1], 32, 8, 128, 128, {}),           # many pieces
     ("f32", [3000, 1, 2048, 129], [1, 1, 1, 1], 32, 8, 128, 128, {}),
-    # chunks of many tokens
+    # chunks of more tokens
     ("s8", [64], [64], 1, 1, 64, 16, {}),
     ("s8", [300, 129, 70], [300, 33, 70], 2, 2, 64, 16, {}),
     ("s8", [1000, 257], [130, 257], 8, 2, 128, 32, {}),
@@ -138,6 +138,31 @@ def test_against_the_definition(pkg, T, case):
     Made(pkg, kind, lengths, chunks, heads, kv, size, page, case).check(T, **more)
 
 
+# Chunks that make a workgroup of 128 rows for each CU: these go over the keys together.
+TILES = [
+    ([600, 300, 257, 700], [300, 300, 257, 290], 32, 32, 64, 16, {}),
+    ([300, 290, 0, 1100, 260, 257], [70, 97, 0, 90, 64, 65], 64, 16, 128, 32, {}),
+    ([513, 400], [260, 300], 64, 64, 80, 48, {}),                              # heads that do not fill their tiles
+    ([400, 200, 90], [260, 280, 90], 48, 48, 96, 16, {}),                      # more tokens than are cached
+    ([400, 300], [260, 270], 64, 64, 192, 16, {}),
+    ([290, 280], [290, 270], 64, 64, 144, 16, {}),
+    ([290, 300], [290, 258], 64, 64, 256, 16, {}),
+    ([700, 600], [300, 290], 64, 64, 64, 32, {"window": 1}),
+    ([700, 600], [128, 140], 128, 64, 128, 32, {"window": 150}),
+    ([300, 400], [260, 270], 64, 64, 128, 16, {"causal": False}),
+    ([1500, 1200], [128, 128], 128, 64, 128, 64, {}),                          # two pieces of the keys
+    ([1500, 700, 300], [258, 257, 259], 32, 32, 64, 16, {"max_length": 1280}),
+    ([5000], [257], 128, 128, 64, 16, {"window": 4000}),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(TILES)))
+def test_chunks_against_the_definition(pkg, T, case):
+    lengths, chunks, heads, kv, size, page, more = TILES[case]
+    Made(pkg, "s8", lengths, chunks, heads, kv, size, page, 100 + case).check(T, **more)
+
+
 @pytest.mark.gpu
 def test_many_sequences(pkg, T):
     """More sequences than a wavefront has lanes, some without tokens."""
@@ -151,21 +176,22 @@ def test_many_sequences(pkg, T):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s8", "f32"])
-@pytest.mark.parametrize("chunks", [[1, 30, 64], [150, 90, 64]])
-def test_pages_outside_the_cache(pkg, T, kind, chunks):
-    m = Made(pkg, kind, [200, 90, 64], chunks, 4, 2, 64, 16, 4)
+@pytest.mark.parametrize("chunks,heads", [([1, 30, 64], 4), ([150, 90, 64], 4), ([300, 300, 300], 64)])
+def test_pages_outside_the_cache(pkg, T, kind, chunks, heads):
+    m = Made(pkg, kind, [200, 90, 64] if heads == 4 else [320, 310, 300], chunks, heads, heads // 2 if heads == 4 else heads, 64, 16, 4)
     m.table[0, [0, 5]] = [-1, 10 ** 6]
     m.table[1, 3] = len(m.cache[0])
-    m.table[2, :4] = -1  # nothing is there at all
+    m.table[2] = -1  # nothing is there at all
     m.check(T)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s8", "f32"])
-@pytest.mark.parametrize("chunks", [[1, 1], [40, 21], [120, 70]])
-def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks):
+@pytest.mark.parametrize("chunks,heads", [([1, 1], 6), ([40, 21], 6), ([120, 70], 6), ([258, 260], 128)])
+def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks, heads):
     import torch
-    m = Made(pkg, kind, [150, 70], chunks, 6, 2, 64, 16, 5)
+    m = Made(pkg, kind, [150, 70] if heads == 6 else [290, 270], chunks, heads, heads // 3 if heads == 6 else heads // 2, 64, 16, 5)
+    group = heads // m.cache[0].shape[1]
     clean = T.n(m.run(T)).copy()
     rows = np.ones((m.cache[0].shape[0], 16), bool)  # slots of no sequence
     for i, n in enumerate(m.lengths):
@@ -184,18 +210,20 @@ def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks):
         m.cache[1][page, 1, inside, 40] = np.nan
     got = T.n(m.run(T))
     mine = np.zeros(got.shape, bool)
-    mine[m.starts[1] - 1, 3:] = True
+    mine[m.starts[1] - 1, group:2 * group] = True
     assert np.array_equal(got[~mine], clean[~mine])
     if kind == "f32":
-        assert np.isposinf(got[m.starts[1] - 1, 3:, 5]).all() and np.isnan(got[m.starts[1] - 1, 3:, 40]).all()
+        assert np.isposinf(got[m.starts[1] - 1, group:2 * group, 5]).all() and np.isnan(got[m.starts[1] - 1, group:2 * group, 40]).all()
         m.check(T)
+    else:
+        assert np.isnan(got[m.starts[1] - 1, group:2 * group]).all()
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("chunks", [[2, 45], [200, 45]])
-def test_scales_of_all_sizes(pkg, T, chunks):
+@pytest.mark.parametrize("chunks,heads,kv", [([2, 45], 4, 2), ([200, 45], 4, 2), ([257, 270], 64, 64)])
+def test_scales_of_all_sizes(pkg, T, chunks, heads, kv):
     """Rows of values from 10^-20 to 10^20, zeros among them, and queries likewise."""
-    m = Made(pkg, "s8", [300, 45], chunks, 4, 2, 128, 16, 6)
+    m = Made(pkg, "s8", [300, 45 if kv == 2 else 270], chunks, heads, kv, 128, 16, 6)
     m.cache[3][:] = np.exp(m.rng.normal(size=m.cache[3].shape) * 15).astype(np.float32)
     m.cache[3][m.rng.random(m.cache[3].shape) < 0.2] = 0
     m.cache[2][m.rng.random(m.cache[2].shape) < 0.2] = 0
@@ -208,25 +236,37 @@ def test_scales_of_all_sizes(pkg, T, chunks):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("chunks", [[3, 30], [250, 30]])
-def test_large_scores(pkg, T, chunks):
+@pytest.mark.parametrize("length,chunk,kv", [(4000, 1, 2), (300, 20, 2), (1100, 128, 128)])
+@pytest.mark.parametrize("order", [1, -1])
+def test_scales_further_apart_than_float32_exponents(pkg, T, length, chunk, kv, order):
+    """The weights of keys whose values are small beside the others' count in full, whichever come first."""
+    m = Made(pkg, "s8", [length], [chunk], kv, kv, 64, 16, 17)
+    at = np.arange(m.lengths[0])
+    scales = np.where((at < length * 3 // 4)[::order], np.float32(1e-25), np.float32(1e25)).astype(np.float32)
+    m.cache[3][m.table[0][at // 16], :, at % 16] = scales[:, None]
+    m.check(T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("chunks,heads,kv", [([3, 30], 4, 2), ([250, 30], 4, 2), ([257, 270], 64, 64)])
+def test_large_scores(pkg, T, chunks, heads, kv):
     """Weights that all fall on one key or underflow."""
     for kind in ("s8", "f32"):
-        m = Made(pkg, kind, [400, 30], chunks, 4, 2, 64, 16, 7)
+        m = Made(pkg, kind, [400, 30 if kv == 2 else 300], chunks, heads, kv, 64, 16, 7)
         m.scale *= 100
         m.check(T)
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("chunk", [1, 64])
-def test_rows_whose_scores_rise_beside_rows_whose_do_not(pkg, T, chunk):
+@pytest.mark.parametrize("chunk,kv", [(1, 1), (64, 1), (128, 128)])
+def test_rows_whose_scores_rise_beside_rows_whose_do_not(pkg, T, chunk, kv):
     """The largest score of one row moves with every key, that of the other stays: neither loses what it has."""
-    m = Made(pkg, "s8", [5000], [chunk], 2, 1, 64, 16, 13)
+    m = Made(pkg, "s8", [5000 if kv == 1 else 1500], [chunk], 2 * kv, kv, 64, 16, 13)
     m.cache[0][:] = m.cache[0][0, 0, 0]
-    at = np.arange(5000)
-    m.cache[2][m.table[0][at // 16], 0, at % 16] = np.linspace(0.001, 0.02, 5000, dtype=np.float32)
-    m.q[:, 0] = m.cache[0][0, 0, 0] / np.float32(100)
-    m.q[:, 1] = -m.q[:, 0]
+    at = np.arange(m.lengths[0])
+    m.cache[2][m.table[0][at // 16], :, at % 16] = np.linspace(0.001, 0.02, len(at), dtype=np.float32)[:, None]
+    m.q[:, 0::2] = m.cache[0][0, 0, 0] / np.float32(100)
+    m.q[:, 1::2] = -m.q[:, 0::2]
     got = m.run(T)
     m.check(T, got)
     want, _ = R.attention(m.q, m.cache, m.table, m.starts, m.lengths, m.scale)

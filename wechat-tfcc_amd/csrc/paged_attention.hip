@@ -214,6 +214,9 @@ __device__ __forceinline__ QueryScale query_scale(float top, float scale) {
   const float up = power(14 - e);
   return {scale > 0.0f ? up : scale < 0.0f ? -up : 0.0f * scale, scale != 0.0f ? fmaxf(power(e - 14) * fabsf(scale), 1.17549435e-38f) : 1.0f};
 }
+// The factor from one frame to a higher one is the square of this.  Sums of weights are multiplied by it twice: where the scales of the values
+// span more than float32's exponents, a sum of 2^90 in the lower frame may be all there is in the higher, and the square itself underflows.
+__device__ __forceinline__ float half_step(float from, float to) { return __builtin_amdgcn_exp2f(0.5f * (from - to)); }
 // log2 of a value's scale for the frame.  A row of zeros, whose scale is 0, counts like one of 2^-90: its weight is summed and may not overflow.
 __device__ __forceinline__ float frame_log(float value_scale) { return fmaxf(__builtin_amdgcn_logf(fabsf(value_scale)), -90.0f); }
 
@@ -253,9 +256,9 @@ __device__ __forceinline__ void join_and_store(Joining<DPAD, WAVES>& s, const At
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       if (s.maxima[w][r] == -INFINITY) continue;  // a wavefront that saw no key of this row
-      const float f = __builtin_amdgcn_exp2f(s.maxima[w][r] - top);
-      total += f * s.sums[w][r];
-      sum += f * *reinterpret_cast<const f32x4*>(&s.outputs[w][r][d]);
+      const float h = half_step(s.maxima[w][r], top);
+      total += s.sums[w][r] * h * h;
+      sum += h * h * *reinterpret_cast<const f32x4*>(&s.outputs[w][r][d]);
     }
     const unsigned token = p.group.quotient((unsigned)in_chunk), inner = (unsigned)in_chunk - token * p.group.d;
     const unsigned long long global = t.first + token, query_head = head * p.group.d + inner;
@@ -395,9 +398,9 @@ struct S8Rows {
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaf(s[i], row_scale, frame_log(value_scale[i / 4][i % 4])));
     top = across_groups_max(top);
     if (__any(top - frame > 15.0f)) {
-      const float next = top - frame > 15.0f ? top - 8.0f : frame, f = next == frame ? 1.0f : __builtin_amdgcn_exp2f(frame - next);
+      const float next = top - frame > 15.0f ? top - 8.0f : frame, h = next == frame ? 1.0f : half_step(frame, next), f = h * h;
       frame = next;
-      l *= f;
+      l = l * h * h;
 #pragma unroll
       for (int i = 0; i < N; ++i) o[i] *= f;
     }
@@ -791,9 +794,9 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
     butterfly_pair<32>(top, a, b);
     top = fmaxf(a, b);
     if (__any(top - frame > 15.0f)) {
-      const float next = top - frame > 15.0f ? top - 8.0f : frame, f = next == frame ? 1.0f : __builtin_amdgcn_exp2f(frame - next);
+      const float next = top - frame > 15.0f ? top - 8.0f : frame, h = next == frame ? 1.0f : half_step(frame, next), f = h * h;
       frame = next;
-      l *= f;
+      l = l * h * h;
 #pragma unroll
       for (int n = 0; n < N; ++n) o[n] *= f;
     }
@@ -1099,9 +1102,9 @@ __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) 
   for (unsigned i = lane; i < p.splits; i += 64) {
     const float* s = p.statistics + (i * rows + row) * 2;
     const bool none = s[0] == -INFINITY;  // the piece has no key of this row
-    const float w = none ? 0.0f : __builtin_amdgcn_exp2f(s[0] - top);
-    weights[i] = none ? -1.0f : w;  // (all wavefronts write the same)
-    total += none ? 0.0f : w * s[1];
+    const float h = none ? 0.0f : half_step(s[0], top);
+    weights[i] = none ? -1.0f : h * h;  // (all wavefronts write the same)
+    total += none ? 0.0f : s[1] * h * h;
   }
   total = wave_sum(total);
   __syncthreads();
