@@ -553,7 +553,7 @@ typedef struct tfcc_rocm_rotary_desc {
 int tfcc_rocm_rotary_f32(void* stream, const tfcc_rocm_rotary_desc* desc);
 
 /* Keys and values of many sequences in pages: row `slot % page_size` of page `slot / page_size` for each head.  type TFCC_ROCM_F32, or
- * TFCC_ROCM_S8 with one scale for each slot and head, as cache_write makes them: scale = max |x| / 127 in float32, integers
+ * TFCC_ROCM_S8 with one scale for each slot and head, as cache_write makes them: scale = max |x| * (1 / 127) in float32, integers
  * x / scale rounded to nearest, ties to even; a row of zeros has scale 0, and a row that holds an infinity or a NaN reads back as
  * NaN.  keys and values have the same strides, and so have the scales; key and value arrays, scales, slots do not overlap.
  * size: up to 256, a multiple of 4 (F32) or 8 (S8), with pointers and strides of keys and values multiples of 16 bytes (F32) or 8 (S8). */

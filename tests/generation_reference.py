@@ -20,7 +20,7 @@ def rotary(x, positions, frequencies, interleaved, magnitude=1.0):
 def quantized(x):
     """(integers, scales) of rows along the last axis: the definition, with the quotient in 64 bits."""
     with np.errstate(invalid="ignore", divide="ignore", over="ignore"):
-        scale = np.abs(x).max(-1) / np.float32(127)
+        scale = np.abs(x).max(-1) * np.float32(1 / 127)
         good = np.isfinite(scale) & (scale > 0)
         n = np.rint(x.astype(np.float64) / np.where(good, scale, 1).astype(np.float64)[..., None])
         return np.where(good[..., None], np.clip(n, -127, 127), 0).astype(np.int8), scale.astype(np.float32)

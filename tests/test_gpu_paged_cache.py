@@ -90,7 +90,7 @@ def test_every_integer_is_the_true_quotients(pkg, T):
     rng = np.random.default_rng(1)
     scale = np.float32(1) + rng.integers(0, 2 ** 23, 4096).astype(np.float32) * np.float32(2.0 ** -23)
     top = scale * np.float32(127)
-    scale = top / np.float32(127)
+    scale = top * np.float32(1 / 127)
     border = ((np.arange(63) * 2 - 62.0) + 0.5)[None] * scale[:, None].astype(np.float64)
     rows = np.zeros((4096, 64), np.float32)
     rows[:, 0] = top
