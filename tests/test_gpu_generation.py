@@ -289,7 +289,7 @@ def test_workspaces_of_any_contents(pkg, T):
     d.tokens, d.heads, d.batch, d.table_stride, d.table_width, d.scale, d.causal = 3, 4, 3, 200, 200, 0.125, 1
     needs = lib.tfcc_rocm_paged_attention_workspace(C.byref(d))
     logits, random = T.t(rng.normal(size=(2, 70001)).astype(np.float32)), T.t(rng.random(2).astype(np.float32))
-    token, odds = torch.empty(2, dtype=torch.int32, device="cuda"), torch.empty(2, device="cuda")
+    token, odds = torch.empty(2, dtype=torch.int64, device="cuda"), torch.empty(2, device="cuda")
     s = pkg.SampleDesc()
     s.logits, s.random, s.tokens, s.probabilities = (t.data_ptr() for t in (logits, random, token, odds))
     s.rows, s.length, s.row_stride = 2, 70001, 70001

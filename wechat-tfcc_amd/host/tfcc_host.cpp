@@ -1741,5 +1741,213 @@ template Variable<int32_t> reduce_sum(const Tensor<uint8_t>&, bool);
 template Variable<int32_t> reduce_sum(const Tensor<int16_t>&, bool);
 
 }  // namespace quantization
+
+// ---------------------------------------------------------------------------------------------
+// between a language model's products
+// ---------------------------------------------------------------------------------------------
+namespace generation {
+
+namespace {
+
+void require_rocm() {
+  if (dynamic_cast<ROCMDevice*>(Device::getThreadDefault()) == nullptr) throw NotImplementedError();
+}
+// [tokens, heads, size]
+template <class T>
+void require_heads(const Tensor<T>& t, const char* text) {
+  if (t.shape().size() != 3 || t.shape(1) == 0 || t.shape(2) == 0) throw InvalidArgumentError(text);
+}
+template <class T>
+void require_list(const Tensor<T>& t, size_t count, const char* text) {
+  if (t.shape().size() != 1 || t.shape(0) != count) throw InvalidArgumentError(text);
+}
+template <class T>
+tfcc_rocm_paged_cache held_by(const PagedCache<T>& c) {
+  tfcc_rocm_paged_cache d{};
+  d.keys = const_cast<T*>(c.keys.data());
+  d.values = const_cast<T*>(c.values.data());
+  d.type = std::is_same<T, int8_t>::value ? TFCC_ROCM_S8 : TFCC_ROCM_F32;
+  d.pages = c.keys.shape(0);
+  d.heads = c.keys.shape(1);
+  d.page_size = c.keys.shape(2);
+  d.size = c.keys.shape(3);
+  d.row_stride = d.size;
+  d.head_stride = d.row_stride * d.page_size;
+  d.page_stride = d.head_stride * d.heads;
+  if (std::is_same<T, int8_t>::value) {
+    d.key_scales = const_cast<float*>(c.keyScales.data());
+    d.value_scales = const_cast<float*>(c.valueScales.data());
+    d.scale_row_stride = 1;
+    d.scale_head_stride = d.page_size;
+    d.scale_page_stride = d.scale_head_stride * d.heads;
+  }
+  return d;
+}
+
+}  // namespace
+
+std::tuple<std::vector<double>, float> rotary_frequencies(unsigned part, double base, RotaryScaling scaling, double factor, unsigned originalLength,
+                                                          double low, double high) {
+  std::vector<double> frequencies(part / 2 + 1);
+  float magnitude = 1.0f;
+  if (tfcc_rocm_rotary_frequencies(part, base, static_cast<int>(scaling), factor, originalLength, low, high, frequencies.data(), &magnitude) != TFCC_ROCM_OK)
+    throw InvalidArgumentError(tfcc_rocm_last_error_string());
+  frequencies.resize(part / 2);
+  return std::make_tuple(std::move(frequencies), magnitude);
+}
+
+std::tuple<Variable<float>, Variable<float>> rotary(const Tensor<float>& q, const Tensor<float>& k, const Tensor<int32_t>& positions,
+                                                    const Tensor<double>& frequencies, bool interleaved, float magnitude) {
+  require_heads(q, "invalid q");
+  require_heads(k, "invalid k");
+  if (k.shape(0) != q.shape(0) || k.shape(2) != q.shape(2)) throw InvalidArgumentError("invalid k");
+  require_list(positions, q.shape(0), "invalid positions");
+  if (frequencies.shape().size() != 1 || frequencies.size() == 0 || frequencies.size() > q.shape(2) / 2) throw InvalidArgumentError("invalid frequencies");
+  require_rocm();
+  Variable<float> turnedQ(q.shape()), turnedK(k.shape());
+  if (q.size() == 0) return std::make_tuple(std::move(turnedQ), std::move(turnedK));
+  tfcc_rocm_rotary_desc d{};
+  const Tensor<float>* const in[2] = {&q, &k};
+  Variable<float>* const out[2] = {&turnedQ, &turnedK};
+  for (int i = 0; i < 2; ++i) {
+    d.in[i] = in[i]->data();
+    d.out[i] = out[i]->data();
+    d.heads[i] = in[i]->shape(1);
+    d.in_head_stride[i] = d.out_head_stride[i] = q.shape(2);
+    d.in_token_stride[i] = d.out_token_stride[i] = static_cast<uint64_t>(q.shape(2)) * d.heads[i];
+  }
+  d.tokens = q.shape(0);
+  d.size = q.shape(2);
+  d.part = 2 * frequencies.size();
+  d.positions = positions.data();
+  d.position_type = TFCC_ROCM_S32;
+  d.frequencies = frequencies.data();
+  d.magnitude = magnitude;
+  d.interleaved = interleaved;
+  check(tfcc_rocm_rotary_f32(current_stream(), &d));
+  return std::make_tuple(std::move(turnedQ), std::move(turnedK));
+}
+
+template <class T>
+PagedCache<T>::PagedCache(unsigned pages, unsigned heads, unsigned pageSize, unsigned size)
+    : keys({pages, heads, pageSize, size}), values({pages, heads, pageSize, size}) {
+  if (keys.size() == 0) throw InvalidArgumentError("invalid cache");
+  require_rocm();
+  data::zeros(keys);
+  data::zeros(values);
+  if (std::is_same<T, int8_t>::value) {
+    keyScales = Variable<float>({pages, heads, pageSize});
+    valueScales = Variable<float>({pages, heads, pageSize});
+    data::zeros(keyScales);
+    data::zeros(valueScales);
+  }
+}
+
+template <class T>
+void cache_write(PagedCache<T>& cache, const Tensor<float>& keys, const Tensor<float>& values, const Tensor<int32_t>& slots) {
+  require_heads(keys, "invalid keys");
+  if (keys.shape(1) != cache.keys.shape(1) || keys.shape(2) != cache.keys.shape(3)) throw InvalidArgumentError("invalid keys");
+  if (values.shape() != keys.shape()) throw InvalidArgumentError("invalid values");
+  require_list(slots, keys.shape(0), "invalid slots");
+  require_rocm();
+  const tfcc_rocm_paged_cache d = held_by(cache);
+  const uint64_t head = d.size, token = head * d.heads;
+  check(tfcc_rocm_cache_write(current_stream(), &d, keys.data(), token, head, values.data(), token, head, keys.shape(0), slots.data(), TFCC_ROCM_S32));
+}
+
+template <class T>
+std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
+                                                        unsigned tokens) {
+  if (table.shape().size() != 2) throw InvalidArgumentError("invalid table");
+  require_list(starts, table.shape(0) + 1, "invalid starts");
+  require_rocm();
+  const tfcc_rocm_paged_cache d = held_by(cache);
+  Variable<float> keys({tokens, d.heads, d.size}), values({tokens, d.heads, d.size});
+  check(tfcc_rocm_cache_read(current_stream(), &d, table.data(), table.shape(1), table.shape(1), table.shape(0), starts.data(), tokens, keys.data(), values.data()));
+  return std::make_tuple(std::move(keys), std::move(values));
+}
+
+template <class T>
+Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
+                                const Tensor<int32_t>& lengths, float scale, bool causal, unsigned window, unsigned maxLength) {
+  require_heads(q, "invalid q");
+  if (q.shape(2) != cache.keys.shape(3) || q.shape(1) % cache.keys.shape(1) != 0) throw InvalidArgumentError("invalid q");
+  if (lengths.shape().size() != 1) throw InvalidArgumentError("invalid lengths");
+  if (table.shape().size() != 2 || table.shape(0) != lengths.shape(0)) throw InvalidArgumentError("invalid table");
+  require_list(starts, lengths.shape(0) + 1, "invalid starts");
+  if (window > 0 && !causal) throw InvalidArgumentError("invalid window");
+  require_rocm();
+  Variable<float> out(q.shape());
+  tfcc_rocm_paged_attention_desc d{};
+  d.cache = held_by(cache);
+  d.q = q.data();
+  d.out = out.data();
+  d.q_head_stride = d.out_head_stride = q.shape(2);
+  d.q_token_stride = d.out_token_stride = static_cast<uint64_t>(q.shape(2)) * q.shape(1);
+  d.tokens = q.shape(0);
+  d.heads = q.shape(1);
+  d.batch = lengths.shape(0);
+  d.starts = starts.data();
+  d.lengths = lengths.data();
+  d.table = table.data();
+  d.table_stride = table.shape(1);
+  d.table_width = table.shape(1);
+  d.max_length = maxLength;
+  d.scale = scale;
+  d.causal = causal;
+  d.window = window;
+  Variable<uint8_t> workspace;
+  if ((d.workspace_bytes = tfcc_rocm_paged_attention_workspace(&d)) > 0) {
+    if (d.workspace_bytes > 0xffffffffu) throw NotImplementedError("a workspace of 4 GiB");
+    workspace = Variable<uint8_t>({static_cast<unsigned>(d.workspace_bytes)});
+    d.workspace = workspace.data();
+  }
+  check(tfcc_rocm_paged_attention_f32(current_stream(), &d));
+  return out;
+}
+
+std::tuple<Variable<int64_t>, Variable<float>> sample(const Tensor<float>& logits, const Tensor<float>& random, const SampleFilters& filters) {
+  if (logits.shape().size() != 2 || logits.shape(1) == 0) throw InvalidArgumentError("invalid logits");
+  const unsigned rows = logits.shape(0), length = logits.shape(1);
+  require_list(random, rows, "invalid random");
+  if (filters.temperature) require_list(*filters.temperature, rows, "invalid temperature");
+  if (filters.topK) require_list(*filters.topK, rows, "invalid topK");
+  if (filters.topP) require_list(*filters.topP, rows, "invalid topP");
+  if (filters.minP) require_list(*filters.minP, rows, "invalid minP");
+  require_rocm();
+  Variable<int64_t> tokens({rows});
+  Variable<float> probabilities({rows});
+  if (rows == 0) return std::make_tuple(std::move(tokens), std::move(probabilities));
+  tfcc_rocm_sample_desc d{};
+  d.logits = logits.data();
+  d.row_stride = length;
+  d.rows = rows;
+  d.length = length;
+  d.random = random.data();
+  d.temperature = filters.temperature ? filters.temperature->data() : nullptr;
+  d.top_k = filters.topK ? filters.topK->data() : nullptr;
+  d.top_p = filters.topP ? filters.topP->data() : nullptr;
+  d.min_p = filters.minP ? filters.minP->data() : nullptr;
+  d.tokens = tokens.data();
+  d.probabilities = probabilities.data();
+  d.workspace_bytes = tfcc_rocm_sample_workspace(rows, length);
+  if (d.workspace_bytes > 0xffffffffu) throw NotImplementedError("a workspace of 4 GiB");
+  Variable<uint8_t> workspace({static_cast<unsigned>(d.workspace_bytes)});
+  d.workspace = workspace.data();
+  check(tfcc_rocm_sample_f32(current_stream(), &d));
+  return std::make_tuple(std::move(tokens), std::move(probabilities));
+}
+
+#define TFCC_PAGED_CACHE(T)                                                                                                             \
+  template struct PagedCache<T>;                                                                                                       \
+  template void cache_write(PagedCache<T>&, const Tensor<float>&, const Tensor<float>&, const Tensor<int32_t>&);                       \
+  template std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>&, const Tensor<int32_t>&, const Tensor<int32_t>&, unsigned); \
+  template Variable<float> paged_attention(const Tensor<float>&, const PagedCache<T>&, const Tensor<int32_t>&, const Tensor<int32_t>&,  \
+                                           const Tensor<int32_t>&, float, bool, unsigned, unsigned);
+TFCC_PAGED_CACHE(float)
+TFCC_PAGED_CACHE(int8_t)
+#undef TFCC_PAGED_CACHE
+
+}  // namespace generation
 }  // namespace rocm
 }  // namespace tfcc

@@ -245,5 +245,48 @@ std::tuple<Variable<int32_t>, Variable<float>, Variable<float>> matmul(
     const Tensor<float>& maxA, const PreparedWeights& w, const Tensor<float>& minB, const Tensor<float>& maxB);
 
 }  // namespace quantization
+
+// What a language model does between its products: rotary positions, a paged cache of keys and values, attention over it, the
+// choice of a token.  The calls of the same names in include/tfcc_rocm.h say what each computes, skips and leaves; here are their tensors and
+// checks.  They need the ROCm device as the thread default.
+namespace generation {
+
+enum class RotaryScaling { PLAIN = 0, LINEAR = 1, BASE = 2, TURNS = 3, INDEX = 4 };
+// part / 2 radians for each position, to be made a tensor once, and the magnitude
+std::tuple<std::vector<double>, float> rotary_frequencies(unsigned part, double base = 10000.0, RotaryScaling scaling = RotaryScaling::PLAIN,
+                                                          double factor = 1.0, unsigned originalLength = 0, double low = 1.0, double high = 4.0);
+// q [tokens, heads, size] and k [tokens, cache heads, size] turned; positions [tokens], frequencies [part / 2]
+std::tuple<Variable<float>, Variable<float>> rotary(const Tensor<float>& q, const Tensor<float>& k, const Tensor<int32_t>& positions,
+                                                    const Tensor<double>& frequencies, bool interleaved = false, float magnitude = 1.0f);
+
+// Memory of a cache, all zeros at first.  T = float, or int8_t with a scale for each row of a head.
+template <class T>
+struct PagedCache {
+  Variable<T> keys, values;                 // [pages, heads, rows, size]
+  Variable<float> keyScales, valueScales;   // [pages, heads, rows], int8_t only
+  PagedCache(unsigned pages, unsigned heads, unsigned pageSize, unsigned size);
+};
+// keys and values [tokens, heads, size] to slots [tokens] (page * rows + row; -1: skipped)
+template <class T>
+void cache_write(PagedCache<T>& cache, const Tensor<float>& keys, const Tensor<float>& values, const Tensor<int32_t>& slots);
+// the first starts[i + 1] - starts[i] tokens of each sequence, back to back: two tensors [tokens, heads, size]; table [batch, pages]
+template <class T>
+std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
+                                                        unsigned tokens);
+// q [tokens, heads, size], starts [batch + 1], lengths [batch]; maxLength: an upper bound of lengths, 0: what the table holds
+template <class T>
+Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
+                                const Tensor<int32_t>& lengths, float scale, bool causal = true, unsigned window = 0, unsigned maxLength = 0);
+
+// [rows] each, or null
+struct SampleFilters {
+  const Tensor<float>* temperature = nullptr;
+  const Tensor<int32_t>* topK = nullptr;
+  const Tensor<float>*topP = nullptr, *minP = nullptr;
+};
+// a token for each row of logits [rows, length] and its probability; random [rows]
+std::tuple<Variable<int64_t>, Variable<float>> sample(const Tensor<float>& logits, const Tensor<float>& random, const SampleFilters& filters = {});
+
+}  // namespace generation
 }  // namespace rocm
 }  // namespace tfcc
