@@ -163,6 +163,22 @@ def test_chunks_against_the_definition(pkg, T, case):
     Made(pkg, "s8", lengths, chunks, heads, kv, size, page, 100 + case).check(T, **more)
 
 
+# Pages that end inside a step's keys: 16 rows and more, and fewer, a page for each key.
+ENDS = [(kind, page, size, chunks, heads) for page in (17, 20, 24, 31, 40, 100, 5) for kind in ("s8", "f32")
+        for size, chunks, heads in ((64, [1, 1, 1], 4), (128, [1, 33, 7], 4), (256, [1, 1, 1], 4), (64, [300, 270, 260], 64))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,page,size,chunks,heads", ENDS)
+def test_pages_that_end_inside_a_step(pkg, T, kind, page, size, chunks, heads):
+    m = Made(pkg, kind, [700, 333, 290], chunks, heads, heads // 2 if heads == 4 else heads, size, page, page)
+    m.check(T)
+    m.table[0, ::3] = -1
+    m.table[1, 1::2] = len(m.cache[0])
+    m.check(T)
+    m.check(T, window=37)
+
+
 @pytest.mark.gpu
 def test_many_sequences(pkg, T):
     """More sequences than a wavefront has lanes, some without tokens."""

@@ -299,6 +299,11 @@ __device__ __forceinline__ bool take_work(const AttentionArgs& p, unsigned rows_
   return true;
 }
 
+// 16 bytes of each lane's own address to LDS, lane i's to m0 + 16 i.
+__device__ __forceinline__ void dma16_global(const void* from, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+
 // The page that holds a key, in two halves: what the table says of it, and, when that is wanted, whether there is such a page (-1: none).
 // What is loaded in one step is looked at in the next: a step does not wait for the table.
 // (Constant memory as far as a launch goes, so that entries come through the scalar cache: among the vector loads, which return in their order,
@@ -444,8 +449,8 @@ struct S8Rows {
   }
 };
 
-// int8 with pages of a multiple of 16 rows whose rows and scales can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
-// of 16.  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
+// int8 with pages of 16 rows and more that can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
+// of 16; WHOLE: pages of a multiple of 16 rows, so that a half lies in one, else in up to two.  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
 // straight into LDS, a ring of STAGES of its own (no barriers), and reads a step from there when it is due.
 template <int BLOCKS, int WAVES>
 struct S8Ring {
@@ -457,7 +462,7 @@ struct S8Ring {
     Joining<64 * BLOCKS, WAVES> joining;
   };
 };
-template <int BLOCKS, int WAVES>
+template <int BLOCKS, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs p) {
   typedef S8Ring<BLOCKS, WAVES> Ring;
   constexpr int STEP = 32 * WAVES, CHUNKS = 4 * BLOCKS /* of 16 bytes in a row */, PER_COPY = 64 / CHUNKS /* rows */, FOURS = PER_COPY / 4;
@@ -471,7 +476,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
   const unsigned size = p.cache.size, row_bytes = (unsigned)p.cache.row;
   const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
   const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
-  const float* const scales = (lane < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head;
+  const float* const scales = (lane < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head + c;
   const int* const table = p.table + (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)t.sequence) * p.table_stride;
   int kb = __builtin_amdgcn_readfirstlane(begin + 32 * (int)wave);
   end = __builtin_amdgcn_readfirstlane(end);
@@ -483,46 +488,73 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
   // exchanged within a row by its number.  Values are read a few bytes of rows 4 g + i at a time: those rows lie side by side.
   unsigned key_at[BLOCKS], value_at[BLOCKS];
   const unsigned slot = lane / CHUNKS, chunk = lane % CHUNKS;
+  const auto key_row = [&](int b) { return b * PER_COPY + slot; };
+  const auto value_row = [&](int b) { return (b * FOURS + slot % FOURS) * 4 + slot / FOURS; };
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b) {
-    const unsigned row = b * PER_COPY + slot, from = (chunk ^ exchange(row)) * 16;
-    key_at[b] = row * row_bytes + (from < size ? from : 0);
-    value_at[b] = ((b * FOURS + slot % FOURS) * 4 + slot / FOURS) * row_bytes + (chunk * 16 < size ? chunk * 16 : 0);
+    const unsigned from = (chunk ^ exchange(key_row(b))) * 16;
+    key_at[b] = key_row(b) * row_bytes + (from < size ? from : 0);
+    value_at[b] = value_row(b) * row_bytes + (chunk * 16 < size ? chunk * 16 : 0);
   }
   const unsigned half_bytes = 15 * row_bytes + size;
   unsigned char* const ring = shared.ring[wave][0];
   const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)ring;
 
-  PageEntry entries[2] = {};
+  // of each half: the page of its first key and, where that may be another one, of its last
+  constexpr int PAGES = WHOLE ? 1 : 2;
+  PageEntry entries[2][PAGES] = {};
   const auto ask_pages = [&](int at) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) entries[h] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 16 * h));
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < PAGES; ++n) entries[h][n] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 16 * h + 15 * n));
   };
-  const auto copy = [&](unsigned stage, int at, const int (&page)[2]) {
+  const auto inside_page = [&](unsigned key) { return key - p.cache.page_size.quotient(key) * p.cache.page_size.d; };
+  // the row of a half that the second page begins with
+  const auto cut_of = [&](unsigned key) { return p.cache.page_size.d - inside_page(key); };
+  const auto copy = [&](unsigned stage, int at, const int (&page)[2][PAGES]) {
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(ring_at + stage * Ring::kBytes));
-    unsigned long long scale_at[2];
+    const float* scale_at[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const unsigned key = (unsigned)at + 16 * h, inside = key - p.cache.page_size.quotient(key) * p.cache.page_size.d;
-      const unsigned long long held = page[h] < 0 ? 0 : (unsigned)page[h], base = held * p.cache.page + inside * p.cache.row;
-      scale_at[h] = held * p.cache.scale_page + inside;
-      const lds_dma_v4i k = make_rsrc(keys + base, half_bytes), v = make_rsrc(values + base, half_bytes);
+      const unsigned key = (unsigned)at + 16 * h, inside = inside_page(key);
+      const unsigned long long held = page[h][0] < 0 ? 0 : (unsigned)page[h][0], base = held * p.cache.page + inside * p.cache.row;
+      scale_at[h] = scales + held * p.cache.scale_page + inside;
+      if constexpr (WHOLE) {
+        const lds_dma_v4i k = make_rsrc(keys + base, half_bytes), v = make_rsrc(values + base, half_bytes);
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) dma16(k, to + (h * BLOCKS + b) * 1024, key_at[b]);
+        for (int b = 0; b < BLOCKS; ++b) dma16(k, to + (h * BLOCKS + b) * 1024, key_at[b]);
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) dma16(v, to + ((2 + h) * BLOCKS + b) * 1024, value_at[b]);
+        for (int b = 0; b < BLOCKS; ++b) dma16(v, to + ((2 + h) * BLOCKS + b) * 1024, value_at[b]);
+      } else {
+        const unsigned long long next = page[h][PAGES - 1] < 0 ? 0 : (unsigned)page[h][PAGES - 1];
+        const long long cut = cut_of(key), other = (long long)(next * p.cache.page) - cut * (long long)p.cache.row;
+        if (c >= cut) scale_at[h] = scales + next * p.cache.scale_page - cut;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) dma16_global(keys + (key_row(b) >= cut ? other : (long long)base) + key_at[b], to + (h * BLOCKS + b) * 1024);
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) dma16_global(values + (value_row(b) >= cut ? other : (long long)base) + value_at[b], to + ((2 + h) * BLOCKS + b) * 1024);
+      }
     }
-    const float* const scale = scales + ((lane & 16) ? scale_at[1] : scale_at[0]) + c;
+    const float* const scale = (lane & 16) ? scale_at[1] : scale_at[0];
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to + Ring::kRows), "v"(scale) : "memory", "m0");
   };
-  unsigned gone = 0;  // two bits a stage: halves that no page holds
+  unsigned gone = 0;  // four bits a stage: of each half, what would be on its first and on its last page is nowhere
   if (kb < end) ask_pages(kb);
   int ahead = kb;  // the first step that no copy is under way for
   const auto send = [&](unsigned stage) {
     if (ahead < end) {
-      const int pages[2] = {page_of(p, entries[0]), page_of(p, entries[1])};
+      int pages[2][PAGES];
+      unsigned none = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          if (n < PAGES) pages[h][n] = page_of(p, entries[h][n]);
+          none |= pages[h][n < PAGES ? n : 0] < 0 ? 1u << (2 * h + n) : 0u;
+        }
       copy(stage, ahead, pages);
-      gone = (gone & ~(3u << (2 * stage))) | ((pages[0] < 0 ? 1u : 0u) | (pages[1] < 0 ? 2u : 0u)) << (2 * stage);
+      gone = (gone & ~(15u << (4 * stage))) | none << (4 * stage);
       ahead += STEP;
       if (ahead < end) ask_pages(ahead);
     }
@@ -564,8 +596,16 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
         for (int b = 0; b < 4; ++b) v[i][b] = w[b];
       }
     }
-    const unsigned none = gone >> (2 * stage) & 3;
-    const unsigned missing = (none & 1 ? 15u : 0u) | (none & 2 ? 240u : 0u);
+    const unsigned none = gone >> (4 * stage) & 15;
+    unsigned missing = (none & 1 ? 15u : 0u) | (none & 4 ? 240u : 0u);
+    if (!WHOLE && none != 0) {
+      missing = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned h = i / 4, behind = 4 * g + i % 4 >= cut_of((unsigned)kb + 16 * h) ? 1 : 0;
+        missing |= (none >> (2 * h + behind) & 1) << i;
+      }
+    }
     // Read: the stage may be written again.  (By the builtin, which the compiler counts with: it would else wait for the reads once more, and
     // with them for the page entries that send() has asked for.)
     asm volatile("" : : : "memory");
@@ -596,14 +636,14 @@ __device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
   return n / 4 * 4 + 4 <= 2 * BLOCKS ? n / 4 * 128 + 4 * L + n % 4 : n / 4 * 128 + 4 * (L % 16) + 2 * (L / 16) + n % 4;
 }
 
-template <int BLOCKS>
+template <int BLOCKS, bool WHOLE>
 __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attention_s8_tile_kernel(AttentionArgs p) {
   constexpr int KS = 4 * BLOCKS, N = 2 * BLOCKS;  // products over a head, tiles of 32 of its values
   struct Stage {
     u32x4 keys[KS][64];       // lane l: key l % 32, values 16 s + 8 (l / 32) + j
     u32x4 values[N][2][64];   // lane l: value_of(l % 32, n), keys 16 m + 8 (j / 4) + 4 (l / 32) + j % 4
     float key_scale[kTileKeys], value_scale[kTileKeys], value_log[kTileKeys];
-    unsigned gone[2];  // a bit of its own for a half that no page holds
+    unsigned gone;  // a bit for each key that no page holds
   };
   __shared__ Stage stages[2];
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = lane / 32;
@@ -632,28 +672,36 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
   // (Entries through the scalar cache would be waited for with the LDS reads.)
   float scale = 0.0f;
   bool gone = false;
-  int named[TASKS];
-  const auto half_of = [&](int k) { return for_keys ? me / 16 % 2 : (me + 128 * k) / WORDS / 2 % 2; };
+  // WHOLE: pages of a multiple of 16 rows, else of 4, 16 at least: the eight keys of a task then lie four and four
+  constexpr int PAGES = WHOLE ? 1 : 2;
+  int named[TASKS][PAGES];
+  // the first key of the step's that the thread's task k fetches of its n-th page
+  const auto key_of = [&](int k, int n) {
+    const unsigned group = (me + 128 * k) / WORDS;
+    return for_keys ? (WHOLE ? me / 16 % 2 * 16 : me % 32) : group / 2 % 2 * 16 + (WHOLE ? 0 : 4 * (group % 2) + 8 * n);
+  };
+  const auto inside_page = [&](unsigned key) { return key - p.cache.page_size.quotient(key) * p.cache.page_size.d; };
   const auto ask_pages = [&](int at) {
 #pragma unroll
-    for (int k = 0; k < TASKS; ++k) {
-      const unsigned index = p.cache.page_size.quotient((unsigned)at + 16 * half_of(k));
-      named[k] = index < p.table_width ? table[index] : -1;
-    }
+    for (int k = 0; k < TASKS; ++k)
+#pragma unroll
+      for (int n = 0; n < PAGES; ++n) {
+        const unsigned index = p.cache.page_size.quotient((unsigned)at + key_of(k, n));
+        named[k][n] = index < p.table_width ? table[index] : -1;
+      }
   };
   const auto fetch = [&](int at) {
-    const unsigned inside[2] = {(unsigned)at - p.cache.page_size.quotient((unsigned)at) * p.cache.page_size.d,
-                                (unsigned)at + 16 - p.cache.page_size.quotient((unsigned)at + 16) * p.cache.page_size.d};
-    const auto page_row = [&](int k, unsigned long long& held) {
-      const bool none = (unsigned)named[k] >= p.cache.pages;
-      held = none ? 0 : (unsigned)named[k];
+    const unsigned halves[2] = {inside_page((unsigned)at), inside_page((unsigned)at + 16)};
+    const auto page_row = [&](int k, int n, unsigned long long& held) {
+      const bool none = (unsigned)named[k][n] >= p.cache.pages;
+      held = none ? 0 : (unsigned)named[k][n];
       return none;
     };
     unsigned long long held;
     if (for_keys) {
-      gone = page_row(0, held);
-      const unsigned first = half_of(0) ? inside[1] : inside[0];
-      const int8_t* const row = keys + held * p.cache.page + (first + (me & 15)) * p.cache.row;
+      gone = page_row(0, 0, held);
+      const unsigned inside = WHOLE ? (me / 16 % 2 ? halves[1] : halves[0]) + (me & 15) : inside_page((unsigned)at + me % 32);
+      const int8_t* const row = keys + held * p.cache.page + inside * p.cache.row;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         const unsigned d = 16 * (me / 32 + 4 * b);
@@ -661,18 +709,22 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
       }
       if (threadIdx.x < 64) {
         const float* const s = (threadIdx.x < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head;
-        scale = s[held * p.cache.scale_page + first + (threadIdx.x & 15)];
+        scale = s[held * p.cache.scale_page + inside];
       }
     } else {
 #pragma unroll
       for (int k = 0; k < TASKS; ++k) {
         const unsigned task = me + 128 * k, word = task % WORDS, group = task / WORDS;
         if (4 * WORDS % 128 == 0 || group < 4) {
-          (void)page_row(k, held);
-          const unsigned first = (group / 2 ? inside[1] : inside[0]) + 4 * (group % 2);
-          const int8_t* const row = values + held * p.cache.page + first * p.cache.row + (4 * word < size ? 4 * word : 0);
+          const int8_t* row[2];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) raw[2 * k + j / 4][j % 4] = *reinterpret_cast<const unsigned*>(row + (8 * (j / 4) + j % 4) * p.cache.row);
+          for (int n = 0; n < 2; ++n) {
+            (void)page_row(k, n < PAGES ? n : 0, held);
+            const unsigned inside = WHOLE ? (group / 2 ? halves[1] : halves[0]) + 4 * (group % 2) + 8 * n : inside_page((unsigned)at + key_of(k, n));
+            row[n] = values + held * p.cache.page + inside * p.cache.row + (4 * word < size ? 4 * word : 0);
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) raw[2 * k + j / 4][j % 4] = *reinterpret_cast<const unsigned*>(row[j / 4] + j % 4 * p.cache.row);
         }
       }
     }
@@ -687,7 +739,8 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
       }
       if (threadIdx.x < 32) {
         s.key_scale[threadIdx.x] = scale;
-        if (threadIdx.x % 16 == 0) s.gone[threadIdx.x / 16] = gone ? 1u << (threadIdx.x / 16) : 0u;
+        const unsigned nowhere = (unsigned)__ballot(gone);
+        if (threadIdx.x == 0) s.gone = nowhere;
       } else if (threadIdx.x < 64) {
         s.value_scale[threadIdx.x - 32] = scale;
         s.value_log[threadIdx.x - 32] = frame_log(scale);
@@ -778,12 +831,12 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[4 * a + i] *= key_scale[i];
     }
-    const unsigned none = s.gone[0] | s.gone[1];
+    const unsigned none = s.gone;
     if (none != 0 || kb < all_low || kb + kTileKeys > all_high) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = kb + 8 * (i / 4) + 4 * (int)half + i % 4;
-        const bool seen = (none >> (i / 8) & 1) == 0 && key >= t.row_low && key < t.row_high;
+        const bool seen = (none >> (key - kb) & 1) == 0 && key >= t.row_low && key < t.row_high;
         x[i] = seen ? x[i] : -INFINITY;
         value_scale[i / 4][i % 4] = seen ? value_scale[i / 4][i % 4] : 0.0f;
       }
@@ -913,9 +966,9 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_any_kernel(AttentionA
 }
 
 // float32: 16 keys in one step of a wavefront.  The next step's keys are loaded into the registers of this one's as soon as the
-// scores are formed, its values once the weights have met them.  UNIFORM: pages of a multiple of 16 rows; `missing`: a bit for each of the
-// lane's four keys that no page holds.
-template <int BLOCKS, int WAVES, bool UNIFORM>
+// scores are formed, its values once the weights have met them.  PAGES that the keys of a step may lie in: 1 (of a multiple of 16 rows),
+// 2 (16 rows at least) or any number, 0.  `missing`: a bit for each of the lane's four keys that no page holds.
+template <int BLOCKS, int WAVES, int PAGES>
 __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs p) {
   constexpr int DPAD = 64 * BLOCKS, STEP = 16 * WAVES;
   __shared__ Joining<DPAD, WAVES> joining;
@@ -939,34 +992,51 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
     row = page < 0 ? 0 : page * p.cache.page + inside_page((unsigned)key) * p.cache.row;
     return page >= 0;
   };
-  PageEntry entry = {};
-  const auto ask_page = [&](int at) {
-    if constexpr (UNIFORM) entry = entry_of(p, table, p.cache.page_size.quotient((unsigned)at));
+  PageEntry entries[PAGES == 2 ? 2 : 1] = {};
+  const auto ask_pages = [&](int at) {
+#pragma unroll
+    for (int n = 0; n < PAGES; ++n) entries[n] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 15 * n));
   };
-  const auto load_keys = [&](int at, int page) {
+  struct Held {
+    int page[2];
+  };
+  const auto pages_of = [&] {
+    Held held = {};
+#pragma unroll
+    for (int n = 0; n < PAGES; ++n) held.page[n] = page_of(p, entries[n]);
+    return held;
+  };
+  // where row r of the step at `at` lies, and whether it is anywhere
+  const auto place = [&](int at, unsigned r, const Held& held, unsigned long long& row) {
+    if constexpr (PAGES == 0) return locate(at + (int)r, row);
+    const unsigned inside = inside_page((unsigned)at), cut = p.cache.page_size.d - inside;
+    const bool behind = PAGES == 2 && r >= cut;
+    const int page = behind ? held.page[1] : held.page[0];
+    row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (behind ? r - cut : inside + r) * p.cache.row;
+    return page >= 0;
+  };
+  const auto load_keys = [&](int at, const Held& held) {
     unsigned long long row;
-    if constexpr (UNIFORM) row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (inside_page((unsigned)at) + c) * p.cache.row;
-    else locate(at + (int)c, row);
+    place(at, c, held, row);
 #pragma unroll
     for (int b = 0; b < 4 * BLOCKS; ++b) k[b] = *reinterpret_cast<const f32x4*>(keys + row + (16 * b + 4 * g < size ? 16 * b + 4 * g : 0));
   };
-  const auto load_values = [&](int at, int page) {
-    missing = UNIFORM && page < 0 ? 15u : 0u;
+  const auto load_values = [&](int at, const Held& held) {
+    missing = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       unsigned long long row;
-      if constexpr (UNIFORM) row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (inside_page((unsigned)at) + 4 * g + i) * p.cache.row;
-      else missing |= locate(at + 4 * (int)g + i, row) ? 0u : 1u << i;
+      missing |= place(at, 4 * g + i, held, row) ? 0u : 1u << i;
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) v[i][b] = *reinterpret_cast<const f32x4*>(values + row + (64 * b + 4 * c < size ? 64 * b + 4 * c : 0));
     }
   };
   if (kb < end) {
-    ask_page(kb);
-    const int page = page_of(p, entry);
-    load_keys(kb, page);
-    load_values(kb, page);
-    if (kb + STEP < end) ask_page(kb + STEP);
+    ask_pages(kb);
+    const Held held = pages_of();
+    load_keys(kb, held);
+    load_values(kb, held);
+    if (kb + STEP < end) ask_pages(kb + STEP);
   }
   // value 16 b + 4 g + j of the row's query in q[b][j]
   f32x4 q[4 * BLOCKS];
@@ -1001,8 +1071,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
     }
     f32x4 s = s0 + s1;
     const bool more = kb + STEP < end;
-    const int page = page_of(p, entry);
-    if (more) load_keys(kb + STEP, page);
+    const Held next_pages = pages_of();
+    if (more) load_keys(kb + STEP, next_pages);
     const bool edge = __any(missing != 0) || kb < t.all_low || kb + 16 > t.all_high;
     unsigned foreign = 0;  // values that are not finite, of keys that some row does not see
     if (edge) {
@@ -1071,8 +1141,8 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
       }
     }
     if (more) {
-      load_values(kb + STEP, page);
-      if (kb + 2 * STEP < end) ask_page(kb + 2 * STEP);
+      load_values(kb + STEP, next_pages);
+      if (kb + 2 * STEP < end) ask_pages(kb + 2 * STEP);
     }
   }
   l = across_groups_sum(l);
@@ -1126,19 +1196,30 @@ __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) 
   }
 }
 
+// What a step's 16 keys may lie in: 1 page, up to 2, or any number (0).
+int pages_of_step(unsigned page_size) { return page_size % 16 == 0 ? 1 : page_size >= 16 ? 2 : 0; }
+
 template <int BLOCKS>
-void launch_s8(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves, bool fast) {
+void launch_s8(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves, bool wide) {
   const auto start = [&](auto kernel, unsigned width) { hipLaunchKernelGGL(kernel, grid, dim3(width * 64), 0, s, a); };
+  const bool whole = a.cache.page_size.d % 16 == 0;
   if constexpr (BLOCKS <= 2)
-    if (waves == 8) return start(fast ? attention_s8_kernel<BLOCKS, 8> : attention_s8_any_kernel<BLOCKS, 8>, 8);
-  start(fast ? attention_s8_kernel<BLOCKS, 4> : attention_s8_any_kernel<BLOCKS, 4>, 4);
+    if (waves == 8) return start(!wide ? attention_s8_any_kernel<BLOCKS, 8> : whole ? attention_s8_kernel<BLOCKS, 8, true> : attention_s8_kernel<BLOCKS, 8, false>, 8);
+  start(!wide ? attention_s8_any_kernel<BLOCKS, 4> : whole ? attention_s8_kernel<BLOCKS, 4, true> : attention_s8_kernel<BLOCKS, 4, false>, 4);
 }
 template <int BLOCKS>
-void launch_f32(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves, bool uniform) {
-  const auto start = [&](auto kernel, unsigned width) { hipLaunchKernelGGL(kernel, grid, dim3(width * 64), 0, s, a); };
+void launch_tiles(const AttentionArgs& a, dim3 grid, hipStream_t s) {
+  hipLaunchKernelGGL((a.cache.page_size.d % 16 == 0 ? attention_s8_tile_kernel<BLOCKS, true> : attention_s8_tile_kernel<BLOCKS, false>), grid, dim3(kTileWaves * 64), 0, s, a);
+}
+template <int BLOCKS>
+void launch_f32(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves) {
+  const auto start = [&](auto one, auto two, auto any, unsigned width) {
+    const int pages = pages_of_step(a.cache.page_size.d);
+    hipLaunchKernelGGL((pages == 1 ? one : pages == 2 ? two : any), grid, dim3(width * 64), 0, s, a);
+  };
   if constexpr (BLOCKS <= 2)
-    if (waves == 8) return start(uniform ? attention_f32_kernel<BLOCKS, 8, true> : attention_f32_kernel<BLOCKS, 8, false>, 8);
-  start(uniform ? attention_f32_kernel<BLOCKS, 4, true> : attention_f32_kernel<BLOCKS, 4, false>, 4);
+    if (waves == 8) return start(attention_f32_kernel<BLOCKS, 8, 1>, attention_f32_kernel<BLOCKS, 8, 2>, attention_f32_kernel<BLOCKS, 8, 0>, 8);
+  start(attention_f32_kernel<BLOCKS, 4, 1>, attention_f32_kernel<BLOCKS, 4, 2>, attention_f32_kernel<BLOCKS, 4, 0>, 4);
 }
 
 int check_attention(const tfcc_rocm_paged_attention_desc& d) {
@@ -1158,16 +1239,15 @@ unsigned most_keys(const tfcc_rocm_paged_attention_desc& d) {
   return d.max_length > 0 && d.max_length < held ? d.max_length : held;
 }
 
-// An int8 cache with pages of a multiple of 16 rows whose rows and scales can be read 16 bytes at a time.
+// An int8 cache with pages of 16 rows and more that can be read 16 bytes at a time, its scales in a row.
 bool wide_reads(const tfcc_rocm_paged_cache& c) {
-  return c.type == TFCC_ROCM_S8 && c.page_size % 16 == 0 && c.size % 16 == 0 && (c.page_stride | c.head_stride | c.row_stride) % 16 == 0 &&
-         c.scale_row_stride == 1 && c.row_stride < (1u << 26) && (c.scale_page_stride | c.scale_head_stride) % 4 == 0 &&
-         (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values) | reinterpret_cast<uintptr_t>(c.key_scales) |
-          reinterpret_cast<uintptr_t>(c.value_scales)) % 16 == 0;
+  return c.type == TFCC_ROCM_S8 && c.page_size >= 16 && c.size % 16 == 0 && (c.page_stride | c.head_stride | c.row_stride) % 16 == 0 &&
+         c.scale_row_stride == 1 && c.row_stride < (1u << 26) &&
+         (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values)) % 16 == 0;
 }
 
 PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
-  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, wide_reads(d.cache));
+  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, wide_reads(d.cache) && d.cache.page_size % 4 == 0);
 }
 
 size_t workspace_of(const tfcc_rocm_paged_attention_desc& d, const PagedAttentionPlan& plan) {
@@ -1228,22 +1308,21 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
   const dim3 grid((unsigned)groups);
   const tfcc_rocm_paged_cache& c = d.cache;
   const unsigned blocks = (c.size + 63) / 64;
-  const bool uniform = c.page_size % 16 == 0, fast = wide_reads(c);
   if (plan.rows == kAttentionChunkRows) {
-    const auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kTileWaves * 64), 0, s, a); };
-    if (blocks == 1) start(attention_s8_tile_kernel<1>);
-    else if (blocks == 2) start(attention_s8_tile_kernel<2>);
-    else if (blocks == 3) start(attention_s8_tile_kernel<3>);
-    else start(attention_s8_tile_kernel<4>);
+    if (blocks == 1) launch_tiles<1>(a, grid, s);
+    else if (blocks == 2) launch_tiles<2>(a, grid, s);
+    else if (blocks == 3) launch_tiles<3>(a, grid, s);
+    else launch_tiles<4>(a, grid, s);
   } else if (c.type == TFCC_ROCM_S8) {
-    if (blocks == 1) launch_s8<1>(a, grid, s, plan.waves, fast);
-    else if (blocks == 2) launch_s8<2>(a, grid, s, plan.waves, fast);
-    else launch_s8<4>(a, grid, s, plan.waves, fast);
+    const bool wide = wide_reads(c);
+    if (blocks == 1) launch_s8<1>(a, grid, s, plan.waves, wide);
+    else if (blocks == 2) launch_s8<2>(a, grid, s, plan.waves, wide);
+    else launch_s8<4>(a, grid, s, plan.waves, wide);
   } else {
-    if (blocks == 1) launch_f32<1>(a, grid, s, plan.waves, uniform);
-    else if (blocks == 2) launch_f32<2>(a, grid, s, plan.waves, uniform);
-    else if (blocks == 3) launch_f32<3>(a, grid, s, plan.waves, uniform);
-    else launch_f32<4>(a, grid, s, plan.waves, uniform);
+    if (blocks == 1) launch_f32<1>(a, grid, s, plan.waves);
+    else if (blocks == 2) launch_f32<2>(a, grid, s, plan.waves);
+    else if (blocks == 3) launch_f32<3>(a, grid, s, plan.waves);
+    else launch_f32<4>(a, grid, s, plan.waves);
   }
   if (int e = check_launch("paged_attention")) return e;
   if (plan.splits > 1) {
