@@ -13,6 +13,9 @@
 //   pick    the list is sorted, the border found in it, the kept weights summed, and the token looked up in its run
 // (That the last workgroup of `runs` did what `pick` does cost 110 us more than the launch, for 128 rows of 100003: each of them
 // has to push the L2 of its part of the GPU out to memory first.)
+// 128 rows of 100003 with top-p and min-p take 12 + 23 + 26 + 11 us, of which the first is bound by HBM, the two in the middle by the vector
+// unit (about 40 operations of four cycles a logit, half of them in 64 bits), the last by the latency of what it does one after another,
+// and so are all four for a single row of 32000: 4 + 5 + 8 + 7.
 // A bin of more tokens than the list holds - a vocabulary of equal logits, top-k of thousands - goes a slower way there: eight bits of
 // the logits' order at a time over the whole row.
 #include "common.hpp"
@@ -65,31 +68,34 @@ __constant__ double kPowers[32] = {
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 
 // What the weights of a row's logits follow from.  exp((x - top) / temperature) * 2^shift is 2^(e + shift) 2^(j / 32) e^f with |f| <= ln 2 / 64
-// and the Taylor polynomial of e^f to the fifth power, whose rest is below 3e-15 of it; the 32 powers lie in LDS.  Weights that
-// round to the integer 0 need not be formed.
+// and the Taylor polynomial of e^f to the fifth power, whose rest is below 3e-15 of it; the 32 powers, with 2^shift in them, lie in LDS.
+// Below `cutoff` a weight is 2^-2 at most, the integer 0: it is taken for 0, and so is that of a NaN or of -infinity.
 struct Row {
-  float top, slope, least;  // below least times the slope from the top a weight is under 2^-2
-  double steps;             // of ln 2 / 32 in a logit
+  float top, slope, cutoff;
+  double steps;  // of ln 2 / 32 in a logit
   int shift;
   const double* powers;
-  __device__ double weight(float x) const {
-    const float below = (x - top) * slope;
-    if (below < least) return 0.0;
-    const double t = x == top ? 0.0 : ((double)x - (double)top) * steps;
-    const double n = rint(t), f = (t - n) * 0.021660849392498290195;
-    const int i = (int)n;
+  __device__ __forceinline__ double weight(float x) const {
+    // (infinity less infinity is no number, of which the smaller of it and 0 is 0)
+    const double t = fmin((double)x - (double)top, 0.0) * steps;
+    const double m = t + 6755399441055744.0;  // 1.5 * 2^52: the nearest integer is in the low bits
+    const int i = (int)(unsigned)(u64)__double_as_longlong(m);
+    const double f = (t - (m - 6755399441055744.0)) * 0.021660849392498290195;
     double e = fma(f, 1.0 / 120, 1.0 / 24);
     e = fma(e, f, 1.0 / 6);
     e = fma(e, f, 0.5);
     e = fma(e, f, 1.0);
     e = fma(e, f, 1.0);
-    return ldexp(e * powers[i & 31], (i >> 5) + shift);
+    const double w = ldexp(e * powers[i & 31], i >> 5);
+    return x >= cutoff ? w : 0.0;  // (what is formed for others is anything)
   }
 };
 __device__ Row row_of(float top, float temperature, int shift, double* powers) {  // powers: 32 in LDS, filled here; the caller waits
-  if (threadIdx.x < 32) powers[threadIdx.x] = kPowers[threadIdx.x];
-  const double slope = 1.0 / (double)temperature;
-  return {top, (float)slope, -0.6931472f * (shift + 2), slope * 46.166241308446828384, shift, powers};
+  if (threadIdx.x < 32) powers[threadIdx.x] = ldexp(kPowers[threadIdx.x], shift);
+  const double slope = 1.0 / (double)temperature, least = -0.6931471805599453 * (shift + 2);
+  float cutoff = fmaxf((float)fmax((double)top + least / slope, -3.4028234663852886e38), -3.402823466e38f);
+  if (((double)cutoff - (double)top) * slope > least && cutoff < INFINITY) cutoff = fmaxf(value_of(key_of(cutoff) - 1), -3.402823466e38f);  // rounded up
+  return {top, (float)slope, cutoff, slope * 46.166241308446828384, shift, powers};
 }
 // to the nearest integer, below 2^52
 __device__ __forceinline__ u64 integer_of(double w) { return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull; }
@@ -227,7 +233,7 @@ __device__ __forceinline__ u64 reach_of(float top_p, u64 all) {
 // What a row asks for.  All of it is loaded at once, from the random numbers where there is nothing to load: a load after another
 // is a microsecond.
 struct Wishes {
-  float temperature, top_p, random;
+  float temperature, top_p, min_p, random;
   int top_k;
   double least;  // of a kept weight
 };
@@ -235,7 +241,7 @@ __device__ __forceinline__ Wishes wishes_of(const SampleArgs& p, unsigned r) {
   const float temperature = (p.temperature ? p.temperature : p.random)[r], top_p = (p.top_p ? p.top_p : p.random)[r];
   const float min_p = (p.min_p ? p.min_p : p.random)[r], random = p.random[r];
   const int top_k = (p.top_k ? p.top_k : reinterpret_cast<const int*>(p.random))[r];
-  return {p.temperature ? temperature : 1.0f, p.top_p ? top_p : 1.0f, random, p.top_k ? top_k : 0,
+  return {p.temperature ? temperature : 1.0f, p.top_p ? top_p : 1.0f, p.min_p ? min_p : 0.0f, random, p.top_k ? top_k : 0,
           ldexp(fmin(p.min_p ? (double)min_p : 0.0, 1.0), p.shift)};
 }
 
@@ -364,6 +370,23 @@ __device__ __forceinline__ Four four_at(const float* x, unsigned at, unsigned le
   return f;
 }
 
+// A lane's part of a run, loaded a run ahead: with one load on its way a wavefront would wait longer than it works.
+struct Ahead {
+  Four f[4];
+};
+__device__ __forceinline__ Ahead run_at(const float* x, unsigned run, unsigned length) {
+  Ahead a;
+  const unsigned at = run * kRun + 4 * (threadIdx.x & 63);
+  if ((run + 1) * kRun <= length) {  // the same for the wavefront
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a.f[j] = *reinterpret_cast<const Four*>(x + at + 256 * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a.f[j] = four_at(x, at + 256 * j, length);
+  }
+  return a;
+}
+
 // Runs [first, behind) of a wavefront.
 struct Share {
   unsigned first, behind;
@@ -376,7 +399,8 @@ __device__ __forceinline__ Share share_of(const SampleArgs& p, unsigned part, un
 __global__ __launch_bounds__(kSampleThreads) void sample_tops_kernel(SampleArgs p) {
   __shared__ u64 tops[kSampleWaves];
   __shared__ unsigned lows[kSampleWaves];
-  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, lane = threadIdx.x & 63;
+  const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
   const RowSpace space = space_of(p, r);
   const float* x = p.logits + r * p.row_stride;
   for (unsigned i = part * kSampleThreads + threadIdx.x; i < kBins; i += p.parts * kSampleThreads) {
@@ -450,38 +474,54 @@ __device__ Head head_of(const SampleArgs& p, const RowSpace& space, const Wishes
   h.bins_of_logit = all > wide && all < 1e30f ? all : wide;
   return h;
 }
-// Falls with the logit: a rounded difference times a factor, cut off.
+// Falls with the logit: a rounded difference times a factor, cut off.  What is not a number, between infinities or for a factor of infinity, is
+// in the first (the middle one of three of which one is no number is the smaller of the others).
 __device__ __forceinline__ unsigned bin_of(const Head& h, float x) {
-  const float at = (h.row.top - x) * h.bins_of_logit;  // not a number between infinities, or for a factor of infinity: the first
-  return at < (float)(kBins - 1) ? (unsigned)at : at >= (float)(kBins - 1) ? kBins - 1 : 0u;
+  return (unsigned)__builtin_amdgcn_fmed3f((h.row.top - x) * h.bins_of_logit, 0.0f, (float)(kBins - 1));
 }
 
 __global__ __launch_bounds__(kSampleThreads) void sample_bins_kernel(SampleArgs p) {
   __shared__ u64 weights[kBins];
   __shared__ double powers[32];
   unsigned* const counts = reinterpret_cast<unsigned*>(weights);
-  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, lane = threadIdx.x & 63;
+  const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
   const RowSpace space = space_of(p, r);
   const float* x = p.logits + r * p.row_stride;
   const Share share = share_of(p, part, wave);
-  Four next = four_at(x, share.first * kRun + 4 * lane, p.length);
+  Ahead next = run_at(x, share.first, p.length);
   for (unsigned i = threadIdx.x; i < kBins; i += kSampleThreads) weights[i] = 0;
   const Wishes wishes = wishes_of(p, r);
   const Head h = head_of(p, space, wishes, powers);
   if ((!h.by_count && !h.by_weight) || h.greedy || (unsigned)(h.top >> 32) <= kNoToken) return;
   __syncthreads();
-  for (unsigned base = share.first * kRun; base < share.behind * kRun; base += 256) {
-    const Four f = next;
-    next = four_at(x, base + 256 + 4 * lane, p.length);
+  if (h.by_count) {
+    for (unsigned run = share.first; run < share.behind; ++run) {
+      const Ahead now = next;
+      next = run_at(x, run + 1, p.length);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (key_of(f.v[i]) <= kNoToken) continue;
-      const unsigned bin = bin_of(h, f.v[i]);
-      if (h.by_count) {
-        atomicAdd(&counts[bin], 1u);
-      } else {
-        const u64 w = integer_of(h.row.weight(f.v[i]));
-        if (w != 0) atomicAdd(&weights[bin], w);
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (now.f[j].v[i] > -INFINITY) atomicAdd(&counts[bin_of(h, now.f[j].v[i])], 1u);
+    }
+  } else {
+    for (unsigned run = share.first; run < share.behind; ++run) {
+      const Ahead now = next;
+      next = run_at(x, run + 1, p.length);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const Four f = now.f[j];
+        u64 w[4];
+        unsigned bin[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // all before the first is added: they wait for LDS together
+          w[i] = integer_of(h.row.weight(f.v[i]));
+          bin[i] = bin_of(h, f.v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (f.v[i] >= h.row.cutoff) atomicAdd(&weights[bin[i]], w[i]);
       }
     }
   }
@@ -515,15 +555,28 @@ struct Finding {
   u64 totals[kSampleWaves];
   Goal goal;
 };
-__device__ Goal goal_of(const Head& h, const RowSpace& space, Finding& s) {
+// A thread's bins, both kinds: asked for before it is known which kind counts.
+struct Bins {
+  static constexpr unsigned each = kBins / kSampleThreads;
+  u64 weights[each];
+  unsigned counts[each];
+  __device__ __forceinline__ explicit Bins(const RowSpace& space) {
+#pragma unroll
+    for (unsigned i = 0; i < each; ++i) {
+      weights[i] = space.weights[threadIdx.x * each + i];
+      counts[i] = space.counts[threadIdx.x * each + i];
+    }
+  }
+};
+__device__ Goal goal_of(const Head& h, const Bins& bins, Finding& s) {
   if (threadIdx.x == 0) s.goal = {0, 0, kBins};
   __syncthreads();
   if (!h.by_count && !h.by_weight) return s.goal;
-  constexpr unsigned each = kBins / kSampleThreads;
+  constexpr unsigned each = Bins::each;
   u64 v[each], mine = 0, all;
 #pragma unroll
   for (unsigned i = 0; i < each; ++i) {
-    v[i] = h.by_count ? space.counts[threadIdx.x * each + i] : space.weights[threadIdx.x * each + i];
+    v[i] = h.by_count ? bins.counts[i] : bins.weights[i];
     mine += v[i];
   }
   u64 upto = before_me(mine, s.totals, all);
@@ -545,45 +598,76 @@ __device__ Goal goal_of(const Head& h, const RowSpace& space, Finding& s) {
 __global__ __launch_bounds__(kSampleThreads) void sample_runs_kernel(SampleArgs p) {
   __shared__ Finding finding;
   __shared__ u64 list[kListOfPart];
+  __shared__ float aboves[kSampleWaves][kRun];
   __shared__ double powers[32];
   __shared__ unsigned listed, place_of_list;
-  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+  const unsigned r = blockIdx.x / p.parts, part = blockIdx.x - r * p.parts, lane = threadIdx.x & 63;
+  const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
   const RowSpace space = space_of(p, r);
   const float* x = p.logits + r * p.row_stride;
   const Share share = share_of(p, part, wave);
-  Four next = four_at(x, share.first * kRun + 4 * lane, p.length);
+  const Bins bins(space);
+  Ahead next = run_at(x, share.first, p.length);
   const Wishes wishes = wishes_of(p, r);
   const double least = wishes.least;
   const Head h = head_of(p, space, wishes, powers);
   if ((unsigned)(h.top >> 32) <= kNoToken || h.greedy) return;
   if (threadIdx.x == 0) listed = 0;
-  const Goal goal = goal_of(h, space, finding);
+  const Goal goal = goal_of(h, bins, finding);
   if (part == 0 && threadIdx.x == 0) *space.goal = goal;
   const unsigned border_bin = (unsigned)goal.bin;
+  float* const above = aboves[wave];
+  // below this a weight is too small for min-p or nothing at all; what is near it is looked at more closely
+  const float enough = wishes.min_p > 0.0f ? fmaxf(h.row.cutoff, h.row.top + (logf(fminf(wishes.min_p, 1.0f)) - 1e-3f) * wishes.temperature * 1.0001f - 1e-6f * fabsf(h.row.top))
+                                           : h.row.cutoff;
   for (unsigned run = share.first; run < share.behind; ++run) {
-    u64 mine = 0;
-    for (unsigned at = run * kRun + 4 * lane; at < (run + 1) * kRun; at += 256) {
-      const Four f = next;
-      next = four_at(x, at + 256, p.length);
+    // The logits that are kept for sure are few for most rows: they are gathered, and a wavefront forms their weights 64 at a time (all formed
+    // where a lane wants one: 33 us, gathered 32, with those that min-p leaves out left out before 26).
+    unsigned gathered = 0;
+    const Ahead now = next;
+    next = run_at(x, run + 1, p.length);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Four f = now.f[j];
+      const unsigned at = run * kRun + 256 * j + 4 * lane;
+      u64 for_list[4], any = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned key = key_of(f.v[i]);
-        if (key <= kNoToken) continue;
-        if (border_bin < kBins) {
-          const unsigned bin = bin_of(h, f.v[i]);
-          if (bin > border_bin) continue;
-          if (bin == border_bin || h.by_count) {
-            const unsigned place = atomicAdd(&listed, 1u);
-            if (place < kListOfPart) list[place] = sort_key(key, at + i);
-            continue;
-          }
-        }
-        const double w = h.row.weight(f.v[i]);
-        mine += w >= least ? integer_of(w) : 0;
+        const unsigned bin = bin_of(h, f.v[i]);
+        const bool there = f.v[i] > -INFINITY;
+        for_list[i] = __ballot(there && (h.by_count ? bin <= border_bin : bin == border_bin));
+        any |= for_list[i];
+        const u64 inner = __ballot(f.v[i] >= enough && !h.by_count && bin < border_bin);
+        if (inner >> lane & 1) above[gathered + __builtin_amdgcn_mbcnt_hi((unsigned)(inner >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)inner, 0))] = f.v[i];
+        gathered += __popcll(inner);
       }
+      if (any != 0) {
+        const unsigned all = __popcll(for_list[0]) + __popcll(for_list[1]) + __popcll(for_list[2]) + __popcll(for_list[3]);
+        unsigned place = 0;
+        if (lane == 0) place = atomicAdd(&listed, all);
+        place = (unsigned)__builtin_amdgcn_readfirstlane((int)place);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned mine = place + __builtin_amdgcn_mbcnt_hi((unsigned)(for_list[i] >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)for_list[i], 0));
+          if ((for_list[i] >> lane & 1) && mine < kListOfPart) list[mine] = sort_key(key_of(f.v[i]), at + i);
+          place += __popcll(for_list[i]);
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    u64 mine = 0;
+#pragma unroll 2
+    for (unsigned i = lane; i < gathered; i += 64) {
+      const double w = h.row.weight(above[i]);
+      mine += w >= least ? integer_of(w) : 0;
     }
     mine = wave_sum64(mine);
     if (lane == 0) space.runs[run] = mine;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
   __syncthreads();
   const unsigned n = listed;
@@ -767,10 +851,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
   }
 }
 
-// About 1024 workgroups in all, each wavefront of which has the same number of runs but for the last ones.
+// Up to 1024 workgroups in all, which run at the same time; each wavefront has the same number of runs but for the last ones.
 unsigned parts_of(unsigned rows, unsigned length) {
   const unsigned long long runs = (length + kRun - 1) / kRun, waves = 1024 * kSampleWaves;
-  unsigned long long each = runs * rows / waves, least = (runs + kMostParts * kSampleWaves - 1) / (kMostParts * kSampleWaves);
+  unsigned long long each = (runs * rows + waves - 1) / waves, least = (runs + kMostParts * kSampleWaves - 1) / (kMostParts * kSampleWaves);
   each = each < least ? least : each;
   return (unsigned)((runs + each * kSampleWaves - 1) / (each * kSampleWaves));
 }
