@@ -20,22 +20,31 @@ static int failures = 0;
 
 int main() {
   // one token of each sequence: a workgroup of eight wavefronts to a CU, pieces where there are fewer workgroups than CUs
-  PagedAttentionPlan p = paged_attention_plan(32, 32, 4, 8, 128, 8192, 1, 0, true);
+  PagedAttentionPlan p = paged_attention_plan(32, 32, 4, 8, 128, 8192, 1, 0, 128, false);
   EXPECT(p.rows == 16 && p.waves == 8 && p.splits == 1 && p.tiles >= 32);
-  p = paged_attention_plan(1, 1, 4, 8, 128, 8192, 1, 0, true);
+  p = paged_attention_plan(1, 1, 4, 8, 128, 8192, 1, 0, 128, false);
   EXPECT(p.rows == 16 && p.splits == 32 && p.split_keys == 256);
-  EXPECT(paged_attention_plan(1, 1, 4, 8, 128, 600, 1, 0, true).splits == 1);
-  EXPECT(paged_attention_plan(1, 1, 4, 8, 128, 100000, 1, 512, true).splits <= 3);  // a window bounds the keys
-  EXPECT(paged_attention_plan(32, 32, 4, 8, 256, 8192, 1, 0, true).waves == 4);
-  EXPECT(paged_attention_plan(100, 100, 4, 8, 128, 8192, 1, 0, true).waves == 4);
+  EXPECT(paged_attention_plan(1, 1, 4, 8, 128, 600, 1, 0, 128, false).splits == 1);
+  EXPECT(paged_attention_plan(1, 1, 4, 8, 128, 100000, 1, 512, 128, false).splits <= 3);  // a window bounds the keys
+  EXPECT(paged_attention_plan(32, 32, 4, 8, 256, 8192, 1, 0, 128, false).waves == 4);
+  EXPECT(paged_attention_plan(100, 100, 4, 8, 128, 8192, 1, 0, 128, false).waves == 4);
   // tiles of 128 rows: chunks that fill two, and a workgroup for each CU
-  EXPECT(paged_attention_plan(4096, 16, 4, 8, 128, 4096, 1, 0, true).rows == 128);
-  EXPECT(paged_attention_plan(4096, 16, 4, 8, 128, 4096, 1, 0, false).rows == 16);
-  EXPECT(paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, true).rows == 128 && paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, true).splits == 2);
-  EXPECT(paged_attention_plan(1024, 1, 4, 8, 128, 1000, 1, 0, true).splits == 1);
-  EXPECT(paged_attention_plan(1536, 1, 4, 8, 128, 4096, 1, 0, true).splits == 1);
-  EXPECT(paged_attention_plan(256, 1, 4, 8, 128, 4096, 1, 0, true).rows == 16);
-  EXPECT(paged_attention_plan(16 * 48, 16, 4, 8, 128, 4096, 1, 0, true).rows == 16);
+  EXPECT(paged_attention_plan(4096, 16, 4, 8, 128, 4096, 1, 0, 128, false).rows == 128);
+  EXPECT(paged_attention_plan(4096, 16, 4, 8, 128, 4096, 1, 0, 0, false).rows == 16);
+  EXPECT(paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, 128, false).rows == 128 && paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, 128, false).splits == 2);
+  EXPECT(paged_attention_plan(1024, 1, 4, 8, 128, 1000, 1, 0, 128, false).splits == 1);
+  EXPECT(paged_attention_plan(1536, 1, 4, 8, 128, 4096, 1, 0, 128, false).splits == 1);
+  EXPECT(paged_attention_plan(256, 1, 4, 8, 128, 4096, 1, 0, 128, false).rows == 16);
+  EXPECT(paged_attention_plan(16 * 48, 16, 4, 8, 128, 4096, 1, 0, 128, false).rows == 16);
+  // float32: tiles of 256 rows from fewer rows on, pieces of long contexts
+  EXPECT(paged_attention_plan(15 * 205, 15, 8, 2, 128, 376, 1, 0, 256, true).rows == 256);
+  EXPECT(paged_attention_plan(674, 1, 6, 4, 96, 675, 1, 0, 256, true).rows == 16);
+  p = paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, 256, true);
+  EXPECT(p.rows == 256 && p.splits == 2 && p.split_keys == 2048);
+  p = paged_attention_plan(256, 1, 4, 8, 128, 4096, 1, 0, 256, true);
+  EXPECT(p.rows == 256 && p.splits == 8);
+  EXPECT(paged_attention_plan(256, 1, 4, 8, 128, 4096, 1, 512, 256, true).rows == 16);
+  EXPECT(paged_attention_plan(64, 64, 8, 8, 128, 4096, 1, 0, 256, true).rows == 16);  // single tokens do not fill a tile
   std::mt19937 g(1);
   for (int turn = 0; turn < 20000; ++turn) {
     const unsigned batch = 1 + g() % 70, group = 1 + g() % 9, heads = 1 + g() % 40, size = 8 * (1 + g() % 32), most = g() % 3 ? g() % 9000 : g() % 300;
@@ -45,11 +54,12 @@ int main() {
     tokens += g() % 5;  // rows behind the last sequence
     const int causal = g() % 4 != 0;
     const unsigned window = causal && g() % 2 ? 1 + g() % 700 : 0;
-    p = paged_attention_plan(tokens, batch, group, heads, size, most, causal, window, g() % 2);
+    const bool float_cache = g() % 2;
+    p = paged_attention_plan(tokens, batch, group, heads, size, most, causal, window, g() % 3 == 0 ? 0 : !float_cache || size <= 64 ? 128 : size <= 128 ? 256 : 0, float_cache);
     unsigned tiles = 0;
     for (unsigned n : chunks) tiles += (n * group + p.rows - 1) / p.rows;
     EXPECT(tiles <= p.tiles);
-    EXPECT(p.rows == kAttentionRows || p.rows == kAttentionChunkRows);
+    EXPECT(p.rows == kAttentionRows || p.rows == 128 || p.rows == 256);
     EXPECT((p.waves == 4 || p.waves == 8) && (p.waves == 4 || size <= 128));
     EXPECT(p.splits >= 1 && p.splits <= kAttentionMostSplits && p.split_keys > 0 && p.split_keys % kAttentionStep == 0);
     // the keys that the rows of one tile see begin at a multiple of 32: with a window they are its rows' tokens and the window's
@@ -57,7 +67,7 @@ int main() {
     if (window > 0 && window + p.rows + 31ull < span) span = window + p.rows + 31ull;
     EXPECT((unsigned long long)p.splits * p.split_keys >= span);
   }
-  p = paged_attention_plan(0, 4, 4, 8, 128, 100, 1, 0, true);
+  p = paged_attention_plan(0, 4, 4, 8, 128, 100, 1, 0, 128, false);
   EXPECT(p.tiles == 0 && p.splits == 1);
   if (failures == 0) std::printf("paged attention plan: all passed\n");
   return failures != 0;

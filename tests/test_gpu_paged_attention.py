@@ -153,14 +153,19 @@ TILES = [
     ([1500, 1200], [128, 128], 128, 64, 128, 64, {}),                          # two pieces of the keys
     ([1500, 700, 300], [258, 257, 259], 32, 32, 64, 16, {"max_length": 1280}),
     ([5000], [257], 128, 128, 64, 16, {"window": 4000}),
+    ([3000, 2500, 100], [160, 140, 100], 32, 8, 128, 16, {}),                  # float32: pieces of a long context, some without keys
+    ([2900, 2300], [300, 260], 32, 32, 64, 20, {}),
+    ([4000, 700], [140, 200], 32, 8, 80, 64, {"max_length": 2500}),
+    ([150, 140, 133, 100] * 4, [100, 99, 70, 65] * 4, 12, 6, 40, 16, {}),      # chunks that fill half of their tiles
 ]
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["s8", "f32"])
 @pytest.mark.parametrize("case", range(len(TILES)))
-def test_chunks_against_the_definition(pkg, T, case):
+def test_chunks_against_the_definition(pkg, T, kind, case):
     lengths, chunks, heads, kv, size, page, more = TILES[case]
-    Made(pkg, "s8", lengths, chunks, heads, kv, size, page, 100 + case).check(T, **more)
+    Made(pkg, kind, lengths, chunks, heads, kv, size, page, 100 + case).check(T, **more)
 
 
 # Pages that end inside a step's keys: 16 rows and more, and fewer, a page for each key.
@@ -233,6 +238,35 @@ def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks, heads):
         m.check(T)
     else:
         assert np.isnan(got[m.starts[1] - 1, group:2 * group]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,chunk,heads,size", [(200, 30, 6, 64), (290, 258, 64, 64), (300, 290, 64, 128), (3000, 300, 32, 128)])
+def test_keys_that_are_not_finite(pkg, T, length, chunk, heads, size):
+    """A score of infinity or NaN makes a row NaN, one of -infinity takes the key out; rows that do not see the key keep every bit."""
+    m = Made(pkg, "f32", [length, 64], [chunk, 30], heads, heads // 2, size, 16, 18)
+    clean = T.n(m.run(T)).copy()
+    at = length - chunk // 2
+    page, inside = m.table[0, at // 16], at % 16
+    m.cache[0][page, 1, inside, 3] = np.inf
+    got = T.n(m.run(T)).astype(np.float64)
+    rows = np.arange(length - chunk, length) >= at  # of the first sequence
+    mine = np.zeros(got.shape, bool)
+    mine[:chunk, 2:4] = rows[:, None, None]
+    assert np.array_equal(got[~mine], clean[~mine])
+    x = m.q[:chunk, 2:4, 3]
+    assert np.isnan(got[:chunk, 2:4][rows][x[rows] > 0]).all()
+    out = rows[:, None] & (x < 0)
+    want = np.zeros((chunk, 2, size))
+    pages = m.table[0][np.arange(length) // 16]
+    k, v = m.cache[0][pages, 1, np.arange(length) % 16].astype(np.float64), m.cache[1][pages, 1, np.arange(length) % 16].astype(np.float64)
+    for t, h in zip(*np.nonzero(out)):
+        seen = np.arange(length) <= length - chunk + t
+        seen[at] = False
+        s = k[seen] @ m.q[t, 2 + h].astype(np.float64) * m.scale
+        w = np.exp(s - s.max())
+        want[t, h] = w / w.sum() @ v[seen]
+    assert out.any() and rel_fro(got[:chunk, 2:4][out], want[out]) < 1e-5
 
 
 @pytest.mark.gpu

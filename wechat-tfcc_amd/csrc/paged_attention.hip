@@ -14,10 +14,13 @@
 // fp16 matrix operations.  Queries are scaled by a power of two for each row.  What meets the values is a weight times a value's scale, and
 // what has to stay in fp16's range is that product, not the weight: a row's weights are 2^(score - frame), and the frame moves where
 // score + log2(scale) exceeds it by 15, to 8 below.  Between moves nothing is rescaled, and what fp16 cannot hold is 2^-32 of
-// the largest product or less.  The sum of the weights is kept in the same frame.  A float32 cache goes through the fp32 matrix operations.
+// the largest product or less.  The sum of the weights is kept in the same frame.  A float32 cache goes through the fp32 matrix operations, and
+// chunks of many tokens over one through three fp16 operations of pieces, which take two fifths of the time.
 //
 // The keys of a tile are dealt to the wavefronts of a workgroup in turns, and in pieces to several workgroups where there are few tiles; each
 // wavefront keeps frame, sum and output of its own, joined in LDS, the pieces by a second launch.  A frame of -infinity: no key was seen.
+#include <type_traits>
+
 #include "lds_dma.hpp"
 #include "paged_attention_plan.hpp"
 #include "paged_cache.hpp"
@@ -30,6 +33,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned long long u64;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
@@ -159,6 +163,24 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return a + b;
 }
 
+// The largest of neighbouring lanes, LANES of them.
+template <int LANES>
+__device__ __forceinline__ unsigned lanes_max(unsigned v) {
+  const auto larger = [](unsigned a, unsigned b) { return a > b ? a : b; };
+  v = larger(v, moved<0xb1, 0xf>(v));  // lanes 1, 2, then those of a half row from its other end, then 8 apart
+  v = larger(v, moved<0x4e, 0xf>(v));
+  if constexpr (LANES >= 8) v = larger(v, moved<0x141, 0xf>(v));
+  if constexpr (LANES >= 16) v = larger(v, moved<0x128, 0xf>(v));
+  if constexpr (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = larger(r[0], r[1]);
+  }
+  if constexpr (LANES >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = larger(r[0], r[1]);
+  }
+  return v;
+}
 // 2^e for e in [-126, 127]; infinity for 128
 __device__ __forceinline__ float power(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 // e with |v| < 2^e, from -100 to 128, so that 2^(14 - e) and its inverse are normal numbers
@@ -622,38 +644,113 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
 }
 
 // Chunks of many tokens, int8 as above: a workgroup takes 128 rows, a wavefront 32 of them, and all go over the same keys, 32 in a step.  Bound: the
-// matrix cores and, with as much to do, the vector unit.  So the keys and values of a step are turned into fp16 once for the four wavefronts, in the
+// matrix cores and, with as much to do, the vector unit (4 chunks of 1024 over 4096, 32 heads over 8 of 128: int8 407 us, matrix operations and LDS
+// reads alone 283; float32 730, with tiles of 16 rows on the fp32 matrix operations 1955).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
 // order in which the matrix cores take them, into one of two LDS buffers while the other is worked on; the next step's rows
 // are on their way to registers meanwhile.  Products of 32 x 32 as above, with
 //   S^T: lane l holds row l % 32 and keys 8 a + 4 (l / 32) + i in [4 a + i]
 //   O^T: likewise values place(8 a + 4 (l / 32) + i, n) of the head in tile n
-constexpr int kTileWaves = 4, kTileKeys = 32;
+constexpr int kTileKeys = 32;
 
 // Which value of a head is row L of tile n of the second product: a word of four values goes to four tiles, or to two rows of two where
-// 64 values are left.
-template <int BLOCKS>
+// 64 values are left; float32: two neighbours go to two tiles.
+template <int BLOCKS, bool S8>
 __device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
+  if (!S8) return n / 2 * 64 + 2 * L + n % 2;
   return n / 4 * 4 + 4 <= 2 * BLOCKS ? n / 4 * 128 + 4 * L + n % 4 : n / 4 * 128 + 4 * (L % 16) + 2 * (L / 16) + n % 4;
 }
 
-template <int BLOCKS, bool WHOLE>
-__global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attention_s8_tile_kernel(AttentionArgs p) {
-  constexpr int KS = 4 * BLOCKS, N = 2 * BLOCKS;  // products over a head, tiles of 32 of its values
+// A row of a float32 cache is two fp16 pieces under a power of two of its own, which is its scale as an int8 row's is: what is said above of
+// int8 holds, with a third operation for the product of the first factor's large piece with the second's small one.  The two
+// small ones' product is 2^-24 of the whole and left out.  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
+// one by one.
+// The wavefront's 32 rows of a float32 cache by the definition, in float32: lanes take keys for the scores and values of the head for the sums.
+// Only rows that see an infinity or a NaN are written.
+template <int BLOCKS>
+__device__ __forceinline__ void rows_one_by_one(const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, int begin, int end, const int* table,
+                                                          const float* keys, const float* values) {
+  const unsigned lane = threadIdx.x & 63, size = p.cache.size;
+  const auto row_at = [&](const float* held, int key) -> const float* {
+    const unsigned index = p.cache.page_size.quotient((unsigned)key);
+    const int page = page_of(p, table, index);
+    return page < 0 ? nullptr : held + (unsigned long long)page * p.cache.page + (key - index * p.cache.page_size.d) * p.cache.row;
+  };
+#pragma unroll 1
+  for (int r = 0; r < 32; ++r) {
+    const int row_token = __builtin_amdgcn_readlane(t.row_token, r);
+    if (row_token < 0) return;
+    const int row_low = __builtin_amdgcn_readlane(t.row_low, r), row_high = __builtin_amdgcn_readlane(t.row_high, r);
+    const int low = row_low > begin ? row_low : begin, high = row_high < end ? row_high : end;
+    const unsigned long long token = t.first + row_token, query_head = head * p.group.d + __builtin_amdgcn_readlane(t.row_head, r);
+    const float* const q = p.q + token * p.q_token + query_head * p.q_head;
+    float m = -INFINITY, l = 0.0f, out[BLOCKS] = {};
+    bool odd = false;
+    const auto look_at = [&](float v) {
+      odd |= (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
+      return v;
+    };
+#pragma unroll 1
+    for (int kb = low; kb < high; kb += 64) {
+      const int key = kb + (int)lane;
+      const float* const row = key < high ? row_at(keys, key) : nullptr;
+      float s = 0.0f;
+      if (row != nullptr)
+#pragma unroll 1
+        for (unsigned d = 0; d < size; ++d) s += q[d] * look_at(row[d]);
+      s *= p.scale;
+      const float next = fmaxf(m, wave_max(row != nullptr ? s : -INFINITY)), f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      const float e = row != nullptr ? __builtin_amdgcn_exp2f(s - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+      l = l * f + wave_sum(e);
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) out[b] *= f;
+#pragma unroll 1
+      for (int i = 0; i < 64 && kb + i < high; ++i) {
+        const float weight = __shfl(e, i, 64);
+        const float* const value = row_at(values, kb + i);
+        if (value == nullptr) continue;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+          if (lane + 64 * b < size) out[b] += weight * look_at(value[lane + 64 * b]);
+      }
+    }
+    if (!__any(odd)) continue;
+    float* to = p.out + token * p.out_token + query_head * p.out_head;
+    if (p.splits > 1) {
+      const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
+      to = p.partial + place * size;
+      if (lane == 0) {
+        p.statistics[place * 2] = m;
+        p.statistics[place * 2 + 1] = l;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+      if (lane + 64 * b < size) to[lane + 64 * b] = p.splits > 1 ? out[b] : m == -INFINITY ? 0.0f : out[b] / l;
+  }
+}
+
+// WAVES: 4, and 8 where a thread's part of a step's rows would else take the registers (float32, heads of 128: four wavefronts spill, 1210 us).
+template <int BLOCKS, int WAVES, bool S8, bool WHOLE>
+__global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void attention_tile_kernel(AttentionArgs p) {
+  constexpr int KS = 4 * BLOCKS, N = 2 * BLOCKS, PIECES = S8 ? 1 : 2;  // products over a head, tiles of 32 of its values
+  static_assert(S8 ? WAVES == 4 : BLOCKS * 4 == WAVES);
   struct Stage {
-    u32x4 keys[KS][64];       // lane l: key l % 32, values 16 s + 8 (l / 32) + j
-    u32x4 values[N][2][64];   // lane l: value_of(l % 32, n), keys 16 m + 8 (j / 4) + 4 (l / 32) + j % 4
+    u32x4 keys[PIECES][KS][64];       // lane l: key l % 32, values 16 s + 8 (l / 32) + j; float32: exchange() within the half
+    u32x4 values[PIECES][N][2][64];   // lane l: value_of(l % 32, n), keys 16 m + 8 (j / 4) + 4 (l / 32) + j % 4
     float key_scale[kTileKeys], value_scale[kTileKeys], value_log[kTileKeys];
-    unsigned gone;  // a bit for each key that no page holds
+    unsigned gone[WAVES / 2];         // keys that no page holds: a bit for each; what each of the first wavefronts knows of it
   };
   __shared__ Stage stages[2];
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = lane / 32;
   Tile t;
   unsigned head, split;
   int begin, end;
-  if (!take_work(p, kAttentionChunkRows, wave * 32 + lane % 32, t, head, split, begin, end)) return;
+  if (!take_work(p, WAVES * 32, wave * 32 + lane % 32, t, head, split, begin, end)) return;
   const unsigned size = p.cache.size;
-  const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
-  const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
+  using Element = std::conditional_t<S8, int8_t, float>;
+  const Element* const keys = static_cast<const Element*>(p.cache.keys) + head * p.cache.head;
+  const Element* const values = static_cast<const Element*>(p.cache.values) + head * p.cache.head;
   const int* const table = p.table + (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)t.sequence) * p.table_stride;
   begin = __builtin_amdgcn_readfirstlane(begin);
   end = __builtin_amdgcn_readfirstlane(end);
@@ -662,12 +759,13 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
   const int low = __builtin_amdgcn_readfirstlane(t.row_low), high = there > 0 ? __builtin_amdgcn_readlane(t.row_high, last) : 0;
   const int all_low = __builtin_amdgcn_readlane(t.row_low, last), all_high = __builtin_amdgcn_readfirstlane(t.row_high);
 
-  // A step's rows: threads of the first half fetch keys, 16 bytes of key (thread % 32) at a time; those of the second values, a word of eight keys
-  // at a time; the first wavefront the scales.
-  constexpr int WORDS = 16 * BLOCKS, TASKS = (4 * WORDS + 127) / 128;
-  const bool for_keys = threadIdx.x < 128;
-  const unsigned me = threadIdx.x % 128;
-  u32x4 raw[BLOCKS <= 2 ? 2 : 4];  // BLOCKS times 16 bytes of a key, or TASKS times eight words
+  // A step's rows: threads of the first half fetch keys, 16 bytes of key (thread % 32) at a time, float32: SIDE threads side by side those of one
+  // key; those of the second values, four values of eight keys at a time, float32: two; the first wavefront the scales.
+  constexpr int HALF = WAVES * 32, SIDE = HALF / kTileKeys, WORDS = S8 ? 16 * BLOCKS : 32 * BLOCKS, TASKS = (4 * WORDS + HALF - 1) / HALF;
+  static_assert(S8 || (TASKS == 1 && 4 * WORDS == HALF));
+  const bool for_keys = threadIdx.x < HALF;
+  const unsigned me = threadIdx.x % HALF;
+  u32x4 raw[S8 && BLOCKS <= 2 ? 2 : 4];  // 16 bytes of a key each, or TASKS times eight words, float32: two keys' values in each
   // Each thread asks for the pages of its own rows, through the vector loads: they come back in order, after the rows that were asked for before.
   // (Entries through the scalar cache would be waited for with the LDS reads.)
   float scale = 0.0f;
@@ -677,8 +775,8 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
   int named[TASKS][PAGES];
   // the first key of the step's that the thread's task k fetches of its n-th page
   const auto key_of = [&](int k, int n) {
-    const unsigned group = (me + 128 * k) / WORDS;
-    return for_keys ? (WHOLE ? me / 16 % 2 * 16 : me % 32) : group / 2 % 2 * 16 + (WHOLE ? 0 : 4 * (group % 2) + 8 * n);
+    const unsigned group = (me + HALF * k) / WORDS;
+    return for_keys ? (!S8 ? me / SIDE : WHOLE ? me / 16 % 2 * 16 : me % 32) : group / 2 % 2 * 16 + (WHOLE ? 0 : 4 * (group % 2) + 8 * n);
   };
   const auto inside_page = [&](unsigned key) { return key - p.cache.page_size.quotient(key) * p.cache.page_size.d; };
   const auto ask_pages = [&](int at) {
@@ -700,47 +798,55 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
     unsigned long long held;
     if (for_keys) {
       gone = page_row(0, 0, held);
-      const unsigned inside = WHOLE ? (me / 16 % 2 ? halves[1] : halves[0]) + (me & 15) : inside_page((unsigned)at + me % 32);
-      const int8_t* const row = keys + held * p.cache.page + inside * p.cache.row;
+      const unsigned inside = WHOLE ? (me / 16 % 2 ? halves[1] : halves[0]) + (me & 15) : inside_page((unsigned)at + key_of(0, 0));
+      const Element* const row = keys + held * p.cache.page + inside * p.cache.row;
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        const unsigned d = 16 * (me / 32 + 4 * b);
+      for (int b = 0; b < (S8 ? BLOCKS : 4); ++b) {
+        const unsigned d = S8 ? 16 * (me / 32 + 4 * b) : 4 * (me % SIDE + SIDE * b);
         raw[b] = *reinterpret_cast<const u32x4*>(row + (d < size ? d : 0));
       }
-      if (threadIdx.x < 64) {
+      if (S8 && threadIdx.x < 64) {
         const float* const s = (threadIdx.x < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head;
         scale = s[held * p.cache.scale_page + inside];
       }
     } else {
 #pragma unroll
       for (int k = 0; k < TASKS; ++k) {
-        const unsigned task = me + 128 * k, word = task % WORDS, group = task / WORDS;
-        if (4 * WORDS % 128 == 0 || group < 4) {
-          const int8_t* row[2];
+        const unsigned task = me + HALF * k, word = task % WORDS, group = task / WORDS;
+        if (4 * WORDS % HALF == 0 || group < 4) {
+          const Element* row[2];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             (void)page_row(k, n < PAGES ? n : 0, held);
             const unsigned inside = WHOLE ? (group / 2 ? halves[1] : halves[0]) + 4 * (group % 2) + 8 * n : inside_page((unsigned)at + key_of(k, n));
-            row[n] = values + held * p.cache.page + inside * p.cache.row + (4 * word < size ? 4 * word : 0);
+            const unsigned d = S8 ? 4 * word : 2 * word;
+            row[n] = values + held * p.cache.page + inside * p.cache.row + (d < size ? d : 0);
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) raw[2 * k + j / 4][j % 4] = *reinterpret_cast<const unsigned*>(row[j / 4] + j % 4 * p.cache.row);
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (S8) raw[2 * k + j / 4][j % 4] = *reinterpret_cast<const unsigned*>(row[j / 4] + j % 4 * p.cache.row);
+            else {
+              const u32x2 two = *reinterpret_cast<const u32x2*>(row[j / 4] + j % 4 * p.cache.row);
+              raw[j / 2][j % 2 * 2] = two[0];
+              raw[j / 2][j % 2 * 2 + 1] = two[1];
+            }
+          }
         }
       }
     }
   };
-  const auto store = [&](Stage& s) {
+  const auto store_s8 = [&](Stage& s) {
     if (for_keys) {
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         const unsigned step = me / 32 + 4 * b;
-        s.keys[step][me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][0], raw[b][1]));
-        s.keys[step][32 + me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][2], raw[b][3]));
+        s.keys[0][step][me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][0], raw[b][1]));
+        s.keys[0][step][32 + me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][2], raw[b][3]));
       }
       if (threadIdx.x < 32) {
         s.key_scale[threadIdx.x] = scale;
         const unsigned nowhere = (unsigned)__ballot(gone);
-        if (threadIdx.x == 0) s.gone = nowhere;
+        if (threadIdx.x < 2) s.gone[threadIdx.x] = nowhere;
       } else if (threadIdx.x < 64) {
         s.value_scale[threadIdx.x - 32] = scale;
         s.value_log[threadIdx.x - 32] = frame_log(scale);
@@ -748,8 +854,8 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
     } else {
 #pragma unroll
       for (int k = 0; k < TASKS; ++k) {
-        const unsigned task = me + 128 * k, word = task % WORDS, group = task / WORDS;
-        if (4 * WORDS % 128 == 0 || group < 4) {
+        const unsigned task = me + HALF * k, word = task % WORDS, group = task / WORDS;
+        if (4 * WORDS % HALF == 0 || group < 4) {
           unsigned w[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) w[j] = raw[2 * k + j / 4][j % 4];
@@ -758,11 +864,100 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
             const unsigned n = word / 32 * 4 + (quarters ? b : b % 2), L = quarters ? word % 32 : word % 16 + 16 * (b / 2);
-            s.values[n][group / 2][32 * (group % 2) + L] = __builtin_bit_cast(u32x4, v[b]);
+            s.values[0][n][group / 2][32 * (group % 2) + L] = __builtin_bit_cast(u32x4, v[b]);
           }
         }
       }
     }
+  };
+  // float32: the power of two that brings a row's largest value to 2^13 .. 2^14, and the row's pieces.  What is read together and written together
+  // of the keys lies in different banks.
+  const auto exchange = [](unsigned lane_of, unsigned step) { return lane_of ^ (lane_of / 32 * 4) ^ (WAVES == 8 ? step % 2 * 2 : 0); };
+  bool odd = false;  // an infinity or a NaN was among what some row sees
+  const auto store_f32 = [&](Stage& s, int at) {
+    const auto larger = [](unsigned a, unsigned b) { return a > b ? a : b; };
+    const auto size_of = [&](unsigned v) { return v & 0x7fffffffu; };
+    if (at < t.low || at + kTileKeys > t.high) {  // what no row sees may be anything
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = at + (int)(for_keys ? me / SIDE : me / WORDS / 2 * 16 + 4 * (me / WORDS % 2) + 8 * (j / 4) + j % 4);
+        const bool none = key < t.low || key >= t.high;
+        raw[j / 2][j % 2 * 2] = none ? 0u : raw[j / 2][j % 2 * 2];
+        raw[j / 2][j % 2 * 2 + 1] = none ? 0u : raw[j / 2][j % 2 * 2 + 1];
+      }
+    }
+    unsigned most = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = larger(most, size_of(raw[b][i]));
+    if (__any(most >= 0x7f800000u)) {  // rare; for the rows that do not see it, as zeros, which change nothing
+      odd = true;
+      most = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          raw[b][i] = size_of(raw[b][i]) >= 0x7f800000u ? 0u : raw[b][i];
+          most = larger(most, size_of(raw[b][i]));
+        }
+    }
+    if (for_keys) {
+      const int e = bound_of(__uint_as_float(lanes_max<SIDE>(most)));
+      const float up = power(14 - e);
+      const unsigned key = me / SIDE, part = me % SIDE;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        f16x2 hi[2], lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) split_two(__uint_as_float(raw[b][2 * i]) * up, __uint_as_float(raw[b][2 * i + 1]) * up, hi[i], lo[i]);
+        const unsigned step = part / 4 + SIDE / 4 * b, to = exchange(part / 2 % 2 * 32 + key, step);
+        reinterpret_cast<u32x2*>(&s.keys[0][step][to])[part % 2] = u32x2{__builtin_bit_cast(unsigned, hi[0]), __builtin_bit_cast(unsigned, hi[1])};
+        reinterpret_cast<u32x2*>(&s.keys[PIECES - 1][step][to])[part % 2] = u32x2{__builtin_bit_cast(unsigned, lo[0]), __builtin_bit_cast(unsigned, lo[1])};
+      }
+      if (part == 0) s.key_scale[key] = power(e - 14);
+      // a bit for each SIDE threads to neighbouring bits: of 8 by a product that moves bit 8 i to 56 + i
+      u64 nowhere = __ballot(gone);
+      if constexpr (SIDE == 8) {
+        nowhere = (nowhere & 0x0101010101010101ull) * 0x0102040810204080ull >> 56;
+      } else {
+        nowhere &= 0x1111111111111111ull;
+        nowhere = (nowhere | nowhere >> 3) & 0x0303030303030303ull;
+        nowhere = (nowhere | nowhere >> 6) & 0x000f000f000f000full;
+        nowhere = (nowhere | nowhere >> 12) & 0x000000ff000000ffull;
+        nowhere |= nowhere >> 24;
+      }
+      if (lane == 0) s.gone[wave] = (unsigned)(nowhere & ((1ull << 64 / SIDE) - 1)) << (64 / SIDE * wave);
+    } else {
+      const unsigned word = me % WORDS, group = me / WORDS;
+      int exponent[8];
+      float up[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // of the lanes that have the row
+        exponent[j] = bound_of(__uint_as_float(lanes_max<WORDS>(larger(size_of(raw[j / 2][j % 2 * 2]), size_of(raw[j / 2][j % 2 * 2 + 1])))));
+        up[j] = power(14 - exponent[j]);
+      }
+      int e = exponent[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) e = word == (unsigned)j ? exponent[j] : e;
+      if (word < 8) {
+        const unsigned key = group / 2 * 16 + 4 * (group % 2) + 8 * (word / 4) + word % 4;
+        s.value_scale[key] = power(e - 14);
+        s.value_log[key] = fmaxf((float)(e - 14), -90.0f);  // as of frame_log()
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        Half8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_two(__uint_as_float(raw[j][b]) * up[2 * j], __uint_as_float(raw[j][2 + b]) * up[2 * j + 1], hi.p[j], lo.p[j]);
+        s.values[0][word / 32 * 2 + b][group / 2][32 * (group % 2) + word % 32] = __builtin_bit_cast(u32x4, hi.v);
+        s.values[PIECES - 1][word / 32 * 2 + b][group / 2][32 * (group % 2) + word % 32] = __builtin_bit_cast(u32x4, lo.v);
+      }
+    }
+  };
+  const auto store = [&](Stage& s, int at) {
+    if constexpr (S8) store_s8(s);
+    else store_f32(s, at);
   };
 
   if (begin < end) {
@@ -808,7 +1003,7 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
 #pragma unroll 1
   for (int kb = begin; kb < end; kb += kTileKeys, turn ^= 1) {
     Stage& s = stages[turn];
-    store(s);
+    store(s, kb);
     if (kb + kTileKeys < end) {
       fetch(kb + kTileKeys);
       if (kb + 2 * kTileKeys < end) ask_pages(kb + 2 * kTileKeys);
@@ -818,7 +1013,9 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
     f32x16 x = {};
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const f16x8 a = __builtin_bit_cast(f16x8, s.keys[k][lane]);
+      const unsigned at = S8 ? lane : exchange(lane, k);
+      const f16x8 a = __builtin_bit_cast(f16x8, s.keys[0][k][at]);
+      if constexpr (!S8) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, s.keys[PIECES - 1][k][at]), q_hi[k], x, 0, 0, 0);
       x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_lo[k], x, 0, 0, 0);
       x = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[k], x, 0, 0, 0);
     }
@@ -826,20 +1023,28 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       const f32x4 key_scale = *reinterpret_cast<const f32x4*>(s.key_scale + 8 * a + 4 * half);
-      value_scale[a] = *reinterpret_cast<const f32x4*>(s.value_scale + 8 * a + 4 * half);
-      value_log[a] = *reinterpret_cast<const f32x4*>(s.value_log + 8 * a + 4 * half);
+      if constexpr (S8) {
+        value_scale[a] = *reinterpret_cast<const f32x4*>(s.value_scale + 8 * a + 4 * half);
+        value_log[a] = *reinterpret_cast<const f32x4*>(s.value_log + 8 * a + 4 * half);
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[4 * a + i] *= key_scale[i];
     }
-    const unsigned none = s.gone;
+    unsigned none = s.gone[0];
+#pragma unroll
+    for (int i = 1; i < WAVES / 2; ++i) none |= s.gone[i];
     if (none != 0 || kb < all_low || kb + kTileKeys > all_high) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int key = kb + 8 * (i / 4) + 4 * (int)half + i % 4;
         const bool seen = (none >> (key - kb) & 1) == 0 && key >= t.row_low && key < t.row_high;
         x[i] = seen ? x[i] : -INFINITY;
-        value_scale[i / 4][i % 4] = seen ? value_scale[i / 4][i % 4] : 0.0f;
+        if constexpr (S8) value_scale[i / 4][i % 4] = seen ? value_scale[i / 4][i % 4] : 0.0f;  // it may be anything
       }
+    }
+    if constexpr (!S8) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) value_log[a] = *reinterpret_cast<const f32x4*>(s.value_log + 8 * a + 4 * half);
     }
     float top = -INFINITY, a, b;
 #pragma unroll
@@ -854,6 +1059,10 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
       for (int n = 0; n < N; ++n) o[n] *= f;
     }
     const float zero = frame == -INFINITY ? 0.0f : frame;
+    if constexpr (!S8) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a) value_scale[a] = *reinterpret_cast<const f32x4*>(s.value_scale + 8 * a + 4 * half);
+    }
     Half8 w_hi[2], w_lo[2];
     float w[16];
 #pragma unroll
@@ -868,7 +1077,8 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const f16x8 v = __builtin_bit_cast(f16x8, s.values[n][h][lane]);
+        const f16x8 v = __builtin_bit_cast(f16x8, s.values[0][n][h][lane]);
+        if constexpr (!S8) o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, s.values[PIECES - 1][n][h][lane]), w_hi[h].v, o[n], 0, 0, 0);
         o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w_lo[h].v, o[n], 0, 0, 0);
         o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w_hi[h].v, o[n], 0, 0, 0);
       }
@@ -876,32 +1086,52 @@ __global__ __launch_bounds__(kTileWaves * 64, BLOCKS <= 2 ? 2 : 1) void attentio
   float a, b;
   butterfly_pair<32>(l, a, b);
   l = a + b;
-  if (t.row_token < 0) return;
-  const unsigned long long token = t.first + t.row_token, query_head = head * p.group.d + t.row_head;
-  float* to = p.out + token * p.out_token + query_head * p.out_head;
-  float factor = 1.0f;
-  if (p.splits > 1) {
-    const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
-    to = p.partial + place * size;
-    if (half == 0) {
-      p.statistics[place * 2] = frame;
-      p.statistics[place * 2 + 1] = l;
-    }
-  } else {
-    factor = frame == -INFINITY ? 0.0f : 1.0f / l;
-  }
-#pragma unroll
-  for (int n = 0; n < N; n += n / 4 * 4 + 4 <= N ? 4 : 2)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const unsigned d = value_of<BLOCKS>(8 * (i / 4) + 4 * half + i % 4, n);
-      if (d >= size) continue;
-      if (n / 4 * 4 + 4 <= N) {
-        *reinterpret_cast<f32x4*>(to + d) = f32x4{o[n][i], o[n + 1][i], o[n + 2][i], o[n + 3][i]} * factor;
-      } else {
-        *reinterpret_cast<f32x2*>(to + d) = f32x2{o[n][i] * factor, o[n + 1][i] * factor};
+  if (t.row_token >= 0) {
+    const unsigned long long token = t.first + t.row_token, query_head = head * p.group.d + t.row_head;
+    float* to = p.out + token * p.out_token + query_head * p.out_head;
+    float factor = 1.0f;
+    if (p.splits > 1) {
+      const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
+      to = p.partial + place * size;
+      if (half == 0) {
+        p.statistics[place * 2] = frame;
+        p.statistics[place * 2 + 1] = l;
       }
+    } else {
+      factor = frame == -INFINITY ? 0.0f : 1.0f / l;
     }
+    if constexpr (S8) {
+#pragma unroll
+      for (int n = 0; n < N; n += n / 4 * 4 + 4 <= N ? 4 : 2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const unsigned d = value_of<BLOCKS, S8>(8 * (i / 4) + 4 * half + i % 4, n);
+          if (d >= size) continue;
+          if (n / 4 * 4 + 4 <= N) {
+            *reinterpret_cast<f32x4*>(to + d) = f32x4{o[n][i], o[n + 1][i], o[n + 2][i], o[n + 3][i]} * factor;
+          } else {
+            *reinterpret_cast<f32x2*>(to + d) = f32x2{o[n][i] * factor, o[n + 1][i] * factor};
+          }
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; n += 2)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const unsigned d = value_of<BLOCKS, S8>(8 * (i / 4) + 4 * half + i % 4, n);
+          if (d < size) *reinterpret_cast<f32x4*>(to + d) = f32x4{o[n][i], o[n + 1][i], o[n][i + 1], o[n + 1][i + 1]} * factor;
+        }
+    }
+  }
+  if constexpr (!S8) {
+    __shared__ unsigned odds[WAVES];
+    if (lane == 0) odds[wave] = odd ? 1u : 0u;
+    __syncthreads();
+    unsigned any = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) any |= odds[w];
+    if (any != 0) return rows_one_by_one<BLOCKS>(p, t, head, split, begin, end, table, keys, values);
+  }
 }
 
 // int8 in any layout, a page for each key, loaded when it is due.
@@ -1209,7 +1439,7 @@ void launch_s8(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves,
 }
 template <int BLOCKS>
 void launch_tiles(const AttentionArgs& a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((a.cache.page_size.d % 16 == 0 ? attention_s8_tile_kernel<BLOCKS, true> : attention_s8_tile_kernel<BLOCKS, false>), grid, dim3(kTileWaves * 64), 0, s, a);
+  hipLaunchKernelGGL((a.cache.page_size.d % 16 == 0 ? attention_tile_kernel<BLOCKS, 4, true, true> : attention_tile_kernel<BLOCKS, 4, true, false>), grid, dim3(256), 0, s, a);
 }
 template <int BLOCKS>
 void launch_f32(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves) {
@@ -1246,8 +1476,16 @@ bool wide_reads(const tfcc_rocm_paged_cache& c) {
          (reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values)) % 16 == 0;
 }
 
+// Rows of the tiles that chunks of many tokens may take, 0: none.
+unsigned chunk_rows(const tfcc_rocm_paged_cache& c) {
+  if (c.page_size < 16 || c.page_size % 4 != 0) return 0;
+  if (c.type == TFCC_ROCM_F32) return c.size <= 64 ? 128 : c.size <= 128 ? 256 : 0;
+  return wide_reads(c) ? 128 : 0;
+}
+
 PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
-  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, wide_reads(d.cache) && d.cache.page_size % 4 == 0);
+  return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, chunk_rows(d.cache),
+                              d.cache.type == TFCC_ROCM_F32);
 }
 
 size_t workspace_of(const tfcc_rocm_paged_attention_desc& d, const PagedAttentionPlan& plan) {
@@ -1308,7 +1546,10 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
   const dim3 grid((unsigned)groups);
   const tfcc_rocm_paged_cache& c = d.cache;
   const unsigned blocks = (c.size + 63) / 64;
-  if (plan.rows == kAttentionChunkRows) {
+  if (plan.rows != kAttentionRows && c.type == TFCC_ROCM_F32) {
+    if (blocks == 1) hipLaunchKernelGGL((attention_tile_kernel<1, 4, false, false>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attention_tile_kernel<2, 8, false, false>), grid, dim3(512), 0, s, a);
+  } else if (plan.rows != kAttentionRows) {
     if (blocks == 1) launch_tiles<1>(a, grid, s);
     else if (blocks == 2) launch_tiles<2>(a, grid, s);
     else if (blocks == 3) launch_tiles<3>(a, grid, s);

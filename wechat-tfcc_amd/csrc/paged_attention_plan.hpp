@@ -14,7 +14,6 @@ struct PagedAttentionPlan {
 };
 
 constexpr unsigned kAttentionRows = 16;    // rows (a token's query heads of one cache head) of a tile
-constexpr unsigned kAttentionChunkRows = 128;  // of a tile of a chunk of many tokens
 constexpr unsigned kAttentionStep = 256;   // keys that eight wavefronts take in one step
 constexpr unsigned kAttentionMostSplits = 256;
 
@@ -24,29 +23,47 @@ inline unsigned paged_attention_tiles(unsigned tokens, unsigned batch, unsigned 
   return (unsigned)(((uint64_t)tokens * group + (uint64_t)(rows - 1) * chunks) / rows);
 }
 
+// chunk_rows: of the tiles that chunks of many tokens may take, 128 or 256; 0: there are none.
 inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, unsigned group, unsigned cache_heads, unsigned size, unsigned max_length,
-                                               int causal, unsigned window, bool chunk_tiles) {
+                                               int causal, unsigned window, unsigned chunk_rows, bool float_cache) {
   PagedAttentionPlan p;
   // chunks of about the same number of tokens
   const uint64_t chunks = tokens < batch ? tokens : batch, mean = chunks == 0 ? 0 : (tokens + chunks - 1) / chunks;
   const auto groups_of = [&](unsigned rows) { return chunks * ((mean * group + rows - 1) / rows) * cache_heads; };
-  // Tiles of 128 rows where they make a workgroup for each CU, of chunks that fill two (16 chunks of 256 tokens, 32 heads over 8 of 128: 374 us,
-  // with tiles of 16 rows 469; one chunk of 1024: 190 and 235; 16 of 64: 182 and 171; one of 256: 208 and 76).
-  p.rows = chunk_tiles && mean * group >= 2 * kAttentionChunkRows && groups_of(kAttentionChunkRows) >= 256 ? kAttentionChunkRows : kAttentionRows;
-  p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
   // a tile spans at most `rows` tokens: the keys that one of them sees
-  uint64_t keys = max_length;
-  if (causal && window > 0 && (uint64_t)window + p.rows + 32 < keys) keys = (uint64_t)window + p.rows + 32;
-  const uint64_t groups = groups_of(p.rows);
+  const auto keys_of = [&](unsigned rows) {
+    const uint64_t span = (uint64_t)window + rows + 32;
+    return causal && window > 0 && span < max_length ? span : (uint64_t)max_length;
+  };
+  bool wide = false;
+  if (chunk_rows > 0 && !float_cache) {
+    // Tiles of 128 rows where they make a workgroup for each CU, of chunks that fill two (16 chunks of 256 tokens, 32 heads over 8 of 128: 374 us,
+    // with tiles of 16 rows 469; one chunk of 1024: 190 and 235; 16 of 64: 182 and 171; one of 256: 208 and 76).
+    wide = mean * group >= 256 && groups_of(chunk_rows) >= 256;
+  } else if (chunk_rows > 0) {
+    // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
+    // (32 heads over 8 of 128, tokens x rows of all tiles: 15 of 205 over 376, 16 heads over 2: 50 us, with tiles of 16 rows 101; 11 of 125 over 227: 34 and 43;
+    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in four pieces 129 and 213).
+    const uint64_t rows = mean * group * chunks * cache_heads;
+    wide = 2 * mean * group >= chunk_rows && (rows >= 18000 || (rows >= 8192 && keys_of(chunk_rows) >= 2048));
+  }
+  p.rows = wide ? chunk_rows : kAttentionRows;
+  p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
+  const uint64_t keys = keys_of(p.rows), groups = groups_of(p.rows);
   // One workgroup of eight wavefronts to a CU is best as long as there are no more than two for each CU: it has the CU's LDS for rows on
   // their way, and little time goes into beginnings and ends (64 sequences of up to 4096 keys, 8 heads of 128 in int8: 88 us, with
   // four wavefronts 97; 200 sequences of 700: 78 and 59).  Eight with heads wider than 128 do not have the registers.
   uint64_t splits = 1;
   p.waves = groups <= 512 && size <= 128 && keys > kAttentionStep / 2 ? 8 : 4;
-  if (p.rows == kAttentionChunkRows) {
+  if (wide && float_cache) {
+    // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 267 us, one 403)
+    p.waves = chunk_rows / 32;
+    const uint64_t fit = groups == 0 ? 1 : 256 * 256 / chunk_rows / groups;
+    splits = keys < 2048 || fit < 1 ? 1 : fit < keys / 512 ? fit : keys / 512;
+    if (splits > 8) splits = 8;
+  } else if (wide) {
     p.waves = 4;
-    splits = groups < 384 ? 2 : 1;  // two of these share a CU
-    if (keys < 4 * kAttentionStep) splits = 1;
+    splits = groups < 384 && keys >= 4 * kAttentionStep ? 2 : 1;  // two of these share a CU
   } else if (groups > 0 && groups < 256) {
     // Fewer than CUs: pieces of the keys, where they save more steps than the launch that joins them costs, three steps of 256 keys with
     // heads of 128 and four with heads of 64 (16 sequences of 4096: two pieces 30 us, one 40; one sequence of 1024: four 12.4, one 14.4;
