@@ -241,6 +241,22 @@ def test_what_a_row_does_not_see_may_be_anything(pkg, T, kind, chunks, heads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,page", [("s8", 16), ("s8", 24), ("s8", 7), ("f32", 16), ("f32", 24), ("f32", 7)])
+@pytest.mark.parametrize("lengths,chunks,heads", [([200, 64], [30, 1], 6), ([4000, 64], [1, 1], 2), ([290, 270], [258, 260], 128), ([3000, 100], [300, 100], 64)])
+def test_queries_that_are_not_finite(pkg, T, kind, page, lengths, chunks, heads):
+    """Their rows are NaN, not the zeros of a row that sees nothing; the others keep every bit."""
+    m = Made(pkg, kind, lengths, chunks, heads, heads // 2, 64, page, 19)
+    clean = T.n(m.run(T)).copy()
+    for value in (np.nan, np.inf, -np.inf):
+        token = chunks[0] - 1
+        m.q[token, 1, 5] = value
+        got = T.n(m.run(T))
+        mine = np.zeros(got.shape, bool)
+        mine[token, 1] = True
+        assert np.isnan(got[mine]).all() and np.array_equal(got[~mine], clean[~mine])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("length,chunk,heads,size", [(200, 30, 6, 64), (290, 258, 64, 64), (300, 290, 64, 128), (3000, 300, 32, 128)])
 def test_keys_that_are_not_finite(pkg, T, length, chunk, heads, size):
     """A score of infinity or NaN makes a row NaN, one of -infinity takes the key out; rows that do not see the key keep every bit."""
@@ -248,15 +264,18 @@ def test_keys_that_are_not_finite(pkg, T, length, chunk, heads, size):
     clean = T.n(m.run(T)).copy()
     at = length - chunk // 2
     page, inside = m.table[0, at // 16], at % 16
+    later = np.arange(length - chunk, length) >= at
+    m.cache[0][page, 1, inside, 3] = np.nan
+    got = T.n(m.run(T))
+    assert np.isnan(got[:chunk, 2:4][later]).all() and np.array_equal(got[:chunk, 2:4][~later], clean[:chunk, 2:4][~later])
     m.cache[0][page, 1, inside, 3] = np.inf
     got = T.n(m.run(T)).astype(np.float64)
-    rows = np.arange(length - chunk, length) >= at  # of the first sequence
     mine = np.zeros(got.shape, bool)
-    mine[:chunk, 2:4] = rows[:, None, None]
+    mine[:chunk, 2:4] = later[:, None, None]
     assert np.array_equal(got[~mine], clean[~mine])
     x = m.q[:chunk, 2:4, 3]
-    assert np.isnan(got[:chunk, 2:4][rows][x[rows] > 0]).all()
-    out = rows[:, None] & (x < 0)
+    assert np.isnan(got[:chunk, 2:4][later][x[later] > 0]).all()
+    out = later[:, None] & (x < 0)
     want = np.zeros((chunk, 2, size))
     pages = m.table[0][np.arange(length) // 16]
     k, v = m.cache[0][pages, 1, np.arange(length) % 16].astype(np.float64), m.cache[1][pages, 1, np.arange(length) % 16].astype(np.float64)

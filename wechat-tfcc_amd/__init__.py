@@ -1125,6 +1125,12 @@ def _heads_of(t, name):
     return t if t.shape[2] <= 1 or t.stride(2) == 1 else t.contiguous()
 
 
+def _written_heads(out, like):
+    """Memory for a result like `like`: its heads contiguous, no two of its elements in one place."""
+    return out.shape == like.shape and out.dtype == like.dtype and (out.shape[2] <= 1 or out.stride(2) == 1) and \
+        all(n <= 1 or step > 0 for n, step in zip(out.shape, out.stride()))
+
+
 def _integers(t, name, count, types):
     if t.dtype not in types or t.dim() != 1 or t.shape[0] != count:
         raise InvalidArgumentError("invalid " + name)
@@ -1153,8 +1159,7 @@ def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0, out=N
         outputs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in inputs]
     else:
         outputs = [t for t in out if t is not None]
-        if len(outputs) != len(inputs) or any(o.shape != t.shape or o.dtype != t.dtype or (size > 1 and o.stride(2) != 1)
-                                              for o, t in zip(outputs, inputs)):
+        if len(outputs) != len(inputs) or not all(_written_heads(o, t) for o, t in zip(outputs, inputs)):
             raise InvalidArgumentError("invalid out")
     d = RotaryDesc()
     for i, (t, o) in enumerate(zip(inputs, outputs)):
@@ -1278,7 +1283,7 @@ def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window
         raise InvalidArgumentError("invalid window")
     if out is None:
         out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
-    elif out.shape != q.shape or out.dtype != torch.float32 or out.stride(2) != 1:
+    elif not _written_heads(out, q):
         raise InvalidArgumentError("invalid out")
     d.q, d.out = _ptr(q), _ptr(out)
     d.q_token_stride, d.q_head_stride, d.out_token_stride, d.out_head_stride = q.stride(0), q.stride(1), out.stride(0), out.stride(1)

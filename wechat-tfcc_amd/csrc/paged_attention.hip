@@ -181,6 +181,8 @@ __device__ __forceinline__ unsigned lanes_max(unsigned v) {
   }
   return v;
 }
+// The frame that goes out with a sum: scores of NaN raise none, but a row that has one is not a row without keys.
+__device__ __forceinline__ float frame_out(float frame, float sum) { return sum != sum && frame == -INFINITY ? 0.0f : frame; }
 // 2^e for e in [-126, 127]; infinity for 128
 __device__ __forceinline__ float power(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 // e with |v| < 2^e, from -100 to 128, so that 2^(14 - e) and its inverse are normal numbers
@@ -467,7 +469,7 @@ struct S8Rows {
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int n = 0; n < N; ++n) list[i * N + n] = o[n][i];
-    join_and_store(joining, p, t, head, split, frame, l, list, [&](int at) { return N * (4 * (int)g + at / N) + at % N; });
+    join_and_store(joining, p, t, head, split, frame_out(frame, l), l, list, [&](int at) { return N * (4 * (int)g + at / N) + at % N; });
   }
 };
 
@@ -715,6 +717,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttentionArgs& p, const Ti
       }
     }
     if (!__any(odd)) continue;
+    m = frame_out(m, l);
     float* to = p.out + token * p.out_token + query_head * p.out_head;
     if (p.splits > 1) {
       const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
@@ -1086,6 +1089,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
   float a, b;
   butterfly_pair<32>(l, a, b);
   l = a + b;
+  frame = frame_out(frame, l);
   if (t.row_token >= 0) {
     const unsigned long long token = t.first + t.row_token, query_head = head * p.group.d + t.row_head;
     float* to = p.out + token * p.out_token + query_head * p.out_head;
@@ -1383,7 +1387,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) list[(b * 4 + i) * 4 + j] = o[b][j][i];
-  join_and_store(joining, p, t, head, split, m, l, list, [&](int at) { return 64 * (at / 16) + 4 * (4 * (int)g + at % 16 / 4); });
+  join_and_store(joining, p, t, head, split, frame_out(m, l), l, list, [&](int at) { return 64 * (at / 16) + 4 * (4 * (int)g + at % 16 / 4); });
 }
 
 // The pieces of a row joined: a workgroup to a row, its threads four values each of one in every kThreads / (size / 4) pieces.
