@@ -36,6 +36,10 @@ int main() {
   EXPECT(paged_attention_plan(1536, 1, 4, 8, 128, 4096, 1, 0, 128, false).splits == 1);
   EXPECT(paged_attention_plan(256, 1, 4, 8, 128, 4096, 1, 0, 128, false).rows == 16);
   EXPECT(paged_attention_plan(16 * 48, 16, 4, 8, 128, 4096, 1, 0, 128, false).rows == 16);
+  EXPECT(paged_attention_plan(39 * 63, 39, 4, 8, 128, 510, 1, 0, 128, false).rows == 128);
+  EXPECT(paged_attention_plan(16 * 48, 16, 4, 8, 128, 2048, 1, 0, 128, false).rows == 16);
+  EXPECT(paged_attention_plan(12 * 138, 12, 8, 1, 256, 589, 1, 0, 128, false).rows == 16);
+  EXPECT(paged_attention_plan(2000, 2000, 4, 8, 128, 510, 1, 0, 128, false).rows == 16);  // single tokens do not fill a tile
   // float32: tiles of 256 rows from fewer rows on, pieces of long contexts
   EXPECT(paged_attention_plan(15 * 205, 15, 8, 2, 128, 376, 1, 0, 256, true).rows == 256);
   EXPECT(paged_attention_plan(674, 1, 6, 4, 96, 675, 1, 0, 256, true).rows == 16);

@@ -35,17 +35,19 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
     const uint64_t span = (uint64_t)window + rows + 32;
     return causal && window > 0 && span < max_length ? span : (uint64_t)max_length;
   };
+  const uint64_t all = mean * group * chunks * cache_heads;  // rows
   bool wide = false;
   if (chunk_rows > 0 && !float_cache) {
-    // Tiles of 128 rows where they make a workgroup for each CU, of chunks that fill two (16 chunks of 256 tokens, 32 heads over 8 of 128: 374 us,
-    // with tiles of 16 rows 469; one chunk of 1024: 190 and 235; 16 of 64: 182 and 171; one of 256: 208 and 76).
-    wide = mean * group >= 256 && groups_of(chunk_rows) >= 256;
+    // Wide tiles where chunks fill half of one and there are rows for the GPU, more of them over long contexts, whose steps tiles of 16 rows
+    // take at the rate of HBM (rows in all: 39 chunks of up to 84 over 510, 32 heads over 8 of 128, 79000: 60 us, with tiles of 16 rows 98; 8 of 49 over 2706 with
+    // a window of 293, 20500: 28 and 34; 12 of 184 over 589, 8 heads over 1 of 256, 13000: 73 and 57; over long contexts one of 1024 over
+    // 4096, 32800: 186 and 243; 16 of 64 over 2048, 24600: 105 and 89).
+    wide = 2 * mean * group >= chunk_rows && all >= (keys_of(chunk_rows) <= 1536 ? 20000 : 32000);
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
     // (32 heads over 8 of 128, tokens x rows of all tiles: 15 of 205 over 376, 16 heads over 2: 50 us, with tiles of 16 rows 101; 11 of 125 over 227: 34 and 43;
     // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in four pieces 129 and 213).
-    const uint64_t rows = mean * group * chunks * cache_heads;
-    wide = 2 * mean * group >= chunk_rows && (rows >= 18000 || (rows >= 8192 && keys_of(chunk_rows) >= 2048));
+    wide = 2 * mean * group >= chunk_rows && (all >= 18000 || (all >= 8192 && keys_of(chunk_rows) >= 2048));
   }
   p.rows = wide ? chunk_rows : kAttentionRows;
   p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
@@ -63,7 +65,7 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
     if (splits > 8) splits = 8;
   } else if (wide) {
     p.waves = 4;
-    splits = groups < 384 && keys >= 4 * kAttentionStep ? 2 : 1;  // two of these share a CU
+    splits = keys >= 2048 && groups < (size <= 128 ? 384 : 192) ? 2 : 1;  // two share a CU, of heads wider than 128 one has it
   } else if (groups > 0 && groups < 256) {
     // Fewer than CUs: pieces of the keys, where they save more steps than the launch that joins them costs, three steps of 256 keys with
     // heads of 128 and four with heads of 64 (16 sequences of 4096: two pieces 30 us, one 40; one sequence of 1024: four 12.4, one 14.4;
