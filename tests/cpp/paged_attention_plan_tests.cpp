@@ -65,7 +65,7 @@ int main() {
     EXPECT(tiles <= p.tiles);
     EXPECT(p.rows == kAttentionRows || p.rows == 128 || p.rows == 256);
     EXPECT((p.waves == 4 || p.waves == 8) && (p.waves == 4 || size <= 128));
-    EXPECT(p.splits >= 1 && p.splits <= kAttentionMostSplits && p.split_keys > 0 && p.split_keys % kAttentionStep == 0);
+    EXPECT(p.splits >= 1 && p.splits <= kAttentionMostSplits && p.split_keys > 0 && p.split_keys % (p.waves * (float_cache ? 16 : 32)) == 0);
     // the keys that the rows of one tile see begin at a multiple of 32: with a window they are its rows' tokens and the window's
     unsigned long long span = most;
     if (window > 0 && window + p.rows + 31ull < span) span = window + p.rows + 31ull;

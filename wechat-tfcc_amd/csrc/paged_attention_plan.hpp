@@ -10,11 +10,11 @@ struct PagedAttentionPlan {
   unsigned tiles;       // an upper bound of the tiles of rows that all chunks make
   unsigned waves;       // of a workgroup, 4 or 8
   unsigned splits;      // pieces of the keys, each with a workgroup for every tile and cache head
-  unsigned split_keys;  // keys of a piece, a multiple of 256
+  unsigned split_keys;  // keys of a piece, a multiple of what its wavefronts take in one step
 };
 
 constexpr unsigned kAttentionRows = 16;    // rows (a token's query heads of one cache head) of a tile
-constexpr unsigned kAttentionStep = 256;   // keys that eight wavefronts take in one step
+constexpr unsigned kAttentionStep = 256;   // keys that eight wavefronts take of an int8 cache in one step
 constexpr unsigned kAttentionMostSplits = 256;
 
 // A chunk of n tokens makes ceil(n * group / rows) tiles; how the tokens are spread over the sequences only the device knows.
@@ -55,8 +55,9 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   // One workgroup of eight wavefronts to a CU is best as long as there are no more than two for each CU: it has the CU's LDS for rows on
   // their way, and little time goes into beginnings and ends (64 sequences of up to 4096 keys, 8 heads of 128 in int8: 88 us, with
   // four wavefronts 97; 200 sequences of 700: 78 and 59).  Eight with heads wider than 128 do not have the registers.
-  uint64_t splits = 1;
+  uint64_t splits = 1, step = kAttentionStep;
   p.waves = groups <= 512 && size <= 128 && keys > kAttentionStep / 2 ? 8 : 4;
+  if (!wide) step = p.waves * (float_cache ? 16 : 32);
   if (wide && float_cache) {
     // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 267 us, one 403)
     p.waves = chunk_rows / 32;
@@ -67,18 +68,21 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
     p.waves = 4;
     splits = keys >= 2048 && groups < (size <= 128 ? 384 : 192) ? 2 : 1;  // two share a CU, of heads wider than 128 one has it
   } else if (groups > 0 && groups < 256) {
-    // Fewer than CUs: pieces of the keys, where they save more steps than the launch that joins them costs, three steps of 256 keys with
-    // heads of 128 and four with heads of 64 (16 sequences of 4096: two pieces 30 us, one 40; one sequence of 1024: four 12.4, one 14.4;
-    // 16 of 1024: two 16.6, one 15.6).
-    const uint64_t steps = (keys + kAttentionStep - 1) / kAttentionStep;
-    splits = 256 / groups;
+    // Fewer than CUs: pieces of the keys, where they save more steps than the launch that joins them costs (int8: 16 sequences of 4096, two
+    // pieces 30 us, one 40; one of 1024: four 12.4, one 14.4; 2 of 938, 24 heads over 4 of 96: four 11.8, one 13.6; one of 777, 12 heads of 64:
+    // four 11.4, one 9.8; float32: 12 of 429, 8 heads over 1 of 256: eight 18, one 35; 2 chunks of 3 over 737, 12 heads of 64: six 11.3, one 15.5;
+    // 7 of 15 over 7203, 20 heads over 5 of 80, 140 workgroups: two 109, one 186).
+    const uint64_t steps = (keys + step - 1) / step;
+    splits = float_cache && keys >= 4096 ? (256 + groups - 1) / groups : 256 / groups;
     splits = splits < steps ? splits : steps;
-    if (splits > 1 && (steps - (steps + splits - 1) / splits) * (size + 128) < 3 * 256) splits = 1;
+    if (splits > 32 && splits > steps / 2) splits = steps / 2 > 32 ? steps / 2 : 32;  // joining them takes its time too (3 of 10389: 41 pieces 18.5 us, 82 21)
     if (splits < 1) splits = 1;
+    const uint64_t saved = steps - (steps + splits - 1) / splits;
+    if (float_cache ? saved * (size + 64) < 5 * 64 : saved * (size + 128) < 640) splits = 1;
   }
   uint64_t each = (keys + splits - 1) / splits;
-  each = (each + kAttentionStep - 1) / kAttentionStep * kAttentionStep;
-  if (each == 0) each = kAttentionStep;
+  each = (each + step - 1) / step * step;
+  if (each == 0) each = step;
   p.split_keys = (unsigned)each;
   p.splits = (unsigned)((keys + each - 1) / each);
   if (p.splits < 1) p.splits = 1;
