@@ -22,12 +22,12 @@ def test_refused_without_a_device(pkg):
     assert call() == 0
 
 
-def check(pkg, T, logits, random, **kw):
+def check(pkg, T, logits, random, most_near=0.05, **kw):
     got, odds = pkg.sample(T.t(logits), T.t(random), **{k: None if v is None else T.t(v) for k, v in kw.items()})
     got, odds = T.n(got), T.n(odds)
     want, exact, margin = R.sample(logits, random, **kw)
     near = margin < 1e-9
-    assert near.mean() < 0.05
+    assert near.mean() <= most_near
     assert np.array_equal(got[~near], want[~near]), (got, want, margin)
     # a weight in 64 bits over a sum of integers of 2^-43 each, rounded to float32 once
     assert (np.abs(odds - exact) <= 2.0 ** -24 * exact + logits.shape[1] * 2.0 ** -43 * exact + 1e-45)[~near].all()
@@ -147,3 +147,17 @@ def test_strides_and_refusals(pkg, T):
                      ((wide, u), dict(top_p=u.double())), ((wide, u.cpu()), {}), ((wide[:, :0], u), {})):
         with pytest.raises(pkg.InvalidArgumentError):
             pkg.sample(*args, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size,offset", [(1.0, 0.0), (1e-3, 1e4), (100.0, -1e6), (1e4, 1e8), (1e30, 1e37), (1e-30, 0.0)])
+@pytest.mark.parametrize("least", [1.0, 0.5, 1e-3, 1e-30])
+def test_least_weights_at_all_sizes(pkg, T, size, offset, least):
+    """Logits far from zero, close together and far apart, with temperatures that fit them and others that do not."""
+    rng = np.random.default_rng(12)
+    logits = (rng.normal(size=(6, 5003)) * size + offset).astype(np.float32)
+    temperature = (np.array([1.0, 0.3, 3.0, 1e-3, 1e3, 1e6]) * size).astype(np.float32)
+    # margins are in units of the largest weight: where the least kept one is below 1e-9 of it, every row with a weight that small is called near
+    near = 1.0 if least < 1e-9 else 0.05
+    for top_p in (None, np.full(6, 0.97, np.float32)):
+        check(pkg, T, logits, rng.random(6).astype(np.float32), near, temperature=temperature, min_p=np.full(6, least, np.float32), top_p=top_p)
