@@ -71,6 +71,20 @@ static void refusals(bool gpu) {
   REFUSED(cache_write(odd, k6, k6, positions), ROCMRuntimeError);
 }
 
+// Sizes whose product does not fit the 32 bits in which a tensor counts its elements: refused before anything is allocated.
+static void sizes(bool gpu) {
+  REFUSED(PagedCache<int8_t>(262145, 8, 16, 128), InvalidArgumentError);  // 2^32 + 16384
+  REFUSED(PagedCache<float>(262145, 8, 16, 128), InvalidArgumentError);
+  REFUSED(PagedCache<int8_t>(1u << 16, 1u << 16, 1, 8), InvalidArgumentError);  // 2^35: nothing is left in 32 bits
+  REFUSED(PagedCache<int8_t>(0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu), InvalidArgumentError);
+  REFUSED(PagedCache<int8_t>(0xffffffffu, 0xffffffffu, 0, 8), InvalidArgumentError);
+  if (!gpu) return;
+  PagedCache<float> cache(2, 1, 16, 256);
+  Variable<int32_t> table({1, 2}), starts({2});
+  REFUSED(cache_read(cache, table, starts, (1u << 24) + 1), InvalidArgumentError);  // 2^32 + 256
+  REFUSED(cache_read(cache, table, starts, 0xffffffffu), InvalidArgumentError);
+}
+
 // Keys that are all alike: the weights of a row are equal, and it gets the mean of the values that it sees.
 template <class T>
 static void means() {
@@ -153,6 +167,7 @@ int main(int argc, char** argv) {
     Session::setThreadDefault(session.get());
   }
   refusals(gpu);
+  sizes(gpu);
   if (gpu) {
     means<float>();
     means<int8_t>();

@@ -1761,6 +1761,16 @@ template <class T>
 void require_list(const Tensor<T>& t, size_t count, const char* text) {
   if (t.shape().size() != 1 || t.shape(0) != count) throw InvalidArgumentError(text);
 }
+// A shape whose elements a tensor can count, in 32 bits; refused before anything is allocated.
+Shape countable(std::initializer_list<unsigned> dims, const char* text) {
+  uint64_t area = 1;
+  for (unsigned d : dims) {
+    if (d == 0) return Shape(dims);
+    if (area > 0xffffffffu / d) throw InvalidArgumentError(text);
+    area *= d;
+  }
+  return Shape(dims);
+}
 template <class T>
 tfcc_rocm_paged_cache held_by(const PagedCache<T>& c) {
   tfcc_rocm_paged_cache d{};
@@ -1830,7 +1840,7 @@ std::tuple<Variable<float>, Variable<float>> rotary(const Tensor<float>& q, cons
 
 template <class T>
 PagedCache<T>::PagedCache(unsigned pages, unsigned heads, unsigned pageSize, unsigned size)
-    : keys({pages, heads, pageSize, size}), values({pages, heads, pageSize, size}) {
+    : keys(countable({pages, heads, pageSize, size}, "invalid cache")), values(keys.shape()) {
   if (keys.size() == 0) throw InvalidArgumentError("invalid cache");
   require_rocm();
   data::zeros(keys);
@@ -1862,7 +1872,7 @@ std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>& cac
   require_list(starts, table.shape(0) + 1, "invalid starts");
   require_rocm();
   const tfcc_rocm_paged_cache d = held_by(cache);
-  Variable<float> keys({tokens, d.heads, d.size}), values({tokens, d.heads, d.size});
+  Variable<float> keys(countable({tokens, d.heads, d.size}, "invalid tokens")), values(keys.shape());
   check(tfcc_rocm_cache_read(current_stream(), &d, table.data(), table.shape(1), table.shape(1), table.shape(0), starts.data(), tokens, keys.data(), values.data()));
   return std::make_tuple(std::move(keys), std::move(values));
 }

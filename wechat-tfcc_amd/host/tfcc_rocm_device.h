@@ -259,7 +259,8 @@ std::tuple<std::vector<double>, float> rotary_frequencies(unsigned part, double 
 std::tuple<Variable<float>, Variable<float>> rotary(const Tensor<float>& q, const Tensor<float>& k, const Tensor<int32_t>& positions,
                                                     const Tensor<double>& frequencies, bool interleaved = false, float magnitude = 1.0f);
 
-// Memory of a cache, all zeros at first.  T = float, or int8_t with a scale for each row of a head.
+// Memory of a cache, all zeros at first.  T = float, or int8_t with a scale for each row of a head.  A tensor here counts its elements in 32
+// bits: a cache or a result of cache_read of more is refused (the C interface takes any size).
 template <class T>
 struct PagedCache {
   Variable<T> keys, values;                 // [pages, heads, rows, size]
