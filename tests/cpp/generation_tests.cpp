@@ -85,6 +85,27 @@ static void sizes(bool gpu) {
   REFUSED(cache_read(cache, table, starts, 0xffffffffu), InvalidArgumentError);
 }
 
+// A cache whose tensors were replaced by smaller ones, or moved out: its descriptor would name memory that is not there.
+static void replaced() {
+  Variable<float> k({3, 2, 8}), q({3, 4, 8});
+  Variable<int32_t> slots({3}), table({1, 2}), starts({2}), lengths({1});
+  const auto refused = [&](PagedCache<int8_t>& cache) {
+    REFUSED(cache_write(cache, k, k, slots), InvalidArgumentError);
+    REFUSED(cache_read(cache, table, starts, 1), InvalidArgumentError);
+    REFUSED(paged_attention(q, cache, table, starts, lengths, 1.0f), InvalidArgumentError);
+  };
+  for (int which = 0; which < 4; ++which) {
+    PagedCache<int8_t> cache(2, 2, 16, 8);
+    if (which == 0) cache.values = Variable<int8_t>({1, 2, 16, 8});
+    if (which == 1) cache.keys = Variable<int8_t>({2, 2, 16});
+    if (which == 2) cache.keyScales = Variable<float>({2, 2, 8});
+    if (which == 3) cache.valueScales = Variable<float>();
+    refused(cache);
+  }
+  PagedCache<int8_t> cache(2, 2, 16, 8), other(std::move(cache));
+  refused(cache);
+}
+
 // Keys that are all alike: the weights of a row are equal, and it gets the mean of the values that it sees.
 template <class T>
 static void means() {
@@ -169,6 +190,7 @@ int main(int argc, char** argv) {
   refusals(gpu);
   sizes(gpu);
   if (gpu) {
+    replaced();
     means<float>();
     means<int8_t>();
     tokens();

@@ -1771,8 +1771,13 @@ Shape countable(std::initializer_list<unsigned> dims, const char* text) {
   }
   return Shape(dims);
 }
+// Its tensors are public: one may have been put in the place of another, or moved out.
 template <class T>
 tfcc_rocm_paged_cache held_by(const PagedCache<T>& c) {
+  const Shape& s = c.keys.shape();
+  if (s.size() != 4 || s.area() == 0 || c.values.shape() != s) throw InvalidArgumentError("invalid cache");
+  if (std::is_same<T, int8_t>::value && (c.keyScales.shape() != Shape({s[0], s[1], s[2]}) || c.valueScales.shape() != c.keyScales.shape()))
+    throw InvalidArgumentError("invalid cache");
   tfcc_rocm_paged_cache d{};
   d.keys = const_cast<T*>(c.keys.data());
   d.values = const_cast<T*>(c.values.data());
@@ -1856,11 +1861,11 @@ PagedCache<T>::PagedCache(unsigned pages, unsigned heads, unsigned pageSize, uns
 template <class T>
 void cache_write(PagedCache<T>& cache, const Tensor<float>& keys, const Tensor<float>& values, const Tensor<int32_t>& slots) {
   require_heads(keys, "invalid keys");
-  if (keys.shape(1) != cache.keys.shape(1) || keys.shape(2) != cache.keys.shape(3)) throw InvalidArgumentError("invalid keys");
+  const tfcc_rocm_paged_cache d = held_by(cache);
+  if (keys.shape(1) != d.heads || keys.shape(2) != d.size) throw InvalidArgumentError("invalid keys");
   if (values.shape() != keys.shape()) throw InvalidArgumentError("invalid values");
   require_list(slots, keys.shape(0), "invalid slots");
   require_rocm();
-  const tfcc_rocm_paged_cache d = held_by(cache);
   const uint64_t head = d.size, token = head * d.heads;
   check(tfcc_rocm_cache_write(current_stream(), &d, keys.data(), token, head, values.data(), token, head, keys.shape(0), slots.data(), TFCC_ROCM_S32));
 }
@@ -1881,15 +1886,15 @@ template <class T>
 Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
                                 const Tensor<int32_t>& lengths, float scale, bool causal, unsigned window, unsigned maxLength) {
   require_heads(q, "invalid q");
-  if (q.shape(2) != cache.keys.shape(3) || q.shape(1) % cache.keys.shape(1) != 0) throw InvalidArgumentError("invalid q");
+  tfcc_rocm_paged_attention_desc d{};
+  d.cache = held_by(cache);
+  if (q.shape(2) != d.cache.size || q.shape(1) % d.cache.heads != 0) throw InvalidArgumentError("invalid q");
   if (lengths.shape().size() != 1) throw InvalidArgumentError("invalid lengths");
   if (table.shape().size() != 2 || table.shape(0) != lengths.shape(0)) throw InvalidArgumentError("invalid table");
   require_list(starts, lengths.shape(0) + 1, "invalid starts");
   if (window > 0 && !causal) throw InvalidArgumentError("invalid window");
   require_rocm();
   Variable<float> out(q.shape());
-  tfcc_rocm_paged_attention_desc d{};
-  d.cache = held_by(cache);
   d.q = q.data();
   d.out = out.data();
   d.q_head_stride = d.out_head_stride = q.shape(2);
