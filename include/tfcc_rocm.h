@@ -584,6 +584,8 @@ int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const
  * starts[batch] on are left as they were, and a key on a page outside the cache or behind the table is not seen.  max_length: an
  * upper bound of lengths[] that the host knows (0: table_width * page_size): how the work is split follows it; keys behind it are not seen.
  * workspace: tfcc_rocm_paged_attention_workspace() bytes, 16-byte aligned, of any contents, not in use by another call at the same time.
+ * tokens * heads < 2^31, and no more workgroups than one launch takes: a chunk has one for every 16 rows (token, query head) of a
+ * cache head, or part of 16, and 2^24 - 1 are the most.
  * Products are exact to float32 whatever the cache's type, but for parts of a row that lie 2^-30 below its largest value, which may be
  * lost.  out overlaps no input. */
 typedef struct tfcc_rocm_paged_attention_desc {

@@ -1492,6 +1492,18 @@ PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
                               d.cache.type == TFCC_ROCM_F32);
 }
 
+// Checks a call and deals it out; one without tokens or sequences has nothing to deal out.
+int plan_call(const tfcc_rocm_paged_attention_desc& d, PagedAttentionPlan& plan) {
+  if (int e = check_attention(d)) return e;
+  if (d.tokens == 0 || d.batch == 0) return TFCC_ROCM_OK;
+  plan = plan_of(d);
+  // a launch takes 2^32 - 1 threads; pieces, whose join has a workgroup for each row, are made of fewer rows than that is for
+  const uint64_t groups = (uint64_t)plan.tiles * plan.splits * d.cache.heads;
+  TFCC_REQUIRE(groups * plan.waves * 64 <= 0xffffffffu && (plan.splits == 1 || (uint64_t)d.tokens * d.heads * kThreads <= 0xffffffffu),
+               "paged_attention: %llu workgroups of %u threads", (unsigned long long)groups, plan.waves * 64);
+  return TFCC_ROCM_OK;
+}
+
 size_t workspace_of(const tfcc_rocm_paged_attention_desc& d, const PagedAttentionPlan& plan) {
   return plan.splits == 1 ? 0 : (size_t)plan.splits * d.tokens * d.heads * (d.cache.size + 2) * sizeof(float);
 }
@@ -1504,22 +1516,21 @@ using namespace tfcc_rocm;
 extern "C" {
 
 size_t tfcc_rocm_paged_attention_workspace(const tfcc_rocm_paged_attention_desc* desc) {
-  if (desc == nullptr || check_attention(*desc) != TFCC_ROCM_OK || desc->tokens == 0 || desc->batch == 0) return 0;
-  return workspace_of(*desc, plan_of(*desc));
+  PagedAttentionPlan plan;
+  if (desc == nullptr || plan_call(*desc, plan) != TFCC_ROCM_OK || desc->tokens == 0 || desc->batch == 0) return 0;
+  return workspace_of(*desc, plan);
 }
 
 int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_desc* desc) {
   TFCC_REQUIRE(desc != nullptr, "paged_attention: null descriptor");
   const tfcc_rocm_paged_attention_desc& d = *desc;
-  if (int e = check_attention(d)) return e;
+  PagedAttentionPlan plan;
+  if (int e = plan_call(d, plan)) return e;
   if (d.tokens == 0 || d.batch == 0) return TFCC_ROCM_OK;
   TFCC_REQUIRE(d.q && d.out && d.starts && d.lengths && (d.table || d.table_width == 0), "paged_attention: null argument");
-  const PagedAttentionPlan plan = plan_of(d);
   const size_t needs = workspace_of(d, plan);
   TFCC_REQUIRE(needs == 0 || (d.workspace != nullptr && d.workspace_bytes >= needs), "paged_attention: a workspace of %zu bytes where %zu are needed",
                d.workspace == nullptr ? (size_t)0 : d.workspace_bytes, needs);
-  const uint64_t groups = (uint64_t)plan.tiles * plan.splits * d.cache.heads;
-  TFCC_REQUIRE(groups <= 0x7fffffffu / 512 && (uint64_t)d.tokens * d.heads <= 0x7fffffffu / kThreads, "paged_attention: %u tiles of rows", plan.tiles);
   AttentionArgs a{};
   a.cache = view_of(d.cache);
   a.q = d.q;
@@ -1547,7 +1558,7 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
   a.statistics = static_cast<float*>(d.workspace) + (size_t)plan.splits * d.tokens * d.heads * d.cache.size;
   a.partial = static_cast<float*>(d.workspace);
   const hipStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)groups);
+  const dim3 grid(plan.tiles * plan.splits * d.cache.heads);
   const tfcc_rocm_paged_cache& c = d.cache;
   const unsigned blocks = (c.size + 63) / 64;
   if (plan.rows != kAttentionRows && c.type == TFCC_ROCM_F32) {
