@@ -665,9 +665,14 @@ __device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
 // A row of a float32 cache is two fp16 pieces under a power of two of its own, which is its scale as an int8 row's is: what is said above of
 // int8 holds, with a third operation for the product of the first factor's large piece with the second's small one.  The two
 // small ones' product is 2^-24 of the whole and left out.  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
-// one by one.
+// one by one.  Weights and scores have float32's exponents to stay in, so numbers from 2^80 on go that way too, and what undoes a value row's power of
+// two is taken 2^kLift times, which the results are freed of: these scales lie between 2^-78 and 2^102.  A weight that brings the largest scale to
+// the frame's 2^8 is 2^-94, those 2^-30 below it are normal numbers, and one that brings the smallest to 2^15 is 2^93, of which 2^34 can be summed.
+constexpr unsigned kFar = 0x67800000u;  // 2^80
+constexpr int kLift = 36;
+
 // The wavefront's 32 rows of a float32 cache by the definition, in float32: lanes take keys for the scores and values of the head for the sums.
-// Only rows that see an infinity or a NaN are written.
+// Only rows that see a number of kFar or above are written.
 template <int BLOCKS>
 __device__ __forceinline__ void rows_one_by_one(const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, int begin, int end, const int* table,
                                                           const float* keys, const float* values) {
@@ -688,7 +693,7 @@ __device__ __forceinline__ void rows_one_by_one(const AttentionArgs& p, const Ti
     float m = -INFINITY, l = 0.0f, out[BLOCKS] = {};
     bool odd = false;
     const auto look_at = [&](float v) {
-      odd |= (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
+      odd |= (__float_as_uint(v) & 0x7fffffffu) >= kFar;
       return v;
     };
 #pragma unroll 1
@@ -876,7 +881,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
   // float32: the power of two that brings a row's largest value to 2^13 .. 2^14, and the row's pieces.  What is read together and written together
   // of the keys lies in different banks.
   const auto exchange = [](unsigned lane_of, unsigned step) { return lane_of ^ (lane_of / 32 * 4) ^ (WAVES == 8 ? step % 2 * 2 : 0); };
-  bool odd = false;  // an infinity or a NaN was among what some row sees
+  bool odd = false;  // a number of kFar or above was among what some row sees
   const auto store_f32 = [&](Stage& s, int at) {
     const auto larger = [](unsigned a, unsigned b) { return a > b ? a : b; };
     const auto size_of = [&](unsigned v) { return v & 0x7fffffffu; };
@@ -894,14 +899,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
     for (int b = 0; b < 4; ++b)
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = larger(most, size_of(raw[b][i]));
-    if (__any(most >= 0x7f800000u)) {  // rare; for the rows that do not see it, as zeros, which change nothing
+    if (__any(most >= kFar)) {  // rare; for the rows that do not see it, as zeros, which change nothing
       odd = true;
       most = 0;
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          raw[b][i] = size_of(raw[b][i]) >= 0x7f800000u ? 0u : raw[b][i];
+          raw[b][i] = size_of(raw[b][i]) >= kFar ? 0u : raw[b][i];
           most = larger(most, size_of(raw[b][i]));
         }
     }
@@ -945,8 +950,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
       for (int j = 1; j < 8; ++j) e = word == (unsigned)j ? exponent[j] : e;
       if (word < 8) {
         const unsigned key = group / 2 * 16 + 4 * (group % 2) + 8 * (word / 4) + word % 4;
-        s.value_scale[key] = power(e - 14);
-        s.value_log[key] = fmaxf((float)(e - 14), -90.0f);  // as of frame_log()
+        s.value_scale[key] = power(e - 14 + kLift);
+        s.value_log[key] = (float)(e - 14 + kLift);
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -1093,6 +1098,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
   if (t.row_token >= 0) {
     const unsigned long long token = t.first + t.row_token, query_head = head * p.group.d + t.row_head;
     float* to = p.out + token * p.out_token + query_head * p.out_head;
+    if constexpr (!S8) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) o[n] *= power(-kLift);
+    }
     float factor = 1.0f;
     if (p.splits > 1) {
       const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
