@@ -69,7 +69,7 @@ __constant__ double kPowers[32] = {
 
 // What the weights of a row's logits follow from.  exp((x - top) / temperature) * 2^shift is 2^(e + shift) 2^(j / 32) e^f with |f| <= ln 2 / 64
 // and the Taylor polynomial of e^f to the fifth power, whose rest is below 3e-15 of it; the 32 powers, with 2^shift in them, lie in LDS.
-// Below `cutoff` a weight is 2^-2 at most, the integer 0: it is taken for 0, and so is that of a NaN or of -infinity.
+// Below `cutoff` a weight is less than 2^-2, the integer 0: it is taken for 0, and so is that of a NaN or of -infinity.  From there on e is -64 or more.
 struct Row {
   float top, slope, cutoff;
   double steps;  // of ln 2 / 32 in a logit
@@ -93,8 +93,9 @@ struct Row {
 __device__ Row row_of(float top, float temperature, int shift, double* powers) {  // powers: 32 in LDS, filled here; the caller waits
   if (threadIdx.x < 32) powers[threadIdx.x] = ldexp(kPowers[threadIdx.x], shift);
   const double slope = 1.0 / (double)temperature, least = -0.6931471805599453 * (shift + 2);
-  float cutoff = fmaxf((float)fmax((double)top + least / slope, -3.4028234663852886e38), -3.402823466e38f);
-  if (((double)cutoff - (double)top) * slope > least && cutoff < INFINITY) cutoff = fmaxf(value_of(key_of(cutoff) - 1), -3.402823466e38f);  // rounded up
+  // the lowest float whose weight is 2^-2 or more: the one below may be any number of e-foldings away
+  float cutoff = top == INFINITY ? INFINITY : fmaxf((float)fmax((double)top + least / slope, -3.4028234663852886e38), -3.402823466e38f);
+  if (((double)cutoff - (double)top) * slope < least) cutoff = value_of(key_of(cutoff) + 1);
   return {top, (float)slope, cutoff, slope * 46.166241308446828384, shift, powers};
 }
 // to the nearest integer, below 2^52
