@@ -110,7 +110,7 @@ int tfcc_rocm_rotary_frequencies(unsigned part, double base, int scaling, double
   if (scaling == TFCC_ROCM_ROTARY_INDEX) {
     const auto index_of = [&](double turns) { return part * log(original_length / (turns * pi2)) / (2 * log(base)); };
     first = fmax(0.0, floor(index_of(high)));
-    last = fmin(part / 2 - 1.0, ceil(index_of(low)));
+    last = ceil(index_of(low));  // behind the last pair where that makes more than `low` turns
     if (last <= first) last = first + 0.001;
   }
   for (unsigned i = 0; i < part / 2; ++i) {
