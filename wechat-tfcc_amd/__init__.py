@@ -1117,10 +1117,13 @@ def _on_device(device, *tensors):
         raise InvalidArgumentError("tensors are not on the current device")
 
 
+_MOST = 0x7fffffff  # of a dimension or a count: the fields of a call have 32 bits
+
+
 def _heads_of(t, name):
     """[tokens, heads, size] of float32 whose heads are contiguous."""
     import torch
-    if t.dim() != 3 or t.dtype != torch.float32:
+    if t.dim() != 3 or t.dtype != torch.float32 or max(t.shape) > _MOST:
         raise InvalidArgumentError("invalid " + name)
     return t if t.shape[2] <= 1 or t.stride(2) == 1 else t.contiguous()
 
@@ -1181,7 +1184,7 @@ def _cache_desc(cache):
         raise InvalidArgumentError("invalid cache")
     keys, values = cache[0], cache[1]
     s8 = len(cache) == 4
-    if keys.dim() != 4 or keys.dtype != (torch.int8 if s8 else torch.float32) or keys.numel() == 0:
+    if keys.dim() != 4 or keys.dtype != (torch.int8 if s8 else torch.float32) or keys.numel() == 0 or max(keys.shape) > _MOST:
         raise InvalidArgumentError("invalid cache keys")
     if values.shape != keys.shape or values.dtype != keys.dtype or values.stride() != keys.stride() or keys.stride(3) != 1:
         raise InvalidArgumentError("invalid cache values")
@@ -1234,7 +1237,7 @@ def cache_write(cache, keys, values, slots):
 
 def _table_of(table, batch, name):
     import torch
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != batch:
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != batch or max(table.shape) > _MOST:
         raise InvalidArgumentError("invalid " + name)
     return table if table.shape[1] <= 1 or table.stride(1) == 1 else table.contiguous()
 
@@ -1251,7 +1254,7 @@ def cache_read(cache, table, starts, tokens):
     _on_device(cache[0].device, table, starts)
     table = _table_of(table, table.shape[0], "table")
     starts = _integers(starts, "starts", table.shape[0] + 1, (torch.int32,))
-    if tokens < 0:
+    if not 0 <= tokens <= _MOST:
         raise InvalidArgumentError("invalid tokens")
     keys, values = (torch.empty((tokens, d.heads, d.size), dtype=torch.float32, device=table.device) for _ in range(2))
     check(lib().tfcc_rocm_cache_read(_stream(), C.byref(d), _ptr(table), table.stride(0), table.shape[1], table.shape[0], _ptr(starts),
@@ -1289,7 +1292,8 @@ def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window
     d.q_token_stride, d.q_head_stride, d.out_token_stride, d.out_head_stride = q.stride(0), q.stride(1), out.stride(0), out.stride(1)
     d.tokens, d.heads, d.batch = q.shape[0], q.shape[1], batch
     d.starts, d.lengths, d.table, d.table_stride, d.table_width = _ptr(starts), _ptr(lengths), _ptr(table), table.stride(0), table.shape[1]
-    d.max_length, d.scale, d.causal, d.window = max_length, scale, 1 if causal else 0, window
+    # no sequence is longer than the largest that their fields hold: a larger bound or window is the same as that
+    d.max_length, d.scale, d.causal, d.window = min(max_length, _MOST), scale, 1 if causal else 0, min(window, _MOST)
     if q.shape[0] == 0 or batch == 0:
         return out
     needs = lib().tfcc_rocm_paged_attention_workspace(C.byref(d))
@@ -1307,7 +1311,7 @@ def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None)
     if done is not None:
         return done
     import torch
-    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[1] == 0:
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.shape[1] == 0 or max(logits.shape) > _MOST:
         raise InvalidArgumentError("invalid logits")
     _on_device(logits.device, random, temperature, top_k, top_p, min_p)
     rows, length = logits.shape
