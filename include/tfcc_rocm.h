@@ -566,7 +566,8 @@ typedef struct tfcc_rocm_paged_cache {
   uint64_t scale_page_stride, scale_head_stride, scale_row_stride;
 } tfcc_rocm_paged_cache;
 /* Token i's keys and values [tokens, heads, size] go to slot slots[i] (TFCC_ROCM_S32 or S64); a slot outside the cache (-1 for a
- * padded token) is skipped.  Two tokens of one call must not name the same slot: its contents are then unspecified. */
+ * padded token) is skipped.  Two tokens of one call must not name the same slot: its contents are then unspecified.  A cache stride of 0 over
+ * more than one page, head or row is refused. */
 int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, const float* keys, uint64_t key_token_stride,
                           uint64_t key_head_stride, const float* values, uint64_t value_token_stride,
                           uint64_t value_head_stride, unsigned tokens, const void* slots, int slot_type);

@@ -176,6 +176,12 @@ int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, cons
   if (int e = check_cache(*cache, "cache_write")) return e;
   TFCC_REQUIRE(slot_type == TFCC_ROCM_S32 || slot_type == TFCC_ROCM_S64, "cache_write: slot type %d", slot_type);
   if (tokens == 0) return TFCC_ROCM_OK;
+  // memory that several rows share can be read, but not written
+  TFCC_REQUIRE((cache->pages == 1 || cache->page_stride > 0) && (cache->heads == 1 || cache->head_stride > 0) && (cache->page_size == 1 || cache->row_stride > 0),
+               "cache_write: a cache stride of 0");
+  TFCC_REQUIRE(cache->type != TFCC_ROCM_S8 || ((cache->pages == 1 || cache->scale_page_stride > 0) && (cache->heads == 1 || cache->scale_head_stride > 0) &&
+                                               (cache->page_size == 1 || cache->scale_row_stride > 0)),
+               "cache_write: a cache scale stride of 0");
   TFCC_REQUIRE(keys && values && slots, "cache_write: null argument");
   TFCC_REQUIRE((uint64_t)tokens * cache->heads <= 0x7fffffffu, "cache_write: %u tokens of %u heads", tokens, cache->heads);
   WriteArgs a{view_of(*cache), keys, values, key_token_stride, key_head_stride, value_token_stride, value_head_stride, slots,
