@@ -537,7 +537,7 @@ enum {
 int tfcc_rocm_rotary_frequencies(unsigned part, double base, int scaling, double factor, unsigned original_length, double low,
                                  double high, double* frequencies, float* magnitude);
 /* Up to two tensors [tokens, heads, size] (queries and keys) in one launch; in[1] NULL: one.  out[i] is in[i] with the same strides, or
- * memory that overlaps neither input.  size <= 1024. */
+ * memory that overlaps neither input.  size <= 1024, tokens < 2^24. */
 typedef struct tfcc_rocm_rotary_desc {
   const float* in[2];
   float* out[2];
@@ -567,13 +567,14 @@ typedef struct tfcc_rocm_paged_cache {
 } tfcc_rocm_paged_cache;
 /* Token i's keys and values [tokens, heads, size] go to slot slots[i] (TFCC_ROCM_S32 or S64); a slot outside the cache (-1 for a
  * padded token) is skipped.  Two tokens of one call must not name the same slot: its contents are then unspecified.  A cache stride of 0 over
- * more than one page, head or row is refused. */
+ * more than one page, head or row is refused.  tokens * heads: up to 2^28 - 16 with a size of
+ * up to 64, 2^27 - 8 up to 128, 2^26 - 4 above. */
 int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, const float* keys, uint64_t key_token_stride,
                           uint64_t key_head_stride, const float* values, uint64_t value_token_stride,
                           uint64_t value_head_stride, unsigned tokens, const void* slots, int slot_type);
 /* The first starts[i + 1] - starts[i] tokens of each sequence, back to back: rows starts[i] .. of dense keys and values [tokens, heads, size].
  * table [batch, table_width], row stride table_stride: the pages of each sequence in order.  starts [batch + 1], ascending from 0.
- * Rows from starts[batch] on are left as they were; rows on a page outside the cache or behind the table are zeros. */
+ * Rows from starts[batch] on are left as they were; rows on a page outside the cache or behind the table are zeros.  tokens: up to 2^26 - 4. */
 int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const int32_t* table, uint64_t table_stride,
                          unsigned table_width, unsigned batch, const int32_t* starts, unsigned tokens, float* keys,
                          float* values);

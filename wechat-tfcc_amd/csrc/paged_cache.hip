@@ -182,19 +182,21 @@ int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, cons
   TFCC_REQUIRE(cache->type != TFCC_ROCM_S8 || ((cache->pages == 1 || cache->scale_page_stride > 0) && (cache->heads == 1 || cache->scale_head_stride > 0) &&
                                                (cache->page_size == 1 || cache->scale_row_stride > 0)),
                "cache_write: a cache scale stride of 0");
+  // threads of a launch: whole workgroups
+  const unsigned lanes = cache->size <= 64 ? 16 : cache->size <= 128 ? 32 : 64;
+  TFCC_REQUIRE((uint64_t)tokens * cache->heads * lanes <= 0xffffffffu - (kCacheThreads - 1), "cache_write: %u tokens of %u heads", tokens, cache->heads);
   TFCC_REQUIRE(keys && values && slots, "cache_write: null argument");
-  TFCC_REQUIRE((uint64_t)tokens * cache->heads <= 0x7fffffffu, "cache_write: %u tokens of %u heads", tokens, cache->heads);
   WriteArgs a{view_of(*cache), keys, values, key_token_stride, key_head_stride, value_token_stride, value_head_stride, slots,
               slot_type == TFCC_ROCM_S64, tokens, tokens * cache->heads, Divisor::of(cache->heads)};
   const hipStream_t s = as_stream(stream);
   const bool s8 = cache->type == TFCC_ROCM_S8;
-  const auto start = [&](auto kernel, unsigned lanes) {
+  const auto start = [&](auto kernel) {
     const unsigned rows = kCacheThreads / lanes;
     hipLaunchKernelGGL(kernel, dim3((a.rows + rows - 1) / rows, 2), dim3(kCacheThreads), 0, s, a);
   };
-  if (cache->size <= 64) start(s8 ? cache_write_kernel<true, 16> : cache_write_kernel<false, 16>, 16);
-  else if (cache->size <= 128) start(s8 ? cache_write_kernel<true, 32> : cache_write_kernel<false, 32>, 32);
-  else start(s8 ? cache_write_kernel<true, 64> : cache_write_kernel<false, 64>, 64);
+  if (lanes == 16) start(s8 ? cache_write_kernel<true, 16> : cache_write_kernel<false, 16>);
+  else if (lanes == 32) start(s8 ? cache_write_kernel<true, 32> : cache_write_kernel<false, 32>);
+  else start(s8 ? cache_write_kernel<true, 64> : cache_write_kernel<false, 64>);
   return check_launch("cache_write");
 }
 
@@ -204,8 +206,9 @@ int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const
   TFCC_REQUIRE(cache != nullptr, "cache_read: null cache");
   if (int e = check_cache(*cache, "cache_read")) return e;
   if (tokens == 0 || batch == 0) return TFCC_ROCM_OK;
+  TFCC_REQUIRE((uint64_t)tokens * (kCacheThreads / kReadTokens) <= 0xffffffffu - (kCacheThreads - 1) && batch <= 0x7fffffffu,  // threads of a launch, as above
+               "cache_read: %u tokens of %u sequences", tokens, batch);
   TFCC_REQUIRE(table && starts && keys && values, "cache_read: null argument");
-  TFCC_REQUIRE(tokens <= 0x7fffffffu && batch <= 0x7fffffffu, "cache_read: %u tokens of %u sequences", tokens, batch);
   ReadArgs a{view_of(*cache), table, table_stride, table_width, batch, starts, tokens, keys, values};
   const hipStream_t s = as_stream(stream);
   const bool s8 = cache->type == TFCC_ROCM_S8;

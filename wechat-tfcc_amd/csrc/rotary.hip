@@ -131,7 +131,7 @@ int tfcc_rocm_rotary_f32(void* stream, const tfcc_rocm_rotary_desc* desc) {
   TFCC_REQUIRE(d.size > 0 && d.size <= kRotaryMost, "rotary: heads of %u values (1 to %u)", d.size, kRotaryMost);
   TFCC_REQUIRE(d.part >= 2 && d.part % 2 == 0 && d.part <= d.size, "rotary: part %u of heads of %u values", d.part, d.size);
   TFCC_REQUIRE(d.position_type == TFCC_ROCM_S32 || d.position_type == TFCC_ROCM_S64, "rotary: position type %d", d.position_type);
-  TFCC_REQUIRE(d.tokens <= 0x7fffffffu, "rotary: %u tokens", d.tokens);
+  TFCC_REQUIRE((uint64_t)d.tokens * kRotaryThreads <= 0xffffffffu, "rotary: %u tokens", d.tokens);  // of a launch
   TFCC_REQUIRE(d.in[1] != nullptr || d.out[1] == nullptr, "rotary: a second result without a second input");
   if (d.tokens == 0) return TFCC_ROCM_OK;
   TFCC_REQUIRE(d.in[0] && d.out[0] && d.positions && d.frequencies, "rotary: null argument");
