@@ -26,3 +26,11 @@ def test_index_ramp(pkg, part, base, length, low, high, factor):
     assert np.allclose(f, plain * (1 - ramp) + plain / factor * ramp, rtol=1e-13)
     if last >= part // 2:  # more than `low` turns: not yet the full factor
         assert f[-1] > plain[-1] / factor * 1.01
+
+
+@pytest.mark.parametrize("kw", [dict(part=2 ** 32 + 64), dict(part=-2 ** 32 + 64), dict(part=-2), dict(original_length=2 ** 32 + 64), dict(original_length=-2 ** 31)])
+def test_numbers_beyond_32_bits_are_refused(pkg, kw):
+    """A length of 2^32 + 64 is not one of 64."""
+    with pytest.raises(pkg.InvalidArgumentError):
+        pkg.rotary_frequencies(**{"part": 64, "scaling": "turns", "factor": 8.0, "original_length": 4096, **kw})
+    pkg.rotary_frequencies(64, scaling="turns", factor=8.0, original_length=2 ** 32 - 1)

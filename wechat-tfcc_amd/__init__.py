@@ -1100,6 +1100,10 @@ def rotary_frequencies(part, base=10000.0, scaling="plain", factor=1.0, original
     tensor of the list once.  scaling: one of ROTARY_SCALINGS."""
     if scaling not in ROTARY_SCALINGS:
         raise InvalidArgumentError("invalid scaling")
+    if not 0 < part <= 1024:
+        raise InvalidArgumentError("invalid part")
+    if not 0 <= original_length <= 0xffffffff:
+        raise InvalidArgumentError("invalid original_length")
     f, magnitude = (C.c_double * max(1, part // 2))(), C.c_float()
     if lib().tfcc_rocm_rotary_frequencies(part, base, ROTARY_SCALINGS[scaling], factor, original_length, low, high, f,
                                           C.byref(magnitude)):
