@@ -40,3 +40,31 @@ def test_infinite_logits_at_all_temperatures(pkg, T, filters):
     kw = dict(top_k=np.full(rows, 30, np.int32), top_p=np.full(rows, 0.99, np.float32), min_p=np.full(rows, 0.5, np.float32))
     got, odds = pkg.sample(T.t(logits), T.t(np.linspace(0, 0.999, rows, dtype=np.float32)), temperature=T.t(temperature), **{k: T.t(kw[k]) for k in filters})
     assert np.array_equal(T.n(got), np.where(np.arange(rows) < rows / 2, 11, 1500)) and (T.n(odds) == 0.5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("least", [1e-3, 1e-7, 1e-12, 1e-30, 1e-44])
+@pytest.mark.parametrize("size", [1.0, 100.0, 1e30, 1e-30])
+def test_small_least_weights(pkg, T, least, size):
+    """How near a row comes to another choice is measured against the least weight itself, so that rows are compared however small that is."""
+    rng = np.random.default_rng(23)
+    rows, length = 12, 5003
+    least = np.float32(least)
+    logits = (rng.normal(size=(rows, length)) * size * 3).astype(np.float32)
+    temperature = (np.linspace(0.05, 3.0, rows) * size).astype(np.float32)
+    random = rng.random(rows).astype(np.float32)
+    got, odds = (T.n(t) for t in pkg.sample(T.t(logits), T.t(random), temperature=T.t(temperature), min_p=T.t(np.full(rows, least))))
+    compared = 0
+    for r in range(rows):
+        x = logits[r].astype(np.float64)
+        w = np.exp((x - x.max()) / float(temperature[r]))
+        kept = np.where(w >= float(least), w, 0)
+        sums = kept.cumsum()
+        goal = float(random[r]) * sums[-1]
+        # weights in 64 bits are off by 2^-48 and less; sums of integers of 2^-51 of the largest by 5003 halves of those
+        if (np.abs(w - float(least)) < 1e-10 * float(least)).any() or (np.abs(sums - goal) < 1e-9 * sums[-1]).any():
+            continue
+        compared += 1
+        at = int((sums <= goal).sum())
+        assert got[r] == at and abs(odds[r] - kept[at] / sums[-1]) <= 2.0 ** -23 * kept[at] / sums[-1]
+    assert compared >= rows - 1
