@@ -530,7 +530,7 @@ enum {
   /* each pair between its plain frequency and that divided by factor: plain * (r + (1 - r) / factor), where r grows from 0 to 1 */
   TFCC_ROCM_ROTARY_TURNS = 3,  /* ... with the turns a pair makes over original_length, from `low` to `high` of them */
   TFCC_ROCM_ROTARY_INDEX = 4   /* ... with the pair's index, from where it makes `high` turns down to 0 where it makes `low`, rounded
-                                * outwards to whole indices; *magnitude = 0.1 ln(factor) + 1 (elsewhere 1) */
+                                * outwards to whole indices; *magnitude = 0.1 ln(factor) + 1 for factors above 1 (elsewhere 1) */
 };
 /* frequencies: part / 2 doubles in HOST memory, to be copied to the device once; magnitude may be NULL.  original_length, low and
  * high are read by TURNS and INDEX only (0 < low < high), factor (> 0) by all but PLAIN. */

@@ -34,3 +34,9 @@ def test_numbers_beyond_32_bits_are_refused(pkg, kw):
     with pytest.raises(pkg.InvalidArgumentError):
         pkg.rotary_frequencies(**{"part": 64, "scaling": "turns", "factor": 8.0, "original_length": 4096, **kw})
     pkg.rotary_frequencies(64, scaling="turns", factor=8.0, original_length=2 ** 32 - 1)
+
+
+@pytest.mark.parametrize("factor,magnitude", [(0.5, 1.0), (1.0, 1.0), (1.5, 0.1 * math.log(1.5) + 1)])
+def test_magnitude(pkg, factor, magnitude):
+    got = pkg.rotary_frequencies(64, scaling="index", factor=factor, original_length=4096)[1]
+    assert math.isclose(got, magnitude, rel_tol=2.0 ** -24) and (got == 1.0 or factor > 1)
