@@ -66,7 +66,7 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
     if (splits > 8) splits = 8;
   } else if (wide) {
     p.waves = 4;
-    splits = keys >= 2048 && groups < (size <= 128 ? 384 : 192) ? 2 : 1;  // two share a CU, of heads wider than 128 one has it
+    splits = keys >= 2048 && groups < 384 && size <= 128 ? 2 : 1;  // two share a CU; of heads wider than 128 one has it, and they are enough
   } else if (groups > 0 && groups < 256) {
     // Fewer than CUs: pieces of the keys, where they save more steps than the launch that joins them costs (int8: 16 sequences of 4096, two
     // pieces 30 us, one 40; one of 1024: four 12.4, one 14.4; 2 of 938, 24 heads over 4 of 96: four 11.8, one 13.6; one of 777, 12 heads of 64:
