@@ -2,7 +2,7 @@
 // the running maximum and sum of each row.
 //
 // The query heads of a token that share a cache head are rows of one product: row r of a sequence is token r / group, head r % group, and
-// a tile holds 16 rows.  Both products run transposed on the matrix cores, with a row in each column:
+// a tile holds 16 rows, or 128 or 256 of chunks of many tokens.  Both products run transposed on the matrix cores, with a row in each column:
 //   S^T = K Q^T   (16 keys x 16 rows): lane l holds row l % 16 and keys 4 (l / 16) + i, i < 4
 //   O^T = V^T P^T (16 values x 16 rows)
 // so a row's maximum, sum and scale sit in the lanes that hold its scores, and the scores are where the second product wants its
@@ -10,7 +10,7 @@
 // exchanged between lanes but two steps of the row maximum.  V is loaded as it lies, row by row; which column of the
 // product stands for which value of a head is free as well and follows the loads.
 //
-// An int8 cache keeps float32 accuracy: an int8 is exact in fp16, a float32 is the sum of two but for 2^-24 of it, so each product is two
+// An int8 cache keeps float32 accuracy: an int8 is exact in fp16, a float32 is the sum of two but for 2^-23 of it, so each product is two
 // fp16 matrix operations.  Queries are scaled by a power of two for each row.  What meets the values is a weight times a value's scale, and
 // what has to stay in fp16's range is that product, not the weight: a row's weights are 2^(score - frame), and the frame moves where
 // score + log2(scale) exceeds it by 15, to 8 below.  Between moves nothing is rescaled, and what fp16 cannot hold is 2^-32 of
@@ -222,7 +222,7 @@ __device__ __forceinline__ f16x8 eight_of(const unsigned (&w)[8]) {
   return h.v;
 }
 
-// float32 as the sum of two fp16, both to the nearest: the error is at most 2^-24 of the value, or half of fp16's smallest number, 2^-25
+// float32 as the sum of two fp16, both to the nearest: the second is 2^-11 of the value at most and the error 2^-23, or half of fp16's smallest number, 2^-25
 __device__ __forceinline__ void split_two(float a, float b, f16x2& hi, f16x2& lo) {
   hi = __builtin_convertvector(f32x2{a, b}, f16x2);
   lo = __builtin_convertvector(f32x2{fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b)}, f16x2);
@@ -664,7 +664,8 @@ __device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
 
 // A row of a float32 cache is two fp16 pieces under a power of two of its own, which is its scale as an int8 row's is: what is said above of
 // int8 holds, with a third operation for the product of the first factor's large piece with the second's small one.  The two
-// small ones' product is 2^-24 of the whole and left out.  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
+// small ones' product, 2^-22 of the whole at most and 2^-25 in the mean, is left out: with the pieces' own 2^-23 each a term is right to 2^-21, where the
+// fp32 operations, at five times their cost, round to 2^-24 (6 chunks of 517 with a window: 4.9e-7 from 64 bits, elementary float32 operations 4.4e-7).  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
 // one by one.  Weights and scores have float32's exponents to stay in, so numbers from 2^80 on go that way too, and what undoes a value row's power of
 // two is taken 2^kLift times, which the results are freed of: these scales lie between 2^-78 and 2^102.  A weight that brings the largest scale to
 // the frame's 2^8 is 2^-94, those 2^-30 below it are normal numbers, and one that brings the smallest to 2^15 is 2^93, of which 2^34 can be summed.

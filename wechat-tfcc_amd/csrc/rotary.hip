@@ -4,7 +4,8 @@
 // 2.4 us).  The angles are those of a token, not of a head: a workgroup takes one token, forms the
 // sines and cosines of its part / 2 pairs once in LDS and runs over its share of the heads.  The angle is a product in 64 bits,
 // reduced to a fraction of a turn there: position 10^6 at one radian a position loses 2^-33 of a radian, where float32 would be
-// off by 0.06.  Sine and cosine of the fraction are float32.
+// off by 0.06.  The fraction and its sine and cosine are float32: it is off by 2^-26 of a turn at most, 0.8 of a unit in the last place of what it turns
+// (4096 tokens at far positions: 5.9e-8 from 64 bits, with angles rounded to nothing less than that 4.2e-8).
 #include <math.h>
 
 #include "common.hpp"
