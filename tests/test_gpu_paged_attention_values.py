@@ -105,3 +105,57 @@ def test_one_large_row_among_others(pkg, T, shape):
             off = 60 * R.EPS * np.abs(want) + (length + 60) * R.EPS * 8
         assert (np.abs(got - want) <= off)[mine].all()
         m.cache[c][page, 1, inside] = before
+
+
+# float32, tiles of 128 and 256 rows; rows, windows and pages that end inside a step of 16 keys
+FAR = [
+    ([300, 270], [258, 260], 64, 32, 64, 16, {}),
+    ([310, 270], [258, 260], 64, 32, 40, 20, {"window": 70}),
+    ([300, 290], [300, 290], 32, 16, 128, 20, {"window": 100}),
+    ([500, 333], [300, 290], 48, 16, 96, 24, {"causal": False}),
+    ([3000, 300], [200, 111], 32, 8, 128, 20, {}),          # pieces
+    ([2700, 2100], [300, 260], 32, 32, 64, 28, {"window": 2300}),
+    ([400, 200, 90], [260, 280, 90], 48, 48, 96, 16, {}),   # more tokens than are cached
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(FAR)))
+@pytest.mark.parametrize("value", [np.inf, np.nan, 1e30, -3e38])
+def test_far_numbers_here_and_there(pkg, T, case, value):
+    """Some value rows and keys with an infinity, a NaN or a number beyond 2^80, pages that are nowhere: rows that see one are those of the definition, all
+    others keep every bit."""
+    lengths, chunks, heads, kv, size, page, more = FAR[case]
+    m = Made(pkg, "f32", lengths, chunks, heads, kv, size, page, 71 + case)
+    m.table[0, 2] = -1
+    m.table[0, -2] = len(m.cache[0])
+    clean = T.n(m.run(T, **more)).copy()
+    group = heads // kv
+    mine = np.zeros(clean.shape, bool)
+    for i, (at, head) in enumerate([(lengths[0] // 2, 1), (lengths[0] - 2, 0), (lengths[1] - 70, 1), (lengths[1] // 2 + 3, kv - 1), (lengths[0] // 3, kv - 1)]):
+        sequence = 1 if i in (2, 3) else 0
+        named, inside = m.table[sequence, at // page], at % page
+        if not 0 <= named < len(m.cache[0]):
+            continue
+        # a key takes part as a zero times that number: nothing of it is in a score, but it is there
+        c = 0 if i == 1 and np.isfinite(value) else 1
+        m.cache[c][named, head, inside, 5] = value
+        if c == 0:
+            m.q[:, :, 5] = 0
+            clean = None
+        n = chunks[sequence]
+        position = lengths[sequence] - n + np.arange(n)
+        sees = (at <= position) & (at > position - more.get("window", 10 ** 9)) if more.get("causal", True) else np.ones(n, bool)
+        mine[m.starts[sequence]:m.starts[sequence + 1], head * group:(head + 1) * group] |= sees[:, None, None]
+    got = T.n(m.run(T, **more)).astype(np.float64)
+    if clean is not None:
+        assert np.array_equal(got[~mine], clean[~mine])
+    want, off = R.attention(m.q, m.cache, m.table, m.starts, m.lengths, m.scale, **more)
+    off = np.where(np.isfinite(want), off, 0)
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        near = np.abs(got - want) <= off
+    # a weight below 2^-149 times infinity is NaN in float32 and infinity in 64 bits
+    lost = np.isinf(want) & np.isnan(got)
+    assert (same | near | lost).all() and not lost.all()
+    assert mine.any()

@@ -666,77 +666,280 @@ __device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
 // int8 holds, with a third operation for the product of the first factor's large piece with the second's small one.  The two
 // small ones' product, 2^-22 of the whole at most and 2^-25 in the mean, is left out: with the pieces' own 2^-23 each a term is right to 2^-21, where the
 // fp32 operations, at five times their cost, round to 2^-24 (6 chunks of 517 with a window: 4.9e-7 from 64 bits, elementary float32 operations 4.4e-7).  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
-// one by one.  Weights and scores have float32's exponents to stay in, so numbers from 2^80 on go that way too, and what undoes a value row's power of
+// once more by the fp32 operations (an infinity in the first page of every sequence: 4 chunks of 1024 over 4096 2530 us, with tiles of 16 rows 2060).  Weights and scores have float32's exponents to stay in, so numbers from 2^80 on go that way too, and what undoes a value row's power of
 // two is taken 2^kLift times, which the results are freed of: these scales lie between 2^-78 and 2^102.  A weight that brings the largest scale to
 // the frame's 2^8 is 2^-94, those 2^-30 below it are normal numbers, and one that brings the smallest to 2^15 is 2^93, of which 2^34 can be summed.
 constexpr unsigned kFar = 0x67800000u;  // 2^80
 constexpr int kLift = 36;
 
-// The wavefront's 32 rows of a float32 cache by the definition, in float32: lanes take keys for the scores and values of the head for the sums.
-// Only rows that see a number of kFar or above are written.
-template <int BLOCKS>
-__device__ __forceinline__ void rows_one_by_one(const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, int begin, int end, const int* table,
-                                                          const float* keys, const float* values) {
-  const unsigned lane = threadIdx.x & 63, size = p.cache.size;
-  const auto row_at = [&](const float* held, int key) -> const float* {
-    const unsigned index = p.cache.page_size.quotient((unsigned)key);
-    const int page = page_of(p, table, index);
-    return page < 0 ? nullptr : held + (unsigned long long)page * p.cache.page + (key - index * p.cache.page_size.d) * p.cache.row;
+// Rows of a tile, 16 of them, over a float32 cache: the keys of steps kb, kb + STEP, ... below end, 16 in each.  The next step's keys are loaded into the registers
+// of this one's as soon as the scores are formed, its values once the weights have met them.  PAGES that the keys of a step may lie in: 1 (of a
+// multiple of 16 rows), 2 (16 rows at least) or any number, 0.  `missing`: a bit for each of the lane's four keys that no page holds.
+// o: value 64 b + 4 (4 g + i) + j of the row in o[b][j][i]; look: sees each step's rows as they were loaded.
+template <int BLOCKS, int STEP, int PAGES, class Look>
+__device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& t, unsigned head, int kb, int end, const int* table, f32x4 (&o)[BLOCKS][4],
+                                            float& m, float& l, Look look) {
+  constexpr int DPAD = 64 * BLOCKS;
+  const unsigned lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
+  const unsigned size = p.cache.size;
+  const float* const keys = static_cast<const float*>(p.cache.keys) + head * p.cache.head;
+  const float* const values = static_cast<const float*>(p.cache.values) + head * p.cache.head;
+
+  kb = __builtin_amdgcn_readfirstlane(kb);
+  end = __builtin_amdgcn_readfirstlane(end);
+  f32x4 k[4 * BLOCKS], v[4][BLOCKS];
+  unsigned missing = 0;
+  const auto inside_page = [&](unsigned key) { return key - p.cache.page_size.quotient(key) * p.cache.page_size.d; };
+  const auto locate = [&](int key, unsigned long long& row) {
+    const int page = page_of(p, table, p.cache.page_size.quotient((unsigned)key));
+    row = page < 0 ? 0 : page * p.cache.page + inside_page((unsigned)key) * p.cache.row;
+    return page >= 0;
   };
-#pragma unroll 1
-  for (int r = 0; r < 32; ++r) {
-    const int row_token = __builtin_amdgcn_readlane(t.row_token, r);
-    if (row_token < 0) return;
-    const int row_low = __builtin_amdgcn_readlane(t.row_low, r), row_high = __builtin_amdgcn_readlane(t.row_high, r);
-    const int low = row_low > begin ? row_low : begin, high = row_high < end ? row_high : end;
-    const unsigned long long token = t.first + row_token, query_head = head * p.group.d + __builtin_amdgcn_readlane(t.row_head, r);
-    const float* const q = p.q + token * p.q_token + query_head * p.q_head;
-    float m = -INFINITY, l = 0.0f, out[BLOCKS] = {};
-    bool odd = false;
-    const auto look_at = [&](float v) {
-      odd |= (__float_as_uint(v) & 0x7fffffffu) >= kFar;
-      return v;
-    };
-#pragma unroll 1
-    for (int kb = low; kb < high; kb += 64) {
-      const int key = kb + (int)lane;
-      const float* const row = key < high ? row_at(keys, key) : nullptr;
-      float s = 0.0f;
-      if (row != nullptr)
-#pragma unroll 1
-        for (unsigned d = 0; d < size; ++d) s += q[d] * look_at(row[d]);
-      s *= p.scale;
-      const float next = fmaxf(m, wave_max(row != nullptr ? s : -INFINITY)), f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-      m = next;
-      const float e = row != nullptr ? __builtin_amdgcn_exp2f(s - (m == -INFINITY ? 0.0f : m)) : 0.0f;
-      l = l * f + wave_sum(e);
+  PageEntry entries[PAGES == 2 ? 2 : 1] = {};
+  const auto ask_pages = [&](int at) {
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) out[b] *= f;
-#pragma unroll 1
-      for (int i = 0; i < 64 && kb + i < high; ++i) {
-        const float weight = __shfl(e, i, 64);
-        const float* const value = row_at(values, kb + i);
-        if (value == nullptr) continue;
+    for (int n = 0; n < PAGES; ++n) entries[n] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 15 * n));
+  };
+  struct Held {
+    int page[2];
+  };
+  const auto pages_of = [&] {
+    Held held = {};
+#pragma unroll
+    for (int n = 0; n < PAGES; ++n) held.page[n] = page_of(p, entries[n]);
+    return held;
+  };
+  // where row r of the step at `at` lies, and whether it is anywhere
+  const auto place = [&](int at, unsigned r, const Held& held, unsigned long long& row) {
+    if constexpr (PAGES == 0) return locate(at + (int)r, row);
+    const unsigned inside = inside_page((unsigned)at), cut = p.cache.page_size.d - inside;
+    const bool behind = PAGES == 2 && r >= cut;
+    const int page = behind ? held.page[1] : held.page[0];
+    row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (behind ? r - cut : inside + r) * p.cache.row;
+    return page >= 0;
+  };
+  const auto load_keys = [&](int at, const Held& held) {
+    unsigned long long row;
+    place(at, c, held, row);
+#pragma unroll
+    for (int b = 0; b < 4 * BLOCKS; ++b) k[b] = *reinterpret_cast<const f32x4*>(keys + row + (16 * b + 4 * g < size ? 16 * b + 4 * g : 0));
+  };
+  const auto load_values = [&](int at, const Held& held) {
+    missing = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      unsigned long long row;
+      missing |= place(at, 4 * g + i, held, row) ? 0u : 1u << i;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) v[i][b] = *reinterpret_cast<const f32x4*>(values + row + (64 * b + 4 * c < size ? 64 * b + 4 * c : 0));
+    }
+  };
+  if (kb < end) {
+    ask_pages(kb);
+    const Held held = pages_of();
+    load_keys(kb, held);
+    load_values(kb, held);
+    if (kb + STEP < end) ask_pages(kb + STEP);
+  }
+  // value 16 b + 4 g + j of the row's query in q[b][j]
+  f32x4 q[4 * BLOCKS];
+  {
+    const float* x = p.q + (unsigned long long)(t.first + (t.row_token < 0 ? 0 : t.row_token)) * p.q_token + (head * p.group.d + t.row_head) * p.q_head;
+#pragma unroll
+    for (int b = 0; b < 4 * BLOCKS; ++b) {
+      const unsigned d = 16 * b + 4 * g;
+      f32x4 v = {0, 0, 0, 0};
+      if (t.row_token >= 0 && d < size) v = *reinterpret_cast<const f32x4*>(x + d) * p.scale;
+      q[b] = v;
+    }
+  }
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[b][j] = f32x4{0, 0, 0, 0};
+  m = -INFINITY;
+  l = 0.0f;
+
+  for (; kb < end; kb += STEP) {
+    look(kb, k, v, missing);
+    f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < 4 * BLOCKS; ++b) {
+      f32x4 x = k[b];
+      if (size != DPAD && 16 * b + 4 * g >= size) x = f32x4{0, 0, 0, 0};
+      s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[0], q[b][0], s0, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[1], q[b][1], s1, 0, 0, 0);
+      s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[2], q[b][2], s0, 0, 0, 0);
+      s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], q[b][3], s1, 0, 0, 0);
+    }
+    f32x4 s = s0 + s1;
+    const bool more = kb + STEP < end;
+    const Held next_pages = pages_of();
+    if (more) load_keys(kb + STEP, next_pages);
+    const bool edge = __any(missing != 0) || kb < t.all_low || kb + 16 > t.all_high;
+    unsigned foreign = 0;  // values that are not finite, of keys that some row does not see
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = kb + 4 * (int)g + i;
+        const bool there = (missing >> i & 1) == 0;
+        s[i] = there && key >= t.row_low && key < t.row_high ? s[i] : -INFINITY;
+        const bool none = !there || key < t.low || key >= t.high;
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
-          if (lane + 64 * b < size) out[b] += weight * look_at(value[lane + 64 * b]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool odd = (__float_as_uint(v[i][b][j]) & 0x7f800000u) == 0x7f800000u;
+            foreign |= odd && !none ? 1u : 0u;
+            v[i][b][j] = none || odd ? 0.0f : v[i][b][j];
+          }
       }
     }
-    if (!__any(odd)) continue;
+    const float top = across_groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
+    if (__any(top > m)) {
+      const float next = fmaxf(m, top);
+      const float f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[b][j] *= f;
+    }
+    const float zero = m == -INFINITY ? 0.0f : m;
+    float e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(s[i] - zero);
+      l += e[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][b][j], e[i], o[b][j], 0, 0, 0);
+    if (edge && __any(foreign != 0)) {
+      // Rare: a key with an infinity or a NaN among its values that only some of the rows see.  A product over all rows would hand
+      // 0 x infinity to the others, so it went in as zeros and is added here, to the rows that see it.
+      for (int at = 0; at < 16; ++at) {
+        const int key = kb + at;
+        const unsigned from = c + 16 * (at / 4);
+        const float e0 = __shfl(e[0], (int)from, 64), e1 = __shfl(e[1], (int)from, 64), e2 = __shfl(e[2], (int)from, 64), e3 = __shfl(e[3], (int)from, 64);
+        const float weight = at % 4 == 0 ? e0 : at % 4 == 1 ? e1 : at % 4 == 2 ? e2 : e3;
+        const unsigned index = p.cache.page_size.quotient((unsigned)key), inside = (unsigned)key - index * p.cache.page_size.d;
+        const int held = page_of(p, table, index);
+        if (held < 0 || key < t.row_low || key >= t.row_high) continue;
+        const float* row = values + held * p.cache.page + inside * p.cache.row;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const unsigned d = 64 * b + 4 * (4 * g + i) + j;
+              const float x = d < size ? row[d] : 0.0f;
+              if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) o[b][j][i] += weight * x;
+            }
+      }
+    }
+    if (more) {
+      load_values(kb + STEP, next_pages);
+      if (kb + 2 * STEP < end) ask_pages(kb + 2 * STEP);
+    }
+  }
+}
+
+// The wavefront's 32 rows of a tile over a float32 cache by the fp32 matrix operations, 16 at a time.  Only rows that see a number of kFar or above are
+// written: the others keep what they have, whatever lies beside them.
+template <int BLOCKS>
+__device__ __forceinline__ void stream_far_rows(const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, int begin, int end, const int* table) {
+  const unsigned lane = threadIdx.x & 63, g = lane / 16, size = p.cache.size;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    Tile u = t;
+    const int row = 16 * half + (int)(lane % 16);
+    u.row_token = __shfl(t.row_token, row, 64);
+    u.row_head = __shfl(t.row_head, row, 64);
+    u.row_low = __shfl(t.row_low, row, 64);
+    u.row_high = __shfl(t.row_high, row, 64);
+    const u64 there = __ballot(u.row_token >= 0) & 0xffff;  // the first ones
+    if (there == 0) return;
+    // what these rows see of the piece, from one of its steps on
+    const int low = __builtin_amdgcn_readfirstlane(u.row_low), high = __builtin_amdgcn_readlane(u.row_high, 63 - __builtin_clzll(there));
+    const int from = low > begin ? begin + (low - begin) / 16 * 16 : begin, upto = high < end ? high : end;
+    bool far = false;
+    const auto look = [&](int kb, const f32x4 (&k)[4 * BLOCKS], const f32x4 (&v)[4][BLOCKS], unsigned missing) {
+      const auto size_of = [](const f32x4& x) {
+        unsigned most = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned bits = __float_as_uint(x[j]) & 0x7fffffffu;
+          most = bits > most ? bits : most;
+        }
+        return most;
+      };
+      // a bit for each key of the step: lanes c, c + 16, ... have key c, the 16 of group g value rows 4 g + i
+      unsigned most = 0;
+#pragma unroll
+      for (int b = 0; b < 4 * BLOCKS; ++b) most = size_of(k[b]) > most ? size_of(k[b]) : most;
+      const u64 key_lanes = __ballot(most >= kFar);
+      unsigned keys = (unsigned)(key_lanes | key_lanes >> 16 | key_lanes >> 32 | key_lanes >> 48) & 0xffffu;
+      unsigned none = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        most = 0;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) most = size_of(v[i][b]) > most ? size_of(v[i][b]) : most;
+        const u64 value_lanes = __ballot(most >= kFar), none_lanes = __ballot((missing >> i & 1) != 0);
+#pragma unroll
+        for (int group = 0; group < 4; ++group) {
+          keys |= (value_lanes >> (16 * group) & 0xffff) != 0 ? 1u << (4 * group + i) : 0u;
+          none |= (unsigned)(none_lanes >> (16 * group) & 1) << (4 * group + i);
+        }
+      }
+      const int first = u.row_low > kb ? u.row_low - kb : 0, behind = u.row_high - kb < 16 ? u.row_high - kb : 16;
+      if (first < behind) far |= (keys & ~none & ((1u << behind) - 1) >> first << first) != 0;
+    };
+    f32x4 o[BLOCKS][4];
+    float m, l;
+    stream_rows<BLOCKS, 16, 2>(p, u, head, from, upto, table, o, m, l, look);
+    l = across_groups_sum(l);
     m = frame_out(m, l);
+    if (u.row_token < 0 || !far) continue;
+    const unsigned long long token = u.first + u.row_token, query_head = head * p.group.d + u.row_head;
     float* to = p.out + token * p.out_token + query_head * p.out_head;
+    const f32x4 zeros = {0, 0, 0, 0};
+    float divisor = l;
     if (p.splits > 1) {
       const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
       to = p.partial + place * size;
-      if (lane == 0) {
+      divisor = 1.0f;
+      if (g == 0) {
         p.statistics[place * 2] = m;
         p.statistics[place * 2 + 1] = l;
       }
     }
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
-      if (lane + 64 * b < size) to[lane + 64 * b] = p.splits > 1 ? out[b] : m == -INFINITY ? 0.0f : out[b] / l;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned d = 64 * b + 4 * (4 * g + i);
+        if (d < size) *reinterpret_cast<f32x4*>(to + d) = m == -INFINITY ? zeros : f32x4{o[b][0][i], o[b][1][i], o[b][2][i], o[b][3][i]} / divisor;
+      }
   }
+}
+
+// The same as a function of its own that finds the work once more: with heads of 128, whose steps have all registers, what it wants takes none from them
+// (4 chunks of 1024 over 4096, 32 heads over 8: 674 us, and 700 with the above in the kernel; heads of 64 the other way round, 51.3 and 49.3 us for 6
+// chunks of 517 with a window, which feel the stack that a call wants).
+template <int BLOCKS, int WAVES>
+__device__ __attribute__((noinline)) void stream_far_rows_apart(const AttentionArgs& p) {
+  Tile t;
+  unsigned head, split;
+  int begin, end;
+  if (!take_work(p, WAVES * 32, threadIdx.x / 64 * 32 + threadIdx.x % 32, t, head, split, begin, end)) return;
+  stream_far_rows<BLOCKS>(p, t, head, split, begin, end, p.table + (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)t.sequence) * p.table_stride);
 }
 
 // WAVES: 4, and 8 where a thread's part of a step's rows would else take the registers (float32, heads of 128: four wavefronts spill, 1210 us).
@@ -1144,7 +1347,10 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
     unsigned any = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) any |= odds[w];
-    if (any != 0) return rows_one_by_one<BLOCKS>(p, t, head, split, begin, end, table, keys, values);
+    if (any != 0) {
+      if constexpr (BLOCKS == 1) stream_far_rows<BLOCKS>(p, t, head, split, begin, end, table);
+      else stream_far_rows_apart<BLOCKS, WAVES>(*(const AttentionArgs*)__builtin_amdgcn_kernarg_segment_ptr());  // the kernel's one argument, where it lies
+    }
   }
 }
 
@@ -1209,9 +1415,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_any_kernel(AttentionA
   rows.template finish<WAVES>(joining, p, t, head, split, g);
 }
 
-// float32: 16 keys in one step of a wavefront (2 sequences of 30011, 8 heads of 128, 478 MB: 89 us, 5.4 TB/s, then 5 for the join).  The next step's keys are loaded into the registers of this one's as soon as the
-// scores are formed, its values once the weights have met them.  PAGES that the keys of a step may lie in: 1 (of a multiple of 16 rows),
-// 2 (16 rows at least) or any number, 0.  `missing`: a bit for each of the lane's four keys that no page holds.
+// float32: 16 keys in one step of a wavefront (2 sequences of 30011, 8 heads of 128, 478 MB: 89 us, 5.4 TB/s, then 5 for the join).
 template <int BLOCKS, int WAVES, int PAGES>
 __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs p) {
   constexpr int DPAD = 64 * BLOCKS, STEP = 16 * WAVES;
@@ -1220,175 +1424,11 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
   unsigned head, split;
   int begin, end;
   if (!take_work(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16, c = lane % 16;
-  const unsigned size = p.cache.size;
-  const float* const keys = static_cast<const float*>(p.cache.keys) + head * p.cache.head;
-  const float* const values = static_cast<const float*>(p.cache.values) + head * p.cache.head;
-  const int* const table = p.table + t.sequence * p.table_stride;
-
-  int kb = __builtin_amdgcn_readfirstlane(begin + 16 * (int)wave);
-  end = __builtin_amdgcn_readfirstlane(end);
-  f32x4 k[4 * BLOCKS], v[4][BLOCKS];
-  unsigned missing = 0;
-  const auto inside_page = [&](unsigned key) { return key - p.cache.page_size.quotient(key) * p.cache.page_size.d; };
-  const auto locate = [&](int key, unsigned long long& row) {
-    const int page = page_of(p, table, p.cache.page_size.quotient((unsigned)key));
-    row = page < 0 ? 0 : page * p.cache.page + inside_page((unsigned)key) * p.cache.row;
-    return page >= 0;
-  };
-  PageEntry entries[PAGES == 2 ? 2 : 1] = {};
-  const auto ask_pages = [&](int at) {
-#pragma unroll
-    for (int n = 0; n < PAGES; ++n) entries[n] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 15 * n));
-  };
-  struct Held {
-    int page[2];
-  };
-  const auto pages_of = [&] {
-    Held held = {};
-#pragma unroll
-    for (int n = 0; n < PAGES; ++n) held.page[n] = page_of(p, entries[n]);
-    return held;
-  };
-  // where row r of the step at `at` lies, and whether it is anywhere
-  const auto place = [&](int at, unsigned r, const Held& held, unsigned long long& row) {
-    if constexpr (PAGES == 0) return locate(at + (int)r, row);
-    const unsigned inside = inside_page((unsigned)at), cut = p.cache.page_size.d - inside;
-    const bool behind = PAGES == 2 && r >= cut;
-    const int page = behind ? held.page[1] : held.page[0];
-    row = (page < 0 ? 0ull : (unsigned)page) * p.cache.page + (behind ? r - cut : inside + r) * p.cache.row;
-    return page >= 0;
-  };
-  const auto load_keys = [&](int at, const Held& held) {
-    unsigned long long row;
-    place(at, c, held, row);
-#pragma unroll
-    for (int b = 0; b < 4 * BLOCKS; ++b) k[b] = *reinterpret_cast<const f32x4*>(keys + row + (16 * b + 4 * g < size ? 16 * b + 4 * g : 0));
-  };
-  const auto load_values = [&](int at, const Held& held) {
-    missing = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      unsigned long long row;
-      missing |= place(at, 4 * g + i, held, row) ? 0u : 1u << i;
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) v[i][b] = *reinterpret_cast<const f32x4*>(values + row + (64 * b + 4 * c < size ? 64 * b + 4 * c : 0));
-    }
-  };
-  if (kb < end) {
-    ask_pages(kb);
-    const Held held = pages_of();
-    load_keys(kb, held);
-    load_values(kb, held);
-    if (kb + STEP < end) ask_pages(kb + STEP);
-  }
-  // value 16 b + 4 g + j of the row's query in q[b][j]
-  f32x4 q[4 * BLOCKS];
-  {
-    const float* x = p.q + (unsigned long long)(t.first + (t.row_token < 0 ? 0 : t.row_token)) * p.q_token + (head * p.group.d + t.row_head) * p.q_head;
-#pragma unroll
-    for (int b = 0; b < 4 * BLOCKS; ++b) {
-      const unsigned d = 16 * b + 4 * g;
-      f32x4 v = {0, 0, 0, 0};
-      if (t.row_token >= 0 && d < size) v = *reinterpret_cast<const f32x4*>(x + d) * p.scale;
-      q[b] = v;
-    }
-  }
-  // value 64 b + 4 (4 g + i) + j of the output in o[b][j][i]
+  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16;
   f32x4 o[BLOCKS][4];
-#pragma unroll
-  for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[b][j] = f32x4{0, 0, 0, 0};
-  float m = -INFINITY, l = 0.0f;
-
-  for (; kb < end; kb += STEP) {
-    f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
-#pragma unroll
-    for (int b = 0; b < 4 * BLOCKS; ++b) {
-      f32x4 x = k[b];
-      if (size != DPAD && 16 * b + 4 * g >= size) x = f32x4{0, 0, 0, 0};
-      s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[0], q[b][0], s0, 0, 0, 0);
-      s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[1], q[b][1], s1, 0, 0, 0);
-      s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[2], q[b][2], s0, 0, 0, 0);
-      s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(x[3], q[b][3], s1, 0, 0, 0);
-    }
-    f32x4 s = s0 + s1;
-    const bool more = kb + STEP < end;
-    const Held next_pages = pages_of();
-    if (more) load_keys(kb + STEP, next_pages);
-    const bool edge = __any(missing != 0) || kb < t.all_low || kb + 16 > t.all_high;
-    unsigned foreign = 0;  // values that are not finite, of keys that some row does not see
-    if (edge) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = kb + 4 * (int)g + i;
-        const bool there = (missing >> i & 1) == 0;
-        s[i] = there && key >= t.row_low && key < t.row_high ? s[i] : -INFINITY;
-        const bool none = !there || key < t.low || key >= t.high;
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool odd = (__float_as_uint(v[i][b][j]) & 0x7f800000u) == 0x7f800000u;
-            foreign |= odd && !none ? 1u : 0u;
-            v[i][b][j] = none || odd ? 0.0f : v[i][b][j];
-          }
-      }
-    }
-    const float top = across_groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])));
-    if (__any(top > m)) {
-      const float next = fmaxf(m, top);
-      const float f = next == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - next);
-      m = next;
-      l *= f;
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[b][j] *= f;
-    }
-    const float zero = m == -INFINITY ? 0.0f : m;
-    float e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      e[i] = __builtin_amdgcn_exp2f(s[i] - zero);
-      l += e[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][b][j], e[i], o[b][j], 0, 0, 0);
-    if (edge && __any(foreign != 0)) {
-      // Rare: a key with an infinity or a NaN among its values that only some of the rows see.  A product over all rows would hand
-      // 0 x infinity to the others, so it went in as zeros and is added here, to the rows that see it.
-      for (int at = 0; at < 16; ++at) {
-        const int key = kb + at;
-        const unsigned from = c + 16 * (at / 4);
-        const float e0 = __shfl(e[0], (int)from, 64), e1 = __shfl(e[1], (int)from, 64), e2 = __shfl(e[2], (int)from, 64), e3 = __shfl(e[3], (int)from, 64);
-        const float weight = at % 4 == 0 ? e0 : at % 4 == 1 ? e1 : at % 4 == 2 ? e2 : e3;
-        const unsigned index = p.cache.page_size.quotient((unsigned)key), inside = (unsigned)key - index * p.cache.page_size.d;
-        const int held = page_of(p, table, index);
-        if (held < 0 || key < t.row_low || key >= t.row_high) continue;
-        const float* row = values + held * p.cache.page + inside * p.cache.row;
-#pragma unroll
-        for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const unsigned d = 64 * b + 4 * (4 * g + i) + j;
-              const float x = d < size ? row[d] : 0.0f;
-              if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) o[b][j][i] += weight * x;
-            }
-      }
-    }
-    if (more) {
-      load_values(kb + STEP, next_pages);
-      if (kb + 2 * STEP < end) ask_pages(kb + 2 * STEP);
-    }
-  }
+  float m, l;
+  stream_rows<BLOCKS, STEP, PAGES>(p, t, head, begin + 16 * (int)wave, end, p.table + t.sequence * p.table_stride, o, m, l,
+                                   [](int, const f32x4 (&)[4 * BLOCKS], const f32x4 (&)[4][BLOCKS], unsigned) {});
   l = across_groups_sum(l);
   float list[DPAD / 4];
 #pragma unroll
