@@ -28,7 +28,7 @@ int main() {
   EXPECT(paged_attention_plan(1, 1, 4, 8, 128, 100000, 1, 512, 128, false).splits <= 3);  // a window bounds the keys
   EXPECT(paged_attention_plan(32, 32, 4, 8, 256, 8192, 1, 0, 128, false).waves == 4);
   EXPECT(paged_attention_plan(100, 100, 4, 8, 128, 8192, 1, 0, 128, false).waves == 4);
-  // tiles of 128 rows: chunks that fill two, and a workgroup for each CU
+  // tiles of 128 rows: chunks that fill half of one, and 20000 rows in all, 32000 over more than 1536 keys
   EXPECT(paged_attention_plan(4096, 16, 4, 8, 128, 4096, 1, 0, 128, false).rows == 128);
   EXPECT(paged_attention_plan(4096, 16, 4, 8, 128, 4096, 1, 0, 0, false).rows == 16);
   EXPECT(paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, 128, false).rows == 128 && paged_attention_plan(1024, 1, 4, 8, 128, 4096, 1, 0, 128, false).splits == 2);

@@ -138,7 +138,7 @@ def test_against_the_definition(pkg, T, case):
     Made(pkg, kind, lengths, chunks, heads, kv, size, page, case).check(T, **more)
 
 
-# Chunks that make a workgroup of 128 rows for each CU: these go over the keys together.
+# Chunks of many tokens; most of them go over the keys together, 128 or 256 rows in a workgroup.
 TILES = [
     ([600, 300, 257, 700], [300, 300, 257, 290], 32, 32, 64, 16, {}),
     ([300, 290, 0, 1100, 260, 257], [70, 97, 0, 90, 64, 65], 64, 16, 128, 32, {}),
@@ -150,7 +150,7 @@ TILES = [
     ([700, 600], [300, 290], 64, 64, 64, 32, {"window": 1}),
     ([700, 600], [128, 140], 128, 64, 128, 32, {"window": 150}),
     ([300, 400], [260, 270], 64, 64, 128, 16, {"causal": False}),
-    ([1500, 1200], [128, 128], 128, 64, 128, 64, {}),                          # two pieces of the keys
+    ([1500, 1200], [128, 128], 128, 64, 128, 64, {}),                          # contexts of more than 1024 keys
     ([1500, 700, 300], [258, 257, 259], 32, 32, 64, 16, {"max_length": 1280}),
     ([5000], [257], 128, 128, 64, 16, {"window": 4000}),
     ([3000, 2500, 100], [160, 140, 100], 32, 8, 128, 16, {}),                  # float32: pieces of a long context, some without keys

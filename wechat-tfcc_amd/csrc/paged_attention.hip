@@ -474,7 +474,7 @@ struct S8Rows {
 };
 
 // int8 with pages of 16 rows and more that can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
-// of 16; WHOLE: pages of a multiple of 16 rows, so that a half lies in one, else in up to two (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 47).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
+// of 16; WHOLE: pages of a multiple of 16 rows, so that a half lies in one, else in up to two (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 49).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
 // straight into LDS, a ring of STAGES of its own (no barriers), and reads a step from there when it is due.
 template <int BLOCKS, int WAVES>
 struct S8Ring {
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_s8_kernel(AttentionArgs 
 
 // Chunks of many tokens, int8 as above: a workgroup takes 128 rows, a wavefront 32 of them, and all go over the same keys, 32 in a step.  Bound: the
 // matrix cores and, with as much to do, the vector unit (4 chunks of 1024 over 4096, 32 heads over 8 of 128: int8 407 us, matrix operations and LDS
-// reads alone 283; float32 730, with tiles of 16 rows on the fp32 matrix operations 1955).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
+// reads alone 283; float32 665, with tiles of 16 rows on the fp32 matrix operations 1930).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
 // order in which the matrix cores take them, into one of two LDS buffers while the other is worked on; the next step's rows
 // are on their way to registers meanwhile.  Products of 32 x 32 as above, with
 //   S^T: lane l holds row l % 32 and keys 8 a + 4 (l / 32) + i in [4 a + i]
@@ -665,7 +665,7 @@ __device__ __forceinline__ constexpr unsigned value_of(unsigned L, unsigned n) {
 // A row of a float32 cache is two fp16 pieces under a power of two of its own, which is its scale as an int8 row's is: what is said above of
 // int8 holds, with a third operation for the product of the first factor's large piece with the second's small one.  The two
 // small ones' product, 2^-22 of the whole at most and 2^-25 in the mean, is left out: with the pieces' own 2^-23 each a term is right to 2^-21, where the
-// fp32 operations, at five times their cost, round to 2^-24 (6 chunks of 517 with a window: 4.9e-7 from 64 bits, elementary float32 operations 4.4e-7).  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
+// fp32 operations, at five times their cost, round to 2^-24 (6 chunks of 517 with a window: 4.3 to 4.9e-7 from 64 bits, elementary float32 operations 4.3 to 4.4e-7).  Infinities and NaN have no such pieces: where a row sees one, the workgroup takes its rows
 // once more by the fp32 operations (an infinity in the first page of every sequence: 4 chunks of 1024 over 4096 2530 us, with tiles of 16 rows 2060).  Weights and scores have float32's exponents to stay in, so numbers from 2^80 on go that way too, and what undoes a value row's power of
 // two is taken 2^kLift times, which the results are freed of: these scales lie between 2^-78 and 2^102.  A weight that brings the largest scale to
 // the frame's 2^8 is 2^-94, those 2^-30 below it are normal numbers, and one that brings the smallest to 2^15 is 2^93, of which 2^34 can be summed.
@@ -942,7 +942,7 @@ __device__ __attribute__((noinline)) void stream_far_rows_apart(const AttentionA
   stream_far_rows<BLOCKS>(p, t, head, split, begin, end, p.table + (unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)t.sequence) * p.table_stride);
 }
 
-// WAVES: 4, and 8 where a thread's part of a step's rows would else take the registers (float32, heads of 128: four wavefronts spill, 1210 us).
+// WAVES: 4, and 8 where a thread's part of a step's rows would else take the registers (float32, heads of 128: four wavefronts spill).
 template <int BLOCKS, int WAVES, bool S8, bool WHOLE>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void attention_tile_kernel(AttentionArgs p) {
   constexpr int KS = 4 * BLOCKS, N = 2 * BLOCKS, PIECES = S8 ? 1 : 2;  // products over a head, tiles of 32 of its values
@@ -1354,7 +1354,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
   }
 }
 
-// int8 in any layout, a page for each key, loaded when it is due (the same 32 sequences with pages of 24 rows: 139 us).
+// int8 in any layout, a page for each key, loaded when it is due (the same 32 sequences with pages of 24 rows: 138 us).
 template <int BLOCKS, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void attention_s8_any_kernel(AttentionArgs p) {
   constexpr int STEP = 32 * WAVES;

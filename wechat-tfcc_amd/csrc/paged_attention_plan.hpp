@@ -39,14 +39,14 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   bool wide = false;
   if (chunk_rows > 0 && !float_cache) {
     // Wide tiles where chunks fill half of one and there are rows for the GPU, more of them over long contexts, whose steps tiles of 16 rows
-    // take at the rate of HBM (rows in all: 39 chunks of up to 84 over 510, 32 heads over 8 of 128, 79000: 60 us, with tiles of 16 rows 98; 8 of 49 over 2706 with
-    // a window of 293, 20500: 28 and 34; 12 of 184 over 589, 8 heads over 1 of 256, 13000: 73 and 57; over long contexts one of 1024 over
-    // 4096, 32800: 186 and 243; 16 of 64 over 2048, 24600: 105 and 89).
+    // take at the rate of HBM (rows in all: 39 chunks of up to 84 over 510, 32 heads over 8 of 128, 79000: 61 us, with tiles of 16 rows 99; 8 of 49 over 2706 with
+    // a window of 293, 64 heads, 20500: 28 and 34; 12 of 184 over 589, 8 heads over 1 of 256, 13000: 74 and 57; over long contexts one of 1024 over
+    // 4096, 32800: 186 and 228; 16 of 64 over 2048, 24600: 105 and 89).
     wide = 2 * mean * group >= chunk_rows && all >= (keys_of(chunk_rows) <= 1536 ? 20000 : 32000);
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
-    // (32 heads over 8 of 128, tokens x rows of all tiles: 15 of 205 over 376, 16 heads over 2: 50 us, with tiles of 16 rows 101; 11 of 125 over 227: 34 and 43;
-    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in four pieces 129 and 213).
+    // (32 heads over 8 of 128, tokens x rows of all tiles: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
+    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in eight pieces 84 and 210).
     wide = 2 * mean * group >= chunk_rows && (all >= 18000 || (all >= 8192 && keys_of(chunk_rows) >= 2048));
   }
   p.rows = wide ? chunk_rows : kAttentionRows;
@@ -59,7 +59,7 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   p.waves = groups <= 512 && size <= 128 && keys > kAttentionStep / 2 ? 8 : 4;
   if (!wide) step = p.waves * (float_cache ? 16 : 32);
   if (wide && float_cache) {
-    // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 267 us, one 403)
+    // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 260 us, one 404)
     p.waves = chunk_rows / 32;
     const uint64_t fit = groups == 0 ? 1 : 256 * 256 / chunk_rows / groups;
     splits = keys < 2048 || fit < 1 ? 1 : fit < keys / 512 ? fit : keys / 512;

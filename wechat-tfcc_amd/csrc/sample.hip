@@ -16,8 +16,9 @@
 // 128 rows of 100003 with top-p and min-p take 12 + 23 + 26 + 11 us, of which the first is bound by HBM, the two in the middle by the vector
 // unit (about 40 operations of four cycles a logit, half of them in 64 bits), the last by the latency of what it does one after another,
 // and so are all four for a single row of 32000: 4 + 5 + 8 + 7.
-// A bin of more tokens than the list holds - a vocabulary of equal logits, top-k of thousands - goes a slower way there: eight bits of
-// the logits' order at a time over the whole row.
+// A bin of more tokens than the list holds - a vocabulary of equal logits, top-k of thousands, top-k at low temperatures, whose last bin holds all
+// from 32 temperatures below the largest on - goes a slower way there: eight bits of the logits' order at a time over the whole row (k = 50, 128 rows of
+// 100003: 57 us at a temperature of 0.7, 101 at 0.3, 739 at 0.2).
 #include "common.hpp"
 
 namespace tfcc_rocm {
