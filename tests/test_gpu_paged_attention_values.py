@@ -159,3 +159,41 @@ def test_far_numbers_here_and_there(pkg, T, case, value):
     lost = np.isinf(want) & np.isnan(got)
     assert (same | near | lost).all() and not lost.all()
     assert mine.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [3, 4, 5])
+def test_far_numbers_between_replays(pkg, T, shape):
+    """A captured call meets infinities that come and go in its cache."""
+    import torch
+    m = Made(pkg, "f32", *SHAPES[shape], 91)
+    cache, q, table, starts, lengths = m.on(T), T.t(m.q), T.t(m.table), T.t(m.starts), T.t(m.lengths)
+    call = lambda: pkg.paged_attention(q, cache, table, starts, lengths, m.scale)
+    clean = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    at = int(m.lengths[0]) // 2
+    named, inside = m.table[0, at // m.page], at % m.page
+    for value in (None, float("inf"), None, 1e33, float("nan"), None):
+        held = cache[1][named, 0, inside, 3].item()
+        if value is not None:
+            cache[1][named, 0, inside, 3] = value
+        eager = call()
+        for _ in range(2):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out.isnan(), eager.isnan()) and torch.equal(out.nan_to_num(0.0), eager.nan_to_num(0.0))
+        assert torch.equal(eager.nan_to_num(0.0), clean.nan_to_num(0.0)) == (value is None)
+        cache[1][named, 0, inside, 3] = held
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["s8", "f32"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+@pytest.mark.parametrize("scale", [-0.125, 0.0, -0.0])
+def test_scales_of_scores_below_and_at_zero(pkg, T, kind, shape, scale):
+    m = Made(pkg, kind, *SHAPES[shape], 93 + shape)
+    m.scale = scale
+    m.check(T)

@@ -675,10 +675,10 @@ constexpr int kLift = 36;
 // Rows of a tile, 16 of them, over a float32 cache: the keys of steps kb, kb + STEP, ... below end, 16 in each.  The next step's keys are loaded into the registers
 // of this one's as soon as the scores are formed, its values once the weights have met them.  PAGES that the keys of a step may lie in: 1 (of a
 // multiple of 16 rows), 2 (16 rows at least) or any number, 0.  `missing`: a bit for each of the lane's four keys that no page holds.
-// o: value 64 b + 4 (4 g + i) + j of the row in o[b][j][i]; look: sees each step's rows as they were loaded.
-template <int BLOCKS, int STEP, int PAGES, class Look>
-__device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& t, unsigned head, int kb, int end, const int* table, f32x4 (&o)[BLOCKS][4],
-                                            float& m, float& l, Look look) {
+// look: sees each step's rows as they were loaded; done: takes value 64 b + 4 (4 g + i) + j of the row in o[b][j][i], its frame and the lane's share of its sum.
+// (Handed out through references, they cost heads of more than 128 values 5 to 8 %.)
+template <int BLOCKS, int STEP, int PAGES, class Look, class Done>
+__device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& t, unsigned head, int kb, int end, const int* table, Look look, Done done) {
   constexpr int DPAD = 64 * BLOCKS;
   const unsigned lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const unsigned size = p.cache.size;
@@ -753,12 +753,12 @@ __device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& 
       q[b] = v;
     }
   }
+  f32x4 o[BLOCKS][4];
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[b][j] = f32x4{0, 0, 0, 0};
-  m = -INFINITY;
-  l = 0.0f;
+  float m = -INFINITY, l = 0.0f;
 
   for (; kb < end; kb += STEP) {
     look(kb, k, v, missing);
@@ -848,6 +848,7 @@ __device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& 
       if (kb + 2 * STEP < end) ask_pages(kb + 2 * STEP);
     }
   }
+  done(o, m, l);
 }
 
 // The wavefront's 32 rows of a tile over a float32 cache by the fp32 matrix operations, 16 at a time.  Only rows that see a number of kFar or above are
@@ -901,32 +902,32 @@ __device__ __forceinline__ void stream_far_rows(const AttentionArgs& p, const Ti
       const int first = u.row_low > kb ? u.row_low - kb : 0, behind = u.row_high - kb < 16 ? u.row_high - kb : 16;
       if (first < behind) far |= (keys & ~none & ((1u << behind) - 1) >> first << first) != 0;
     };
-    f32x4 o[BLOCKS][4];
-    float m, l;
-    stream_rows<BLOCKS, 16, 2>(p, u, head, from, upto, table, o, m, l, look);
-    l = across_groups_sum(l);
-    m = frame_out(m, l);
-    if (u.row_token < 0 || !far) continue;
-    const unsigned long long token = u.first + u.row_token, query_head = head * p.group.d + u.row_head;
-    float* to = p.out + token * p.out_token + query_head * p.out_head;
-    const f32x4 zeros = {0, 0, 0, 0};
-    float divisor = l;
-    if (p.splits > 1) {
-      const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
-      to = p.partial + place * size;
-      divisor = 1.0f;
-      if (g == 0) {
-        p.statistics[place * 2] = m;
-        p.statistics[place * 2 + 1] = l;
+    const auto write = [&](const f32x4 (&o)[BLOCKS][4], float m, float l) {
+      l = across_groups_sum(l);
+      m = frame_out(m, l);
+      if (u.row_token < 0 || !far) return;
+      const unsigned long long token = u.first + u.row_token, query_head = head * p.group.d + u.row_head;
+      float* to = p.out + token * p.out_token + query_head * p.out_head;
+      const f32x4 zeros = {0, 0, 0, 0};
+      float divisor = l;
+      if (p.splits > 1) {
+        const unsigned long long place = ((unsigned long long)split * p.tokens + token) * p.cache.heads * p.group.d + query_head;
+        to = p.partial + place * size;
+        divisor = 1.0f;
+        if (g == 0) {
+          p.statistics[place * 2] = m;
+          p.statistics[place * 2 + 1] = l;
+        }
       }
-    }
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b)
+      for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const unsigned d = 64 * b + 4 * (4 * g + i);
-        if (d < size) *reinterpret_cast<f32x4*>(to + d) = m == -INFINITY ? zeros : f32x4{o[b][0][i], o[b][1][i], o[b][2][i], o[b][3][i]} / divisor;
-      }
+        for (int i = 0; i < 4; ++i) {
+          const unsigned d = 64 * b + 4 * (4 * g + i);
+          if (d < size) *reinterpret_cast<f32x4*>(to + d) = m == -INFINITY ? zeros : f32x4{o[b][0][i], o[b][1][i], o[b][2][i], o[b][3][i]} / divisor;
+        }
+    };
+    stream_rows<BLOCKS, 16, 2>(p, u, head, from, upto, table, look, write);
   }
 }
 
@@ -1425,19 +1426,19 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
   int begin, end;
   if (!take_work(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16;
-  f32x4 o[BLOCKS][4];
-  float m, l;
-  stream_rows<BLOCKS, STEP, PAGES>(p, t, head, begin + 16 * (int)wave, end, p.table + t.sequence * p.table_stride, o, m, l,
-                                   [](int, const f32x4 (&)[4 * BLOCKS], const f32x4 (&)[4][BLOCKS], unsigned) {});
-  l = across_groups_sum(l);
-  float list[DPAD / 4];
+  const auto store = [&](const f32x4 (&o)[BLOCKS][4], float m, float l) {
+    l = across_groups_sum(l);
+    float list[DPAD / 4];
 #pragma unroll
-  for (int b = 0; b < BLOCKS; ++b)
+    for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) list[(b * 4 + i) * 4 + j] = o[b][j][i];
-  join_and_store(joining, p, t, head, split, frame_out(m, l), l, list, [&](int at) { return 64 * (at / 16) + 4 * (4 * (int)g + at % 16 / 4); });
+        for (int j = 0; j < 4; ++j) list[(b * 4 + i) * 4 + j] = o[b][j][i];
+    join_and_store(joining, p, t, head, split, frame_out(m, l), l, list, [&](int at) { return 64 * (at / 16) + 4 * (4 * (int)g + at % 16 / 4); });
+  };
+  stream_rows<BLOCKS, STEP, PAGES>(p, t, head, begin + 16 * (int)wave, end, p.table + t.sequence * p.table_stride,
+                                   [](int, const f32x4 (&)[4 * BLOCKS], const f32x4 (&)[4][BLOCKS], unsigned) {}, store);
 }
 
 // The pieces of a row joined: a workgroup to a row, its threads four values each of one in every kThreads / (size / 4) pieces.
