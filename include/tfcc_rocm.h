@@ -584,12 +584,13 @@ int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const
  * cached ones.  Query head h reads cache head h / (heads / cache heads).  causal: a token sees the keys up to its own position and,
  * with window > 0, only the last `window` of those; causal 0: all lengths[i].  A token that sees no key gets zeros, rows from
  * starts[batch] on are left as they were, and a key on a page outside the cache or behind the table is not seen.  max_length: an
- * upper bound of lengths[] that the host knows (0: table_width * page_size): how the work is split follows it; keys behind it are not seen.
+ * upper bound of lengths[] that the host knows (0: table_width * page_size): how the work is split follows it and the
+ * mean chunk, one kernel for all sequences; keys behind it are not seen.
  * workspace: tfcc_rocm_paged_attention_workspace() bytes, 16-byte aligned, of any contents, not in use by another call at the same time.
  * tokens * heads < 2^31, and no more workgroups than one launch takes: a chunk has one for every 16 rows (token, query head) of a
  * cache head, or part of 16, and 2^24 - 1 are the most.
  * Sums and weights are float32, whatever the cache's type.  A term of a product is right to 2^-23 of it, over a float32 cache with many rows to
- * 2^-21, but for parts of a row that lie 2^-30 below its largest value, which may be lost (F32, many rows: and below 2^-139; S8: where the scales are 2^-100 to 2^100 - where all of a row's values have scales below
+ * 2^-21, but for parts of a row that lie 2^-30 below its largest value, which may be lost (F32, many rows: and below 2^-139; S8: where the scales are 2^-100 to 2^96 - where all of a row's values have scales below
  * 2^-(90 + n), 2^-(33 - n) of the largest product is lost).  Sums of weights times values are divided last: where those reach 2^128, they are
  * infinite.  Where rows of many see an infinity, a NaN or a number of 2^80 or more in a float32 cache, they and those beside them are worked out
  * twice, in up to four times the time.  out overlaps no input. */

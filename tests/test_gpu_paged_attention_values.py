@@ -1,5 +1,5 @@
 """Attention over a paged cache with queries, keys and values of all sizes, the same throughout a row: float32 accuracy over a float32 cache and over an
-int8 one with scales from 2^-100 to 2^100."""
+int8 one with scales from 2^-100 to 2^96."""
 import numpy as np
 import pytest
 

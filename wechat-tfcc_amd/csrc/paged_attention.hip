@@ -932,7 +932,7 @@ __device__ __forceinline__ void stream_far_rows(const AttentionArgs& p, const Ti
 }
 
 // The same as a function of its own that finds the work once more: with heads of 128, whose steps have all registers, what it wants takes none from them
-// (4 chunks of 1024 over 4096, 32 heads over 8: 674 us, and 700 with the above in the kernel; heads of 64 the other way round, 51.3 and 49.3 us for 6
+// (4 chunks of 1024 over 4096, 32 heads over 8: 667 us, and 679 with the above in the kernel; heads of 64 the other way round, 51.3 and 49.4 us for 6
 // chunks of 517 with a window, which feel the stack that a call wants).
 template <int BLOCKS, int WAVES>
 __device__ __attribute__((noinline)) void stream_far_rows_apart(const AttentionArgs& p) {
