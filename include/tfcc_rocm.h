@@ -43,6 +43,7 @@ enum {
   TFCC_ROCM_U64 = 7,
   TFCC_ROCM_F32 = 8,
   TFCC_ROCM_F64 = 9,
+  TFCC_ROCM_S4 = 10, /* paged caches only: two in a byte */
 };
 
 const char* tfcc_rocm_last_error_string(void);
@@ -556,10 +557,13 @@ int tfcc_rocm_rotary_f32(void* stream, const tfcc_rocm_rotary_desc* desc);
  * TFCC_ROCM_S8 with one scale for each slot and head, as cache_write makes them: scale = max |x| * (1 / 127) in float32, integers
  * x / scale rounded to nearest, ties to even; a row of zeros has scale 0, and a row that holds an infinity or a NaN reads back as
  * NaN.  keys and values have the same strides, and so have the scales; key and value arrays, scales, slots do not overlap.
- * size: up to 256, a multiple of 4 (F32) or 8 (S8), with pointers and strides of keys and values multiples of 16 bytes (F32) or 8 (S8). */
+ * size: up to 256, a multiple of 4 (F32) or 8 (S8), with pointers and strides of keys and values multiples of 16 bytes (F32) or 8 (S8).
+ * TFCC_ROCM_S4 is the same with integers of 4 bits: scale = max |x| * (1 / 7), integers from -7 to 7 as they are written (-8 is read as such); byte j of
+ * a row holds value 2j in its low half and 2j + 1 in its high one, both in two's complement.  size: a multiple of 16; strides of keys and
+ * values count bytes, multiples of 8 as the pointers are. */
 typedef struct tfcc_rocm_paged_cache {
   void *keys, *values;
-  float *key_scales, *value_scales; /* S8 only */
+  float *key_scales, *value_scales; /* S8 and S4 */
   int type;
   unsigned pages, heads, page_size, size;
   uint64_t page_stride, head_stride, row_stride;
@@ -578,6 +582,15 @@ int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, cons
 int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const int32_t* table, uint64_t table_stride,
                          unsigned table_width, unsigned batch, const int32_t* starts, unsigned tokens, float* keys,
                          float* values);
+
+/* Rows of pages to other places of the same cache, for keys, values and scales of all heads: run i copies rows[i] slots from sources[i] on to
+ * those from destinations[i] on (S32 or S64 as cache_write's slots; rows NULL: up to the end of the source's page).  A run ends with either slot's
+ * page; one whose source or destination lies outside the cache (-1 for a padded one) or whose rows are 0 or less is skipped.  A forked
+ * sequence's last page, pages moved together.  Any number of runs may have the same source; no slot that a run writes may be a source or a destination of another run
+ * of the call, or of its own: its contents are then unspecified.  A cache stride of 0 over more than one page, head or row is refused, and so are more
+ * than 2^23 - 1 workgroups, of which a run has one for every 16 KiB (8 KiB where rows or strides are no multiples of 16 bytes) of a page's keys in all heads, and for every 1024 of its scales. */
+int tfcc_rocm_cache_copy(void* stream, const tfcc_rocm_paged_cache* cache, const void* sources, const void* destinations, int slot_type,
+                         const int32_t* rows, unsigned runs);
 
 /* out = softmax(scale * q k^T) v of a chunk of tokens of each sequence over what the cache holds of it, the chunk itself among that.
  * q and out [tokens, heads, size]; sequence i's chunk is rows starts[i] .. starts[i + 1] - 1 and its last token the last of lengths[i]
@@ -613,6 +626,18 @@ typedef struct tfcc_rocm_paged_attention_desc {
 } tfcc_rocm_paged_attention_desc;
 size_t tfcc_rocm_paged_attention_workspace(const tfcc_rocm_paged_attention_desc* desc); /* 0 for a call that is refused, or needs none */
 int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_desc* desc);
+/* The same with shaped scores and a prefix that is seen as a whole; the same workspace.
+ *   x = scale * q k^T;  with a cap > 0 x = cap * tanh(x / cap);  with slopes x -= slopes[head] * |position of the token - position of the key|
+ * A sequence's i first prefixes[i] tokens (of those that are cached) are seen by all tokens of its chunk, the later ones of the prefix by the
+ * earlier too: a token sees the keys up to its own position and those of the prefix.  A prefix wants causal and no window.  A cap is finite;
+ * slopes may be of any sign, and the bias is formed in float32.  Scores that overflow are those of an infinity: cap or -cap.  All three
+ * unset: the call above. */
+typedef struct tfcc_rocm_attention_scores {
+  float cap;               /* 0: none */
+  const float* slopes;     /* [heads] or NULL */
+  const int32_t* prefixes; /* [batch] or NULL; 0 and below: none */
+} tfcc_rocm_attention_scores;
+int tfcc_rocm_paged_attention_scores_f32(void* stream, const tfcc_rocm_paged_attention_desc* desc, const tfcc_rocm_attention_scores* scores);
 
 /* One token for each row of logits [rows, length], given a random number in [0, 1) for each.  Weights are exp((x - max) / temperature);
  * tokens stand in the order of falling logits, equal ones by position.  Of these, the first top_k are kept; of those, the
@@ -640,6 +665,30 @@ typedef struct tfcc_rocm_sample_desc {
 } tfcc_rocm_sample_desc;
 size_t tfcc_rocm_sample_workspace(unsigned rows, unsigned length);
 int tfcc_rocm_sample_f32(void* stream, const tfcc_rocm_sample_desc* desc);
+
+/* Root-mean-square norm of rows, the residual stream's addition in front of it: h = x + residual (float32; x where residual is NULL),
+ *   out = h * weight / sqrt(mean(h^2) + eps)
+ * as float32, as 8-bit integers for the integer products, or both.  The integers: steps = 128 + n with n = 127 t / max |t| rounded to nearest,
+ * ties to even, t = h * weight (the root is the same for the whole row), decided as if in exact arithmetic, scales = max |out| / 127, and sums = the sum of a
+ * row's steps: with offset_a = -128, what tfcc_rocm_gemm_u8s8s32 takes as a and rowsum_a.  A row of zeros has scale 0; a row whose h or h * weight holds an infinity or
+ * a NaN has steps of 128 and a scale of NaN.  Means, roots and products are formed in 64 bits and rounded once.
+ * sum (h), sums: NULL where they are not wanted.  sum may be x or residual, out may be x, with the same strides; nothing else overlaps.
+ * Rows that are written do not share memory.  rows: up to 2^26 - 4 with a width of up to 1024, 2^24 - 1 up to 4096, 2^22 - 1 above. */
+typedef struct tfcc_rocm_rms_norm_desc {
+  const float *x, *residual, *weight;
+  float *sum, *out;
+  uint8_t* steps;
+  float* scales; /* [rows], with steps */
+  int32_t* sums; /* [rows] */
+  uint64_t x_row_stride, residual_row_stride, sum_row_stride, out_row_stride, steps_row_stride;
+  unsigned rows, width;
+  float eps;
+} tfcc_rocm_rms_norm_desc;
+int tfcc_rocm_rms_norm_f32(void* stream, const tfcc_rocm_rms_norm_desc* desc);
+/* out[i, j] = (in[i, j] - offset) * scales[i] * column_scales[j] (NULL: 1): the results of an integer product, or the steps above, as float32.
+ * in: S32, S8 or U8, dense like out.  The difference is exact before it is rounded to float32.  rows * width < 2^31. */
+int tfcc_rocm_dequantize_rows(void* stream, const void* in, int in_type, unsigned rows, unsigned width, int32_t offset, const float* scales,
+                              const float* column_scales, float* out);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,8 @@ The functions mirror the reference's operator interface for this path:
   quantize / requantize / dequantize   tfcc::quantization::*  (tfcc/core/operations/tfcc_quantization.cpp:26-98)
 and, without a counterpart there, what a model that answers token by token needs between its products:
   rotary, rotary_frequencies           positions on the heads of queries and keys
-  cache_write, cache_read, paged_attention   a paged cache of keys and values, float32 or int8, and attention over it
+  cache_write, cache_read, cache_copy, paged_attention   a paged cache of keys and values, float32, int8 or 4 bits, and attention over it
+  rms_norm, rms_norm_quantized, dequantize_rows   the norm in front of the products, and 8-bit rows with scales
   sample                               a token for each row of logits
 """
 import ctypes as C
@@ -20,7 +21,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtfcc_rocm.so")
 CSRC_DIR = os.path.join(_HERE, "csrc")
 
-S8, U8, S16, U16, S32, U32, S64, U64, F32, F64 = range(10)
+S8, U8, S16, U16, S32, U32, S64, U64, F32, F64, S4 = range(11)
 
 
 class TfccRocmError(RuntimeError):
@@ -106,6 +107,13 @@ class PagedAttentionDesc(C.Structure):
          ("table", C.c_void_p), ("table_stride", C.c_uint64), ("table_width", C.c_uint), ("max_length", C.c_uint),
          ("scale", C.c_float), ("causal", C.c_int), ("window", C.c_uint), ("workspace", C.c_void_p),
          ("workspace_bytes", C.c_size_t)]
+
+
+class RmsNormDesc(C.Structure):
+    """tfcc_rocm_rms_norm_desc"""
+    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "weight", "sum", "out", "steps", "scales", "sums")] + \
+        [(n, C.c_uint64) for n in ("x_row_stride", "residual_row_stride", "sum_row_stride", "out_row_stride", "steps_row_stride")] + \
+        [("rows", C.c_uint), ("width", C.c_uint), ("eps", C.c_float)]
 
 
 class SampleDesc(C.Structure):
@@ -204,10 +212,13 @@ SYMBOLS = {
     "tfcc_rocm_rotary_f32": (_I, [_VP, C.POINTER(RotaryDesc)]),
     "tfcc_rocm_cache_write": (_I, [_VP, C.POINTER(PagedCache), _VP, _U64, _U64, _VP, _U64, _U64, _U, _VP, _I]),
     "tfcc_rocm_cache_read": (_I, [_VP, C.POINTER(PagedCache), _VP, _U64, _U, _U, _VP, _U, _VP, _VP]),
+    "tfcc_rocm_cache_copy": (_I, [_VP, C.POINTER(PagedCache), _VP, _VP, _I, _VP, _U]),
     "tfcc_rocm_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedAttentionDesc)]),
     "tfcc_rocm_paged_attention_f32": (_I, [_VP, C.POINTER(PagedAttentionDesc)]),
     "tfcc_rocm_sample_workspace": (C.c_size_t, [_U, _U]),
     "tfcc_rocm_sample_f32": (_I, [_VP, C.POINTER(SampleDesc)]),
+    "tfcc_rocm_rms_norm_f32": (_I, [_VP, C.POINTER(RmsNormDesc)]),
+    "tfcc_rocm_dequantize_rows": (_I, [_VP, _VP, _I, _U, _U, C.c_int32, _VP, _VP, _VP]),
 }
 
 _lib = None
@@ -1182,22 +1193,27 @@ def rotary(q, k, positions, frequencies, interleaved=False, magnitude=1.0, out=N
 
 
 def _cache_desc(cache):
-    """A tfcc_rocm_paged_cache over (keys, values) of float32 or (keys, values, key scales, value scales) of int8."""
+    """A tfcc_rocm_paged_cache over (keys, values) of float32 or (keys, values, key scales, value scales) of int8, or of uint8 with two
+    integers of 4 bits in each."""
     import torch
     if len(cache) not in (2, 4):
         raise InvalidArgumentError("invalid cache")
     keys, values = cache[0], cache[1]
-    s8 = len(cache) == 4
-    if keys.dim() != 4 or keys.dtype != (torch.int8 if s8 else torch.float32) or keys.numel() == 0 or max(keys.shape) > _MOST:
+    scaled = len(cache) == 4
+    if keys.dim() != 4 or keys.dtype not in ((torch.int8, torch.uint8) if scaled else (torch.float32,)) or keys.numel() == 0 or max(keys.shape) > _MOST:
         raise InvalidArgumentError("invalid cache keys")
     if values.shape != keys.shape or values.dtype != keys.dtype or values.stride() != keys.stride() or keys.stride(3) != 1:
         raise InvalidArgumentError("invalid cache values")
     _on_device(keys.device, *cache)
     d = PagedCache()
-    d.keys, d.values, d.type = _ptr(keys), _ptr(values), S8 if s8 else F32
+    d.keys, d.values, d.type = _ptr(keys), _ptr(values), {torch.float32: F32, torch.int8: S8, torch.uint8: S4}[keys.dtype]
     d.pages, d.heads, d.page_size, d.size = keys.shape
     d.page_stride, d.head_stride, d.row_stride = keys.stride()[:3]
-    if s8:
+    if d.type == S4:
+        if keys.shape[3] > 1024:
+            raise InvalidArgumentError("invalid cache keys")
+        d.size = 2 * keys.shape[3]
+    if scaled:
         for t in cache[2:]:
             if t.shape != keys.shape[:3] or t.dtype != torch.float32 or t.stride() != cache[2].stride():
                 raise InvalidArgumentError("invalid cache scales")
@@ -1208,13 +1224,14 @@ def _cache_desc(cache):
 
 def paged_cache(pages, heads, page_size, size, dtype=None, device="cuda"):
     """Zeroed memory of a paged cache as the calls below take it: (keys, values), each [pages, heads, page_size, size], and for
-    int8 (the default) (..., key scales, value scales), each [pages, heads, page_size].  Any tensors of these shapes will do,
-    views of other strides among them."""
+    int8 (the default) (..., key scales, value scales), each [pages, heads, page_size].  uint8: integers of 4 bits, two to a byte, so that
+    keys and values are [pages, heads, page_size, size / 2].  Any tensors of these shapes will do, views of other strides among them."""
     import torch
     dtype = torch.int8 if dtype is None else dtype
-    if dtype not in (torch.int8, torch.float32):
-        raise InvalidArgumentError("a cache is int8 or float32")
-    held = tuple(torch.zeros((pages, heads, page_size, size), dtype=dtype, device=device) for _ in range(2))
+    if dtype not in (torch.int8, torch.uint8, torch.float32) or (dtype == torch.uint8 and size % 2):
+        raise InvalidArgumentError("a cache is int8, uint8 (two 4-bit integers each) or float32")
+    width = size // 2 if dtype == torch.uint8 else size
+    held = tuple(torch.zeros((pages, heads, page_size, width), dtype=dtype, device=device) for _ in range(2))
     if dtype == torch.float32:
         return held
     return held + tuple(torch.zeros((pages, heads, page_size), dtype=torch.float32, device=device) for _ in range(2))
@@ -1222,7 +1239,7 @@ def paged_cache(pages, heads, page_size, size, dtype=None, device="cuda"):
 
 def cache_write(cache, keys, values, slots):
     """Keys and values [tokens, heads, size] of new tokens into the cache's slots (page * page_size + row; int32 or int64 [tokens];
-    -1: the token is skipped), as int8 with a scale for each token and head or as they are: tfcc_rocm_cache_write."""
+    -1: the token is skipped), as integers of 8 or 4 bits with a scale for each token and head or as they are: tfcc_rocm_cache_write."""
     done = _native().cache_write(cache, keys, values, slots)
     if done is not None:
         return
@@ -1264,6 +1281,24 @@ def cache_read(cache, table, starts, tokens):
     check(lib().tfcc_rocm_cache_read(_stream(), C.byref(d), _ptr(table), table.stride(0), table.shape[1], table.shape[0], _ptr(starts),
                                      tokens, _ptr(keys), _ptr(values)))
     return keys, values
+
+
+def cache_copy(cache, sources, destinations, rows=None):
+    """Runs of rows[i] slots (int32 [runs]; None: up to the end of the source's page) from slot sources[i] on to those from destinations[i]
+    on (int32 or int64 [runs], page * page_size + row; -1: the run is skipped), each inside a page, for keys, values and scales of all
+    heads: tfcc_rocm_cache_copy.  What a run writes is no other run's source or destination."""
+    if _native().cache_copy(cache, sources, destinations, rows) is not None:
+        return
+    import torch
+    d = _cache_desc(cache)
+    _on_device(cache[0].device, sources, destinations, rows)
+    runs = sources.numel()
+    sources = _integers(sources, "sources", runs, (torch.int32, torch.int64))
+    destinations = _integers(destinations, "destinations", runs, (sources.dtype,))
+    rows = None if rows is None else _integers(rows, "rows", runs, (torch.int32,))
+    if runs > _MOST:
+        raise InvalidArgumentError("invalid sources")
+    check(lib().tfcc_rocm_cache_copy(_stream(), C.byref(d), _ptr(sources), _ptr(destinations), _type_code(sources.dtype), _ptr(rows), runs))
 
 
 def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window=0, max_length=0, out=None):
@@ -1338,3 +1373,90 @@ def sample(logits, random, temperature=None, top_k=None, top_p=None, min_p=None)
     d.workspace, d.workspace_bytes = _ptr(workspace), needs
     check(lib().tfcc_rocm_sample_f32(_stream(), C.byref(d)))
     return tokens, probabilities
+
+
+def _rows(t, name, width=None):
+    """[..., width] of float32 as a matrix whose rows are contiguous."""
+    import torch
+    if t.dim() < 1 or t.dtype != torch.float32 or (width is not None and t.shape[-1] != width):
+        raise InvalidArgumentError("invalid " + name)
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty((0, t.shape[-1]))
+    if max(m.shape) > _MOST:
+        raise InvalidArgumentError("invalid " + name)
+    return m if m.shape[1] <= 1 or m.stride(1) == 1 else m.contiguous()
+
+
+def _norm(x, weight, eps, residual, quantized):
+    import torch
+    _on_device(x.device, weight, residual)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise InvalidArgumentError("invalid x")
+    width = x.shape[-1]
+    rows = _rows(x, "x")
+    if weight.dtype != torch.float32 or tuple(weight.shape) != (width,):
+        raise InvalidArgumentError("invalid weight")
+    weight = weight.contiguous()
+    if residual is not None and residual.shape != x.shape:
+        raise InvalidArgumentError("invalid residual")
+    if not 0 <= eps <= 3.4028234e38:
+        raise InvalidArgumentError("invalid eps")
+    added = None if residual is None else _rows(residual, "residual")
+    d = RmsNormDesc()
+    d.x, d.weight, d.residual, d.rows, d.width, d.eps = _ptr(rows), _ptr(weight), _ptr(added), rows.shape[0], width, eps
+    d.x_row_stride, d.residual_row_stride = rows.stride(0), 0 if added is None else added.stride(0)
+    d.sum_row_stride = d.out_row_stride = d.steps_row_stride = width
+    held = None if residual is None else torch.empty(x.shape, dtype=torch.float32, device=x.device)
+    d.sum = _ptr(held)
+    if quantized:
+        steps = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        sums = torch.empty(x.shape[:-1], dtype=torch.int32, device=x.device)
+        d.steps, d.scales, d.sums = _ptr(steps), _ptr(scales), _ptr(sums)
+        results = steps, scales, sums, held
+    else:
+        out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+        d.out = _ptr(out)
+        results = out, held
+    if rows.shape[0]:
+        check(lib().tfcc_rocm_rms_norm_f32(_stream(), C.byref(d)))
+    return results
+
+
+def rms_norm(x, weight, eps, residual=None):
+    """x [..., width], the residual added first where there is one, divided by the root of its rows' mean squares (and eps) and multiplied
+    by weight [width]: tfcc_rocm_rms_norm_f32.  Returns (result, x + residual or None)."""
+    done = _native().rms_norm(x, weight, eps, residual, False)
+    return _norm(x, weight, eps, residual, False) if done is None else done
+
+
+def rms_norm_quantized(x, weight, eps, residual=None):
+    """The same result as 8-bit integers with a scale for each row, (steps - 128) * scale: (steps uint8 [..., width], scales float32 [...],
+    the rows' sums of steps int32 [...], x + residual or None).  Steps and sums are what quantization_matmul_offsets takes with an offset_a of
+    -128; dequantize_rows turns its result into float32."""
+    done = _native().rms_norm(x, weight, eps, residual, True)
+    return _norm(x, weight, eps, residual, True) if done is None else done
+
+
+def dequantize_rows(a, scales, offset=0, column_scales=None):
+    """(a - offset) * scales of the rows (* column_scales): tfcc_rocm_dequantize_rows.  a: int32, int8 or uint8 [..., width], scales
+    float32 [...], column_scales float32 [width]."""
+    done = _native().dequantize_rows(a, scales, offset, column_scales)
+    if done is not None:
+        return done
+    import torch
+    _on_device(a.device, scales, column_scales)
+    if a.dim() < 1 or a.dtype not in (torch.int32, torch.int8, torch.uint8) or a.numel() > _MOST:
+        raise InvalidArgumentError("invalid a")
+    if scales.dtype != torch.float32 or scales.shape != a.shape[:-1]:
+        raise InvalidArgumentError("invalid scales")
+    if column_scales is not None and (column_scales.dtype != torch.float32 or tuple(column_scales.shape) != (a.shape[-1],)):
+        raise InvalidArgumentError("invalid column_scales")
+    if not -0x80000000 <= offset <= _MOST:
+        raise InvalidArgumentError("invalid offset")
+    a, scales = a.contiguous(), scales.contiguous()
+    columns = None if column_scales is None else column_scales.contiguous()
+    out = torch.empty(a.shape, dtype=torch.float32, device=a.device)
+    if a.numel():
+        check(lib().tfcc_rocm_dequantize_rows(_stream(), _ptr(a), _type_code(a.dtype), a.numel() // a.shape[-1], a.shape[-1], offset, _ptr(scales),
+                                              _ptr(columns), _ptr(out)))
+    return out

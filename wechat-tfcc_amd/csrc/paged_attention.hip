@@ -1509,6 +1509,7 @@ void launch_f32(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves
 
 int check_attention(const tfcc_rocm_paged_attention_desc& d) {
   if (int e = check_cache(d.cache, "paged_attention")) return e;
+  TFCC_REQUIRE(d.cache.type != TFCC_ROCM_S4, "paged_attention: a cache of type %d", d.cache.type);
   TFCC_REQUIRE(d.heads > 0 && d.heads % d.cache.heads == 0, "paged_attention: %u heads over %u cache heads", d.heads, d.cache.heads);
   TFCC_REQUIRE(d.tokens <= 0x7fffffffu && d.batch <= 0x7fffffffu && (uint64_t)d.tokens * d.heads <= 0x7fffffffu, "paged_attention: %u tokens of %u heads", d.tokens, d.heads);
   TFCC_REQUIRE(d.window == 0 || d.causal, "paged_attention: a window without causal");

@@ -2,7 +2,8 @@
 //
 // Write: a row is one head of one token.  Its lanes hold four values each (a power of two of lanes, 16 to 64, several rows to a
 // wavefront), so the row is read once: the largest absolute value is joined over its lanes, and
-//   scale = amax * (1 / 127) (float32),  n = x / scale rounded to nearest, ties to even.
+//   scale = amax * (1 / 127) (float32),  n = x / scale rounded to nearest, ties to even
+// (1 / 7 for integers of 4 bits, which lie two to a byte).
 // The quotient is not formed: n is taken from x * (1 / scale), which can miss only next to a border, and the remainder x - n * scale,
 // which a fused multiply-add gives exactly there (|x| <= 127.5 scale, so it is a multiple of the smaller last place of x and scale
 // and at most about scale / 2: 24 bits hold it), moves it to the neighbour or, on a tie, to the even one.  So every
@@ -15,6 +16,10 @@
 
 namespace tfcc_rocm {
 namespace {
+
+// What a cache holds of a value: the type's code.  Integers go from -kLargest to kLargest.
+template <int TYPE>
+constexpr int kLargest = TYPE == TFCC_ROCM_S8 ? 127 : 7;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // needs no more than a float's alignment
@@ -42,16 +47,17 @@ __device__ __forceinline__ unsigned row_max(unsigned u) {
   return u;
 }
 
+template <int LARGEST>
 __device__ __forceinline__ int nearest(float x, float scale, float inverse) {
   float n = rintf(x * inverse);
   const float left = fmaf(-n, scale, x), half = 0.5f * scale;
   const bool odd = ((int)n & 1) != 0;
   if (left > half || (left == half && odd)) n += 1.0f;
   else if (left < -half || (left == -half && odd)) n -= 1.0f;
-  return (int)fminf(fmaxf(n, -127.0f), 127.0f);
+  return (int)fminf(fmaxf(n, -(float)LARGEST), (float)LARGEST);
 }
 
-template <bool S8, int LANES>
+template <int TYPE, int LANES>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(WriteArgs p) {
   const unsigned row = blockIdx.x * (kCacheThreads / LANES) + threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
   if (row >= p.rows) return;
@@ -67,7 +73,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(WriteArgs p)
   const bool mine = d < p.cache.size;
   f32x4 x = {0, 0, 0, 0};
   if (mine) x = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(in + d));
-  if constexpr (!S8) {
+  if constexpr (TYPE == TFCC_ROCM_F32) {
     float* out = static_cast<float*>(const_cast<void*>(value ? p.cache.values : p.cache.keys)) + at;
     if (mine) *reinterpret_cast<f32x4*>(out + d) = x;
   } else {
@@ -78,17 +84,22 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(WriteArgs p)
       top = top > u ? top : u;
     }
     top = row_max<LANES>(top);
-    const float scale = __uint_as_float(top) * (1.0f / 127.0f);
+    const float scale = __uint_as_float(top) * (1.0f / kLargest<TYPE>);
     int n[4] = {0, 0, 0, 0};
     if (top < 0x7f800000u && scale > 0.0f) {
       // a subnormal scale has no finite reciprocal: both are lifted by 2^64, which changes no quotient
       const float lift = scale < 1e-30f ? 18446744073709551616.0f : 1.0f, s = scale * lift, inverse = 1.0f / s;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) n[i] = nearest(x[i] * lift, s, inverse);
+      for (int i = 0; i < 4; ++i) n[i] = nearest<kLargest<TYPE>>(x[i] * lift, s, inverse);
     }
     int8_t* out = static_cast<int8_t*>(const_cast<void*>(value ? p.cache.values : p.cache.keys)) + at;
-    if (mine)
-      *reinterpret_cast<unsigned*>(out + d) = ((unsigned)n[0] & 255u) | ((unsigned)n[1] & 255u) << 8 | ((unsigned)n[2] & 255u) << 16 | (unsigned)n[3] << 24;
+    if constexpr (TYPE == TFCC_ROCM_S8) {
+      if (mine)
+        *reinterpret_cast<unsigned*>(out + d) = ((unsigned)n[0] & 255u) | ((unsigned)n[1] & 255u) << 8 | ((unsigned)n[2] & 255u) << 16 | (unsigned)n[3] << 24;
+    } else {
+      if (mine)
+        *reinterpret_cast<uint16_t*>(out + d / 2) = (uint16_t)(((unsigned)n[0] & 15u) | ((unsigned)n[1] & 15u) << 4 | ((unsigned)n[2] & 15u) << 8 | ((unsigned)n[3] & 15u) << 12);
+    }
     if (d == 0)
       const_cast<float*>(value ? p.cache.value_scales : p.cache.key_scales)[page * p.cache.scale_page + head * p.cache.scale_head + inside * p.cache.scale_row] = scale;
   }
@@ -107,7 +118,7 @@ struct ReadArgs {
 constexpr unsigned kReadTokens = 4;  // of a workgroup
 
 // LANES lanes of four values to a row, as above; a workgroup finds its tokens' slots once for all their heads.
-template <bool S8, int LANES>
+template <int TYPE, int LANES>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(ReadArgs p) {
   __shared__ unsigned pages[kReadTokens], insides[kReadTokens];
   constexpr unsigned kOutside = 0xffffffffu, kBehind = 0xfffffffeu;
@@ -147,18 +158,86 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(ReadArgs p) {
     for (unsigned head = threadIdx.x / LANES; head < p.cache.heads; head += step) {
       f32x4 x = {0, 0, 0, 0};
       if (page != kOutside) {
-        const unsigned long long at = page * p.cache.page + head * p.cache.head + inside * p.cache.row + d;
-        if constexpr (S8) {
-          const unsigned n = *reinterpret_cast<const unsigned*>(static_cast<const int8_t*>(held) + at);
-          const float scale = scales[page * p.cache.scale_page + head * p.cache.scale_head + inside * p.cache.scale_row];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(n >> (8 * i)) * scale;
+        const unsigned long long at = page * p.cache.page + head * p.cache.head + inside * p.cache.row;
+        if constexpr (TYPE == TFCC_ROCM_F32) {
+          x = *reinterpret_cast<const f32x4*>(static_cast<const float*>(held) + at + d);
         } else {
-          x = *reinterpret_cast<const f32x4*>(static_cast<const float*>(held) + at);
+          const float scale = scales[page * p.cache.scale_page + head * p.cache.scale_head + inside * p.cache.scale_row];
+          if constexpr (TYPE == TFCC_ROCM_S8) {
+            const unsigned n = *reinterpret_cast<const unsigned*>(static_cast<const int8_t*>(held) + at + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(n >> (8 * i)) * scale;
+          } else {
+            const int n = *reinterpret_cast<const uint16_t*>(static_cast<const int8_t*>(held) + at + d / 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (float)(n << (28 - 4 * i) >> 28) * scale;
+          }
         }
       }
       __builtin_nontemporal_store(x, reinterpret_cast<f32x4_any*>(out + ((unsigned long long)(first + t) * p.cache.heads + head) * p.cache.size + d));
     }
+  }
+}
+
+// Runs of rows to other places of the cache.  Bound: HBM, a launch for a few pages.  What a run moves of keys or values, [heads][rows][chunks] of
+// UNIT bytes, is gone over as one range, cut into pieces for several workgroups: a thread has all its loads under way before it stores the first.  Pieces
+// behind those move the scales, 4 bytes to a unit.
+constexpr unsigned kCopyEach = 4, kCopyUnits = kCacheThreads * kCopyEach;
+struct CopyArgs {
+  void* rows_of[2];
+  float* scales_of[2];
+  unsigned long long page, head, row, scale_page, scale_head, scale_row;  // in bytes
+  const void *sources, *destinations;
+  const int* rows;
+  int wide_slots;
+  unsigned pages, units, scale_units, row_pieces;
+  Divisor page_size, chunks, pieces;
+};
+
+template <class Unit>
+__device__ __forceinline__ void copy_piece(unsigned piece, unsigned units, const Divisor& chunks, const Divisor& page_size, unsigned rows, char* memory,
+                                           unsigned long long from, unsigned long long to, unsigned long long head_stride, unsigned long long row_stride) {
+  Unit held[kCopyEach];
+  unsigned long long at[kCopyEach];
+  bool mine[kCopyEach];
+#pragma unroll
+  for (unsigned i = 0; i < kCopyEach; ++i) {
+    const unsigned unit = piece * kCopyUnits + i * kCacheThreads + threadIdx.x;
+    const unsigned line = chunks.quotient(unit), chunk = unit - line * chunks.d, head = page_size.quotient(line), row = line - head * page_size.d;
+    mine[i] = unit < units && row < rows;
+    at[i] = head * head_stride + row * row_stride + chunk * (unsigned long long)sizeof(Unit);
+    if (mine[i]) held[i] = *reinterpret_cast<const Unit*>(memory + from + at[i]);
+  }
+#pragma unroll
+  for (unsigned i = 0; i < kCopyEach; ++i)
+    if (mine[i]) *reinterpret_cast<Unit*>(memory + to + at[i]) = held[i];
+}
+
+template <unsigned UNIT>
+__global__ __launch_bounds__(kCacheThreads) void cache_copy_kernel(CopyArgs p) {
+  const unsigned run = p.pieces.quotient(blockIdx.x), piece = blockIdx.x - run * p.pieces.d;
+  const auto slot_of = [&](const void* slots) { return p.wide_slots ? static_cast<const long long*>(slots)[run] : static_cast<const int*>(slots)[run]; };
+  const long long source = slot_of(p.sources), destination = slot_of(p.destinations), slots = (long long)p.pages * p.page_size.d;
+  if (source < 0 || source >= slots || destination < 0 || destination >= slots) return;
+  const auto page_of = [&](long long slot) {
+    return slot < 0x80000000ll ? p.page_size.quotient((unsigned)slot) : (unsigned long long)slot / p.page_size.d;
+  };
+  const unsigned long long from_page = page_of(source), to_page = page_of(destination);
+  const unsigned from_row = (unsigned)(source - from_page * p.page_size.d), to_row = (unsigned)(destination - to_page * p.page_size.d);
+  unsigned rows = p.page_size.d - (from_row > to_row ? from_row : to_row);
+  if (p.rows != nullptr) {
+    const int wanted = p.rows[run];
+    if (wanted <= 0) return;
+    rows = (unsigned)wanted < rows ? (unsigned)wanted : rows;
+  }
+  if (piece < p.row_pieces) {
+    typedef unsigned unit __attribute__((ext_vector_type(UNIT / 4)));
+    copy_piece<unit>(piece, p.units, p.chunks, p.page_size, rows, static_cast<char*>(p.rows_of[blockIdx.y]), from_page * p.page + from_row * p.row,
+                     to_page * p.page + to_row * p.row, p.head, p.row);
+  } else {
+    const Divisor one = {1, 1u << 31, 31};
+    copy_piece<unsigned>(piece - p.row_pieces, p.scale_units, one, p.page_size, rows, reinterpret_cast<char*>(p.scales_of[blockIdx.y]),
+                         from_page * p.scale_page + from_row * p.scale_row, to_page * p.scale_page + to_row * p.scale_row, p.scale_head, p.scale_row);
   }
 }
 
@@ -176,12 +255,7 @@ int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, cons
   if (int e = check_cache(*cache, "cache_write")) return e;
   TFCC_REQUIRE(slot_type == TFCC_ROCM_S32 || slot_type == TFCC_ROCM_S64, "cache_write: slot type %d", slot_type);
   if (tokens == 0) return TFCC_ROCM_OK;
-  // memory that several rows share can be read, but not written
-  TFCC_REQUIRE((cache->pages == 1 || cache->page_stride > 0) && (cache->heads == 1 || cache->head_stride > 0) && (cache->page_size == 1 || cache->row_stride > 0),
-               "cache_write: a cache stride of 0");
-  TFCC_REQUIRE(cache->type != TFCC_ROCM_S8 || ((cache->pages == 1 || cache->scale_page_stride > 0) && (cache->heads == 1 || cache->scale_head_stride > 0) &&
-                                               (cache->page_size == 1 || cache->scale_row_stride > 0)),
-               "cache_write: a cache scale stride of 0");
+  if (int e = check_written(*cache, "cache_write")) return e;
   // threads of a launch: whole workgroups
   const unsigned lanes = cache->size <= 64 ? 16 : cache->size <= 128 ? 32 : 64;
   TFCC_REQUIRE((uint64_t)tokens * cache->heads * lanes <= 0xffffffffu - (kCacheThreads - 1), "cache_write: %u tokens of %u heads", tokens, cache->heads);
@@ -189,14 +263,13 @@ int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, cons
   WriteArgs a{view_of(*cache), keys, values, key_token_stride, key_head_stride, value_token_stride, value_head_stride, slots,
               slot_type == TFCC_ROCM_S64, tokens, tokens * cache->heads, Divisor::of(cache->heads)};
   const hipStream_t s = as_stream(stream);
-  const bool s8 = cache->type == TFCC_ROCM_S8;
-  const auto start = [&](auto kernel) {
+  const auto start = [&](auto s4, auto s8, auto f32) {
     const unsigned rows = kCacheThreads / lanes;
-    hipLaunchKernelGGL(kernel, dim3((a.rows + rows - 1) / rows, 2), dim3(kCacheThreads), 0, s, a);
+    hipLaunchKernelGGL((cache->type == TFCC_ROCM_S4 ? s4 : cache->type == TFCC_ROCM_S8 ? s8 : f32), dim3((a.rows + rows - 1) / rows, 2), dim3(kCacheThreads), 0, s, a);
   };
-  if (lanes == 16) start(s8 ? cache_write_kernel<true, 16> : cache_write_kernel<false, 16>);
-  else if (lanes == 32) start(s8 ? cache_write_kernel<true, 32> : cache_write_kernel<false, 32>);
-  else start(s8 ? cache_write_kernel<true, 64> : cache_write_kernel<false, 64>);
+  if (lanes == 16) start(cache_write_kernel<TFCC_ROCM_S4, 16>, cache_write_kernel<TFCC_ROCM_S8, 16>, cache_write_kernel<TFCC_ROCM_F32, 16>);
+  else if (lanes == 32) start(cache_write_kernel<TFCC_ROCM_S4, 32>, cache_write_kernel<TFCC_ROCM_S8, 32>, cache_write_kernel<TFCC_ROCM_F32, 32>);
+  else start(cache_write_kernel<TFCC_ROCM_S4, 64>, cache_write_kernel<TFCC_ROCM_S8, 64>, cache_write_kernel<TFCC_ROCM_F32, 64>);
   return check_launch("cache_write");
 }
 
@@ -211,14 +284,56 @@ int tfcc_rocm_cache_read(void* stream, const tfcc_rocm_paged_cache* cache, const
   TFCC_REQUIRE(table && starts && keys && values, "cache_read: null argument");
   ReadArgs a{view_of(*cache), table, table_stride, table_width, batch, starts, tokens, keys, values};
   const hipStream_t s = as_stream(stream);
-  const bool s8 = cache->type == TFCC_ROCM_S8;
-  const auto start = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((tokens + kReadTokens - 1) / kReadTokens, 2), dim3(kCacheThreads), 0, s, a);
+  const auto start = [&](auto s4, auto s8, auto f32) {
+    hipLaunchKernelGGL((cache->type == TFCC_ROCM_S4 ? s4 : cache->type == TFCC_ROCM_S8 ? s8 : f32), dim3((tokens + kReadTokens - 1) / kReadTokens, 2), dim3(kCacheThreads), 0, s, a);
   };
-  if (cache->size <= 64) start(s8 ? cache_read_kernel<true, 16> : cache_read_kernel<false, 16>);
-  else if (cache->size <= 128) start(s8 ? cache_read_kernel<true, 32> : cache_read_kernel<false, 32>);
-  else start(s8 ? cache_read_kernel<true, 64> : cache_read_kernel<false, 64>);
+  if (cache->size <= 64) start(cache_read_kernel<TFCC_ROCM_S4, 16>, cache_read_kernel<TFCC_ROCM_S8, 16>, cache_read_kernel<TFCC_ROCM_F32, 16>);
+  else if (cache->size <= 128) start(cache_read_kernel<TFCC_ROCM_S4, 32>, cache_read_kernel<TFCC_ROCM_S8, 32>, cache_read_kernel<TFCC_ROCM_F32, 32>);
+  else start(cache_read_kernel<TFCC_ROCM_S4, 64>, cache_read_kernel<TFCC_ROCM_S8, 64>, cache_read_kernel<TFCC_ROCM_F32, 64>);
   return check_launch("cache_read");
+}
+
+int tfcc_rocm_cache_copy(void* stream, const tfcc_rocm_paged_cache* cache, const void* sources, const void* destinations, int slot_type,
+                         const int32_t* rows, unsigned runs) {
+  TFCC_REQUIRE(cache != nullptr, "cache_copy: null cache");
+  const tfcc_rocm_paged_cache& c = *cache;
+  if (int e = check_cache(c, "cache_copy")) return e;
+  TFCC_REQUIRE(slot_type == TFCC_ROCM_S32 || slot_type == TFCC_ROCM_S64, "cache_copy: slot type %d", slot_type);
+  if (runs == 0) return TFCC_ROCM_OK;
+  if (int e = check_written(c, "cache_copy")) return e;
+  CopyArgs a{};
+  const unsigned element = element_bytes(c), bytes = row_bytes(c);
+  const bool wide = (bytes | c.page_stride * element | c.head_stride * element | c.row_stride * element | reinterpret_cast<uintptr_t>(c.keys) |
+                     reinterpret_cast<uintptr_t>(c.values)) % 16 == 0;
+  const unsigned unit = wide ? 16 : 8;
+  a.rows_of[0] = c.keys;
+  a.rows_of[1] = c.values;
+  a.scales_of[0] = c.key_scales;
+  a.scales_of[1] = c.value_scales;
+  a.page = c.page_stride * element;
+  a.head = c.head_stride * element;
+  a.row = c.row_stride * element;
+  a.scale_page = c.scale_page_stride * 4;
+  a.scale_head = c.scale_head_stride * 4;
+  a.scale_row = c.scale_row_stride * 4;
+  a.sources = sources;
+  a.destinations = destinations;
+  a.rows = rows;
+  a.wide_slots = slot_type == TFCC_ROCM_S64;
+  a.pages = c.pages;
+  a.page_size = Divisor::of(c.page_size);
+  a.chunks = Divisor::of(bytes / unit);
+  const uint64_t units = (uint64_t)c.heads * c.page_size * (bytes / unit), scales = has_scales(c) ? (uint64_t)c.heads * c.page_size : 0;
+  const uint64_t row_pieces = (units + kCopyUnits - 1) / kCopyUnits, pieces = row_pieces + (scales + kCopyUnits - 1) / kCopyUnits;
+  TFCC_REQUIRE(units <= 0x7fffffffu - kCopyUnits && pieces * runs <= 0x7fffffffu / kCacheThreads, "cache_copy: %u runs of up to %llu bytes", runs,
+               (unsigned long long)units * unit);
+  TFCC_REQUIRE(sources && destinations, "cache_copy: null argument");
+  a.units = (unsigned)units;
+  a.scale_units = (unsigned)scales;
+  a.row_pieces = (unsigned)row_pieces;
+  a.pieces = Divisor::of((unsigned)pieces);
+  hipLaunchKernelGGL((wide ? cache_copy_kernel<16> : cache_copy_kernel<8>), dim3((unsigned)pieces * runs, 2), dim3(kCacheThreads), 0, as_stream(stream), a);
+  return check_launch("cache_copy");
 }
 
 }  // extern "C"

@@ -34,18 +34,33 @@ inline CacheView view_of(const tfcc_rocm_paged_cache& c) {
           c.scale_head_stride, c.scale_row_stride, c.pages, c.heads, c.size, Divisor::of(c.page_size)};
 }
 
+// Integers of 8 or 4 bits with scales.
+inline bool has_scales(const tfcc_rocm_paged_cache& c) { return c.type != TFCC_ROCM_F32; }
+// Bytes of a row of a head, and of an element that strides count.
+inline unsigned row_bytes(const tfcc_rocm_paged_cache& c) { return c.type == TFCC_ROCM_F32 ? 4 * c.size : c.type == TFCC_ROCM_S8 ? c.size : c.size / 2; }
+inline unsigned element_bytes(const tfcc_rocm_paged_cache& c) { return c.type == TFCC_ROCM_F32 ? 4 : 1; }
+
 inline int check_cache(const tfcc_rocm_paged_cache& c, const char* what) {
-  TFCC_REQUIRE(c.type == TFCC_ROCM_F32 || c.type == TFCC_ROCM_S8, "%s: a cache of type %d", what, c.type);
-  const bool s8 = c.type == TFCC_ROCM_S8;
-  const unsigned unit = s8 ? 8 : 4, bytes = s8 ? 8 : 16;
-  TFCC_REQUIRE(c.keys && c.values && (!s8 || (c.key_scales && c.value_scales)), "%s: null cache", what);
-  TFCC_REQUIRE(c.size > 0 && c.size <= kCacheMostSize && c.size % unit == 0, "%s: heads of %u values (a multiple of %u up to %u)", what,
-               c.size, unit, kCacheMostSize);
+  TFCC_REQUIRE(c.type == TFCC_ROCM_F32 || c.type == TFCC_ROCM_S8 || c.type == TFCC_ROCM_S4, "%s: a cache of type %d", what, c.type);
+  const bool scaled = has_scales(c);
+  const unsigned unit = scaled ? 8 : 4, bytes = scaled ? 8 : 16, values = c.type == TFCC_ROCM_S4 ? 16 : unit;
+  TFCC_REQUIRE(c.keys && c.values && (!scaled || (c.key_scales && c.value_scales)), "%s: null cache", what);
+  TFCC_REQUIRE(c.size > 0 && c.size <= kCacheMostSize && c.size % values == 0, "%s: heads of %u values (a multiple of %u up to %u)", what,
+               c.size, values, kCacheMostSize);
   TFCC_REQUIRE(c.heads > 0 && c.heads <= 65535, "%s: %u cache heads", what, c.heads);
   TFCC_REQUIRE(c.page_size > 0 && c.page_size <= (1u << 24), "%s: pages of %u rows", what, c.page_size);
   TFCC_REQUIRE(c.pages > 0 && c.pages <= 0x7fffffffu, "%s: %u pages", what, c.pages);
   TFCC_REQUIRE((c.page_stride | c.head_stride | c.row_stride) % unit == 0, "%s: cache strides that are not multiples of %u", what, unit);
   TFCC_REQUIRE((reinterpret_cast<uintptr_t>(c.keys) | reinterpret_cast<uintptr_t>(c.values)) % bytes == 0, "%s: cache memory off %u bytes", what, bytes);
+  return TFCC_ROCM_OK;
+}
+
+// Memory that several rows share can be read, but not written.
+inline int check_written(const tfcc_rocm_paged_cache& c, const char* what) {
+  TFCC_REQUIRE((c.pages == 1 || c.page_stride > 0) && (c.heads == 1 || c.head_stride > 0) && (c.page_size == 1 || c.row_stride > 0), "%s: a cache stride of 0", what);
+  TFCC_REQUIRE(!has_scales(c) || ((c.pages == 1 || c.scale_page_stride > 0) && (c.heads == 1 || c.scale_head_stride > 0) &&
+                                  (c.page_size == 1 || c.scale_row_stride > 0)),
+               "%s: a cache scale stride of 0", what);
   return TFCC_ROCM_OK;
 }
 

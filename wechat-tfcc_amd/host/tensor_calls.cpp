@@ -385,23 +385,28 @@ bool number(PyObject* o, int64_t* v) {
   return !overflow && x >= 0 && x <= INT32_MAX;
 }
 
-// The memory of a paged cache: a tuple of two tensors of float32, or of two of int8 and two of scales.
+// The memory of a paged cache: a tuple of two tensors of float32, or of two of int8, or of uint8 with two integers of 4 bits in each, and two of scales.
 bool cache_of(PyObject* o, c10::DeviceIndex device, tfcc_rocm_paged_cache& c) {
   if (!PyTuple_CheckExact(o)) return false;
   const Py_ssize_t n = PyTuple_GET_SIZE(o);
   if (n != 2 && n != 4) return false;
-  const at::ScalarType type = n == 4 ? at::kChar : at::kFloat;
+  at::ScalarType type = n == 4 ? at::kChar : at::kFloat;
   const Tensor* keys = rows_of(PyTuple_GET_ITEM(o, 0), type, 4, device);
+  if (!keys && n == 4) keys = rows_of(PyTuple_GET_ITEM(o, 0), type = at::kByte, 4, device);
   const Tensor* values = rows_of(PyTuple_GET_ITEM(o, 1), type, 4, device);
   if (!keys || !values || keys->sizes() != values->sizes() || keys->strides() != values->strides()) return false;
   if (!fits(keys->size(0)) || !fits(keys->size(1)) || !fits(keys->size(2)) || !fits(keys->size(3))) return false;
   c.keys = data(keys);
   c.values = data(values);
-  c.type = n == 4 ? TFCC_ROCM_S8 : TFCC_ROCM_F32;
+  c.type = type == at::kChar ? TFCC_ROCM_S8 : type == at::kByte ? TFCC_ROCM_S4 : TFCC_ROCM_F32;
   c.pages = static_cast<unsigned>(keys->size(0));
   c.heads = static_cast<unsigned>(keys->size(1));
   c.page_size = static_cast<unsigned>(keys->size(2));
   c.size = static_cast<unsigned>(keys->size(3));
+  if (type == at::kByte) {
+    if (c.size > 1024) return false;
+    c.size *= 2;
+  }
   c.page_stride = keys->stride(0);
   c.head_stride = keys->stride(1);
   c.row_stride = keys->stride(2);
@@ -507,6 +512,24 @@ PyObject* cache_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// cache_copy(cache, sources, destinations, rows or None): True where it was done
+PyObject* cache_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !THPVariable_CheckExact(args[1])) return none();
+  Here here(args[1]);
+  tfcc_rocm_paged_cache c{};
+  const int64_t runs = THPVariable_Unpack(args[1]).numel();
+  const Tensor *sources, *destinations, *rows = args[3] == Py_None ? nullptr : plain(args[3], at::kInt, here.device);
+  const int type = integers(args[1], runs, here.device, &sources);
+  if (type < 0 || integers(args[2], runs, here.device, &destinations) != type || !fits(runs) || !cache_of(args[0], here.device, c)) return none();
+  if (args[3] != Py_None && (!rows || rows->dim() != 1 || rows->size(0) != runs)) return none();
+  void* stream = here.stream();
+  if (launch([&] { return tfcc_rocm_cache_copy(stream, &c, data(sources), data(destinations), type, data<int32_t>(rows), static_cast<unsigned>(runs)); }) != TFCC_ROCM_OK)
+    return none();
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length)
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -590,11 +613,79 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// rms_norm(x, weight, eps, residual or None, quantized)
+PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5 || !PyFloat_CheckExact(args[2]) || !PyBool_Check(args[4])) return none();
+  Here here(args[0]);
+  const Tensor *x = plain(args[0], at::kFloat, here.device), *weight = plain(args[1], at::kFloat, here.device);
+  const Tensor* residual = args[3] == Py_None ? nullptr : plain(args[3], at::kFloat, here.device);
+  if (!x || !weight || (args[3] != Py_None && !residual) || x->dim() < 1 || x->numel() == 0 || weight->dim() != 1) return none();
+  const int64_t width = x->size(x->dim() - 1), rows = x->numel() / width;
+  if (weight->size(0) != width || (residual && residual->sizes() != x->sizes()) || !fits(width) || !fits(rows)) return none();
+  tfcc_rocm_rms_norm_desc d{};
+  Tensor sum, out, scales, sums;
+  if (residual) sum = empty(x->sizes(), at::kFloat, here.device);
+  d.x = data<float>(x);
+  d.weight = data<float>(weight);
+  d.residual = data<float>(residual);
+  d.sum = residual ? data<float>(sum) : nullptr;
+  d.rows = static_cast<unsigned>(rows);
+  d.width = static_cast<unsigned>(width);
+  d.eps = static_cast<float>(PyFloat_AS_DOUBLE(args[2]));
+  d.x_row_stride = d.residual_row_stride = d.sum_row_stride = d.out_row_stride = d.steps_row_stride = static_cast<uint64_t>(width);
+  const bool quantized = args[4] == Py_True;
+  out = empty(x->sizes(), quantized ? at::kByte : at::kFloat, here.device);
+  if (quantized) {
+    const at::IntArrayRef shape = x->sizes().slice(0, x->dim() - 1);
+    scales = empty(shape, at::kFloat, here.device);
+    sums = empty(shape, at::kInt, here.device);
+    d.steps = data<uint8_t>(out);
+    d.scales = data<float>(scales);
+    d.sums = data<int32_t>(sums);
+  } else {
+    d.out = data<float>(out);
+  }
+  void* stream = here.stream();
+  if (launch([&] { return tfcc_rocm_rms_norm_f32(stream, &d); }) != TFCC_ROCM_OK) return none();
+  PyObject* held = residual ? wrap(std::move(sum)) : none();
+  if (quantized) return pack({wrap(std::move(out)), wrap(std::move(scales)), wrap(std::move(sums)), held});
+  return pack({wrap(std::move(out)), held});
+  END_HANDLE_TH_ERRORS
+}
+
+// dequantize_rows(a, scales, offset, column_scales or None)
+PyObject* dequantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4 || !THPVariable_CheckExact(args[0]) || !PyLong_CheckExact(args[2])) return none();
+  Here here(args[0]);
+  const at::ScalarType type = THPVariable_Unpack(args[0]).scalar_type();
+  const int code = quantized_code(type);
+  const Tensor *a = plain(args[0], type, here.device), *scales = plain(args[1], at::kFloat, here.device);
+  const Tensor* columns = args[3] == Py_None ? nullptr : plain(args[3], at::kFloat, here.device);
+  if (!a || !scales || (args[3] != Py_None && !columns) || code < 0 || a->dim() < 1 || a->numel() == 0) return none();
+  const int64_t width = a->size(a->dim() - 1), rows = a->numel() / width;
+  if (scales->sizes() != a->sizes().slice(0, a->dim() - 1) || (columns && (columns->dim() != 1 || columns->size(0) != width)) || !fits(width) || !fits(rows)) return none();
+  int overflow = 0;
+  const long long offset = PyLong_AsLongLongAndOverflow(args[2], &overflow);
+  if (overflow || offset < INT32_MIN || offset > INT32_MAX) return none();
+  Tensor out = empty(a->sizes(), at::kFloat, here.device);
+  void* stream = here.stream();
+  if (launch([&] {
+        return tfcc_rocm_dequantize_rows(stream, data(a), code, static_cast<unsigned>(rows), static_cast<unsigned>(width), static_cast<int32_t>(offset),
+                                         data<float>(scales), data<float>(columns), data<float>(out));
+      }) != TFCC_ROCM_OK)
+    return none();
+  return wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define TENSOR_CALL(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(NAME)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TENSOR_CALL(blas_matmul), TENSOR_CALL(reduce_sum), TENSOR_CALL(quantization_matmul),
                          TENSOR_CALL(quantization_matmul_requantize), TENSOR_CALL(gemv_dequant), TENSOR_CALL(gemv_dequant_packed),
                          TENSOR_CALL(quantize), TENSOR_CALL(dequantize), TENSOR_CALL(rotary),
-                         TENSOR_CALL(cache_write), TENSOR_CALL(cache_read), TENSOR_CALL(paged_attention), TENSOR_CALL(sample), {nullptr, nullptr, 0, nullptr}};
+                         TENSOR_CALL(cache_write), TENSOR_CALL(cache_read), TENSOR_CALL(cache_copy), TENSOR_CALL(paged_attention), TENSOR_CALL(sample),
+                         TENSOR_CALL(rms_norm), TENSOR_CALL(dequantize_rows), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
