@@ -109,6 +109,11 @@ class PagedAttentionDesc(C.Structure):
          ("workspace_bytes", C.c_size_t)]
 
 
+class AttentionScores(C.Structure):
+    """tfcc_rocm_attention_scores"""
+    _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("prefixes", C.c_void_p)]
+
+
 class RmsNormDesc(C.Structure):
     """tfcc_rocm_rms_norm_desc"""
     _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "weight", "sum", "out", "steps", "scales", "sums")] + \
@@ -215,6 +220,7 @@ SYMBOLS = {
     "tfcc_rocm_cache_copy": (_I, [_VP, C.POINTER(PagedCache), _VP, _VP, _I, _VP, _U]),
     "tfcc_rocm_paged_attention_workspace": (C.c_size_t, [C.POINTER(PagedAttentionDesc)]),
     "tfcc_rocm_paged_attention_f32": (_I, [_VP, C.POINTER(PagedAttentionDesc)]),
+    "tfcc_rocm_paged_attention_scores_f32": (_I, [_VP, C.POINTER(PagedAttentionDesc), C.POINTER(AttentionScores)]),
     "tfcc_rocm_sample_workspace": (C.c_size_t, [_U, _U]),
     "tfcc_rocm_sample_f32": (_I, [_VP, C.POINTER(SampleDesc)]),
     "tfcc_rocm_rms_norm_f32": (_I, [_VP, C.POINTER(RmsNormDesc)]),
@@ -1301,19 +1307,23 @@ def cache_copy(cache, sources, destinations, rows=None):
     check(lib().tfcc_rocm_cache_copy(_stream(), C.byref(d), _ptr(sources), _ptr(destinations), _type_code(sources.dtype), _ptr(rows), runs))
 
 
-def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window=0, max_length=0, out=None):
+def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window=0, max_length=0, out=None, cap=0.0, slopes=None, prefixes=None):
     """Attention of a chunk of new tokens of each sequence over what the cache holds of it: tfcc_rocm_paged_attention_f32.  q
     [tokens, heads, size]: the chunks back to back, sequence i's rows starts[i] to starts[i + 1] - 1 (int32 [batch + 1]); lengths
     (int32 [batch]): cached tokens, the chunk's own among them; table: int32 [batch, pages].  max_length: an upper bound of lengths
-    that the program knows, which the work is dealt out by.  Rows of out behind the last sequence are left as they were."""
+    that the program knows, which the work is dealt out by.  Rows of out behind the last sequence are left as they were.
+
+    Shaped scores (tfcc_rocm_paged_attention_scores_f32): cap > 0 makes x = scale * q k^T cap * tanh(x / cap), slopes (float32 [heads])
+    take slope * |distance of the positions| off it, and of sequence i all tokens see the first prefixes[i] cached ones (int32 [batch];
+    causal, no window)."""
     if out is None:
-        done = _native().paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length)
+        done = _native().paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length, cap, slopes, prefixes)
         if done is not None:
             return done
     import torch
     d = PagedAttentionDesc()
     d.cache = _cache_desc(cache)
-    _on_device(cache[0].device, q, table, starts, lengths, out)
+    _on_device(cache[0].device, q, table, starts, lengths, out, slopes, prefixes)
     q = _heads_of(q, "q")
     if q.shape[2] != d.cache.size or q.shape[1] == 0 or q.shape[1] % d.cache.heads:
         raise InvalidArgumentError("invalid q")
@@ -1323,6 +1333,12 @@ def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window
     starts = _integers(starts, "starts", batch + 1, (torch.int32,))
     if window < 0 or max_length < 0 or (window and not causal):
         raise InvalidArgumentError("invalid window")
+    if not 0 <= cap <= 3.4028234e38:
+        raise InvalidArgumentError("invalid cap")
+    slopes = None if slopes is None else _integers(slopes, "slopes", q.shape[1], (torch.float32,))
+    prefixes = None if prefixes is None else _integers(prefixes, "prefixes", batch, (torch.int32,))
+    if prefixes is not None and (window or not causal):
+        raise InvalidArgumentError("invalid prefixes")
     if out is None:
         out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
     elif not _written_heads(out, q):
@@ -1338,7 +1354,8 @@ def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window
     needs = lib().tfcc_rocm_paged_attention_workspace(C.byref(d))
     workspace = torch.empty(needs, dtype=torch.uint8, device=q.device) if needs else None
     d.workspace, d.workspace_bytes = _ptr(workspace), needs
-    check(lib().tfcc_rocm_paged_attention_f32(_stream(), C.byref(d)))
+    scores = AttentionScores(cap, _ptr(slopes), _ptr(prefixes))
+    check(lib().tfcc_rocm_paged_attention_scores_f32(_stream(), C.byref(d), C.byref(scores)))
     return out
 
 

@@ -530,10 +530,10 @@ PyObject* cache_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length)
+// paged_attention(q, cache, table, starts, lengths, scale, causal, window, max_length, cap, slopes or None, prefixes or None)
 PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 9 || !PyFloat_CheckExact(args[5]) || !PyBool_Check(args[6])) return none();
+  if (n != 12 || !PyFloat_CheckExact(args[5]) || !PyBool_Check(args[6]) || !PyFloat_CheckExact(args[9])) return none();
   Here here(args[0]);
   tfcc_rocm_paged_attention_desc d{};
   const Tensor* q = rows_of(args[0], at::kFloat, 3, here.device);
@@ -544,6 +544,17 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t batch = table->size(0);
   if (lengths->dim() != 1 || lengths->size(0) != batch || starts->dim() != 1 || starts->size(0) != batch + 1) return none();
   if (!fits(q->size(0)) || !fits(q->size(1)) || q->size(2) != d.cache.size || !fits(batch) || !fits(table->size(1))) return none();
+  tfcc_rocm_attention_scores scores{static_cast<float>(PyFloat_AS_DOUBLE(args[9])), nullptr, nullptr};
+  if (args[10] != Py_None) {
+    const Tensor* slopes = plain(args[10], at::kFloat, here.device);
+    if (!slopes || slopes->dim() != 1 || slopes->size(0) != q->size(1)) return none();
+    scores.slopes = data<float>(slopes);
+  }
+  if (args[11] != Py_None) {
+    const Tensor* prefixes = plain(args[11], at::kInt, here.device);
+    if (!prefixes || prefixes->dim() != 1 || prefixes->size(0) != batch) return none();
+    scores.prefixes = data<int32_t>(prefixes);
+  }
   Tensor out = empty(q->sizes(), at::kFloat, here.device);
   d.q = data<float>(q);
   d.out = data<float>(out);
@@ -570,7 +581,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     d.workspace = data(workspace);
   }
   void* stream = here.stream();
-  if (launch([&] { return tfcc_rocm_paged_attention_f32(stream, &d); }) != TFCC_ROCM_OK) return none();
+  if (launch([&] { return tfcc_rocm_paged_attention_scores_f32(stream, &d, &scores); }) != TFCC_ROCM_OK) return none();
   return wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }

@@ -2,6 +2,7 @@
 // ROCm device: every GPU action goes through the C ABI of libtfcc_rocm.so.
 #include <algorithm>
 #include <chrono>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <limits>
@@ -1774,22 +1775,24 @@ Shape countable(std::initializer_list<unsigned> dims, const char* text) {
 // Its tensors are public: one may have been put in the place of another, or moved out.
 template <class T>
 tfcc_rocm_paged_cache held_by(const PagedCache<T>& c) {
+  constexpr bool scaled = !std::is_same<T, float>::value, halves = std::is_same<T, Int4>::value;
+  typedef typename CacheElement<T>::type Element;
   const Shape& s = c.keys.shape();
-  if (s.size() != 4 || s.area() == 0 || c.values.shape() != s) throw InvalidArgumentError("invalid cache");
-  if (std::is_same<T, int8_t>::value && (c.keyScales.shape() != Shape({s[0], s[1], s[2]}) || c.valueScales.shape() != c.keyScales.shape()))
+  if (s.size() != 4 || s.area() == 0 || c.values.shape() != s || (halves && s[3] > 1024)) throw InvalidArgumentError("invalid cache");
+  if (scaled && (c.keyScales.shape() != Shape({s[0], s[1], s[2]}) || c.valueScales.shape() != c.keyScales.shape()))
     throw InvalidArgumentError("invalid cache");
   tfcc_rocm_paged_cache d{};
-  d.keys = const_cast<T*>(c.keys.data());
-  d.values = const_cast<T*>(c.values.data());
-  d.type = std::is_same<T, int8_t>::value ? TFCC_ROCM_S8 : TFCC_ROCM_F32;
+  d.keys = const_cast<Element*>(c.keys.data());
+  d.values = const_cast<Element*>(c.values.data());
+  d.type = halves ? TFCC_ROCM_S4 : scaled ? TFCC_ROCM_S8 : TFCC_ROCM_F32;
   d.pages = c.keys.shape(0);
   d.heads = c.keys.shape(1);
   d.page_size = c.keys.shape(2);
-  d.size = c.keys.shape(3);
-  d.row_stride = d.size;
+  d.size = halves ? 2 * c.keys.shape(3) : c.keys.shape(3);
+  d.row_stride = c.keys.shape(3);
   d.head_stride = d.row_stride * d.page_size;
   d.page_stride = d.head_stride * d.heads;
-  if (std::is_same<T, int8_t>::value) {
+  if (scaled) {
     d.key_scales = const_cast<float*>(c.keyScales.data());
     d.value_scales = const_cast<float*>(c.valueScales.data());
     d.scale_row_stride = 1;
@@ -1845,12 +1848,12 @@ std::tuple<Variable<float>, Variable<float>> rotary(const Tensor<float>& q, cons
 
 template <class T>
 PagedCache<T>::PagedCache(unsigned pages, unsigned heads, unsigned pageSize, unsigned size)
-    : keys(countable({pages, heads, pageSize, size}, "invalid cache")), values(keys.shape()) {
-  if (keys.size() == 0) throw InvalidArgumentError("invalid cache");
+    : keys(countable({pages, heads, pageSize, std::is_same<T, Int4>::value ? size / 2 : size}, "invalid cache")), values(keys.shape()) {
+  if (keys.size() == 0 || (std::is_same<T, Int4>::value && size % 2 != 0)) throw InvalidArgumentError("invalid cache");
   require_rocm();
   data::zeros(keys);
   data::zeros(values);
-  if (std::is_same<T, int8_t>::value) {
+  if (!std::is_same<T, float>::value) {
     keyScales = Variable<float>({pages, heads, pageSize});
     valueScales = Variable<float>({pages, heads, pageSize});
     data::zeros(keyScales);
@@ -1883,8 +1886,19 @@ std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>& cac
 }
 
 template <class T>
+void cache_copy(PagedCache<T>& cache, const Tensor<int32_t>& sources, const Tensor<int32_t>& destinations, const Tensor<int32_t>* rows) {
+  if (sources.shape().size() != 1) throw InvalidArgumentError("invalid sources");
+  const unsigned runs = sources.shape(0);
+  require_list(destinations, runs, "invalid destinations");
+  if (rows) require_list(*rows, runs, "invalid rows");
+  require_rocm();
+  const tfcc_rocm_paged_cache d = held_by(cache);
+  check(tfcc_rocm_cache_copy(current_stream(), &d, sources.data(), destinations.data(), TFCC_ROCM_S32, rows ? rows->data() : nullptr, runs));
+}
+
+template <class T>
 Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
-                                const Tensor<int32_t>& lengths, float scale, bool causal, unsigned window, unsigned maxLength) {
+                                const Tensor<int32_t>& lengths, float scale, bool causal, unsigned window, unsigned maxLength, const ScoreShape& shape) {
   require_heads(q, "invalid q");
   tfcc_rocm_paged_attention_desc d{};
   d.cache = held_by(cache);
@@ -1893,6 +1907,12 @@ Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cac
   if (table.shape().size() != 2 || table.shape(0) != lengths.shape(0)) throw InvalidArgumentError("invalid table");
   require_list(starts, lengths.shape(0) + 1, "invalid starts");
   if (window > 0 && !causal) throw InvalidArgumentError("invalid window");
+  if (!(shape.cap >= 0.0f && std::isfinite(shape.cap))) throw InvalidArgumentError("invalid cap");
+  if (shape.slopes) require_list(*shape.slopes, q.shape(1), "invalid slopes");
+  if (shape.prefixes) {
+    require_list(*shape.prefixes, lengths.shape(0), "invalid prefixes");
+    if (!causal || window > 0) throw InvalidArgumentError("invalid prefixes");
+  }
   require_rocm();
   Variable<float> out(q.shape());
   d.q = q.data();
@@ -1917,9 +1937,82 @@ Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cac
     workspace = Variable<uint8_t>({static_cast<unsigned>(d.workspace_bytes)});
     d.workspace = workspace.data();
   }
-  check(tfcc_rocm_paged_attention_f32(current_stream(), &d));
+  const tfcc_rocm_attention_scores scores{shape.cap, shape.slopes ? shape.slopes->data() : nullptr, shape.prefixes ? shape.prefixes->data() : nullptr};
+  check(tfcc_rocm_paged_attention_scores_f32(current_stream(), &d, &scores));
   return out;
 }
+
+namespace {
+
+// The common part of both norms; `shape` is that of the rows' scales.
+tfcc_rocm_rms_norm_desc describe_norm(const Tensor<float>& x, const Tensor<float>& weight, float eps, const Tensor<float>* residual, Variable<float>& sum,
+                                      std::vector<unsigned>& shape) {
+  if (x.shape().size() < 1 || x.shape(x.shape().size() - 1) == 0) throw InvalidArgumentError("invalid x");
+  const unsigned width = x.shape(x.shape().size() - 1);
+  require_list(weight, width, "invalid weight");
+  if (residual && residual->shape() != x.shape()) throw InvalidArgumentError("invalid residual");
+  if (!(eps >= 0.0f && std::isfinite(eps))) throw InvalidArgumentError("invalid eps");
+  require_rocm();
+  for (size_t i = 0; i + 1 < x.shape().size(); ++i) shape.push_back(x.shape(i));
+  if (shape.empty()) shape.push_back(1);
+  tfcc_rocm_rms_norm_desc d{};
+  d.x = x.data();
+  d.weight = weight.data();
+  if (residual) {
+    sum = Variable<float>(x.shape());
+    d.residual = residual->data();
+    d.sum = sum.data();
+  }
+  d.rows = x.size() / width;
+  d.width = width;
+  d.eps = eps;
+  d.x_row_stride = d.residual_row_stride = d.sum_row_stride = d.out_row_stride = d.steps_row_stride = width;
+  return d;
+}
+
+}  // namespace
+
+std::tuple<Variable<float>, Variable<float>> rms_norm(const Tensor<float>& x, const Tensor<float>& weight, float eps, const Tensor<float>* residual) {
+  Variable<float> sum;
+  std::vector<unsigned> shape;
+  tfcc_rocm_rms_norm_desc d = describe_norm(x, weight, eps, residual, sum, shape);
+  Variable<float> out(x.shape());
+  d.out = out.data();
+  if (d.rows > 0) check(tfcc_rocm_rms_norm_f32(current_stream(), &d));
+  return std::make_tuple(std::move(out), std::move(sum));
+}
+
+QuantizedRows rms_norm_quantized(const Tensor<float>& x, const Tensor<float>& weight, float eps, const Tensor<float>* residual) {
+  QuantizedRows r;
+  std::vector<unsigned> shape;
+  tfcc_rocm_rms_norm_desc d = describe_norm(x, weight, eps, residual, r.sum, shape);
+  r.steps = Variable<uint8_t>(x.shape());
+  r.scales = Variable<float>(Shape(shape));
+  r.sums = Variable<int32_t>(Shape(shape));
+  d.steps = r.steps.data();
+  d.scales = r.scales.data();
+  d.sums = r.sums.data();
+  if (d.rows > 0) check(tfcc_rocm_rms_norm_f32(current_stream(), &d));
+  return r;
+}
+
+template <class T>
+Variable<float> dequantize_rows(const Tensor<T>& a, const Tensor<float>& scales, int32_t offset, const Tensor<float>* columnScales) {
+  if (a.shape().size() < 1) throw InvalidArgumentError("invalid a");
+  const unsigned width = a.shape(a.shape().size() - 1), rows = width == 0 ? 0 : a.size() / width;
+  if (width != 0 && scales.size() != rows) throw InvalidArgumentError("invalid scales");
+  if (columnScales) require_list(*columnScales, width, "invalid columnScales");
+  if (a.size() > 0x7fffffffu) throw InvalidArgumentError("invalid a");
+  require_rocm();
+  Variable<float> out(a.shape());
+  const int code = std::is_same<T, int32_t>::value ? TFCC_ROCM_S32 : std::is_same<T, int8_t>::value ? TFCC_ROCM_S8 : TFCC_ROCM_U8;
+  if (a.size() > 0)
+    check(tfcc_rocm_dequantize_rows(current_stream(), a.data(), code, rows, width, offset, scales.data(), columnScales ? columnScales->data() : nullptr, out.data()));
+  return out;
+}
+template Variable<float> dequantize_rows(const Tensor<int32_t>&, const Tensor<float>&, int32_t, const Tensor<float>*);
+template Variable<float> dequantize_rows(const Tensor<int8_t>&, const Tensor<float>&, int32_t, const Tensor<float>*);
+template Variable<float> dequantize_rows(const Tensor<uint8_t>&, const Tensor<float>&, int32_t, const Tensor<float>*);
 
 std::tuple<Variable<int64_t>, Variable<float>> sample(const Tensor<float>& logits, const Tensor<float>& random, const SampleFilters& filters) {
   if (logits.shape().size() != 2 || logits.shape(1) == 0) throw InvalidArgumentError("invalid logits");
@@ -1957,10 +2050,12 @@ std::tuple<Variable<int64_t>, Variable<float>> sample(const Tensor<float>& logit
   template struct PagedCache<T>;                                                                                                       \
   template void cache_write(PagedCache<T>&, const Tensor<float>&, const Tensor<float>&, const Tensor<int32_t>&);                       \
   template std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>&, const Tensor<int32_t>&, const Tensor<int32_t>&, unsigned); \
+  template void cache_copy(PagedCache<T>&, const Tensor<int32_t>&, const Tensor<int32_t>&, const Tensor<int32_t>*);                    \
   template Variable<float> paged_attention(const Tensor<float>&, const PagedCache<T>&, const Tensor<int32_t>&, const Tensor<int32_t>&,  \
-                                           const Tensor<int32_t>&, float, bool, unsigned, unsigned);
+                                           const Tensor<int32_t>&, float, bool, unsigned, unsigned, const ScoreShape&);
 TFCC_PAGED_CACHE(float)
 TFCC_PAGED_CACHE(int8_t)
+TFCC_PAGED_CACHE(Int4)
 #undef TFCC_PAGED_CACHE
 
 }  // namespace generation

@@ -246,8 +246,8 @@ std::tuple<Variable<int32_t>, Variable<float>, Variable<float>> matmul(
 
 }  // namespace quantization
 
-// What a language model does between its products: rotary positions, a paged cache of keys and values, attention over it, the
-// choice of a token.  The calls of the same names in include/tfcc_rocm.h say what each computes, skips and leaves; here are their tensors and
+// What a language model does between its products: the norm in front of them, rotary positions, a paged cache of keys and values, attention
+// over it, the choice of a token.  The calls of the same names in include/tfcc_rocm.h say what each computes, skips and leaves; here are their tensors and
 // checks.  They need the ROCm device as the thread default.
 namespace generation {
 
@@ -259,12 +259,22 @@ std::tuple<std::vector<double>, float> rotary_frequencies(unsigned part, double 
 std::tuple<Variable<float>, Variable<float>> rotary(const Tensor<float>& q, const Tensor<float>& k, const Tensor<int32_t>& positions,
                                                     const Tensor<double>& frequencies, bool interleaved = false, float magnitude = 1.0f);
 
-// Memory of a cache, all zeros at first.  T = float, or int8_t with a scale for each row of a head.  A tensor here counts its elements in 32
+// Integers of 4 bits, two to a byte.
+struct Int4 {};
+template <class T>
+struct CacheElement {
+  typedef T type;
+};
+template <>
+struct CacheElement<Int4> {
+  typedef uint8_t type;
+};
+// Memory of a cache, all zeros at first.  T = float, or int8_t or Int4 with a scale for each row of a head.  A tensor here counts its elements in 32
 // bits: a cache or a result of cache_read of more is refused (the C interface takes any size).
 template <class T>
 struct PagedCache {
-  Variable<T> keys, values;                 // [pages, heads, rows, size]
-  Variable<float> keyScales, valueScales;   // [pages, heads, rows], int8_t only
+  Variable<typename CacheElement<T>::type> keys, values;  // [pages, heads, rows, size], Int4: size / 2 bytes
+  Variable<float> keyScales, valueScales;                 // [pages, heads, rows], int8_t and Int4
   PagedCache(unsigned pages, unsigned heads, unsigned pageSize, unsigned size);
 };
 // keys and values [tokens, heads, size] to slots [tokens] (page * rows + row; -1: skipped)
@@ -274,10 +284,34 @@ void cache_write(PagedCache<T>& cache, const Tensor<float>& keys, const Tensor<f
 template <class T>
 std::tuple<Variable<float>, Variable<float>> cache_read(const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
                                                         unsigned tokens);
+// rows[i] slots (null: up to the end of the source's page) from sources[i] on to those from destinations[i] on, each [runs]
+template <class T>
+void cache_copy(PagedCache<T>& cache, const Tensor<int32_t>& sources, const Tensor<int32_t>& destinations, const Tensor<int32_t>* rows = nullptr);
+// A cap of the scores, 0: none; a slope for each query head [heads] and a prefix of each sequence [batch], or null
+struct ScoreShape {
+  float cap = 0.0f;
+  const Tensor<float>* slopes = nullptr;
+  const Tensor<int32_t>* prefixes = nullptr;
+};
 // q [tokens, heads, size], starts [batch + 1], lengths [batch]; maxLength: an upper bound of lengths, 0: what the table holds
 template <class T>
 Variable<float> paged_attention(const Tensor<float>& q, const PagedCache<T>& cache, const Tensor<int32_t>& table, const Tensor<int32_t>& starts,
-                                const Tensor<int32_t>& lengths, float scale, bool causal = true, unsigned window = 0, unsigned maxLength = 0);
+                                const Tensor<int32_t>& lengths, float scale, bool causal = true, unsigned window = 0, unsigned maxLength = 0,
+                                const ScoreShape& shape = {});
+
+// x [..., width] (plus the residual) over the root of its rows' mean squares, times weight [width]; and the sum, empty without a residual
+std::tuple<Variable<float>, Variable<float>> rms_norm(const Tensor<float>& x, const Tensor<float>& weight, float eps, const Tensor<float>* residual = nullptr);
+// The same as (steps - 128) * scale of the row; sums: of a row's steps, which with an offset of -128 is what the integer product takes
+struct QuantizedRows {
+  Variable<uint8_t> steps;
+  Variable<float> scales;
+  Variable<int32_t> sums;
+  Variable<float> sum;  // x + residual, empty without one
+};
+QuantizedRows rms_norm_quantized(const Tensor<float>& x, const Tensor<float>& weight, float eps, const Tensor<float>* residual = nullptr);
+// (a - offset) * scales of the rows (* columnScales [width]); a [..., width] of int32_t, int8_t or uint8_t
+template <class T>
+Variable<float> dequantize_rows(const Tensor<T>& a, const Tensor<float>& scales, int32_t offset = 0, const Tensor<float>* columnScales = nullptr);
 
 // [rows] each, or null
 struct SampleFilters {
