@@ -176,6 +176,31 @@ def test_shaped_chunks_against_the_definition(pkg, T, kind, shape, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,longest,chunk,heads,kv,size,page", [(70, 900, 1, 16, 8, 64, 16), (150, 300, 3, 12, 4, 32, 32), (64, 1300, 1, 8, 8, 128, 64), (130, 40, 1, 4, 4, 48, 24),
+                                                                    (40, 700, 2, 8, 8, 256, 32), (65, 3000, 1, 24, 4, 96, 16), (20, 1500, 9, 66, 2, 64, 20)])
+def test_many_sequences_of_all_lengths(pkg, T, batch, longest, chunk, heads, kv, size, page):
+    """More workgroups than run at once, taken by falling length: lengths of zero, equal ones, sequences without a chunk."""
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(0, longest + 1, batch)
+    lengths[::7], lengths[3::9] = longest, 0
+    chunks = np.where(rng.random(batch) < 0.15, 0, rng.integers(1, chunk + 1, batch))
+    m = Made(pkg, "s4", lengths.tolist(), chunks.tolist(), heads, kv, size, page, batch)
+    m.check(T)
+    m.check(T, max_length=longest // 2)
+    m.check(T, **m.shaped({}, cap=3.0, slopes=True))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,heads,kv,size,page", [([5000, 3000, 1100] * 11, 8, 4, 128, 32), ([4100] * 40, 12, 6, 64, 16), ([2500, 1] * 50, 4, 2, 256, 64),
+                                                        ([4000, 900] * 16, 8, 8, 32, 20), ([9000], 64, 32, 128, 64)])
+def test_workgroups_of_many_wavefronts(pkg, T, lengths, heads, kv, size, page):
+    m = Made(pkg, "s4", lengths, [1] * len(lengths), heads, kv, size, page, len(lengths))
+    m.check(T)
+    m.check(T, window=1500)
+    m.check(T, **m.shaped({}, cap=3.0, slopes=True, prefixes=[40] * len(lengths)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s4", "s8", "f32"])
 @pytest.mark.parametrize("lengths,chunks,heads,kv", [([400, 90], [3, 1], 8, 2), ([700, 300], [300, 290], 64, 64)])
 def test_prefixes(pkg, T, kind, lengths, chunks, heads, kv):

@@ -79,7 +79,7 @@ unsigned chunk_rows(const tfcc_rocm_paged_cache& c) {
 
 PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
   return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, chunk_rows(d.cache),
-                              d.cache.type == TFCC_ROCM_F32);
+                              d.cache.type == TFCC_ROCM_F32, d.cache.type == TFCC_ROCM_S4);
 }
 
 // Checks a call and deals it out; one without tokens or sequences has nothing to deal out.
@@ -130,6 +130,11 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   a.pieces = Divisor::of(plan.splits);
   a.splits = plan.splits;
   a.split_keys = plan.split_keys;
+  if (d.cache.type == TFCC_ROCM_S4 && d.batch > 1 && plan.rows == kAttentionRows && (uint64_t)plan.tiles * plan.splits * d.cache.heads > 256) {
+    int shift = 0;
+    while (a.max_length >> shift > 16) ++shift;
+    a.longest_first = shift + 1;
+  }
   a.statistics = static_cast<float*>(d.workspace) + (size_t)plan.splits * d.tokens * d.heads * d.cache.size;
   a.partial = static_cast<float*>(d.workspace);
   const hipStream_t s = as_stream(stream);

@@ -44,6 +44,7 @@ struct AttentionArgs {
   Divisor group, cache_heads, pieces;
   float *partial, *statistics;  // [splits][tokens][heads][size], [splits][tokens][heads][2]
   unsigned splits, split_keys;
+  int longest_first;  // 0: sequences in the batch's order, else by length / 2^(longest_first - 1)
   // of shaped scores: a cap in the units of log2 and its inverse (0: none), a slope for each query head, a prefix of each sequence
   float cap, cap_inverse;
   const float* slopes;
@@ -91,7 +92,9 @@ __device__ __forceinline__ unsigned wave_scan(unsigned v) {
   return v;
 }
 
-// The chunks' tiles are counted off along the batch, 64 sequences at a time.
+// The chunks' tiles are counted off along the batch, 64 sequences at a time; with longest_first (a shift and 1) those
+// 64 are taken by falling length, in 16 buckets: workgroups begin in their order, and where there are more than run at once, a long one that begins late is what the others
+// have to wait for (64 sequences of 1024 to 4096, 4 bits, 8 heads of 128: 48 us, in the batch's order 56).
 template <bool SHAPED>
 __device__ __forceinline__ Tile find_tile(const AttentionArgs& p, unsigned tile, unsigned rows_of_tile, unsigned row) {
   const unsigned lane = threadIdx.x & 63;
@@ -110,12 +113,33 @@ __device__ __forceinline__ Tile find_tile(const AttentionArgs& p, unsigned tile,
       next = next > (int)p.tokens ? (int)p.tokens : next;
       count = first >= 0 && next > first ? next - first : 0;
     }
-    const unsigned mine = ((unsigned)count * p.group.d + rows_of_tile - 1) / rows_of_tile, upto = wave_scan(mine) + before;
-    const unsigned long long past = __ballot(upto > tile);
+    unsigned mine = ((unsigned)count * p.group.d + rows_of_tile - 1) / rows_of_tile, upto = wave_scan(mine) + before;
+    unsigned long long past = __ballot(upto > tile);
     if (past != 0) {
+      unsigned from = b;
+      if (p.longest_first != 0) {
+        const unsigned there = p.batch - base < 64 ? p.batch - base : 64;
+        const int bucket = lane >= there ? -1 : held <= 0 ? 0 : (held >> (p.longest_first - 1)) < 15 ? held >> (p.longest_first - 1) : 15;
+        unsigned rank = lane, longer = 0;  // lanes behind the batch stay where they are
+#pragma unroll
+        for (int i = 15; i >= 0; --i) {
+          const unsigned long long equal = __ballot(bucket == i);
+          const unsigned before_me = __builtin_amdgcn_mbcnt_hi((unsigned)(equal >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)equal, longer));
+          rank = bucket == i ? before_me : rank;
+          longer += (unsigned)__builtin_popcountll(equal);
+        }
+        const auto sent = [&](int v) { return __builtin_amdgcn_ds_permute((int)(4 * rank), v); };
+        first = sent(first);
+        count = sent(count);
+        held = sent(held);
+        mine = (unsigned)sent((int)mine);
+        from = (unsigned)sent((int)b);
+        upto = wave_scan(mine) + before;
+        past = __ballot(upto > tile);
+      }
       const int at = __builtin_ctzll(past);
       t.any = true;
-      t.sequence = base + at;
+      t.sequence = (unsigned)__builtin_amdgcn_readlane((int)from, at);
       t.first = __builtin_amdgcn_readlane(first, at);
       t.count = __builtin_amdgcn_readlane(count, at);
       length = __builtin_amdgcn_readlane(held, at);
@@ -291,16 +315,17 @@ __device__ __forceinline__ f16x8 eight_of(const unsigned (&w)[8]) {
   return h.v;
 }
 
-// The integers of 4 bits of a word as fp16, exactly: out[i] holds those of its bits 4 i and 16 + 4 i, i < 4.  As above with u the int4 + 8; where u lies four bits
-// up, 0x6400 + 16 u is 1024 + 16 u, a sixteenth of which is 64 + u.
+// The integers of 4 bits of a word as fp16, exactly: out[i] holds those of its bits 4 i and 16 + 4 i, i < 4.  As above with u the int4 + 8, whose highest bit is
+// the other one; where it lies four bits up, 0x6400 + 16 u is 1024 + 16 u, a sixteenth of which is 64 + u.  (Two operations for two integers: the mask, the bit and
+// the bias are one.)
 __device__ __forceinline__ void eight_int4(unsigned w, f16x2 (&out)[4]) {
-  const unsigned low = 0x000f000fu, high = 0x00f000f0u, bias = 0x64006400u;
+  const unsigned low = 0x000f000fu, low_bias = 0x64086408u, high = 0x00f000f0u, high_bias = 0x64806480u;
   const f16x2 less = {(_Float16)1032.0f, (_Float16)1032.0f}, sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, less_high = {(_Float16)-72.0f, (_Float16)-72.0f};
-  const unsigned u = w ^ 0x88888888u, v = u >> 8;
-  out[0] = __builtin_bit_cast(f16x2, (u & low) | bias) - less;
-  out[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (u & high) | bias), sixteenth, less_high);
-  out[2] = __builtin_bit_cast(f16x2, (v & low) | bias) - less;
-  out[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (v & high) | bias), sixteenth, less_high);
+  const unsigned v = w >> 8;
+  out[0] = __builtin_bit_cast(f16x2, (w & low) ^ low_bias) - less;
+  out[1] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & high) ^ high_bias), sixteenth, less_high);
+  out[2] = __builtin_bit_cast(f16x2, (v & low) ^ low_bias) - less;
+  out[3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (v & high) ^ high_bias), sixteenth, less_high);
 }
 // The eight of a word: in the order 0, 4, 1, 5, 2, 6, 3, 7, which the other factor of a product follows.
 __device__ __forceinline__ f16x8 word_int4(unsigned w) {
@@ -308,22 +333,19 @@ __device__ __forceinline__ f16x8 word_int4(unsigned w) {
   eight_int4(w, h.p);
   return h.v;
 }
-// Integer E of eight words in h[E].
-__device__ __forceinline__ void eight_of_int4(const unsigned (&w)[8], f16x8 (&out)[8]) {
-  Half8 h[8];
+// Integer 4 HIGH + e of eight words in out[e], e < 4.
+template <int HIGH>
+__device__ __forceinline__ void four_of_int4(const unsigned (&w)[8], f16x8 (&out)[4]) {
+  Half8 h[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    f16x2 low[4], high[4];
-    eight_int4(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u), low);
-    eight_int4(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u), high);
+    f16x2 pair[4];
+    eight_int4(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], HIGH ? 0x07060302u : 0x05040100u), pair);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      h[e].p[i] = low[e];
-      h[4 + e].p[i] = high[e];
-    }
+    for (int e = 0; e < 4; ++e) h[e].p[i] = pair[e];
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = h[e].v;
+  for (int e = 0; e < 4; ++e) out[e] = h[e].v;
 }
 
 // float32 as the sum of two fp16, both to the nearest: the second is 2^-11 of the value at most and the error 2^-23, or half of fp16's smallest number, 2^-25
@@ -456,13 +478,24 @@ __device__ __forceinline__ int page_of(const AttentionArgs& p, const int* table,
   return page >= 0 && (unsigned)page < p.cache.pages ? page : -1;
 }
 
-// A tile's rows over a cache of integers: queries and running results of one wavefront.  BLOCKS: of 64 bytes in a row; PER: values in a byte.
+// How rows of 64 BLOCKS integers go to lanes: PER of them to a byte, BYTES in a row, N to a lane as values, and as keys RUN (of 16 bytes, or 8 where a row has
+// 32) side by side in each 4 RUN of them.
+template <int TYPE, int BLOCKS>
+struct ScaledLayout {
+  static constexpr int PER = TYPE == TFCC_ROCM_S4 ? 2 : 1, BYTES = 64 * BLOCKS / PER, N = 4 * BLOCKS, RUN = BYTES < 64 ? 8 * PER : 16 * PER, KS = 2 * BLOCKS,
+                       KEY_WORDS = BYTES / 16, VALUE_WORDS = BYTES < 64 ? 1 : BYTES / 64;
+};
+
+// A tile's rows over a cache of integers: queries and running results of one wavefront.
 template <int TYPE, int BLOCKS, bool SHAPED>
-struct ScaledRows {
-  static constexpr int PER = TYPE == TFCC_ROCM_S4 ? 2 : 1, N = 4 * BLOCKS * PER, KS = 2 * BLOCKS * PER;
-  // The head's value PER (64 b + 16 g + x) is the first of byte x of the lane's 16 in block b.  Eight of them side by side, in the order in which
-  // a word's integers come out, in [2 PER b + h][j], as two fp16 under a power of two.
-  f16x8 q_hi[KS], q_lo[KS];
+struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
+  using Layout = ScaledLayout<TYPE, BLOCKS>;
+  using Layout::KEY_WORDS;
+  using Layout::KS;
+  using Layout::N;
+  using Layout::RUN;
+  using Layout::VALUE_WORDS;
+  f16x8 q_hi[KS], q_lo[KS];                  // the lane's values of the head, eight side by side in each, in the order in which integers come out of words, as two fp16 under a power of two
   f32x4 o[N];                                // value N (4 g + i) + n in [n][i]
   float row_scale, frame = -INFINITY, l = 0.0f;
   ScoreShape shape;                          // SHAPED: and then row_scale is in the scores
@@ -473,7 +506,7 @@ struct ScaledRows {
     const float* q = p.q + (unsigned long long)(t.first + (t.row_token < 0 ? 0 : t.row_token)) * p.q_token + (head * p.group.d + t.row_head) * p.q_head;
 #pragma unroll
     for (int b = 0; b < 2 * KS; ++b) {
-      const unsigned d = PER * (64 * (b / (4 * PER)) + 16 * g) + 4 * (b % (4 * PER));
+      const unsigned d = 4 * RUN * (4 * b / RUN) + RUN * g + 4 * b % RUN;
       f32x4 v = {0, 0, 0, 0};
       if (t.row_token >= 0 && d < p.cache.size) v = *reinterpret_cast<const f32x4*>(q + d);
       x[b] = v;
@@ -501,23 +534,24 @@ struct ScaledRows {
     if constexpr (SHAPED) shape.start(p, t, head);
   }
 
-  // k: 16 bytes from byte 64 b + 16 g of key 16 h + c in [h][b]; key_scale: of keys 16 h + 4 g + i, and so s[4 h + i], scores but for row_scale
-  __device__ __forceinline__ void score(const u32x4 (&k)[2][BLOCKS], const f32x4 (&key_scale)[2], float (&s)[8]) const {
+  // k: the lane's words of key 16 h + c in [h]; key_scale: of keys 16 h + 4 g + i, and so s[4 h + i], scores but for row_scale
+  __device__ __forceinline__ void score(const unsigned (&k)[2][KEY_WORDS], const f32x4 (&key_scale)[2], float (&s)[8]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       f32x4 acc = {0, 0, 0, 0};
+      constexpr int EACH = RUN / 8;  // products of a lane's run
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        f16x8 part[2 * PER];
+      for (int b = 0; b < KS; b += EACH) {
+        f16x8 part[EACH];
 #pragma unroll
-        for (int i = 0; i < 2 * PER; ++i) {
-          if constexpr (TYPE == TFCC_ROCM_S4) part[i] = word_int4(k[h][b][i]);
-          else part[i] = eight_int8(k[h][b][2 * i], k[h][b][2 * i + 1]);
+        for (int i = 0; i < EACH; ++i) {
+          if constexpr (TYPE == TFCC_ROCM_S4) part[i] = word_int4(k[h][b + i]);
+          else part[i] = eight_int8(k[h][2 * (b + i)], k[h][2 * (b + i) + 1]);
         }
 #pragma unroll
-        for (int i = 0; i < 2 * PER; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[i], q_lo[2 * PER * b + i], acc, 0, 0, 0);
+        for (int i = 0; i < EACH; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[i], q_lo[b + i], acc, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 2 * PER; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[i], q_hi[2 * PER * b + i], acc, 0, 0, 0);
+        for (int i = 0; i < EACH; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[i], q_hi[b + i], acc, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * h + i] = acc[i] * key_scale[h][i];
@@ -547,7 +581,7 @@ struct ScaledRows {
   }
 
   // v: words from value N c of key 16 h + 4 g + i in [4 h + i]
-  __device__ __forceinline__ void add(float (&s)[8], const f32x4 (&value_scale)[2], const unsigned (&v)[8][BLOCKS]) {
+  __device__ __forceinline__ void add(float (&s)[8], const f32x4 (&value_scale)[2], const unsigned (&v)[8][VALUE_WORDS]) {
     const float row_scale = SHAPED ? 1.0f : this->row_scale;
     float top = -INFINITY;
 #pragma unroll
@@ -572,28 +606,33 @@ struct ScaledRows {
 #pragma unroll
     for (int i = 0; i < 4; ++i) split_two(w[2 * i], w[2 * i + 1], w_hi.p[i], w_lo.p[i]);
 #pragma unroll
-    for (int b = 0; b < BLOCKS; ++b) {
+    for (int b = 0; b < VALUE_WORDS; ++b) {
       unsigned word[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) word[i] = v[i][b];
-      f16x8 part[4 * PER];
-      if constexpr (TYPE == TFCC_ROCM_S4) {
-        eight_of_int4(word, part);
-      } else {
-        part[0] = eight_of<0>(word);
-        part[1] = eight_of<1>(word);
-        part[2] = eight_of<2>(word);
-        part[3] = eight_of<3>(word);
+#pragma unroll
+      for (int half = 0; half < N / VALUE_WORDS / 4; ++half) {
+        const int at = N / VALUE_WORDS * b + 4 * half;
+        f16x8 part[4];
+        if constexpr (TYPE == TFCC_ROCM_S4) {
+          if (half == 0) four_of_int4<0>(word, part);
+          else four_of_int4<1>(word, part);
+        } else {
+          part[0] = eight_of<0>(word);
+          part[1] = eight_of<1>(word);
+          part[2] = eight_of<2>(word);
+          part[3] = eight_of<3>(word);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[at + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[n], w_lo.v, o[at + n], 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) o[at + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[n], w_hi.v, o[at + n], 0, 0, 0);
       }
-#pragma unroll
-      for (int n = 0; n < 4 * PER; ++n) o[4 * PER * b + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[n], w_lo.v, o[4 * PER * b + n], 0, 0, 0);
-#pragma unroll
-      for (int n = 0; n < 4 * PER; ++n) o[4 * PER * b + n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(part[n], w_hi.v, o[4 * PER * b + n], 0, 0, 0);
     }
   }
 
   template <int WAVES>
-  __device__ __forceinline__ void finish(Joining<64 * BLOCKS * PER, WAVES>& joining, const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, unsigned g) {
+  __device__ __forceinline__ void finish(Joining<64 * BLOCKS, WAVES>& joining, const AttentionArgs& p, const Tile& t, unsigned head, unsigned split, unsigned g) {
     l = across_groups_sum(l);
     float list[4 * N];  // neighbours in the list are neighbours in the head
 #pragma unroll
@@ -604,23 +643,28 @@ struct ScaledRows {
   }
 };
 
-// int8 with pages of 16 rows and more that can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
-// of 16; WHOLE: pages of a multiple of 16 rows, so that a half lies in one, else in up to two (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 49).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
+// Integers with pages of 16 rows and more that can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
+// of 16; WITHIN: pages of a multiple of 16 rows, so that a half lies in one, or of 32 for a whole step (4 bits), else (0) a half in up to two (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 49).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
 // straight into LDS, a ring of STAGES of its own (no barriers), and reads a step from there when it is due.
 template <int TYPE, int BLOCKS, int WAVES>
 struct ScaledRing {
-  static constexpr int kRows = 4 * BLOCKS * 1024, kBytes = kRows + 256;  // keys and values, scales
-  static constexpr int kStages = BLOCKS == 1 ? 4 : 2;
-  static constexpr int kCopies = 4 * BLOCKS + 1;
+  static constexpr int kRow = ScaledLayout<TYPE, BLOCKS>::BYTES, kHalf = 16 * kRow, kRows = 4 * kHalf, kBytes = kRows + 256;  // keys and values, scales
+  static constexpr int kStages = TYPE == TFCC_ROCM_S4 || kRow >= 128 ? 2 : 4;
+  static constexpr int kCopies = (kRow < 64 ? 2 : 4 * (kRow / 64)) + 1;
   union {
     alignas(16) unsigned char ring[WAVES][kStages][kBytes];
-    Joining<64 * BLOCKS * (TYPE == TFCC_ROCM_S4 ? 2 : 1), WAVES> joining;
+    Joining<64 * BLOCKS, WAVES> joining;
   };
 };
-template <int TYPE, int BLOCKS, int WAVES, bool WHOLE, bool SHAPED>
-__global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionArgs p) {
+template <int TYPE, int BLOCKS, int WAVES, int WITHIN, bool SHAPED>
+__global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4 : BLOCKS == 2 ? 3 : 2) : 1) void attention_scaled_kernel(AttentionArgs p) {
+  constexpr bool WHOLE = WITHIN != 0;
   typedef ScaledRing<TYPE, BLOCKS, WAVES> Ring;
-  constexpr int STEP = 32 * WAVES, CHUNKS = 4 * BLOCKS /* of 16 bytes in a row */, PER_COPY = 64 / CHUNKS /* rows */, FOURS = PER_COPY / 4;
+  typedef ScaledLayout<TYPE, BLOCKS> Layout;
+  constexpr int STEP = 32 * WAVES, CHUNKS = Layout::BYTES / 16 /* of 16 bytes in a row */;
+  // Rows of 32 bytes: one copy brings both halves' keys, or values.
+  constexpr bool BOTH = CHUNKS == 2;
+  constexpr int LINES = BOTH ? 1 : CHUNKS / 4 /* copies of a half */, PER_COPY = 16 / LINES /* rows of it */, FOURS = PER_COPY / 4;
   __shared__ Ring shared;
   Tile t;
   unsigned head, split;
@@ -628,7 +672,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
   if (!take_work<SHAPED>(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
   const unsigned lane = threadIdx.x & 63, g = lane / 16, c = lane % 16;
   const unsigned wave = (unsigned)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64));
-  const unsigned size = TYPE == TFCC_ROCM_S4 ? p.cache.size / 2 : p.cache.size /* of a row, in bytes */, row_bytes = (unsigned)p.cache.row;
+  const unsigned size = p.cache.size / Layout::PER /* of a row, in bytes */, row_bytes = (unsigned)p.cache.row;
   const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
   const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
   const float* const scales = (lane < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head + c;
@@ -636,22 +680,26 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
   int kb = __builtin_amdgcn_readfirstlane(begin + 32 * (int)wave);
   end = __builtin_amdgcn_readfirstlane(end);
 
-  const auto exchange = [](unsigned row) { return BLOCKS == 1 ? row / 4 % 4 : row % CHUNKS; };
+  const auto exchange = [](unsigned row) { return BOTH ? row / 8 : CHUNKS == 4 ? row / 4 % 4 : row % CHUNKS; };
   // A copy brings PER_COPY whole rows, CHUNKS lanes to a row: lanes side by side ask for memory side by side (with a lane for each row the copies
   // take four times as long).  A lane puts its 16 bytes at its own place in LDS; which of the row's chunks that is, and which row, is free
   // and chosen so that what is read together lies in different banks.  Keys are read 16 rows at a time, a chunk of each: chunks are
   // exchanged within a row by its number.  Values are read a few bytes of rows 4 g + i at a time: those rows lie side by side.
-  unsigned key_at[BLOCKS], value_at[BLOCKS];
-  const unsigned slot = lane / CHUNKS, chunk = lane % CHUNKS;
+  unsigned key_at[LINES], value_at[LINES];
+  const unsigned slot = lane / CHUNKS % 16, chunk = lane % CHUNKS;
   const auto key_row = [&](int b) { return b * PER_COPY + slot; };
   const auto value_row = [&](int b) { return (b * FOURS + slot % FOURS) * 4 + slot / FOURS; };
 #pragma unroll
-  for (int b = 0; b < BLOCKS; ++b) {
+  for (int b = 0; b < LINES; ++b) {
     const unsigned from = (chunk ^ exchange(key_row(b))) * 16;
     key_at[b] = key_row(b) * row_bytes + (from < size ? from : 0);
     value_at[b] = value_row(b) * row_bytes + (chunk * 16 < size ? chunk * 16 : 0);
   }
-  const unsigned half_bytes = 15 * row_bytes + size;
+  if (BOTH && WITHIN == 32 && lane >= 32) {
+    key_at[0] += 16 * row_bytes;
+    value_at[0] += 16 * row_bytes;
+  }
+  const unsigned half_bytes = (WITHIN == 32 ? 31 : 15) * row_bytes + size;  // from a half's first row on, or a step's
   unsigned char* const ring = shared.ring[wave][0];
   const unsigned ring_at = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)ring;
 
@@ -660,7 +708,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
   PageEntry entries[2][PAGES] = {};
   const auto ask_pages = [&](int at) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < (WITHIN == 32 ? 1 : 2); ++h)
 #pragma unroll
       for (int n = 0; n < PAGES; ++n) entries[h][n] = entry_of(p, table, p.cache.page_size.quotient((unsigned)at + 16 * h + 15 * n));
   };
@@ -669,27 +717,60 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
   const auto cut_of = [&](unsigned key) { return p.cache.page_size.d - inside_page(key); };
   const auto copy = [&](unsigned stage, int at, const int (&page)[2][PAGES]) {
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(ring_at + stage * Ring::kBytes));
+    if constexpr (WITHIN == 32) {
+      const unsigned inside = inside_page((unsigned)at);
+      const unsigned long long held = page[0][0] < 0 ? 0 : (unsigned)page[0][0], base = held * p.cache.page + inside * p.cache.row;
+      const lds_dma_v4i k = make_rsrc(keys + base, half_bytes), v = make_rsrc(values + base, half_bytes);
+#pragma unroll
+      for (int h = 0; h < (BOTH ? 1 : 2); ++h)
+#pragma unroll
+        for (int b = 0; b < LINES; ++b) {
+          if (h == 0) dma16(k, to + b * 1024, key_at[b]);
+          else dma16s(k, to + (LINES + b) * 1024, key_at[b], 16 * row_bytes);
+        }
+#pragma unroll
+      for (int h = 0; h < (BOTH ? 1 : 2); ++h)
+#pragma unroll
+        for (int b = 0; b < LINES; ++b) {
+          if (h == 0) dma16(v, to + 2 * Ring::kHalf + b * 1024, value_at[b]);
+          else dma16s(v, to + 2 * Ring::kHalf + (LINES + b) * 1024, value_at[b], 16 * row_bytes);
+        }
+      const float* const scale = scales + held * p.cache.scale_page + inside + (lane & 16);
+      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to + Ring::kRows), "v"(scale) : "memory", "m0");
+      return;
+    }
     const float* scale_at[2];
+    unsigned long long row_at[2];  // BOTH: of the lane's row of keys, and of values, in the first half and in the second
+    unsigned long long value_row_at[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const unsigned key = (unsigned)at + 16 * h, inside = inside_page(key);
       const unsigned long long held = page[h][0] < 0 ? 0 : (unsigned)page[h][0], base = held * p.cache.page + inside * p.cache.row;
       scale_at[h] = scales + held * p.cache.scale_page + inside;
-      if constexpr (WHOLE) {
+      if constexpr (BOTH && WHOLE) {
+        row_at[h] = value_row_at[h] = base;
+      } else if constexpr (WHOLE) {
         const lds_dma_v4i k = make_rsrc(keys + base, half_bytes), v = make_rsrc(values + base, half_bytes);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) dma16(k, to + (h * BLOCKS + b) * 1024, key_at[b]);
+        for (int b = 0; b < LINES; ++b) dma16(k, to + (h * LINES + b) * 1024, key_at[b]);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) dma16(v, to + ((2 + h) * BLOCKS + b) * 1024, value_at[b]);
+        for (int b = 0; b < LINES; ++b) dma16(v, to + ((2 + h) * LINES + b) * 1024, value_at[b]);
       } else {
         const unsigned long long next = page[h][PAGES - 1] < 0 ? 0 : (unsigned)page[h][PAGES - 1];
         const long long cut = cut_of(key), other = (long long)(next * p.cache.page) - cut * (long long)p.cache.row;
         if (c >= cut) scale_at[h] = scales + next * p.cache.scale_page - cut;
+        row_at[h] = key_row(0) >= cut ? other : (long long)base;
+        value_row_at[h] = value_row(0) >= cut ? other : (long long)base;
+        if constexpr (BOTH) continue;
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) dma16_global(keys + (key_row(b) >= cut ? other : (long long)base) + key_at[b], to + (h * BLOCKS + b) * 1024);
+        for (int b = 0; b < LINES; ++b) dma16_global(keys + (key_row(b) >= cut ? other : (long long)base) + key_at[b], to + (h * LINES + b) * 1024);
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) dma16_global(values + (value_row(b) >= cut ? other : (long long)base) + value_at[b], to + ((2 + h) * BLOCKS + b) * 1024);
+        for (int b = 0; b < LINES; ++b) dma16_global(values + (value_row(b) >= cut ? other : (long long)base) + value_at[b], to + ((2 + h) * LINES + b) * 1024);
       }
+    }
+    if constexpr (BOTH) {
+      dma16_global(keys + (lane < 32 ? row_at[0] : row_at[1]) + key_at[0], to);
+      dma16_global(values + (lane < 32 ? value_row_at[0] : value_row_at[1]) + value_at[0], to + 2 * Ring::kHalf);
     }
     const float* const scale = (lane & 16) ? scale_at[1] : scale_at[0];
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to + Ring::kRows), "v"(scale) : "memory", "m0");
@@ -705,7 +786,7 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          if (n < PAGES) pages[h][n] = page_of(p, entries[h][n]);
+          if (n < PAGES) pages[h][n] = WITHIN == 32 && h > 0 ? pages[0][n] : page_of(p, entries[h][n]);
           none |= pages[h][n < PAGES ? n : 0] < 0 ? 1u << (2 * h + n) : 0u;
         }
       copy(stage, ahead, pages);
@@ -714,11 +795,13 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
       if (ahead < end) ask_pages(ahead);
     }
   };
+  // The queries first: loads come back in their order, and behind the copies they would wait for all stages to be filled.  (The pages' entries, which the copies
+  // need, are on their way meanwhile.)
+  ScaledRows<TYPE, BLOCKS, SHAPED> rows;
+  rows.start(p, t, head, g);
 #pragma unroll 1
   for (unsigned stage = 0; stage < Ring::kStages; ++stage) send(stage);
 
-  ScaledRows<TYPE, BLOCKS, SHAPED> rows;
-  rows.start(p, t, head, g);
   unsigned stage = 0;
 #pragma unroll 1
   for (; kb < end; kb += STEP) {
@@ -726,22 +809,34 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_kernel(AttentionA
     if (kb + (Ring::kStages - 1) * STEP < end) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((Ring::kStages - 1) * Ring::kCopies) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     const unsigned char* const from = ring + stage * Ring::kBytes;
-    u32x4 k[2][BLOCKS];
-    unsigned v[8][BLOCKS];
+    unsigned k[2][Layout::KEY_WORDS], v[8][Layout::VALUE_WORDS];
     f32x4 key_scale[2], value_scale[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      const unsigned char* const row = from + h * Ring::kHalf + c * Ring::kRow;
+      if constexpr (BOTH) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(row + (g ^ 2 * exchange(c)) * 8);
+        k[h][0] = w[0];
+        k[h][1] = w[1];
+      } else {
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) k[h][b] = *reinterpret_cast<const u32x4*>(from + h * BLOCKS * 1024 + c * (CHUNKS * 16) + ((4 * b + g) ^ exchange(c)) * 16);
+        for (int b = 0; b < LINES; ++b) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(row + ((4 * b + g) ^ exchange(c)) * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) k[h][4 * b + i] = w[i];
+        }
+      }
       key_scale[h] = *reinterpret_cast<const f32x4*>(from + Ring::kRows + (16 * h + 4 * g) * 4);
       value_scale[h] = *reinterpret_cast<const f32x4*>(from + Ring::kRows + 128 + (16 * h + 4 * g) * 4);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const unsigned char* const at = from + (2 + i / 4) * BLOCKS * 1024 + (g / FOURS) * 1024 + ((i % 4) * FOURS + g % FOURS) * (CHUNKS * 16) + 4 * BLOCKS * c;
-      if constexpr (BLOCKS == 1) {
+      const unsigned char* const at = from + (2 + i / 4) * Ring::kHalf + (g / FOURS) * 1024 + ((i % 4) * FOURS + g % FOURS) * Ring::kRow + Ring::kRow / 16 * c;
+      if constexpr (BOTH) {
+        v[i][0] = *reinterpret_cast<const unsigned short*>(at);
+      } else if constexpr (LINES == 1) {
         v[i][0] = *reinterpret_cast<const unsigned*>(at);
-      } else if constexpr (BLOCKS == 2) {
+      } else if constexpr (LINES == 2) {
         const u32x2 w = *reinterpret_cast<const u32x2*>(at);
         v[i][0] = w[0];
         v[i][1] = w[1];
@@ -1223,21 +1318,25 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
 #pragma unroll
           for (int j = 0; j < 8; ++j) w[j] = raw[2 * k + j / 4][j % 4];
           constexpr int EACH = S4 ? 8 : 4;  // values in a word, which go where four and four do
-          f16x8 v[EACH];
-          if constexpr (S4) {
-            eight_of_int4(w, v);
-          } else {
-            v[0] = eight_of<0>(w);
-            v[1] = eight_of<1>(w);
-            v[2] = eight_of<2>(w);
-            v[3] = eight_of<3>(w);
-          }
 #pragma unroll
-          for (int e = 0; e < EACH; ++e) {
-            const unsigned four = EACH / 4 * word + e / 4, b = e % 4;
+          for (int f = 0; f < EACH / 4; ++f) {
+            f16x8 v[4];
+            if constexpr (S4) {
+              if (f == 0) four_of_int4<0>(w, v);
+              else four_of_int4<1>(w, v);
+            } else {
+              v[0] = eight_of<0>(w);
+              v[1] = eight_of<1>(w);
+              v[2] = eight_of<2>(w);
+              v[3] = eight_of<3>(w);
+            }
+            const unsigned four = EACH / 4 * word + f;
             const bool quarters = (four / 32 + 1) * 4 <= N;
-            const unsigned n = four / 32 * 4 + (quarters ? b : b % 2), L = quarters ? four % 32 : four % 16 + 16 * (b / 2);
-            s.values[0][n][group / 2][32 * (group % 2) + L] = __builtin_bit_cast(u32x4, v[e]);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+              const unsigned n = four / 32 * 4 + (quarters ? b : b % 2), L = quarters ? four % 32 : four % 16 + 16 * (b / 2);
+              s.values[0][n][group / 2][32 * (group % 2) + L] = __builtin_bit_cast(u32x4, v[b]);
+            }
           }
         }
       }
@@ -1533,13 +1632,14 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
 template <int TYPE, int BLOCKS, int WAVES, bool SHAPED>
 __global__ __launch_bounds__(WAVES * 64) void attention_scaled_any_kernel(AttentionArgs p) {
   constexpr int STEP = 32 * WAVES;
-  __shared__ Joining<64 * BLOCKS * (TYPE == TFCC_ROCM_S4 ? 2 : 1), WAVES> joining;
+  typedef ScaledLayout<TYPE, BLOCKS> Layout;
+  __shared__ Joining<64 * BLOCKS, WAVES> joining;
   Tile t;
   unsigned head, split;
   int begin, end;
   if (!take_work<SHAPED>(p, kAttentionRows, threadIdx.x % 16, t, head, split, begin, end)) return;
   const unsigned lane = threadIdx.x & 63, wave = threadIdx.x / 64, g = lane / 16, c = lane % 16;
-  const unsigned size = TYPE == TFCC_ROCM_S4 ? p.cache.size / 2 : p.cache.size;  // of a row, in bytes
+  const unsigned size = p.cache.size / Layout::PER;  // of a row, in bytes
   const int8_t* const keys = static_cast<const int8_t*>(p.cache.keys) + head * p.cache.head;
   const int8_t* const values = static_cast<const int8_t*>(p.cache.values) + head * p.cache.head;
   const float* const key_scales = p.cache.key_scales + head * p.cache.scale_head;
@@ -1556,19 +1656,19 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_any_kernel(Attent
   rows.start(p, t, head, g);
 #pragma unroll 1
   for (int kb = begin + 32 * (int)wave; kb < end; kb += STEP) {
-    u32x4 k[2][BLOCKS];
-    unsigned v[8][BLOCKS], missing = 0;
+    unsigned k[2][Layout::KEY_WORDS], v[8][Layout::VALUE_WORDS], missing = 0;
     f32x4 key_scale[2], value_scale[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       unsigned long long row, scale;
       locate(kb + 16 * h + (int)c, row, scale);
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        const unsigned d = 64 * b + 16 * g;  // rows are 8-byte aligned
-        const u32x2 w0 = *reinterpret_cast<const u32x2*>(keys + row + (d < size ? d : 0));
-        const u32x2 w1 = *reinterpret_cast<const u32x2*>(keys + row + (d + 8 < size ? d + 8 : 0));
-        k[h][b] = u32x4{w0[0], w0[1], w1[0], w1[1]};
+      for (int b = 0; b < Layout::KEY_WORDS; b += 2) {  // rows are 8-byte aligned
+        constexpr int RUN = Layout::RUN / Layout::PER / 4;  // words
+        const unsigned d = 4 * (4 * RUN * (b / RUN) + RUN * g + b % RUN);
+        const u32x2 w = *reinterpret_cast<const u32x2*>(keys + row + (d < size ? d : 0));
+        k[h][b] = w[0];
+        k[h][b + 1] = w[1];
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -1576,9 +1676,10 @@ __global__ __launch_bounds__(WAVES * 64) void attention_scaled_any_kernel(Attent
         key_scale[h][i] = key_scales[scale];
         value_scale[h][i] = value_scales[scale];
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) {
-          const unsigned d = 4 * BLOCKS * c + 4 * b;
-          v[4 * h + i][b] = *reinterpret_cast<const unsigned*>(values + row + (d < size ? d : 0));
+        for (int b = 0; b < Layout::VALUE_WORDS; ++b) {
+          const unsigned d = Layout::BYTES / 16 * c + 4 * b;
+          const int8_t* const at = values + row + (d < size ? d : 0);
+          v[4 * h + i][b] = Layout::BYTES < 64 ? *reinterpret_cast<const unsigned short*>(at) : *reinterpret_cast<const unsigned*>(at);
         }
       }
     }
@@ -1619,19 +1720,23 @@ __global__ __launch_bounds__(WAVES * 64) void attention_f32_kernel(AttentionArgs
 // What a step's 16 keys may lie in: 1 page, up to 2, or any number (0).
 int pages_of_step(unsigned page_size) { return page_size % 16 == 0 ? 1 : page_size >= 16 ? 2 : 0; }
 
-// BLOCKS: of 64 bytes in a row
+template <int TYPE, int BLOCKS, int WAVES, bool SHAPED>
+void launch_scaled_of(const AttentionArgs& a, dim3 grid, hipStream_t s, bool wide) {
+  const auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(WAVES * 64), 0, s, a); };
+  const unsigned rows = a.cache.page_size.d;
+  if (!wide) return start(attention_scaled_any_kernel<TYPE, BLOCKS, WAVES, SHAPED>);
+  if constexpr (TYPE == TFCC_ROCM_S4)
+    if (rows % 32 == 0) return start(attention_scaled_kernel<TYPE, BLOCKS, WAVES, 32, SHAPED>);
+  start(rows % 16 == 0 ? attention_scaled_kernel<TYPE, BLOCKS, WAVES, 16, SHAPED> : attention_scaled_kernel<TYPE, BLOCKS, WAVES, 0, SHAPED>);
+}
 template <int TYPE, int BLOCKS, bool SHAPED>
 void launch_scaled(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves, bool wide) {
-  const auto start = [&](auto kernel, unsigned width) { hipLaunchKernelGGL(kernel, grid, dim3(width * 64), 0, s, a); };
-  const bool whole = a.cache.page_size.d % 16 == 0;
-  if constexpr (BLOCKS <= (TYPE == TFCC_ROCM_S4 ? 1 : 2))
-    if (waves == 8)
-      return start(!wide ? attention_scaled_any_kernel<TYPE, BLOCKS, 8, SHAPED>
-                   : whole ? attention_scaled_kernel<TYPE, BLOCKS, 8, true, SHAPED> : attention_scaled_kernel<TYPE, BLOCKS, 8, false, SHAPED>, 8);
-  start(!wide ? attention_scaled_any_kernel<TYPE, BLOCKS, 4, SHAPED>
-        : whole ? attention_scaled_kernel<TYPE, BLOCKS, 4, true, SHAPED> : attention_scaled_kernel<TYPE, BLOCKS, 4, false, SHAPED>, 4);
+  if constexpr (TYPE == TFCC_ROCM_S4 && BLOCKS <= 2)
+    if (waves == 12) return launch_scaled_of<TYPE, BLOCKS, 12, SHAPED>(a, grid, s, wide);
+  if constexpr (TYPE == TFCC_ROCM_S8 ? BLOCKS <= 2 : BLOCKS == 4)
+    if (waves == 8) return launch_scaled_of<TYPE, BLOCKS, 8, SHAPED>(a, grid, s, wide);
+  launch_scaled_of<TYPE, BLOCKS, 4, SHAPED>(a, grid, s, wide);
 }
-// BLOCKS: of 64 values in a head
 template <int TYPE, int BLOCKS, bool SHAPED>
 void launch_tiles(const AttentionArgs& a, dim3 grid, hipStream_t s) {
   const bool whole = a.cache.page_size.d % 16 == 0;
@@ -1648,7 +1753,7 @@ void launch_f32(const AttentionArgs& a, dim3 grid, hipStream_t s, unsigned waves
   start(attention_f32_kernel<BLOCKS, 4, 1, SHAPED>, attention_f32_kernel<BLOCKS, 4, 2, SHAPED>, attention_f32_kernel<BLOCKS, 4, 0, SHAPED>, 4);
 }
 
-// The kernel of a call that has been dealt out; wide: a cache of integers that can be read 16 bytes at a time.
+// The kernel of a call that has been dealt out, BLOCKS of 64 values in a head; wide: a cache of integers that can be read 16 bytes at a time.
 template <bool SHAPED>
 void launch_attention(const AttentionArgs& a, int type, bool wide, const PagedAttentionPlan& plan, hipStream_t s) {
   const dim3 grid(plan.tiles * plan.splits * a.cache.heads);
@@ -1660,19 +1765,21 @@ void launch_attention(const AttentionArgs& a, int type, bool wide, const PagedAt
     else if (blocks == 3) launch_tiles<TYPE, 3, SHAPED>(a, grid, s);
     else launch_tiles<TYPE, 4, SHAPED>(a, grid, s);
   };
+  const auto scaled = [&](auto code) {
+    constexpr int TYPE = decltype(code)::value;
+    if (blocks == 1) launch_scaled<TYPE, 1, SHAPED>(a, grid, s, plan.waves, wide);
+    else if (blocks == 2) launch_scaled<TYPE, 2, SHAPED>(a, grid, s, plan.waves, wide);
+    else launch_scaled<TYPE, 4, SHAPED>(a, grid, s, plan.waves, wide);
+  };
   if (plan.rows != kAttentionRows && type == TFCC_ROCM_F32) {
     if (blocks == 1) hipLaunchKernelGGL((attention_tile_kernel<TFCC_ROCM_F32, 1, 4, false, SHAPED>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attention_tile_kernel<TFCC_ROCM_F32, 2, 8, false, SHAPED>), grid, dim3(512), 0, s, a);
   } else if (plan.rows != kAttentionRows) {
     if (type == TFCC_ROCM_S4) tiles(std::integral_constant<int, TFCC_ROCM_S4>());
     else tiles(std::integral_constant<int, TFCC_ROCM_S8>());
-  } else if (type == TFCC_ROCM_S8) {
-    if (blocks == 1) launch_scaled<TFCC_ROCM_S8, 1, SHAPED>(a, grid, s, plan.waves, wide);
-    else if (blocks == 2) launch_scaled<TFCC_ROCM_S8, 2, SHAPED>(a, grid, s, plan.waves, wide);
-    else launch_scaled<TFCC_ROCM_S8, 4, SHAPED>(a, grid, s, plan.waves, wide);
-  } else if (type == TFCC_ROCM_S4) {
-    if (blocks <= 2) launch_scaled<TFCC_ROCM_S4, 1, SHAPED>(a, grid, s, plan.waves, wide);
-    else launch_scaled<TFCC_ROCM_S4, 2, SHAPED>(a, grid, s, plan.waves, wide);
+  } else if (type != TFCC_ROCM_F32) {
+    if (type == TFCC_ROCM_S4) scaled(std::integral_constant<int, TFCC_ROCM_S4>());
+    else scaled(std::integral_constant<int, TFCC_ROCM_S8>());
   } else {
     if (blocks == 1) launch_f32<1, SHAPED>(a, grid, s, plan.waves);
     else if (blocks == 2) launch_f32<2, SHAPED>(a, grid, s, plan.waves);

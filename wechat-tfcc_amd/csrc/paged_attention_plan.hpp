@@ -8,7 +8,7 @@ namespace tfcc_rocm {
 struct PagedAttentionPlan {
   unsigned rows;        // of a tile
   unsigned tiles;       // an upper bound of the tiles of rows that all chunks make
-  unsigned waves;       // of a workgroup, 4 or 8
+  unsigned waves;       // of a workgroup, 4, 8 or 12
   unsigned splits;      // pieces of the keys, each with a workgroup for every tile and cache head
   unsigned split_keys;  // keys of a piece, a multiple of what its wavefronts take in one step
 };
@@ -23,9 +23,9 @@ inline unsigned paged_attention_tiles(unsigned tokens, unsigned batch, unsigned 
   return (unsigned)(((uint64_t)tokens * group + (uint64_t)(rows - 1) * chunks) / rows);
 }
 
-// chunk_rows: of the tiles that chunks of many tokens may take, 128 or 256; 0: there are none.
+// chunk_rows: of the tiles that chunks of many tokens may take, 128 or 256; 0: there are none.  halves: a cache of 4-bit integers.
 inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, unsigned group, unsigned cache_heads, unsigned size, unsigned max_length,
-                                               int causal, unsigned window, unsigned chunk_rows, bool float_cache) {
+                                               int causal, unsigned window, unsigned chunk_rows, bool float_cache, bool halves = false) {
   PagedAttentionPlan p;
   // chunks of about the same number of tokens
   const uint64_t chunks = tokens < batch ? tokens : batch, mean = chunks == 0 ? 0 : (tokens + chunks - 1) / chunks;
@@ -57,6 +57,12 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   // four wavefronts 97; 200 sequences of 700: 78 and 59).  Eight with heads wider than 128 do not have the registers.
   uint64_t splits = 1, step = kAttentionStep;
   p.waves = groups <= 512 && size <= 128 && keys > kAttentionStep / 2 ? 8 : 4;
+  if (halves) {
+    // What holds a workgroup of 4-bit integers up is its operations: as many wavefronts to a CU as registers allow, 12 (heads wider than 128: 8), in one workgroup where there is
+    // no more than one to a CU and enough to do, else in several, whose beginnings and ends others fill.  (Us with one and with several, 8 heads of 128: 32 sequences of 4096 33 and 40,
+    // 64 of up to 4096 54 and 48, 40 of up to 1000 22 and 14; 12 heads, one of 4000 13 and 11; 8 heads of 256, 32 of 4096 50 and 56.)
+    p.waves = groups <= 256 && keys > 1024 && groups * keys > 256 * 384 ? (size <= 128 ? 12 : 8) : 4;
+  }
   if (!wide) step = p.waves * (float_cache ? 16 : 32);
   if (wide && float_cache) {
     // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 260 us, one 404)
