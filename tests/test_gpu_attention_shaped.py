@@ -122,18 +122,20 @@ def test_4_bits_against_the_definition(pkg, T, case):
     Made(pkg, "s4", lengths, chunks, heads, kv, size, page, case).check(T, **more)
 
 
+def fits(shape, more):
+    """A prefix has neither a window nor all keys."""
+    return "prefix" not in shape or not (more.get("window") or not more.get("causal", True))
+
+
 def shape_of(m, shape, more):
     if "prefix" not in shape:
         return m.shaped(more, **shape)
-    if more.get("window") or not more.get("causal", True):
-        pytest.skip("a prefix has neither a window nor all keys")
     return m.shaped(more, shape.get("cap", 0.0), shape.get("slopes", False), m.rng.integers(-3, m.lengths + 40))
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s4", "s8", "f32"])
-@pytest.mark.parametrize("shape", range(len(SHAPES)))
-@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("case,shape", [(c, s) for c in range(len(CASES)) for s in range(len(SHAPES)) if fits(SHAPES[s], CASES[c][-1])])
 def test_shaped_against_the_definition(pkg, T, kind, shape, case):
     lengths, chunks, heads, kv, size, page, more = CASES[case]
     m = Made(pkg, kind, lengths, chunks, heads, kv, size, page, 100 + case)
@@ -167,8 +169,7 @@ def test_chunks_of_4_bits_against_the_definition(pkg, T, case):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s4", "s8", "f32"])
-@pytest.mark.parametrize("shape", [2, 4])
-@pytest.mark.parametrize("case", range(len(TILES)))
+@pytest.mark.parametrize("case,shape", [(c, s) for c in range(len(TILES)) for s in (2, 4) if fits(SHAPES[s], TILES[c][-1])])
 def test_shaped_chunks_against_the_definition(pkg, T, kind, shape, case):
     lengths, chunks, heads, kv, size, page, more = TILES[case]
     m = Made(pkg, kind, lengths, chunks, heads, kv, size, page, 50 + case)

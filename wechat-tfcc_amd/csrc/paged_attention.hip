@@ -130,7 +130,7 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   a.pieces = Divisor::of(plan.splits);
   a.splits = plan.splits;
   a.split_keys = plan.split_keys;
-  if (d.cache.type == TFCC_ROCM_S4 && d.batch > 1 && plan.rows == kAttentionRows && (uint64_t)plan.tiles * plan.splits * d.cache.heads > 256) {
+  if ((uint64_t)plan.tiles * plan.splits * d.cache.heads > (plan.rows == kAttentionRows ? 256 : 65536 / plan.rows)) {  // more workgroups than CUs, of wide tiles than run at once
     int shift = 0;
     while (a.max_length >> shift > 16) ++shift;
     a.longest_first = shift + 1;
@@ -139,8 +139,9 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   a.partial = static_cast<float*>(d.workspace);
   const hipStream_t s = as_stream(stream);
   if (scores != nullptr) {
-    a.cap = scores->cap * 1.44269504088896341f;
-    a.cap_inverse = scores->cap > 0.0f ? 1.0f / a.cap : 0.0f;
+    // caps that no score comes near are none: in the units of log2 they may not be numbers
+    a.cap = scores->cap < 1.2676506e30f ? scores->cap * 1.44269504088896341f : 0.0f;
+    a.cap_inverse = a.cap > 0.0f ? fminf(1.0f / a.cap, 3.4028234e38f) : 0.0f;
     a.slopes = scores->slopes;
     a.prefixes = scores->prefixes;
     launch_shaped_attention(a, d.cache.type, wide_reads(d.cache), plan, s);

@@ -94,7 +94,7 @@ __device__ __forceinline__ unsigned wave_scan(unsigned v) {
 
 // The chunks' tiles are counted off along the batch, 64 sequences at a time; with longest_first (a shift and 1) those
 // 64 are taken by falling length, in 16 buckets: workgroups begin in their order, and where there are more than run at once, a long one that begins late is what the others
-// have to wait for (64 sequences of 1024 to 4096, 4 bits, 8 heads of 128: 48 us, in the batch's order 56).
+// have to wait for (64 sequences of 1024 to 4096, 8 heads of 128: 4 bits 48 us, in the batch's order 56, int8 80 and 85; 12 chunks of 500 over up to 3000, 4 bits: 313 and 364).
 template <bool SHAPED>
 __device__ __forceinline__ Tile find_tile(const AttentionArgs& p, unsigned tile, unsigned rows_of_tile, unsigned row) {
   const unsigned lane = threadIdx.x & 63;
@@ -143,7 +143,10 @@ __device__ __forceinline__ Tile find_tile(const AttentionArgs& p, unsigned tile,
       t.first = __builtin_amdgcn_readlane(first, at);
       t.count = __builtin_amdgcn_readlane(count, at);
       length = __builtin_amdgcn_readlane(held, at);
-      t.row0 = (int)((tile - (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), at)) * rows_of_tile);
+      unsigned within = tile - (unsigned)__builtin_amdgcn_readlane((int)(upto - mine), at);
+      // of a chunk the last rows, which see most
+      if (p.longest_first != 0) within = (unsigned)__builtin_amdgcn_readlane((int)mine, at) - 1 - within;
+      t.row0 = (int)(within * rows_of_tile);
       break;
     }
     before = (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
@@ -230,31 +233,37 @@ __device__ __forceinline__ int bound_of(float v) {
 // A row's scores with a cap and a bias that depends on distance.  In the units of log2, as all scores here.
 //
 // tanh to about float32's last place, of the result and not of 1: below 0.55, x + x^3 P(x^2) with P of degree 4 fitted for the smallest relative error (2^-29), above,
-// 1 - 2 / (2^(2 log2(e) x) + 1).  Most scores are far below their cap: where those of a whole wavefront are, the second is passed over.
-// The bias is slope * distance.  A row's softmax does not change with what all its scores have in common, so distances are counted
-// from the nearest key that the row may see, and a position before the first key counts as that.
+// 1 - 2 / (2^(2 log2(e) x) + 1).  Most scores are far below their cap: where those of a whole wavefront are, the second is passed over.  A score as
+// it comes (`raw`) takes the factor of its row and the cap's inverse in one, and leaves in units of `unit`, the cap where nothing is added to it: a
+// cap costs nine operations, a bias two.
+// The bias is slope * distance.  A row's softmax does not change with what all its scores have in common, so a position behind the last key
+// that the row may see counts as that key's, and one before the first as the first's: differences are whole numbers, exact up to 2^24.
 struct ScoreShape {
-  float cap = 0.0f, cap_inverse = 0.0f, slope = 0.0f;
-  int position = 0, nearest = 0;
+  float cap = 0.0f, slope = 0.0f, factor = 1.0f, unit = 1.0f;
+  int position = 0;
   bool biased = false;
 
-  __device__ __forceinline__ void start(const AttentionArgs& p, const Tile& t, unsigned head) {
+  // factor_of_row: of the scores as they come
+  __device__ __forceinline__ void start(const AttentionArgs& p, const Tile& t, unsigned head, float factor_of_row) {
     cap = p.cap;
-    cap_inverse = p.cap_inverse;
     biased = p.slopes != nullptr;
+    factor_of_row = fminf(factor_of_row, 3.4028234e38f);  // a score of 0 stays one where the factor overflows
+    factor = cap > 0.0f ? fminf(factor_of_row * p.cap_inverse, 3.4028234e38f) : biased ? factor_of_row : 1.0f;
+    unit = biased ? 1.0f : cap > 0.0f ? cap : factor_of_row;
     if (biased && t.row_token >= 0) {
       slope = p.slopes[head * p.group.d + t.row_head] * 1.44269504088896341f;
-      position = t.row_position > 0 ? t.row_position : 0;
-      nearest = position > t.row_high - 1 ? position - (t.row_high - 1) : 0;
+      position = t.row_position < t.row_high - 1 ? t.row_position : t.row_high - 1;
+      position = position > 0 ? position : 0;
     }
   }
-  template <int N, class Key>
-  __device__ __forceinline__ void apply(float (&s)[N], Key key_of) const {
-    if (cap_inverse > 0.0f) {
+  // key: of s[0]; AWAY(i): that of s[i] less it
+  template <int N, class Away>
+  __device__ __forceinline__ void apply(float (&s)[N], int key, Away away) const {
+    if (cap > 0.0f) {
       float most = 0.0f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        s[i] *= cap_inverse;
+        s[i] *= factor;
         most = fmaxf(most, fabsf(s[i]));
       }
       const bool large = __any(!(most < 0.55f));
@@ -271,15 +280,13 @@ struct ScoreShape {
           const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.88539008177792681f) + 1.0f), 1.0f);
           r = fabsf(x) < 0.55f ? r : far;
         }
-        s[i] = cap * r;
+        s[i] = r;
       }
     }
     if (biased) {
+      const float first = (float)(key - position), times = cap > 0.0f ? cap : factor;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int away = position - key_of(i);
-        s[i] = fmaf(-slope, (float)((away < 0 ? -away : away) - nearest), s[i]);
-      }
+      for (int i = 0; i < N; ++i) s[i] = fmaf(-slope, fabsf(first + (float)away(i)), s[i] * times);
     }
   }
 };
@@ -351,7 +358,11 @@ __device__ __forceinline__ void four_of_int4(const unsigned (&w)[8], f16x8 (&out
 // float32 as the sum of two fp16, both to the nearest: the second is 2^-11 of the value at most and the error 2^-23, or half of fp16's smallest number, 2^-25
 __device__ __forceinline__ void split_two(float a, float b, f16x2& hi, f16x2& lo) {
   hi = __builtin_convertvector(f32x2{a, b}, f16x2);
-  lo = __builtin_convertvector(f32x2{fmaf((float)hi[0], -1.0f, a), fmaf((float)hi[1], -1.0f, b)}, f16x2);
+  // a - hi, which is exact: one operation that takes half a register as fp16 (of a conversion and a difference the compiler makes two)
+  float rest_a, rest_b;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest_a) : "v"(hi), "v"(a));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest_b) : "v"(hi), "v"(b));
+  lo = __builtin_convertvector(f32x2{rest_a, rest_b}, f16x2);
 }
 
 // Powers of two for a row of queries whose largest value is `top`: `up` brings it to 2^13 .. 2^14 under the sign of the scale (0 for a scale of 0),
@@ -498,7 +509,7 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
   f16x8 q_hi[KS], q_lo[KS];                  // the lane's values of the head, eight side by side in each, in the order in which integers come out of words, as two fp16 under a power of two
   f32x4 o[N];                                // value N (4 g + i) + n in [n][i]
   float row_scale, frame = -INFINITY, l = 0.0f;
-  ScoreShape shape;                          // SHAPED: and then row_scale is in the scores
+  ScoreShape shape;
 
   __device__ __forceinline__ void start(const AttentionArgs& p, const Tile& t, unsigned head, unsigned g) {
     f32x4 x[2 * KS];
@@ -531,7 +542,10 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) o[n] = f32x4{0, 0, 0, 0};
-    if constexpr (SHAPED) shape.start(p, t, head);
+    if constexpr (SHAPED) {
+      shape.start(p, t, head, row_scale);
+      row_scale = shape.unit;
+    }
   }
 
   // k: the lane's words of key 16 h + c in [h]; key_scale: of keys 16 h + 4 g + i, and so s[4 h + i], scores but for row_scale
@@ -560,11 +574,7 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
 
   // SHAPED: the scores as they are meant, of keys kb + 16 h + 4 g + i
   __device__ __forceinline__ void form(int kb, unsigned g, float (&s)[8]) const {
-    if constexpr (SHAPED) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] *= fminf(row_scale, 3.4028234e38f);  // a score of 0 stays one where the factor overflows
-      shape.apply(s, [&](int i) { return kb + 16 * (i / 4) + 4 * (int)g + i % 4; });
-    }
+    if constexpr (SHAPED) shape.apply(s, kb + 4 * (int)g, [](int i) { return 16 * (i / 4) + i % 4; });
   }
 
   // `missing`: a bit for each of the lane's eight keys that no page holds
@@ -582,7 +592,6 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
 
   // v: words from value N c of key 16 h + 4 g + i in [4 h + i]
   __device__ __forceinline__ void add(float (&s)[8], const f32x4 (&value_scale)[2], const unsigned (&v)[8][VALUE_WORDS]) {
-    const float row_scale = SHAPED ? 1.0f : this->row_scale;
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaf(s[i], row_scale, frame_log(value_scale[i / 4][i % 4])));
@@ -987,7 +996,7 @@ __device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& 
     for (int j = 0; j < 4; ++j) o[b][j] = f32x4{0, 0, 0, 0};
   float m = -INFINITY, l = 0.0f;
   ScoreShape shape;
-  if constexpr (SHAPED) shape.start(p, t, head);
+  if constexpr (SHAPED) shape.start(p, t, head, 1.0f);
 
   for (; kb < end; kb += STEP) {
     look(kb, k, v, missing);
@@ -1004,8 +1013,8 @@ __device__ __forceinline__ void stream_rows(const AttentionArgs& p, const Tile& 
     f32x4 s = s0 + s1;
     if constexpr (SHAPED) {
       float formed[4] = {s[0], s[1], s[2], s[3]};
-      shape.apply(formed, [&](int i) { return kb + 4 * (int)g + i; });
-      s = f32x4{formed[0], formed[1], formed[2], formed[3]};
+      shape.apply(formed, kb + 4 * (int)g, [](int i) { return i; });
+      s = f32x4{formed[0], formed[1], formed[2], formed[3]} * shape.unit;
     }
     const bool more = kb + STEP < end;
     const Held next_pages = pages_of();
@@ -1439,7 +1448,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
   }
   // the row's query, as above: value 16 s + 8 (l / 32) + j in [s][j]
   f16x8 q_hi[KS], q_lo[KS];
-  float query_factor;
+  float row_scale;
   {
     const float* const q = p.q + (unsigned long long)(t.first + (t.row_token < 0 ? 0 : t.row_token)) * p.q_token + (head * p.group.d + t.row_head) * p.q_head;
     f32x4 x[2 * KS];
@@ -1456,7 +1465,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
     butterfly_pair<32>(top, a, b);
     const QueryScale scale = query_scale(fmaxf(a, b), p.scale);
     const float up = scale.up;
-    query_factor = scale.scale;
+    row_scale = scale.scale;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       Half8 hi, lo;
@@ -1469,13 +1478,15 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
       q_lo[s] = lo.v;
     }
   }
-  const float row_scale = SHAPED ? 1.0f : query_factor;  // SHAPED: it is in the scores
   f32x16 o[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) o[n] = f32x16{};
   float frame = -INFINITY, l = 0.0f;
   ScoreShape shape;
-  if constexpr (SHAPED) shape.start(p, t, head);
+  if constexpr (SHAPED) {
+    shape.start(p, t, head, row_scale);
+    row_scale = shape.unit;
+  }
 
   unsigned turn = 0;
 #pragma unroll 1
@@ -1511,8 +1522,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
     if constexpr (SHAPED) {
       float formed[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) formed[i] = x[i] * fminf(query_factor, 3.4028234e38f);
-      shape.apply(formed, [&](int i) { return kb + 8 * (i / 4) + 4 * (int)half + i % 4; });
+      for (int i = 0; i < 16; ++i) formed[i] = x[i];
+      shape.apply(formed, kb + 4 * (int)half, [](int i) { return 8 * (i / 4) + i % 4; });
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = formed[i];
     }
