@@ -176,6 +176,44 @@ def test_shaped_chunks_against_the_definition(pkg, T, kind, shape, case):
     m.check(T, **shape_of(m, SHAPES[shape], more))
 
 
+# Wide tiles of 4-bit integers: chunks that fill half of them, and 450 workgroups, or 280 over up to 512 keys; heads of 80 have rows of 40 bytes.
+WIDE = [
+    ([600, 400, 300], [260, 270, 290], 128, 64, 128, 32, {}),
+    ([300, 290, 0, 500, 260], [70, 97, 0, 90, 64], 128, 64, 128, 16, {}),
+    ([700, 600, 90], [300, 200, 90], 128, 64, 96, 20, {}),
+    ([513, 600, 90], [260, 300, 90], 128, 64, 80, 48, {}),
+    ([513, 600], [260, 300], 128, 64, 112, 20, {"window": 100}),
+    ([700, 600], [128, 140], 256, 64, 128, 32, {"window": 1}),
+    ([300, 400], [260, 270], 128, 64, 128, 16, {"causal": False}),
+    ([1500, 700, 300], [258, 257, 259], 64, 64, 128, 64, {"max_length": 1280}),
+    ([400, 200, 90], [260, 280, 90], 96, 48, 128, 24, {}),                     # more tokens than are cached
+    ([3000, 2500], [200, 160], 256, 64, 128, 32, {}),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(WIDE)))
+def test_wide_tiles_of_4_bits(pkg, T, case):
+    lengths, chunks, heads, kv, size, page, more = WIDE[case]
+    there = [n for n in chunks if n]
+    each = -(-(-(-sum(there) // len(chunks)) * heads // kv) // 128)
+    assert len(chunks) * each * kv >= (280 if max(lengths) <= 512 else 450)
+    m = Made(pkg, "s4", lengths, chunks, heads, kv, size, page, case)
+    m.check(T, **more)
+    m.check(T, **m.shaped(more, cap=4.0, slopes=True, prefixes=None if more.get("window") or "causal" in more else [100] * len(lengths)))
+    if case in (0, 3):
+        m.table[0, 0], m.table[1, 2], m.table[2, -1] = -1, m.cache[0].shape[0], 2 ** 31 - 1
+        m.check(T)
+        # what no row sees, and what only the last rows see, may be anything
+        before = T.n(m.run(T))
+        for i, (n, chunk) in enumerate(zip(lengths, chunks)):
+            for s in m.cache[2:]:
+                s[m.table[i][(n - 1) // page], :, (n - 1) % page] = np.nan
+        got, last = T.n(m.run(T)), m.starts[1:] - 1
+        rest = np.setdiff1d(np.arange(len(m.q)), last)
+        assert np.isnan(got[last]).all() and np.array_equal(got[rest], before[rest])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,longest,chunk,heads,kv,size,page", [(70, 900, 1, 16, 8, 64, 16), (150, 300, 3, 12, 4, 32, 32), (64, 1300, 1, 8, 8, 128, 64), (130, 40, 1, 4, 4, 48, 24),
                                                                     (40, 700, 2, 8, 8, 256, 32), (65, 3000, 1, 24, 4, 96, 16), (20, 1500, 9, 66, 2, 64, 20)])

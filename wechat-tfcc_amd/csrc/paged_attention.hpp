@@ -466,6 +466,10 @@ __device__ __forceinline__ void dma16_global(const void* from, unsigned to) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
 }
 
+__device__ __forceinline__ void dma4_global(const void* from, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(from) : "memory", "m0");
+}
+
 // The page that holds a key, in two halves: what the table says of it, and, when that is wanted, whether there is such a page (-1: none).
 // What is loaded in one step is looked at in the next: a step does not wait for the table.
 // (Constant memory as far as a launch goes, so that entries come through the scalar cache: among the vector loads, which return in their order,
@@ -653,13 +657,13 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
 };
 
 // Integers with pages of 16 rows and more that can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
-// of 16; WITHIN: pages of a multiple of 16 rows, so that a half lies in one, or of 32 for a whole step (4 bits), else (0) a half in up to two (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 49).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
+// of 16; WITHIN: pages of a multiple of 16 rows, so that a half lies in one, or of 32 for a whole step (4 bits), else (0) a half in up to two, and so where rows are no multiples of 16 bytes (-1, 4 bits) (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 49).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
 // straight into LDS, a ring of STAGES of its own (no barriers), and reads a step from there when it is due.
-template <int TYPE, int BLOCKS, int WAVES>
+template <int TYPE, int BLOCKS, int WAVES, bool NARROW>
 struct ScaledRing {
   static constexpr int kRow = ScaledLayout<TYPE, BLOCKS>::BYTES, kHalf = 16 * kRow, kRows = 4 * kHalf, kBytes = kRows + 256;  // keys and values, scales
   static constexpr int kStages = TYPE == TFCC_ROCM_S4 || kRow >= 128 ? 2 : 4;
-  static constexpr int kCopies = (kRow < 64 ? 2 : 4 * (kRow / 64)) + 1;
+  static constexpr int kCopies = (NARROW ? kRow / 4 : kRow < 64 ? 2 : 4 * (kRow / 64)) + 1;
   union {
     alignas(16) unsigned char ring[WAVES][kStages][kBytes];
     Joining<64 * BLOCKS, WAVES> joining;
@@ -667,8 +671,9 @@ struct ScaledRing {
 };
 template <int TYPE, int BLOCKS, int WAVES, int WITHIN, bool SHAPED>
 __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4 : BLOCKS == 2 ? 3 : 2) : 1) void attention_scaled_kernel(AttentionArgs p) {
-  constexpr bool WHOLE = WITHIN != 0;
-  typedef ScaledRing<TYPE, BLOCKS, WAVES> Ring;
+  constexpr bool WHOLE = WITHIN > 0;
+  constexpr bool NARROW = WITHIN < 0;
+  typedef ScaledRing<TYPE, BLOCKS, WAVES, NARROW> Ring;
   typedef ScaledLayout<TYPE, BLOCKS> Layout;
   constexpr int STEP = 32 * WAVES, CHUNKS = Layout::BYTES / 16 /* of 16 bytes in a row */;
   // Rows of 32 bytes: one copy brings both halves' keys, or values.
@@ -726,6 +731,31 @@ __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4
   const auto cut_of = [&](unsigned key) { return p.cache.page_size.d - inside_page(key); };
   const auto copy = [&](unsigned stage, int at, const int (&page)[2][PAGES]) {
     const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)(ring_at + stage * Ring::kBytes));
+    if constexpr (NARROW) {
+      // 4 bytes to a lane, which go where the above puts them: lane l of copy n has word l % WORDS of place n * ROWS + l / WORDS
+      constexpr int WORDS = Ring::kRow / 4, ROWS = 64 / WORDS;
+      const unsigned word = lane % WORDS;
+      const float* scale_of[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned key = (unsigned)at + 16 * h, inside = inside_page(key), cut = cut_of(key);
+        const unsigned long long first = page[h][0] < 0 ? 0 : (unsigned)page[h][0], next = page[h][PAGES - 1] < 0 ? 0 : (unsigned)page[h][PAGES - 1];
+        const long long base = (long long)(first * p.cache.page + inside * p.cache.row), other = (long long)(next * p.cache.page) - cut * (long long)p.cache.row;
+        scale_of[h] = c >= cut ? scales + next * p.cache.scale_page - cut : scales + first * p.cache.scale_page + inside;
+#pragma unroll 1  // (unrolled, their addresses take registers that a step does not have)
+        for (int n = 0; n < 16 / ROWS; ++n) {
+          const unsigned row = n * ROWS + lane / WORDS, from = ((word / 4 ^ exchange(row)) * 4 + word % 4) * 4;
+          dma4_global(keys + (row >= cut ? other : base) + (row * row_bytes + (from < size ? from : 0)), to + h * Ring::kHalf + n * 256);
+        }
+#pragma unroll 1
+        for (int n = 0; n < 16 / ROWS; ++n) {
+          const unsigned place = n * ROWS + lane / WORDS, row = (place / PER_COPY * FOURS + place % PER_COPY % FOURS) * 4 + place % PER_COPY / FOURS, from = word * 4;
+          dma4_global(values + (row >= cut ? other : base) + (row * row_bytes + (from < size ? from : 0)), to + (2 + h) * Ring::kHalf + n * 256);
+        }
+      }
+      dma4_global((lane & 16) ? scale_of[1] : scale_of[0], to + Ring::kRows);
+      return;
+    }
     if constexpr (WITHIN == 32) {
       const unsigned inside = inside_page((unsigned)at);
       const unsigned long long held = page[0][0] < 0 ? 0 : (unsigned)page[0][0], base = held * p.cache.page + inside * p.cache.row;
@@ -745,7 +775,7 @@ __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4
           else dma16s(v, to + 2 * Ring::kHalf + (LINES + b) * 1024, value_at[b], 16 * row_bytes);
         }
       const float* const scale = scales + held * p.cache.scale_page + inside + (lane & 16);
-      asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to + Ring::kRows), "v"(scale) : "memory", "m0");
+      dma4_global(scale, to + Ring::kRows);
       return;
     }
     const float* scale_at[2];
@@ -782,7 +812,7 @@ __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4
       dma16_global(values + (lane < 32 ? value_row_at[0] : value_row_at[1]) + value_at[0], to + 2 * Ring::kHalf);
     }
     const float* const scale = (lane & 16) ? scale_at[1] : scale_at[0];
-    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" : : "s"(to + Ring::kRows), "v"(scale) : "memory", "m0");
+    dma4_global(scale, to + Ring::kRows);
   };
   unsigned gone = 0;  // four bits a stage: of each half, what would be on its first and on its last page is nowhere
   if (kb < end) ask_pages(kb);
@@ -1191,6 +1221,7 @@ __device__ __attribute__((noinline)) void stream_far_rows_apart(const AttentionA
 template <int TYPE, int BLOCKS, int WAVES, bool WHOLE, bool SHAPED>
 __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void attention_tile_kernel(AttentionArgs p) {
   constexpr bool S8 = TYPE != TFCC_ROCM_F32 /* integers with scales */, S4 = TYPE == TFCC_ROCM_S4;
+  static_assert(!S4 || BLOCKS == 2);
   constexpr int KS = 4 * BLOCKS, N = 2 * BLOCKS, PIECES = S8 ? 1 : 2;  // products over a head, tiles of 32 of its values
   static_assert(S8 ? WAVES == 4 : BLOCKS * 4 == WAVES);
   struct Stage {
@@ -1221,7 +1252,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
   // key; those of the second values, four values of eight keys at a time, float32: two; the first wavefront the scales.
   constexpr int HALF = WAVES * 32, SIDE = HALF / kTileKeys, WORDS = S4 ? 8 * BLOCKS : S8 ? 16 * BLOCKS : 32 * BLOCKS, TASKS = (4 * WORDS + HALF - 1) / HALF;
   static_assert(S8 || (TASKS == 1 && 4 * WORDS == HALF));
-  constexpr int CHUNKS = S4 ? (BLOCKS + 1) / 2 : S8 ? BLOCKS : 4;  // of 16 bytes of a key to a thread
+  constexpr int CHUNKS = S4 ? 1 : S8 ? BLOCKS : 4;  // of 16 bytes of a key to a thread
   const unsigned row_bytes = S4 ? size / 2 : size;                 // S8 and S4
   const bool for_keys = threadIdx.x < HALF;
   const unsigned me = threadIdx.x % HALF;
@@ -1263,7 +1294,12 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
 #pragma unroll
       for (int b = 0; b < CHUNKS; ++b) {
         const unsigned d = S8 ? 16 * (me / 32 + 4 * b) : 4 * (me % SIDE + SIDE * b);
-        raw[b] = *reinterpret_cast<const u32x4*>(row + (d < (S8 ? row_bytes : size) ? d : 0));
+        if constexpr (S4) {  // rows of a multiple of 8 bytes
+          const u32x2 first = *reinterpret_cast<const u32x2*>(row + (d < row_bytes ? d : 0)), second = *reinterpret_cast<const u32x2*>(row + (d + 8 < row_bytes ? d + 8 : 0));
+          raw[b] = u32x4{first[0], first[1], second[0], second[1]};
+        } else {
+          raw[b] = *reinterpret_cast<const u32x4*>(row + (d < size ? d : 0));
+        }
       }
       if (S8 && threadIdx.x < 64) {
         const float* const s = (threadIdx.x < 32 ? p.cache.key_scales : p.cache.value_scales) + head * p.cache.scale_head;
@@ -1301,10 +1337,8 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
       for (int b = 0; b < CHUNKS; ++b) {
         const unsigned chunk = me / 32 + 4 * b;
         if constexpr (S4) {
-          if (2 * BLOCKS % 4 == 0 || chunk < 2 * BLOCKS) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s.keys[0][2 * chunk + i / 2][i % 2 * 32 + me % 32] = __builtin_bit_cast(u32x4, word_int4(raw[b][i]));
-          }
+          for (int i = 0; i < 4; ++i) s.keys[0][2 * chunk + i / 2][i % 2 * 32 + me % 32] = __builtin_bit_cast(u32x4, word_int4(raw[b][i]));
         } else {
           s.keys[0][chunk][me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][0], raw[b][1]));
           s.keys[0][chunk][32 + me % 32] = __builtin_bit_cast(u32x4, eight_int8(raw[b][2], raw[b][3]));
@@ -1736,8 +1770,11 @@ void launch_scaled_of(const AttentionArgs& a, dim3 grid, hipStream_t s, bool wid
   const auto start = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(WAVES * 64), 0, s, a); };
   const unsigned rows = a.cache.page_size.d;
   if (!wide) return start(attention_scaled_any_kernel<TYPE, BLOCKS, WAVES, SHAPED>);
-  if constexpr (TYPE == TFCC_ROCM_S4)
+  if constexpr (TYPE == TFCC_ROCM_S4) {
+    const unsigned long long bytes = a.cache.size / 2 | a.cache.page | a.cache.head | a.cache.row | reinterpret_cast<uintptr_t>(a.cache.keys) | reinterpret_cast<uintptr_t>(a.cache.values);
+    if (bytes % 16 != 0) return start(attention_scaled_kernel<TYPE, BLOCKS, WAVES, -1, SHAPED>);
     if (rows % 32 == 0) return start(attention_scaled_kernel<TYPE, BLOCKS, WAVES, 32, SHAPED>);
+  }
   start(rows % 16 == 0 ? attention_scaled_kernel<TYPE, BLOCKS, WAVES, 16, SHAPED> : attention_scaled_kernel<TYPE, BLOCKS, WAVES, 0, SHAPED>);
 }
 template <int TYPE, int BLOCKS, bool SHAPED>
@@ -1769,13 +1806,6 @@ template <bool SHAPED>
 void launch_attention(const AttentionArgs& a, int type, bool wide, const PagedAttentionPlan& plan, hipStream_t s) {
   const dim3 grid(plan.tiles * plan.splits * a.cache.heads);
   const unsigned blocks = (a.cache.size + 63) / 64;
-  const auto tiles = [&](auto code) {
-    constexpr int TYPE = decltype(code)::value;
-    if (blocks == 1) launch_tiles<TYPE, 1, SHAPED>(a, grid, s);
-    else if (blocks == 2) launch_tiles<TYPE, 2, SHAPED>(a, grid, s);
-    else if (blocks == 3) launch_tiles<TYPE, 3, SHAPED>(a, grid, s);
-    else launch_tiles<TYPE, 4, SHAPED>(a, grid, s);
-  };
   const auto scaled = [&](auto code) {
     constexpr int TYPE = decltype(code)::value;
     if (blocks == 1) launch_scaled<TYPE, 1, SHAPED>(a, grid, s, plan.waves, wide);
@@ -1786,8 +1816,11 @@ void launch_attention(const AttentionArgs& a, int type, bool wide, const PagedAt
     if (blocks == 1) hipLaunchKernelGGL((attention_tile_kernel<TFCC_ROCM_F32, 1, 4, false, SHAPED>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attention_tile_kernel<TFCC_ROCM_F32, 2, 8, false, SHAPED>), grid, dim3(512), 0, s, a);
   } else if (plan.rows != kAttentionRows) {
-    if (type == TFCC_ROCM_S4) tiles(std::integral_constant<int, TFCC_ROCM_S4>());
-    else tiles(std::integral_constant<int, TFCC_ROCM_S8>());
+    if (type == TFCC_ROCM_S4) launch_tiles<TFCC_ROCM_S4, 2, SHAPED>(a, grid, s);
+    else if (blocks == 1) launch_tiles<TFCC_ROCM_S8, 1, SHAPED>(a, grid, s);
+    else if (blocks == 2) launch_tiles<TFCC_ROCM_S8, 2, SHAPED>(a, grid, s);
+    else if (blocks == 3) launch_tiles<TFCC_ROCM_S8, 3, SHAPED>(a, grid, s);
+    else launch_tiles<TFCC_ROCM_S8, 4, SHAPED>(a, grid, s);
   } else if (type != TFCC_ROCM_F32) {
     if (type == TFCC_ROCM_S4) scaled(std::integral_constant<int, TFCC_ROCM_S4>());
     else scaled(std::integral_constant<int, TFCC_ROCM_S8>());

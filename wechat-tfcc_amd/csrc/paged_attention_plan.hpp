@@ -37,7 +37,12 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   };
   const uint64_t all = mean * group * chunks * cache_heads;  // rows
   bool wide = false;
-  if (chunk_rows > 0 && !float_cache) {
+  if (chunk_rows > 0 && halves) {
+    // 4-bit integers are cheap to unpack, and tiles of 16 rows, whose wavefronts wait for nobody, are ahead until there are wide tiles for nearly two to a CU, or over few keys for more than one
+    // (us with wide tiles and with 16 rows, 8 heads of 128, groups of 4 or 8: 2 chunks of 700 over 2500, 272 workgroups: 153 and 92; 10 of 200 over 1000, 400: 65 and 59; one of 1024 over
+    // 1100, groups of 8, 512: 75 and 81; 8 of 200 over 300, 320: 27 and 34; 16 of 512, 1536: 103 and 163).
+    wide = 2 * mean * group >= chunk_rows && groups_of(chunk_rows) >= (keys_of(chunk_rows) <= 512 ? 280 : 450);
+  } else if (chunk_rows > 0 && !float_cache) {
     // Wide tiles where chunks fill half of one and there are rows for the GPU, more of them over long contexts, whose steps tiles of 16 rows
     // take at the rate of HBM (rows in all: 39 chunks of up to 84 over 510, 32 heads over 8 of 128, 79000: 61 us, with tiles of 16 rows 99; 8 of 49 over 2706 with
     // a window of 293, 64 heads, 20500: 28 and 34; 12 of 184 over 589, 8 heads over 1 of 256, 13000: 74 and 57; over long contexts one of 1024 over
@@ -46,8 +51,9 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
     // (32 heads over 8 of 128, tokens x rows of all tiles: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
-    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in eight pieces 84 and 210).
-    wide = 2 * mean * group >= chunk_rows && (all >= 18000 || (all >= 8192 && keys_of(chunk_rows) >= 2048));
+    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in eight pieces 84 and 210).  Tiles of 128 rows, of which a CU takes two, want a workgroup for about every CU
+    // (12 heads of 64: 3 of 600 over 2000, 144 workgroups, 124 and 86; 10 of 200 over 1000, 240, 63 and 47; 12 of 300 over 1500, 288, 95 and 115).
+    wide = 2 * mean * group >= chunk_rows && ((all >= 18000 && (chunk_rows > 128 || groups_of(chunk_rows) >= 250)) || (all >= 8192 && keys_of(chunk_rows) >= 2048));
   }
   p.rows = wide ? chunk_rows : kAttentionRows;
   p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
