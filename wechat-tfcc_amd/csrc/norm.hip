@@ -1,7 +1,7 @@
 // Root-mean-square norm with the residual's addition, as float32 or as 8-bit integers with a scale for each row, and rows of integers
 // back to float32.  Bound: HBM; for few rows the latency of a launch.
 //
-// One pass: a row's threads keep t = h * weight in registers while the sum of squares (and the largest |t|) is joined, then round it.  The integers of a row do not
+// One pass: a row's threads keep h and the weights in registers while the sum of squares (and the largest |t|, t = h * weight) is joined, then round their products.  The integers of a row do not
 // depend on its root: n = 127 t / max |t|.  A product of two float32 is exact in 64 bits, so t and the largest are, and n is that of
 // the true quotient: t * (127 / max) is off by 2^-51 of itself, and where that may matter, next to a border, 127 t is compared with (n +- 1/2) max
 // in exact sums of two doubles.  64-bit operations run at the rate of 32-bit ones here, and a value takes a dozen of them: the norm stays bound by HBM.
@@ -16,6 +16,10 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));  // nee
 typedef unsigned u32_any __attribute__((aligned(1)));
 
 constexpr unsigned kNormMost = 16384;  // values of a row that registers hold
+// Up to so many rows a thread takes four values: with a workgroup for each CU or less a row's own time counts (float32, 4096 wide: 16 rows 4.0 us,
+// with sixteen values to a thread 4.5; 256 rows 5.1 and 5.6).  More rows fill the CUs either way, and fewer wavefronts join faster.
+// The integers of a row of 4096 are not faster so (16 rows: 5.9 us, with sixteen values to a thread 5.5).
+constexpr unsigned kFewRows = 256;
 
 struct NormArgs {
   const float *x, *residual, *weight;
@@ -121,9 +125,10 @@ __device__ __forceinline__ RowFactors factors_of(const NormArgs& p, const RowTot
   return f;
 }
 
-// A row to THREADS threads, HELD times four values of it to a thread: 4 HELD THREADS values at most.
+// A row to THREADS threads, HELD times four values of it to a thread: 4 HELD THREADS values at most.  The form with integers is held to the registers
+// of 8 wavefronts to a SIMD (3000 rows of 9537: 85 us, without 108); the plain one would spill there (110 us, without 95).
 template <unsigned THREADS, unsigned HELD, bool STEPS>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel(NormArgs p) {
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, STEPS && HELD > 1 ? 8 : 4) void rms_norm_kernel(NormArgs p) {
   constexpr unsigned ROWS = THREADS < 256 ? 256 / THREADS : 1;
   static_assert(THREADS == 64 || ROWS == 1);
   __shared__ double shared[2][16];
@@ -152,7 +157,8 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
         }
     }
   }
-  double t[HELD][4], squares = 0.0, top = 0.0, rest = 0.0;
+  const auto product = [&](unsigned i, unsigned j) { return (double)h[i][j] * (double)w[i][j]; };
+  double squares = 0.0, top = 0.0, rest = 0.0;
 #pragma unroll
   for (unsigned i = 0; i < HELD; ++i) {
     const unsigned at = 4 * (me + THREADS * i);
@@ -170,10 +176,10 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
     for (unsigned j = 0; j < 4; ++j) {
       const double v = h[i][j];
       squares = fma(v, v, squares);
-      t[i][j] = v * (double)w[i][j];
       if constexpr (STEPS) {
-        top = max64(top, fabs(t[i][j]));
-        rest = fma(t[i][j], 0.0, rest);  // 0, or NaN where t is not finite
+        const double t = product(i, j);
+        top = max64(top, fabs(t));
+        rest = fma(t, 0.0, rest);  // 0, or NaN where t is not finite
       }
     }
   }
@@ -189,7 +195,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
     if (p.out != nullptr) {
       f32x4 y;
 #pragma unroll
-      for (unsigned j = 0; j < 4; ++j) y[j] = (float)(t[i][j] * f.root);
+      for (unsigned j = 0; j < 4; ++j) y[j] = (float)(product(i, j) * f.root);
       float* const out = p.out + row * p.out_row + at;
       if (some == 4) {
         *reinterpret_cast<f32x4_any*>(out) = y;
@@ -203,7 +209,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void rms_norm_kernel
       unsigned word = 0;
 #pragma unroll
       for (unsigned j = 0; j < 4; ++j) {
-        const int q = 128 + (f.factor > 0.0 ? step_of(t[i][j], totals.top, f.factor) : 0);
+        const int q = 128 + (f.factor > 0.0 ? step_of(product(i, j), totals.top, f.factor) : 0);
         count += j < some ? q : 0;
         word |= (unsigned)q << (8 * j);
       }
@@ -359,8 +365,12 @@ int tfcc_rocm_rms_norm_f32(void* stream, const tfcc_rocm_rms_norm_desc* desc) {
   const auto start = [&](auto plain, auto quantized, unsigned threads, unsigned each) {
     hipLaunchKernelGGL((d.steps != nullptr ? quantized : plain), dim3((d.rows + each - 1) / each), dim3(threads), 0, s, a);
   };
-  if (d.width <= 1024) start(rms_norm_kernel<64, 4, false>, rms_norm_kernel<64, 4, true>, 256, 4);
+  const bool few = d.rows <= kFewRows;
+  if (d.width <= 1024 && few) start(rms_norm_kernel<256, 1, false>, rms_norm_kernel<256, 1, true>, 256, 1);
+  else if (d.width <= 1024) start(rms_norm_kernel<64, 4, false>, rms_norm_kernel<64, 4, true>, 256, 4);
+  else if (d.width <= 4096 && few && d.steps == nullptr) start(rms_norm_kernel<1024, 1, false>, nullptr, 1024, 1);
   else if (d.width <= 4096) start(rms_norm_kernel<256, 4, false>, rms_norm_kernel<256, 4, true>, 256, 1);
+  else if (d.width <= 8192) start(rms_norm_kernel<512, 4, false>, rms_norm_kernel<512, 4, true>, 512, 1);
   else if (d.width <= kNormMost) start(rms_norm_kernel<1024, 4, false>, rms_norm_kernel<1024, 4, true>, 1024, 1);
   else start(rms_norm_wide_kernel<false>, rms_norm_wide_kernel<true>, 1024, 1);
   return check_launch("rms_norm");

@@ -6,10 +6,12 @@
 // (1 / 7 for integers of 4 bits, which lie two to a byte).
 // The quotient is not formed: n is taken from x * (1 / scale), which can miss only next to a border, and the remainder x - n * scale,
 // which a fused multiply-add gives exactly there (|x| <= 127.5 scale, so it is a multiple of the smaller last place of x and scale
-// and at most about scale / 2: 24 bits hold it), moves it to the neighbour or, on a tie, to the even one.  So every
-// integer is that of the true quotient, at eight operations instead of a 64-bit division.
-// What is read and written once, the rows on their way in and out, passes the caches by, so that the int8 rows stay in the last level for
-// those who read them next (16 prompts of up to 2048 tokens of 8 x 128, written and read back, 274 MB each way: 75 + 73 us without, 81 + 49, 3.4 and 5.6 TB/s, with).
+// and at most about scale / 2: 24 bits hold it), tells: below scale / 2 n is right, and where one of a lane's four is not, all are taken again and moved
+// to the neighbour or, on a tie, to the even one.  So every integer is that of the true quotient, at four operations a value (with the
+// moves formed for every value, the join of the largest through LDS and keys and values in workgroups of their own the kernel was bound by its operations).
+// 16 x 2048 tokens of 8 x 128, 268 MB in: 67 us, 4.5 TB/s, for 4 bits, 69 us, 4.9 TB/s, for 8 (104 and 101 so), 80 us, 6.7 TB/s, as float32.
+// What is read and written once, the rows on their way in and out, passes the caches by, so that the integers stay in the last level for
+// those who read them next.
 // The amax is formed on the bits of |x|, which order infinities and NaNs above all numbers: a row with one gets a scale that is not
 // finite, integers 0, and reads back as NaN.
 #include "paged_cache.hpp"
@@ -35,12 +37,23 @@ struct WriteArgs {
 };
 
 constexpr unsigned kCacheThreads = 256;
+constexpr float kAlign = 12582912.0f;  // 1.5 x 2^23: the last place of a sum with it is 1
+
 
 // largest of the LANES lanes of a row, as bits
 template <int LANES>
 __device__ __forceinline__ unsigned row_max(unsigned u) {
+  // sixteen lanes turn among themselves without LDS
+  const auto turned = [&](auto by) {
+    const unsigned o = (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, 0x120 + decltype(by)::value, 0xf, 0xf, true);
+    u = u > o ? u : o;
+  };
+  turned(std::integral_constant<int, 8>{});
+  turned(std::integral_constant<int, 4>{});
+  turned(std::integral_constant<int, 2>{});
+  turned(std::integral_constant<int, 1>{});
 #pragma unroll
-  for (int m = LANES / 2; m > 0; m /= 2) {
+  for (int m = LANES / 2; m > 8; m /= 2) {
     const unsigned o = (unsigned)__shfl_xor((int)u, m, 64);
     u = u > o ? u : o;
   }
@@ -62,46 +75,62 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(WriteArgs p)
   const unsigned row = blockIdx.x * (kCacheThreads / LANES) + threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
   if (row >= p.rows) return;
   const unsigned token = p.heads.quotient(row), head = row - token * p.heads.d;
+  const bool mine = d < p.cache.size;
+  f32x4 both[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  if (mine) {
+    both[0] = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p.keys + token * p.key_token + head * p.key_head + d));
+    both[1] = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(p.values + token * p.value_token + head * p.value_head + d));
+  }
   const long long slot = p.wide_slots ? static_cast<const long long*>(p.slots)[token] : static_cast<const int*>(p.slots)[token];
   if (slot < 0 || slot >= (long long)p.cache.pages * p.cache.page_size.d) return;
   // (a division of 64 bits takes as long as a sixth of all the rest)
   const unsigned long long page = slot < 0x80000000ll ? p.cache.page_size.quotient((unsigned)slot) : (unsigned long long)slot / p.cache.page_size.d;
   const unsigned inside = (unsigned)(slot - page * p.cache.page_size.d);
-  const bool value = blockIdx.y != 0;
-  const float* in = value ? p.values + token * p.value_token + head * p.value_head : p.keys + token * p.key_token + head * p.key_head;
   const unsigned long long at = page * p.cache.page + head * p.cache.head + inside * p.cache.row;
-  const bool mine = d < p.cache.size;
-  f32x4 x = {0, 0, 0, 0};
-  if (mine) x = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any*>(in + d));
-  if constexpr (TYPE == TFCC_ROCM_F32) {
-    float* out = static_cast<float*>(const_cast<void*>(value ? p.cache.values : p.cache.keys)) + at;
-    if (mine) *reinterpret_cast<f32x4*>(out + d) = x;
-  } else {
-    unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned u = __float_as_uint(x[i]) & 0x7fffffffu;
-      top = top > u ? top : u;
-    }
-    top = row_max<LANES>(top);
-    const float scale = __uint_as_float(top) * (1.0f / kLargest<TYPE>);
-    int n[4] = {0, 0, 0, 0};
-    if (top < 0x7f800000u && scale > 0.0f) {
-      // a subnormal scale has no finite reciprocal: both are lifted by 2^64, which changes no quotient
-      const float lift = scale < 1e-30f ? 18446744073709551616.0f : 1.0f, s = scale * lift, inverse = 1.0f / s;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) n[i] = nearest<kLargest<TYPE>>(x[i] * lift, s, inverse);
-    }
-    int8_t* out = static_cast<int8_t*>(const_cast<void*>(value ? p.cache.values : p.cache.keys)) + at;
-    if constexpr (TYPE == TFCC_ROCM_S8) {
-      if (mine)
-        *reinterpret_cast<unsigned*>(out + d) = ((unsigned)n[0] & 255u) | ((unsigned)n[1] & 255u) << 8 | ((unsigned)n[2] & 255u) << 16 | (unsigned)n[3] << 24;
+  for (int value = 0; value < 2; ++value) {
+    const f32x4 x = both[value];
+    if constexpr (TYPE == TFCC_ROCM_F32) {
+      float* out = static_cast<float*>(const_cast<void*>(value ? p.cache.values : p.cache.keys)) + at;
+      if (mine) *reinterpret_cast<f32x4*>(out + d) = x;
     } else {
-      if (mine)
-        *reinterpret_cast<uint16_t*>(out + d / 2) = (uint16_t)(((unsigned)n[0] & 15u) | ((unsigned)n[1] & 15u) << 4 | ((unsigned)n[2] & 15u) << 8 | ((unsigned)n[3] & 15u) << 12);
+      unsigned top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned u = __float_as_uint(x[i]) & 0x7fffffffu;
+        top = top > u ? top : u;
+      }
+      top = row_max<LANES>(top);
+      const float scale = __uint_as_float(top) * (1.0f / kLargest<TYPE>);
+      unsigned bits[4] = {0, 0, 0, 0};  // the integers, right in their lowest bits
+      if (top < 0x7f800000u && scale > 0.0f) {
+        // the sum leaves the integer in its low bits; v_rcp_f32 is off by a unit in the last place, which only the remainder's test has to know
+        const float inverse = __builtin_amdgcn_rcpf(scale), half = 0.5f * scale;
+        float over = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float sum = fmaf(x[i], inverse, kAlign);
+          bits[i] = __float_as_uint(sum);
+          over = fmaxf(over, fabsf(fmaf(kAlign - sum, scale, x[i])));
+        }
+        if (!(over < half) || scale < 1e-30f) {
+          // a subnormal scale has no finite reciprocal: both are lifted by 2^64, which changes no quotient
+          const float lift = scale < 1e-30f ? 18446744073709551616.0f : 1.0f, s = scale * lift, inverse = 1.0f / s;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) bits[i] = (unsigned)nearest<kLargest<TYPE>>(x[i] * lift, s, inverse);
+        }
+      }
+      int8_t* out = static_cast<int8_t*>(const_cast<void*>(value ? p.cache.values : p.cache.keys)) + at;
+      if constexpr (TYPE == TFCC_ROCM_S8) {
+        const unsigned low = __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u), high = __builtin_amdgcn_perm(bits[3], bits[2], 0x04000c0cu);
+        if (mine) *reinterpret_cast<unsigned*>(out + d) = low | high;
+      } else {
+        const unsigned pair = (bits[0] & 15u) | (bits[1] & 15u) << 4 | (bits[2] & 15u) << 8 | (bits[3] & 15u) << 12;
+        if (mine) *reinterpret_cast<uint16_t*>(out + d / 2) = (uint16_t)pair;
+      }
+      if (d == 0)
+        const_cast<float*>(value ? p.cache.value_scales : p.cache.key_scales)[page * p.cache.scale_page + head * p.cache.scale_head + inside * p.cache.scale_row] = scale;
     }
-    if (d == 0)
-      const_cast<float*>(value ? p.cache.value_scales : p.cache.key_scales)[page * p.cache.scale_page + head * p.cache.scale_head + inside * p.cache.scale_row] = scale;
   }
 }
 
@@ -265,7 +294,7 @@ int tfcc_rocm_cache_write(void* stream, const tfcc_rocm_paged_cache* cache, cons
   const hipStream_t s = as_stream(stream);
   const auto start = [&](auto s4, auto s8, auto f32) {
     const unsigned rows = kCacheThreads / lanes;
-    hipLaunchKernelGGL((cache->type == TFCC_ROCM_S4 ? s4 : cache->type == TFCC_ROCM_S8 ? s8 : f32), dim3((a.rows + rows - 1) / rows, 2), dim3(kCacheThreads), 0, s, a);
+    hipLaunchKernelGGL((cache->type == TFCC_ROCM_S4 ? s4 : cache->type == TFCC_ROCM_S8 ? s8 : f32), dim3((a.rows + rows - 1) / rows), dim3(kCacheThreads), 0, s, a);
   };
   if (lanes == 16) start(cache_write_kernel<TFCC_ROCM_S4, 16>, cache_write_kernel<TFCC_ROCM_S8, 16>, cache_write_kernel<TFCC_ROCM_F32, 16>);
   else if (lanes == 32) start(cache_write_kernel<TFCC_ROCM_S4, 32>, cache_write_kernel<TFCC_ROCM_S8, 32>, cache_write_kernel<TFCC_ROCM_F32, 32>);
