@@ -46,6 +46,51 @@ __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) 
   }
 }
 
+// Few pieces: LANES lanes to a row (at least a quarter of its values), which sum them one after the other.  HBM is its bound where there are many rows
+// (10 chunks of 512, 12 heads of 64, two pieces: 12 us, and 77 with a workgroup to a row).
+constexpr unsigned kFewPieces = 8;
+template <unsigned LANES>
+__global__ __launch_bounds__(kThreads) void join_few_kernel(AttentionArgs p) {
+  const unsigned heads = p.cache.heads * p.group.d, size = p.cache.size, d = threadIdx.x % LANES * 4;
+  const unsigned row = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES, rows = p.tokens * heads;
+  if (row >= rows || d >= size) return;
+  const unsigned token = row / heads, head = row - token * heads;
+  if ((int)token >= p.starts[p.batch] || (int)token < p.starts[0]) return;
+  const unsigned long long each = (unsigned long long)rows * size;  // of a piece
+  const float* const partial = p.partial + (unsigned long long)row * size + d;
+  const f32x2* const statistics = reinterpret_cast<const f32x2*>(p.statistics) + row;
+  float top = -INFINITY, total = 0.0f;
+  f32x4 sum = {0, 0, 0, 0};
+  // four pieces' loads at a time; what is summed so far is in units of 2^top
+  for (unsigned first = 0; first < p.splits; first += 4) {
+    f32x2 held[4];
+    f32x4 part[4];
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+      const unsigned piece = first + i < p.splits ? first + i : first;
+      held[i] = statistics[(unsigned long long)piece * rows];
+      part[i] = *reinterpret_cast<const f32x4*>(partial + piece * each);
+    }
+    const float before = top;
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) top = fmaxf(top, held[i][0]);
+    if (before != -INFINITY && before != top) {
+      const float h = half_step(before, top);
+      total = total * h * h;
+      sum *= h * h;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i) {
+      if (first + i >= p.splits || held[i][0] == -INFINITY) continue;  // none, or one without a key of this row
+      const float h = half_step(held[i][0], top);
+      total += held[i][1] * h * h;
+      sum += h * h * part[i];
+    }
+  }
+  const f32x4 none = {0, 0, 0, 0};
+  *reinterpret_cast<f32x4*>(p.out + token * p.out_token + head * p.out_head + d) = top == -INFINITY ? none : sum / total;
+}
+
 int check_attention(const tfcc_rocm_paged_attention_desc& d) {
   if (int e = check_cache(d.cache, "paged_attention")) return e;
   TFCC_REQUIRE(d.heads > 0 && d.heads % d.cache.heads == 0, "paged_attention: %u heads over %u cache heads", d.heads, d.cache.heads);
@@ -152,7 +197,12 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   if (int e = check_launch("paged_attention")) return e;
   if (plan.splits > 1) {
     const unsigned rows = d.tokens * d.heads;
-    hipLaunchKernelGGL(join_pieces_kernel, dim3(rows), dim3(kThreads), 0, s, a);
+    if (plan.splits > kFewPieces) {
+      hipLaunchKernelGGL(join_pieces_kernel, dim3(rows), dim3(kThreads), 0, s, a);
+    } else {
+      const unsigned lanes = a.cache.size <= 64 ? 16 : a.cache.size <= 128 ? 32 : 64, each = kThreads / lanes;
+      hipLaunchKernelGGL((lanes == 16 ? join_few_kernel<16> : lanes == 32 ? join_few_kernel<32> : join_few_kernel<64>), dim3((rows + each - 1) / each), dim3(kThreads), 0, s, a);
+    }
     return check_launch("paged_attention join");
   }
   return TFCC_ROCM_OK;

@@ -1401,25 +1401,30 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
         raw[j / 2][j % 2 * 2 + 1] = none ? 0u : raw[j / 2][j % 2 * 2 + 1];
       }
     }
-    unsigned most = 0;
+    unsigned most = 0, rows[8];  // of all, and of two values side by side: those that a thread for values has of a row
+    const auto measure = [&] {
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most = larger(most, size_of(raw[b][i]));
+      for (int j = 0; j < 8; ++j) {
+        rows[j] = larger(size_of(raw[j / 2][j % 2 * 2]), size_of(raw[j / 2][j % 2 * 2 + 1]));
+        most = larger(most, rows[j]);
+      }
+    };
+    measure();
     if (__any(most >= kFar)) {  // rare; for the rows that do not see it, as zeros, which change nothing
       odd = true;
       most = 0;
 #pragma unroll
       for (int b = 0; b < 4; ++b)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          raw[b][i] = size_of(raw[b][i]) >= kFar ? 0u : raw[b][i];
-          most = larger(most, size_of(raw[b][i]));
-        }
+        for (int i = 0; i < 4; ++i) raw[b][i] = size_of(raw[b][i]) >= kFar ? 0u : raw[b][i];
+      measure();
     }
+    // in the place where float32 has it, e with |v| < 2^(e - 126), 26 or more: 2^(140 - e) brings v to 2^13 .. 2^14
+    const auto exponent_of = [&](unsigned v) { return larger(v, 26u << 23) & 0x7f800000u; };
+    constexpr unsigned kUp = 267u << 23;
     if (for_keys) {
-      const int e = bound_of(__uint_as_float(lanes_max<SIDE>(most)));
-      const float up = power(14 - e);
+      const unsigned e = exponent_of(lanes_max<SIDE>(most));
+      const float up = __uint_as_float(kUp - e);
       const unsigned key = me / SIDE, part = me % SIDE;
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -1430,7 +1435,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
         reinterpret_cast<u32x2*>(&s.keys[0][step][to])[part % 2] = u32x2{__builtin_bit_cast(unsigned, hi[0]), __builtin_bit_cast(unsigned, hi[1])};
         reinterpret_cast<u32x2*>(&s.keys[PIECES - 1][step][to])[part % 2] = u32x2{__builtin_bit_cast(unsigned, lo[0]), __builtin_bit_cast(unsigned, lo[1])};
       }
-      if (part == 0) s.key_scale[key] = power(e - 14);
+      if (part == 0) s.key_scale[key] = __uint_as_float(e - (13u << 23));
       // a bit for each SIDE threads to neighbouring bits: of 8 by a product that moves bit 8 i to 56 + i
       u64 nowhere = __ballot(gone);
       if constexpr (SIDE == 8) {
@@ -1445,20 +1450,20 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
       if (lane == 0) s.gone[wave] = (unsigned)(nowhere & ((1ull << 64 / SIDE) - 1)) << (64 / SIDE * wave);
     } else {
       const unsigned word = me % WORDS, group = me / WORDS;
-      int exponent[8];
+      unsigned exponent[8];
       float up[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {  // of the lanes that have the row
-        exponent[j] = bound_of(__uint_as_float(lanes_max<WORDS>(larger(size_of(raw[j / 2][j % 2 * 2]), size_of(raw[j / 2][j % 2 * 2 + 1])))));
-        up[j] = power(14 - exponent[j]);
+        exponent[j] = exponent_of(lanes_max<WORDS>(rows[j]));
+        up[j] = __uint_as_float(kUp - exponent[j]);
       }
-      int e = exponent[0];
+      unsigned e = exponent[0];
 #pragma unroll
       for (int j = 1; j < 8; ++j) e = word == (unsigned)j ? exponent[j] : e;
       if (word < 8) {
         const unsigned key = group / 2 * 16 + 4 * (group % 2) + 8 * (word / 4) + word % 4;
-        s.value_scale[key] = power(e - 14 + kLift);
-        s.value_log[key] = (float)(e - 14 + kLift);
+        s.value_scale[key] = __uint_as_float(e + (unsigned)((kLift - 13) * (1 << 23)));
+        s.value_log[key] = (float)((int)(e >> 23) - 140 + kLift);
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {

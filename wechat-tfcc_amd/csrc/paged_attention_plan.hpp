@@ -50,10 +50,11 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
     wide = 2 * mean * group >= chunk_rows && all >= (keys_of(chunk_rows) <= 1536 ? 20000 : 32000);
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
-    // (32 heads over 8 of 128, tokens x rows of all tiles: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
-    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in eight pieces 84 and 210).  Tiles of 128 rows, of which a CU takes two, want a workgroup for about every CU
-    // (12 heads of 64: 3 of 600 over 2000, 144 workgroups, 124 and 86; 10 of 200 over 1000, 240, 63 and 47; 12 of 300 over 1500, 288, 95 and 115).
-    wide = 2 * mean * group >= chunk_rows && ((all >= 18000 && (chunk_rows > 128 || groups_of(chunk_rows) >= 250)) || (all >= 8192 && keys_of(chunk_rows) >= 2048));
+    // (32 heads over 8 of 128: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
+    // one of 674, 24 heads over 4 of 96: 73 and 62; 4 of 128 over 1500 in four pieces 75 and 170; 12 heads of 64: 5 of 512 over 2000 in two pieces 99 and 185, over 1024 59 and 93;
+    // 2 of 512 over 1024 38 and 46, over 512 27 and 22).  Tiles of 128 rows, of which a CU takes two, want a workgroup for about every CU over short ones
+    // (8 of up to 300 over up to 700, 192 workgroups, 55 and 48; 12 of 300 over 1500, 288, 95 and 115).
+    wide = 2 * mean * group >= chunk_rows && ((all >= 18000 && (chunk_rows > 128 || groups_of(chunk_rows) >= 250)) || (all >= 8192 && keys_of(chunk_rows) >= 1000));
   }
   p.rows = wide ? chunk_rows : kAttentionRows;
   p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
@@ -71,10 +72,10 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   }
   if (!wide) step = p.waves * (float_cache ? 16 : 32);
   if (wide && float_cache) {
-    // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 260 us, one 404)
+    // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 260 us, one 404; over 1024 77 and 116; 2 of 512 over 512 52 and 64)
     p.waves = chunk_rows / 32;
     const uint64_t fit = groups == 0 ? 1 : 256 * 256 / chunk_rows / groups;
-    splits = keys < 2048 || fit < 1 ? 1 : fit < keys / 512 ? fit : keys / 512;
+    splits = keys < 512 || fit < 1 ? 1 : fit < keys / 256 ? fit : keys / 256;
     if (splits > 8) splits = 8;
   } else if (wide) {
     p.waves = 4;
