@@ -239,6 +239,36 @@ def test_workgroups_of_many_wavefronts(pkg, T, lengths, heads, kv, size, page):
     m.check(T, **m.shaped({}, cap=3.0, slopes=True, prefixes=[40] * len(lengths)))
 
 
+PIECES = [
+    # kind, lengths, chunks, heads, kv heads, size, page of calls whose keys come in 2 to 19 pieces, and in 2 and 3 with wide tiles
+    ("s4", [1000], [1], 64, 64, 64, 16),
+    ("s8", [1500, 90], [2, 1], 60, 60, 64, 16),
+    ("f32", [1000, 300], [1, 3], 24, 24, 64, 16),
+    ("s8", [1790], [1], 32, 8, 128, 32),
+    ("f32", [1000, 300], [1, 3], 12, 12, 64, 16),
+    ("s4", [2300, 40], [1, 1], 8, 2, 128, 32),
+    ("f32", [1000, 20, 640], [512, 20, 600], 12, 12, 64, 16),
+    ("f32", [1500, 1100], [160, 120], 32, 8, 128, 16),
+    ("s8", [2100, 40], [1060, 40], 32, 8, 128, 16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rising", [1, -1])
+@pytest.mark.parametrize("case", range(len(PIECES)))
+def test_pieces_joined(pkg, T, case, rising):
+    """Scores that rise or fall by 60 over the keys, so that the largest is in one piece and the others' sums shrink to it; prefixes, by which pieces are
+    empty for some rows and not for others; and rows that see nothing."""
+    kind, lengths, chunks, heads, kv, size, page = PIECES[case]
+    m = Made(pkg, kind, lengths, chunks, heads, kv, size, page, 100 + case)
+    m.check(T)
+    slopes = np.full(heads, rising * 60.0 / max(lengths), np.float32)
+    m.check(T, slopes=slopes)
+    m.check(T, slopes=-slopes / 6, cap=3.0, prefixes=np.array([n // 3 for n in lengths], np.int32))
+    m.lengths[-1] = 0
+    m.check(T, slopes=slopes)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["s4", "s8", "f32"])
 @pytest.mark.parametrize("lengths,chunks,heads,kv", [([400, 90], [3, 1], 8, 2), ([700, 300], [300, 290], 64, 64)])

@@ -51,7 +51,7 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
     // (32 heads over 8 of 128: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
-    // one of 674, 24 heads over 4 of 96: 73 and 62; 4 of 128 over 1500 in four pieces 75 and 170; 12 heads of 64: 5 of 512 over 2000 in two pieces 99 and 185, over 1024 59 and 93;
+    // one of 674, 24 heads over 4 of 96: 73 and 62; 4 of 128 over 1500 in three pieces 75 and 170; 12 heads of 64: 5 of 512 over 2000 in two pieces 99 and 185, over 1024 59 and 93;
     // 2 of 512 over 1024 38 and 46, over 512 27 and 22).  Tiles of 128 rows, of which a CU takes two, want a workgroup for about every CU over short ones
     // (8 of up to 300 over up to 700, 192 workgroups, 55 and 48; 12 of 300 over 1500, 288, 95 and 115).
     wide = 2 * mean * group >= chunk_rows && ((all >= 18000 && (chunk_rows > 128 || groups_of(chunk_rows) >= 250)) || (all >= 8192 && keys_of(chunk_rows) >= 1000));
