@@ -119,6 +119,34 @@ def test_every_integer_is_the_true_quotients(pkg, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,most", [("uint8", 7), ("int8", 127)])
+@pytest.mark.parametrize("size", [32, 128, 256])
+def test_scales_of_all_exponents(pkg, T, kind, most, size):
+    """From subnormal ones to float32's largest, with values on the borders between two integers, next to them and elsewhere."""
+    import torch
+    rng = np.random.default_rng(size)
+    top = np.ldexp(1 + rng.random(1024), rng.permutation(np.arange(1024) % 276) - 148).astype(np.float32)
+    top[:2] = np.float32(3.4028234e38), np.float32(2.0 ** -149)
+    scale = top * np.float32(1 / most)
+    border = (rng.integers(-most, most, (1024, size)) + 0.5) * scale[:, None].astype(np.float64)
+    with np.errstate(over="ignore", under="ignore"):
+        rows = border.astype(np.float32)
+        near = np.nextafter(rows, np.float32(np.inf) * rng.choice([-1, 1], rows.shape).astype(np.float32))
+        rows = np.where(rng.random(rows.shape) < 0.4, near, rows)
+        rows = np.where(rng.random(rows.shape) < 0.3, (rng.uniform(-1, 1, rows.shape) * top[:, None].astype(np.float64)).astype(np.float32), rows)
+    rows = np.clip(rows, -top[:, None], top[:, None])
+    rows[:, size - 1] = top
+    cache = pkg.paged_cache(64, 1, 16, size, getattr(torch, kind))
+    pkg.cache_write(cache, T.t(rows[:, None]), T.t(-rows[:, None]), T.t(np.arange(1024, dtype=np.int32)))
+    good = scale > 0
+    n = np.rint(rows.astype(np.float64) / np.where(good, scale, 1).astype(np.float64)[:, None])
+    n = np.where(good[:, None], np.clip(n, -most, most), 0).astype(np.int8)
+    for i, sign in ((0, 1), (1, -1)):
+        want = R.pack(sign * n) if kind == "uint8" else sign * n
+        assert np.array_equal(T.n(cache[i]).reshape(1024, -1), want) and np.array_equal(T.n(cache[2 + i]).reshape(-1), scale)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("heads,page,size,tokens,pages", WRITTEN)
 def test_read_back(pkg, T, heads, page, size, tokens, pages):
     import torch

@@ -84,6 +84,14 @@ def test_against_the_definition(pkg, T, width, residual):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width", [(256, 1023), (257, 1023), (256, 2050), (257, 2050), (600, 4096), (300, 5001), (300, 9537)])
+def test_few_rows_and_many(pkg, T, rows, width):
+    rng = np.random.default_rng(rows + width)
+    x = (rng.normal(size=(rows, width)) * np.exp(rng.normal(size=(rows, 1)) * 4)).astype(np.float32)
+    check(T, pkg, x, (rng.random(width) + 0.5).astype(np.float32), 1e-6, rng.normal(size=x.shape).astype(np.float32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(1, 1, 16), (0, 8), (3, 0, 8), (2, 3, 5, 20), (300, 256), (16,)])
 def test_shapes(pkg, T, shape):
     rng = np.random.default_rng(1)
