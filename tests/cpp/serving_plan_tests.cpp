@@ -36,9 +36,13 @@ int main() {
   EXPECT(four(100 * 63, 100, 1, 8, 128, 512).rows == 16 && four(100 * 64, 100, 1, 8, 128, 512).rows == 128);  // chunks that fill half of one
   // float32: wide tiles from 8192 rows on over 1000 keys, in as many pieces as run at the same time
   EXPECT(float32(5 * 512, 5, 1, 12, 64, 1000).rows == 128 && float32(5 * 512, 5, 1, 12, 64, 999).rows == 16 && float32(5 * 512, 5, 1, 12, 64, 1000).splits == 2);
-  EXPECT(float32(4 * 128, 4, 1, 12, 64, 1500).rows == 16 && float32(4 * 128, 4, 4, 8, 128, 1500).rows == 256 && float32(4 * 128, 4, 4, 8, 128, 1500).splits == 3);  // of 512 keys
+  EXPECT(float32(4 * 128, 4, 1, 12, 64, 1500).rows == 16 && float32(4 * 128, 4, 4, 8, 128, 1500).rows == 256 && float32(4 * 128, 4, 4, 8, 128, 1500).splits == 4);
   EXPECT(float32(2 * 512, 2, 4, 8, 128, 512).splits == 2 && float32(2 * 512, 2, 4, 8, 128, 511).splits == 1);
-  EXPECT(float32(6 * 600, 6, 1, 12, 64, 1200).splits == 1);  // 360 workgroups
+  EXPECT(float32(2 * 512, 2, 4, 8, 128, 512).split_keys == 256 && float32(5 * 512, 5, 1, 12, 64, 1000).split_keys == 512);
+  // one more over long contexts
+  EXPECT(float32(5 * 600, 5, 1, 12, 64, 1024).splits == 2 && float32(5 * 600, 5, 1, 12, 64, 1023).splits == 1 && float32(6 * 600, 6, 1, 12, 64, 1200).splits == 1);
+  EXPECT(float32(3 * 600, 3, 1, 12, 64, 1536).splits == 3 && float32(3 * 600, 3, 1, 12, 64, 1535).splits == 2 && float32(1024, 1, 1, 12, 64, 4096).splits == 5);
+  EXPECT(float32(20 * 64, 20, 4, 8, 128, 4000).splits == 1);
   std::mt19937 g(2);
   for (int turn = 0; turn < 20000; ++turn) {
     const unsigned batch = 1 + g() % 70, group = 1 + g() % 9, heads = 1 + g() % 40, size = 16 * (1 + g() % 16), most = g() % 3 ? g() % 9000 : g() % 300;

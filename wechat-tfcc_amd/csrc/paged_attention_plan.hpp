@@ -51,7 +51,7 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
     // (32 heads over 8 of 128: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
-    // one of 674, 24 heads over 4 of 96: 73 and 62; 4 of 128 over 1500 in three pieces 75 and 170; 12 heads of 64: 5 of 512 over 2000 in two pieces 99 and 185, over 1024 59 and 93;
+    // one of 674, 24 heads over 4 of 96: 73 and 62; 4 of 128 over 1500 in four pieces 68 and 170; 12 heads of 64: 5 of 512 over 2000 in two pieces 99 and 185, over 1024 59 and 93;
     // 2 of 512 over 1024 38 and 46, over 512 27 and 22).  Tiles of 128 rows, of which a CU takes two, want a workgroup for about every CU over short ones
     // (8 of up to 300 over up to 700, 192 workgroups, 55 and 48; 12 of 300 over 1500, 288, 95 and 115).
     wide = 2 * mean * group >= chunk_rows && ((all >= 18000 && (chunk_rows > 128 || groups_of(chunk_rows) >= 250)) || (all >= 8192 && keys_of(chunk_rows) >= 1000));
@@ -74,7 +74,12 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   if (wide && float_cache) {
     // as many as run at the same time (one of 1024 tokens over 4096, 128 workgroups: two pieces 260 us, one 404; over 1024 77 and 116; 2 of 512 over 512 52 and 64)
     p.waves = chunk_rows / 32;
-    const uint64_t fit = groups == 0 ? 1 : 256 * 256 / chunk_rows / groups;
+    step = p.waves * 16;
+    uint64_t fit = groups == 0 ? 1 : 256 * 256 / chunk_rows / groups;
+    // One more where that leaves many places free: of two or three pieces the tiles that see few keys, or are not there, make room for the others' (12 heads of 64, two and
+    // one: 6 of up to 517 over up to 1201 67 us and 82, 3 of 1000 over 6000 401 and 471; three and two: one prompt of 1900 67 and 85, 3 of up to 600 over up to 2000 72 and 95,
+    // but 5 of up to 512 over up to 1024, pieces of 350, 64 and 56, 6 of up to 517 over up to 1201 with 16 heads, 384 workgroups, 98 and 86; six and five: one of 1024 over 4096 104 and 82; tiles of 256 rows, 20 of 64 over 1000, 144 and 120).
+    if (chunk_rows == 128 && ((fit == 1 && groups <= 320) || (fit == 2 && groups <= 192)) && keys >= 512 * (fit + 1)) ++fit;
     splits = keys < 512 || fit < 1 ? 1 : fit < keys / 256 ? fit : keys / 256;
     if (splits > 8) splits = 8;
   } else if (wide) {
