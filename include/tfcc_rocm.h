@@ -603,7 +603,7 @@ int tfcc_rocm_cache_copy(void* stream, const tfcc_rocm_paged_cache* cache, const
  * tokens * heads < 2^31, and no more workgroups than one launch takes: a chunk has one for every 16 rows (token, query head) of a
  * cache head, or part of 16, and 2^24 - 1 are the most.
  * Sums and weights are float32, whatever the cache's type.  A term of a product is right to 2^-23 of it, over a float32 cache with many rows to
- * 2^-21, but for parts of a row that lie 2^-30 below its largest value, which may be lost (F32, many rows: and below 2^-139; S8: where the scales are 2^-100 to 2^96 - where all of a row's values have scales below
+ * 2^-21, but for parts of a row that lie 2^-30 below its largest value, which may be lost (F32, many rows: and below 2^-139; S8 and S4: where the scales are 2^-100 to 2^96 - where all of a row's values have scales below
  * 2^-(90 + n), 2^-(33 - n) of the largest product is lost).  Sums of weights times values are divided last: where those reach 2^128, they are
  * infinite.  Where rows of many see an infinity, a NaN or a number of 2^80 or more in a float32 cache, they and those beside them are worked out
  * twice, in up to four times the time.  out overlaps no input. */

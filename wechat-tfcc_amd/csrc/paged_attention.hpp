@@ -14,7 +14,8 @@
 // fp16 matrix operations.  Queries are scaled by a power of two for each row.  What meets the values is a weight times a value's scale, and
 // what has to stay in fp16's range is that product, not the weight: a row's weights are 2^(score - frame), and the frame moves where
 // score + log2(scale) exceeds it by 15, to 8 below.  Between moves nothing is rescaled, and what fp16 cannot hold is 2^-32 of
-// the largest product or less.  The sum of the weights is kept in the same frame.  A float32 cache goes through the fp32 matrix operations, and
+// the largest product or less.  The sum of the weights is kept in the same frame.  Integers of 4 bits are those of 8 but for the way they are unpacked: the
+// bytes on their way halve, the operations do not.  A float32 cache goes through the fp32 matrix operations, and
 // chunks of many tokens over one through three fp16 operations of pieces, which take two fifths of the time.
 //
 // The keys of a tile are dealt to the wavefronts of a workgroup in turns, and in pieces to several workgroups where there are few tiles; each
@@ -235,7 +236,8 @@ __device__ __forceinline__ int bound_of(float v) {
 // tanh to about float32's last place, of the result and not of 1: below 0.55, x + x^3 P(x^2) with P of degree 4 fitted for the smallest relative error (2^-29), above,
 // 1 - 2 / (2^(2 log2(e) x) + 1).  Most scores are far below their cap: where those of a whole wavefront are, the second is passed over.  A score as
 // it comes (`raw`) takes the factor of its row and the cap's inverse in one, and leaves in units of `unit`, the cap where nothing is added to it: a
-// cap costs nine operations, a bias two.
+// cap costs nine operations, a bias two (int8, 32 sequences of up to 6000 with a window of 4096, 8 heads of 256, at the rate of HBM: 97 us with a cap, 92 without; 4 chunks of 1024
+// over 4096 in 4 bits, bound by operations: 385 us plain, 503 with a cap, 415 with slopes).
 // The bias is slope * distance.  A row's softmax does not change with what all its scores have in common, so a position behind the last key
 // that the row may see counts as that key's, and one before the first as the first's: differences are whole numbers, exact up to 2^24.
 struct ScoreShape {
@@ -657,8 +659,11 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
 };
 
 // Integers with pages of 16 rows and more that can be read 16 bytes at a time.  A wavefront takes 32 keys in a step, two halves
-// of 16; WITHIN: pages of a multiple of 16 rows, so that a half lies in one, or of 32 for a whole step (4 bits), else (0) a half in up to two, and so where rows are no multiples of 16 bytes (-1, 4 bits) (32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, and 49).  Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps
-// straight into LDS, a ring of STAGES of its own (no barriers), and reads a step from there when it is due.
+// of 16; WITHIN: pages of a multiple of 16 rows, so that a half lies in one, or of 32 for a whole step (4 bits), else (0) a half in up to two, and so where
+// rows are no multiples of 16 bytes (-1, 4 bits), which come four bytes to a lane.  8 bits, 32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, pages of 24 rows 49.
+// Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps straight into LDS, a ring of kStages of its own
+// (no barriers), and reads a step from there when it is due.  4 bits: as much by the vector unit, whose operations take 57 % of the time (64 sequences of 1024 to 4096,
+// 8 heads of 128, 197 MB: 48 to 51 us, 3.9 to 4.1 TB/s; 32 of 16384, 571 MB: 117 to 130 us, 4.4 to 4.9 TB/s).
 template <int TYPE, int BLOCKS, int WAVES, bool NARROW>
 struct ScaledRing {
   static constexpr int kRow = ScaledLayout<TYPE, BLOCKS>::BYTES, kHalf = 16 * kRow, kRows = 4 * kHalf, kBytes = kRows + 256;  // keys and values, scales
@@ -834,12 +839,15 @@ __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4
       if (ahead < end) ask_pages(ahead);
     }
   };
-  // The queries first: loads come back in their order, and behind the copies they would wait for all stages to be filled.  (The pages' entries, which the copies
-  // need, are on their way meanwhile.)
+  // Loads come back in their order: queries behind the copies wait for all stages to be filled, before them the copies wait for the queries.  4 bits, whose stages
+  // take longer to work on than to fill: the queries first (64 sequences of up to 4096: 49.3 us, behind the copies 49.8); 8 bits: behind (32 of up to 4096: 46.2 us, before
+  // them 46.7, 32 of up to 2000 25.6 and 26.6).
+  constexpr bool QUERIES_FIRST = TYPE == TFCC_ROCM_S4;
   ScaledRows<TYPE, BLOCKS, SHAPED> rows;
-  rows.start(p, t, head, g);
+  if constexpr (QUERIES_FIRST) rows.start(p, t, head, g);
 #pragma unroll 1
   for (unsigned stage = 0; stage < Ring::kStages; ++stage) send(stage);
+  if constexpr (!QUERIES_FIRST) rows.start(p, t, head, g);
 
   unsigned stage = 0;
 #pragma unroll 1
@@ -912,8 +920,8 @@ __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4
 }
 
 // Chunks of many tokens, int8 as above: a workgroup takes 128 rows, a wavefront 32 of them, and all go over the same keys, 32 in a step.  Bound: the
-// matrix cores and, with as much to do, the vector unit (4 chunks of 1024 over 4096, 32 heads over 8 of 128: int8 407 us, matrix operations and LDS
-// reads alone 283; float32 665, with tiles of 16 rows on the fp32 matrix operations 1930).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
+// matrix cores and, with as much to do, the vector unit (4 chunks of 1024 over 4096, 32 heads over 8 of 128: int8 377 us, matrix operations and LDS
+// reads alone 283; 4 bits 385; float32 589, with tiles of 16 rows on the fp32 matrix operations 1930).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
 // order in which the matrix cores take them, into one of two LDS buffers while the other is worked on; the next step's rows
 // are on their way to registers meanwhile.  Products of 32 x 32 as above, with
 //   S^T: lane l holds row l % 32 and keys 8 a + 4 (l / 32) + i in [4 a + i]

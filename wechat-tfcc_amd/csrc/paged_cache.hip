@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(WriteArgs p)
   }
   const long long slot = p.wide_slots ? static_cast<const long long*>(p.slots)[token] : static_cast<const int*>(p.slots)[token];
   if (slot < 0 || slot >= (long long)p.cache.pages * p.cache.page_size.d) return;
-  // (a division of 64 bits takes as long as a sixth of all the rest)
+  // (a division of 64 bits takes its time)
   const unsigned long long page = slot < 0x80000000ll ? p.cache.page_size.quotient((unsigned)slot) : (unsigned long long)slot / p.cache.page_size.d;
   const unsigned inside = (unsigned)(slot - page * p.cache.page_size.d);
   const unsigned long long at = page * p.cache.page + head * p.cache.head + inside * p.cache.row;
@@ -146,7 +146,8 @@ struct ReadArgs {
 
 constexpr unsigned kReadTokens = 4;  // of a workgroup
 
-// LANES lanes of four values to a row, as above; a workgroup finds its tokens' slots once for all their heads.
+// LANES lanes of four values to a row, as above; a workgroup finds its tokens' slots once for all their heads (16 sequences of up to 2048 tokens of
+// 8 x 128: from 4 bits 44 us, 5.9 TB/s, from 8 bits 49 us, 5.6 TB/s).
 template <int TYPE, int LANES>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(ReadArgs p) {
   __shared__ unsigned pages[kReadTokens], insides[kReadTokens];
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(ReadArgs p) {
 
 // Runs of rows to other places of the cache.  Bound: HBM, a launch for a few pages.  What a run moves of keys or values, [heads][rows][chunks] of
 // UNIT bytes, is gone over as one range, cut into pieces for several workgroups: a thread has all its loads under way before it stores the first.  Pieces
-// behind those move the scales, 4 bytes to a unit.
+// behind those move the scales, 4 bytes to a unit.  (1500 whole pages of 64 rows of 8 x 128 in 4 bits, 209 MB moved: 45 us, 4.6 TB/s, and 34 where the last-level
+// cache holds them; 500 of 32 rows in float32, 262 MB: 41 us, 6.4 TB/s; four half pages 3.8 us.)
 constexpr unsigned kCopyEach = 4, kCopyUnits = kCacheThreads * kCopyEach;
 struct CopyArgs {
   void* rows_of[2];
