@@ -240,13 +240,16 @@ def test_workgroups_of_many_wavefronts(pkg, T, lengths, heads, kv, size, page):
 
 
 PIECES = [
-    # kind, lengths, chunks, heads, kv heads, size, page of calls whose keys come in 2 to 19 pieces, and in 2 and 3 with wide tiles
+    # kind, lengths, chunks, heads, kv heads, size, page of calls whose keys come in 3 to 137 pieces, some in one, and in 2 and 3 with wide tiles
     ("s4", [1000], [1], 64, 64, 64, 16),
     ("s8", [1500, 90], [2, 1], 60, 60, 64, 16),
     ("f32", [1000, 300], [1, 3], 24, 24, 64, 16),
     ("s8", [1790], [1], 32, 8, 128, 32),
     ("f32", [1000, 300], [1, 3], 12, 12, 64, 16),
     ("s4", [2300, 40], [1, 1], 8, 2, 128, 32),
+    ("f32", [9000], [1], 8, 1, 256, 16),
+    ("s8", [70000], [1], 4, 1, 80, 64),
+    ("s4", [33000], [2], 2, 1, 32, 32),
     ("f32", [1000, 20, 640], [512, 20, 600], 12, 12, 64, 16),
     ("f32", [1500, 1100], [160, 120], 32, 8, 128, 16),
     ("s8", [2100, 40], [1060, 40], 32, 8, 128, 16),

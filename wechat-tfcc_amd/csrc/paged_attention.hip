@@ -6,41 +6,60 @@ namespace {
 
 constexpr int kThreads = 256;  // of the launch that joins pieces
 
-// The pieces of a row joined: a workgroup to a row, its threads four values each of one in every kThreads / (size / 4) pieces.
+// The pieces of a row joined: a workgroup to 64 values of a row, whose threads take four values each of one in every kShares pieces.  Bound: latency, so the first loads of
+// pieces are under way before their weights are known (float32, 2 sequences of 10335, 8 heads over 1 of 256, 81 pieces: 27.1 us in all, with a workgroup to a row, weights first, 32.4; int8, one of 100000, 8 heads over 1 of 128: 19.8 and 23.2).
+constexpr unsigned kShares = kThreads / 16, kAtOnce = 8;
 __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) {
   __shared__ float weights[kAttentionMostSplits];
   __shared__ __align__(16) f32x4 sums[kThreads];
-  const unsigned lane = threadIdx.x & 63, heads = p.cache.heads * p.group.d, size = p.cache.size, quads = size / 4;
+  const unsigned lane = threadIdx.x & 63, heads = p.cache.heads * p.group.d, size = p.cache.size;
+  const unsigned share = threadIdx.x / 16, d = blockIdx.y * 64 + threadIdx.x % 16 * 4;
   const unsigned long long row = blockIdx.x, rows = (unsigned long long)p.tokens * heads;
   const unsigned token = blockIdx.x / heads, head = blockIdx.x - token * heads;
   if ((int)token >= p.starts[p.batch] || (int)token < p.starts[0]) return;
-  float top = -INFINITY, total = 0.0f;
-  for (unsigned i = lane; i < p.splits; i += 64) {
-    top = fmaxf(top, p.statistics[(i * rows + row) * 2]);
+  const float* const partial = p.partial + row * size + (d < size ? d : 0);
+  f32x2 statistics[kAttentionMostSplits / 64];
+#pragma unroll
+  for (unsigned k = 0; k < kAttentionMostSplits / 64; ++k) {
+    const unsigned i = lane + 64 * k;
+    statistics[k] = f32x2{-INFINITY, 0.0f};
+    if (i < p.splits) statistics[k] = *reinterpret_cast<const f32x2*>(p.statistics + (i * rows + row) * 2);
   }
+  f32x4 part[kAtOnce];
+#pragma unroll
+  for (unsigned k = 0; k < kAtOnce; ++k) {
+    const unsigned i = share + kShares * k;
+    part[k] = f32x4{0, 0, 0, 0};
+    if (i < p.splits) part[k] = *reinterpret_cast<const f32x4*>(partial + i * rows * size);
+  }
+  float top = -INFINITY, total = 0.0f;
+#pragma unroll
+  for (unsigned k = 0; k < kAttentionMostSplits / 64; ++k) top = fmaxf(top, statistics[k][0]);
   top = wave_max(top);
-  for (unsigned i = lane; i < p.splits; i += 64) {
-    const float* s = p.statistics + (i * rows + row) * 2;
-    const bool none = s[0] == -INFINITY;  // the piece has no key of this row
-    const float h = none ? 0.0f : half_step(s[0], top);
-    weights[i] = none ? -1.0f : h * h;  // (all wavefronts write the same)
-    total += none ? 0.0f : s[1] * h * h;
+#pragma unroll
+  for (unsigned k = 0; k < kAttentionMostSplits / 64; ++k) {
+    const bool none = statistics[k][0] == -INFINITY;  // no such piece, or one without a key of this row
+    const float h = none ? 0.0f : half_step(statistics[k][0], top);
+    weights[lane + 64 * k] = none ? -1.0f : h * h;  // (all wavefronts write the same)
+    total += none ? 0.0f : statistics[k][1] * h * h;
   }
   total = wave_sum(total);
   __syncthreads();
-  const unsigned shares = kThreads / quads, share = threadIdx.x / quads, d = threadIdx.x % quads * 4;
   f32x4 sum = {0, 0, 0, 0};
-  if (share < shares) {
-#pragma unroll 8
-    for (unsigned i = share; i < p.splits; i += shares) {
-      const float w = weights[i];
-      if (!(w < 0.0f)) sum += w * *reinterpret_cast<const f32x4*>(p.partial + (i * rows + row) * size + d);
-    }
+#pragma unroll
+  for (unsigned k = 0; k < kAtOnce; ++k) {
+    const float w = weights[share + kShares * k];
+    if (!(w < 0.0f)) sum += w * part[k];
+  }
+  for (unsigned i = share + kShares * kAtOnce; i < p.splits; i += kShares) {
+    const float w = weights[i];
+    if (!(w < 0.0f)) sum += w * *reinterpret_cast<const f32x4*>(partial + i * rows * size);
   }
   sums[threadIdx.x] = sum;
   __syncthreads();
-  if (share == 0) {
-    for (unsigned i = 1; i < shares; ++i) sum += sums[threadIdx.x + i * quads];
+  if (share == 0 && d < size) {
+#pragma unroll
+    for (unsigned i = 1; i < kShares; ++i) sum += sums[threadIdx.x + 16 * i];
     const f32x4 none = {0, 0, 0, 0};
     *reinterpret_cast<f32x4*>(p.out + token * p.out_token + head * p.out_head + d) = top == -INFINITY ? none : sum / total;
   }
@@ -198,7 +217,7 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   if (plan.splits > 1) {
     const unsigned rows = d.tokens * d.heads;
     if (plan.splits > kFewPieces) {
-      hipLaunchKernelGGL(join_pieces_kernel, dim3(rows), dim3(kThreads), 0, s, a);
+      hipLaunchKernelGGL(join_pieces_kernel, dim3(rows, (a.cache.size + 63) / 64), dim3(kThreads), 0, s, a);
     } else {
       const unsigned lanes = a.cache.size <= 64 ? 16 : a.cache.size <= 128 ? 32 : 64, each = kThreads / lanes;
       hipLaunchKernelGGL((lanes == 16 ? join_few_kernel<16> : lanes == 32 ? join_few_kernel<32> : join_few_kernel<64>), dim3((rows + each - 1) / each), dim3(kThreads), 0, s, a);
