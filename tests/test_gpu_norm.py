@@ -84,7 +84,7 @@ def test_against_the_definition(pkg, T, width, residual):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,width", [(256, 1023), (257, 1023), (256, 2050), (257, 2050), (600, 4096), (300, 5001), (300, 9537)])
+@pytest.mark.parametrize("rows,width", [(1, 64), (33, 64), (1001, 63), (35, 128), (1003, 97), (300, 129), (301, 256), (299, 300), (257, 512), (600, 1030), (256, 1023), (257, 1023), (256, 2050), (257, 2050), (600, 4096), (300, 5001), (300, 9537)])
 def test_few_rows_and_many(pkg, T, rows, width):
     rng = np.random.default_rng(rows + width)
     x = (rng.normal(size=(rows, width)) * np.exp(rng.normal(size=(rows, 1)) * 4)).astype(np.float32)

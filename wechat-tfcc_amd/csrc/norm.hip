@@ -43,11 +43,12 @@ __device__ __forceinline__ void butterfly_pair64(double v, double& a, double& b)
   a = __hiloint2double(__float_as_int(hi_a), __float_as_int(lo_a));
   b = __hiloint2double(__float_as_int(hi_b), __float_as_int(lo_b));
 }
-template <class Join>
+// Of LANES neighbours, 16 or more.
+template <unsigned LANES, class Join>
 __device__ __forceinline__ double wave_join64(double v, Join join) {
   double a, b;
-  butterfly_pair64<32>(v, a, b); v = join(a, b);
-  butterfly_pair64<16>(v, a, b); v = join(a, b);
+  if constexpr (LANES > 32) { butterfly_pair64<32>(v, a, b); v = join(a, b); }
+  if constexpr (LANES > 16) { butterfly_pair64<16>(v, a, b); v = join(a, b); }
   butterfly_pair64<8>(v, a, b); v = join(a, b);
   butterfly_pair64<4>(v, a, b); v = join(a, b);
   butterfly_pair64<2>(v, a, b); v = join(a, b);
@@ -61,11 +62,12 @@ struct RowTotals {
 __device__ __forceinline__ double add64(double a, double b) { return a + b; }
 __device__ __forceinline__ double max64(double a, double b) { return fmax(a, b); }
 
-// Sum and maximum over the threads of a row, THREADS of them (a multiple of 64); shared: two rows of THREADS / 64.
+// Sum and maximum over the threads of a row, THREADS of them (16, 32 or a multiple of 64); shared: two rows of THREADS / 64.
 template <unsigned THREADS, bool STEPS>
 __device__ __forceinline__ RowTotals row_totals(double squares, double top, double (*shared)[16]) {
-  squares = wave_join64(squares, add64);
-  if constexpr (STEPS) top = wave_join64(top, max64);
+  constexpr unsigned lanes = THREADS < 64 ? THREADS : 64;
+  squares = wave_join64<lanes>(squares, add64);
+  if constexpr (STEPS) top = wave_join64<lanes>(top, max64);
   if constexpr (THREADS > 64) {
     constexpr unsigned waves = THREADS / 64;
     const unsigned wave = threadIdx.x / 64;
@@ -87,7 +89,7 @@ __device__ __forceinline__ RowTotals row_totals(double squares, double top, doub
 template <unsigned THREADS>
 __device__ __forceinline__ int row_count(int count, int* shared) {
 #pragma unroll
-  for (int m = 32; m > 0; m /= 2) count += __shfl_xor(count, m, 64);
+  for (int m = THREADS < 64 ? THREADS / 2 : 32; m > 0; m /= 2) count += __shfl_xor(count, m, 64);
   if constexpr (THREADS > 64) {
     if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = count;
     __syncthreads();
@@ -127,16 +129,18 @@ __device__ __forceinline__ RowFactors factors_of(const NormArgs& p, const RowTot
   return f;
 }
 
-// A row to THREADS threads, HELD times four values of it to a thread: 4 HELD THREADS values at most.  The form with integers is held to the registers
+// A row to THREADS threads, HELD times four values of it to a thread: 4 HELD THREADS values at most, and the fewest that hold a row: short ones share a
+// wavefront (60000 rows of 64: float32 11.9 us, 5.2 TB/s, 8 bits 13.4; with a wavefront to a row and sixteen values to a thread 29.5 and 47.6), and a value that is not there
+// costs as much as one that is (16384 of 256: 12.7 and 15.3 us, with places for 1024 13.9 and 19.3).  The form with integers is held to the registers
 // of 8 wavefronts to a SIMD (3000 rows of 9537: 85 us, without 108); the plain one would spill there (110 us, without 95).
 template <unsigned THREADS, unsigned HELD, bool STEPS>
 __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, STEPS && HELD > 1 ? 8 : 4) void rms_norm_kernel(NormArgs p) {
   constexpr unsigned ROWS = THREADS < 256 ? 256 / THREADS : 1;
-  static_assert(THREADS == 64 || ROWS == 1);
+  static_assert(THREADS <= 64 || ROWS == 1);
   __shared__ double shared[2][16];
   __shared__ int shared_count[16];
   const unsigned long long row = (unsigned long long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
-  if (row >= p.rows) return;  // whole wavefronts, of rows that have one each
+  if (row >= p.rows) return;  // whole wavefronts, or their halves and quarters that rows have
   const unsigned me = threadIdx.x % THREADS;
   const float* const x = p.x + row * p.x_row;
   const float* const residual = p.residual != nullptr ? p.residual + row * p.residual_row : nullptr;
@@ -368,9 +372,14 @@ int tfcc_rocm_rms_norm_f32(void* stream, const tfcc_rocm_rms_norm_desc* desc) {
     hipLaunchKernelGGL((d.steps != nullptr ? quantized : plain), dim3((d.rows + each - 1) / each), dim3(threads), 0, s, a);
   };
   const bool few = d.rows <= kFewRows;
-  if (d.width <= 1024 && few) start(rms_norm_kernel<256, 1, false>, rms_norm_kernel<256, 1, true>, 256, 1);
+  if (d.width <= 64) start(rms_norm_kernel<16, 1, false>, rms_norm_kernel<16, 1, true>, 256, 16);
+  else if (d.width <= 128) start(rms_norm_kernel<32, 1, false>, rms_norm_kernel<32, 1, true>, 256, 8);
+  else if (d.width <= 1024 && few) start(rms_norm_kernel<256, 1, false>, rms_norm_kernel<256, 1, true>, 256, 1);
+  else if (d.width <= 256) start(rms_norm_kernel<64, 1, false>, rms_norm_kernel<64, 1, true>, 256, 4);
+  else if (d.width <= 512) start(rms_norm_kernel<64, 2, false>, rms_norm_kernel<64, 2, true>, 256, 4);
   else if (d.width <= 1024) start(rms_norm_kernel<64, 4, false>, rms_norm_kernel<64, 4, true>, 256, 4);
   else if (d.width <= 4096 && few && d.steps == nullptr) start(rms_norm_kernel<1024, 1, false>, nullptr, 1024, 1);
+  else if (d.width <= 2048) start(rms_norm_kernel<256, 2, false>, rms_norm_kernel<256, 2, true>, 256, 1);
   else if (d.width <= 4096) start(rms_norm_kernel<256, 4, false>, rms_norm_kernel<256, 4, true>, 256, 1);
   else if (d.width <= 8192) start(rms_norm_kernel<512, 4, false>, rms_norm_kernel<512, 4, true>, 512, 1);
   else if (d.width <= kNormMost) start(rms_norm_kernel<1024, 4, false>, rms_norm_kernel<1024, 4, true>, 1024, 1);
