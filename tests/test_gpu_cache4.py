@@ -180,7 +180,8 @@ def filled(pkg, T, kind, pages, heads, page, size, seed):
     return cache
 
 
-COPIED = [(1, 16, 64, 6), (8, 32, 128, 20), (3, 24, 80, 9), (5, 7, 48, 12), (2, 1, 16, 30), (12, 200, 256, 7), (4, 64, 208, 40)]
+COPIED = [(1, 16, 64, 6), (8, 32, 128, 20), (3, 24, 80, 9), (5, 7, 48, 12), (2, 1, 16, 30), (12, 200, 256, 7), (4, 64, 208, 40),
+          (1, 16, 256, 600), (3, 24, 80, 512), (8, 16, 128, 510), (8, 100, 128, 530), (1, 1, 16, 700)]  # more runs and fewer than scales go apart for
 
 
 @pytest.mark.gpu

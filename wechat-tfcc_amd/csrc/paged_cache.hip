@@ -213,6 +213,9 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(ReadArgs p) {
 // UNIT bytes, is gone over as one range, cut into pieces for several workgroups: a thread has all its loads under way before it stores the first.  Pieces
 // behind those move the scales, 4 bytes to a unit.  (1500 whole pages of 64 rows of 8 x 128 in 4 bits, 209 MB moved: 45 us, 4.6 TB/s, and 34 where the last-level
 // cache holds them; 500 of 32 rows in float32, 262 MB: 41 us, 6.4 TB/s; four half pages 3.8 us.)
+// From so many runs on a page whose rows are one piece has its scales moved by the same workgroup: fewer of them outweigh that the scales wait for the rows (pages of 16 rows of
+// 8 x 128 in 4 bits, 3000 runs: 19.9 us, apart 24.9; 300: 4.5 and 4.6; 100: 3.7 and 3.3).
+constexpr unsigned kManyRuns = 256;
 constexpr unsigned kCopyEach = 4, kCopyUnits = kCacheThreads * kCopyEach;
 struct CopyArgs {
   void* rows_of[2];
@@ -222,6 +225,7 @@ struct CopyArgs {
   const int* rows;
   int wide_slots;
   unsigned pages, units, scale_units, row_pieces;
+  int together;  // a run's one piece of rows moves its scales as well
   Divisor page_size, chunks, pieces;
 };
 
@@ -265,9 +269,10 @@ __global__ __launch_bounds__(kCacheThreads) void cache_copy_kernel(CopyArgs p) {
     typedef unsigned unit __attribute__((ext_vector_type(UNIT / 4)));
     copy_piece<unit>(piece, p.units, p.chunks, p.page_size, rows, static_cast<char*>(p.rows_of[blockIdx.y]), from_page * p.page + from_row * p.row,
                      to_page * p.page + to_row * p.row, p.head, p.row);
-  } else {
+  }
+  if (piece >= p.row_pieces || p.together) {
     const Divisor one = {1, 1u << 31, 31};
-    copy_piece<unsigned>(piece - p.row_pieces, p.scale_units, one, p.page_size, rows, reinterpret_cast<char*>(p.scales_of[blockIdx.y]),
+    copy_piece<unsigned>(p.together ? 0 : piece - p.row_pieces, p.scale_units, one, p.page_size, rows, reinterpret_cast<char*>(p.scales_of[blockIdx.y]),
                          from_page * p.scale_page + from_row * p.scale_row, to_page * p.scale_page + to_row * p.scale_row, p.scale_head, p.scale_row);
   }
 }
@@ -355,8 +360,10 @@ int tfcc_rocm_cache_copy(void* stream, const tfcc_rocm_paged_cache* cache, const
   a.page_size = Divisor::of(c.page_size);
   a.chunks = Divisor::of(bytes / unit);
   const uint64_t units = (uint64_t)c.heads * c.page_size * (bytes / unit), scales = has_scales(c) ? (uint64_t)c.heads * c.page_size : 0;
-  const uint64_t row_pieces = (units + kCopyUnits - 1) / kCopyUnits, pieces = row_pieces + (scales + kCopyUnits - 1) / kCopyUnits;
-  TFCC_REQUIRE(units <= 0x7fffffffu - kCopyUnits && pieces * runs <= 0x7fffffffu / kCacheThreads, "cache_copy: %u runs of up to %llu bytes", runs,
+  const uint64_t row_pieces = (units + kCopyUnits - 1) / kCopyUnits, scale_pieces = (scales + kCopyUnits - 1) / kCopyUnits;
+  a.together = runs >= kManyRuns && row_pieces == 1 && scale_pieces == 1;
+  const uint64_t pieces = row_pieces + (a.together ? 0 : scale_pieces);
+  TFCC_REQUIRE(units <= 0x7fffffffu - kCopyUnits && (row_pieces + scale_pieces) * runs <= 0x7fffffffu / kCacheThreads, "cache_copy: %u runs of up to %llu bytes", runs,
                (unsigned long long)units * unit);
   TFCC_REQUIRE(sources && destinations, "cache_copy: null argument");
   a.units = (unsigned)units;
