@@ -27,7 +27,8 @@ static PagedAttentionPlan float32(unsigned tokens, unsigned batch, unsigned grou
 int main() {
   // single tokens: one workgroup of twelve wavefronts to a CU, heads wider than 128 eight, or several of four
   EXPECT(four(32, 32, 4, 8, 128, 4096).waves == 12 && four(32, 32, 4, 8, 256, 4096).waves == 8 && four(64, 64, 4, 8, 128, 4096).waves == 4);
-  EXPECT(four(32, 32, 4, 8, 128, 1024).waves == 4 && four(32, 32, 4, 8, 128, 1025).waves == 12);
+  EXPECT(four(32, 32, 4, 8, 128, 512).waves == 4 && four(32, 32, 4, 8, 128, 513).waves == 12 && four(16, 16, 4, 8, 128, 513).waves == 12 && four(15, 15, 4, 8, 128, 513).waves == 4);
+  EXPECT(four(32, 32, 4, 8, 256, 1024).waves == 4 && four(32, 32, 4, 8, 256, 1025).waves == 8);
   EXPECT(four(1, 1, 1, 12, 64, 4096).waves == 4 && four(1, 1, 1, 12, 64, 9000).waves == 12);  // enough to do for all
   EXPECT(four(32, 32, 4, 8, 128, 4096).splits == 1 && four(1, 1, 4, 8, 128, 4096).splits > 1);
   // wide tiles: workgroups for nearly two to a CU, over few keys for more than one

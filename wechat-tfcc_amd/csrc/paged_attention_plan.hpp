@@ -67,8 +67,9 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   if (halves) {
     // What holds a workgroup of 4-bit integers up is its operations: as many wavefronts to a CU as registers allow, 12 (heads wider than 128: 8), in one workgroup where there is
     // no more than one to a CU and enough to do, else in several, whose beginnings and ends others fill.  (Us with one and with several, 8 heads of 128: 32 sequences of 4096 33 and 40,
-    // 64 of up to 4096 54 and 48, 40 of up to 1000 22 and 14; 12 heads, one of 4000 13 and 11; 8 heads of 256, 32 of 4096 50 and 56.)
-    p.waves = groups <= 256 && keys > 1024 && groups * keys > 256 * 384 ? (size <= 128 ? 12 : 8) : 4;
+    // 64 of up to 4096 54 and 48, 40 of up to 1000 22 and 14, 32 of up to 1000 13.2 and 15.1, 16 of 600 10.1 and 10.7, 4 of 3000 12.6 and 11.8; 12 heads, one of 4000 11.1 and 9.6;
+    // 8 heads of 256, 32 of 4096 50 and 56, of 1000 22.8 and 21.7.)
+    p.waves = groups <= 256 && ((groups >= 128 && keys > 512 && size <= 128) || (keys > 1024 && groups * keys > 256 * 384)) ? (size <= 128 ? 12 : 8) : 4;
   }
   if (!wide) step = p.waves * (float_cache ? 16 : 32);
   if (wide && float_cache) {
