@@ -1213,9 +1213,8 @@ __device__ __forceinline__ void stream_far_rows(const AttentionArgs& p, const Ti
   }
 }
 
-// The same as a function of its own that finds the work once more: with heads of 128, whose steps have all registers, what it wants takes none from them
-// (4 chunks of 1024 over 4096, 32 heads over 8: 667 us, and 679 with the above in the kernel; heads of 64 the other way round, 51.3 and 49.4 us for 6
-// chunks of 517 with a window, which feel the stack that a call wants).
+// The same as a function of its own that finds the work once more: what it wants takes no registers from the kernel's steps (4 chunks of 1024 over 4096, 32 heads
+// over 8 of 128: 667 us, and 679 with the above in the kernel; 12 heads of 64: 30 chunks of up to 500 over up to 800 115 and 119, with biases and prefixes 129 and 134).
 template <int BLOCKS, int WAVES, bool SHAPED>
 __device__ __attribute__((noinline)) void stream_far_rows_apart(const AttentionArgs& p) {
   Tile t;
@@ -1679,10 +1678,7 @@ __global__ __launch_bounds__(WAVES * 64, WAVES == 4 && BLOCKS > 2 ? 1 : 2) void 
     unsigned any = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) any |= odds[w];
-    if (any != 0) {
-      if constexpr (BLOCKS == 1) stream_far_rows<BLOCKS, SHAPED>(p, t, head, split, begin, end, table);
-      else stream_far_rows_apart<BLOCKS, WAVES, SHAPED>(*(const AttentionArgs*)__builtin_amdgcn_kernarg_segment_ptr());  // the kernel's one argument, where it lies
-    }
+    if (any != 0) stream_far_rows_apart<BLOCKS, WAVES, SHAPED>(*(const AttentionArgs*)__builtin_amdgcn_kernarg_segment_ptr());  // the kernel's one argument, where it lies
   }
 }
 
