@@ -671,7 +671,7 @@ int tfcc_rocm_sample_f32(void* stream, const tfcc_rocm_sample_desc* desc);
  * as float32, as 8-bit integers for the integer products, or both.  The integers: steps = 128 + n with n = 127 t / max |t| rounded to nearest,
  * ties to even, t = h * weight (the root is the same for the whole row), decided as if in exact arithmetic, scales = max |out| / 127, and sums = the sum of a
  * row's steps: with offset_a = -128, what tfcc_rocm_gemm_u8s8s32 takes as a and rowsum_a.  A row of zeros has scale 0; a row whose h or h * weight holds an infinity or
- * a NaN has steps of 128 and a scale of NaN.  Means, roots and products are formed in 64 bits and rounded once.
+ * a NaN has steps of 128 and a scale of NaN; out is what the formula says of such rows, with steps or without (0 beside an infinite h).  Means, roots and products are formed in 64 bits and rounded once.
  * sum (h), sums: NULL where they are not wanted.  sum may be x or residual, out may be x, with the same strides; nothing else overlaps.
  * Rows that are written do not share memory.  rows: up to 2^26 - 4 with a width of up to 1024, 2^24 - 1 up to 4096, 2^22 - 1 above. */
 typedef struct tfcc_rocm_rms_norm_desc {

@@ -56,8 +56,10 @@ __device__ __forceinline__ double wave_join64(double v, Join join) {
   return v;
 }
 
+constexpr double kInfinity = __builtin_inf();
 struct RowTotals {
-  double squares, top;
+  double squares;
+  double top;  // the largest |t|; infinity where one is not finite.  (The squares say nothing of it: the root is the same whether integers are asked for or not.)
 };
 __device__ __forceinline__ double add64(double a, double b) { return a + b; }
 __device__ __forceinline__ double max64(double a, double b) { return fmax(a, b); }
@@ -121,8 +123,9 @@ struct RowFactors {
   double factor;  // 127 / largest |t|; 0: all steps are 128
   float scale;
 };
-__device__ __forceinline__ RowFactors factors_of(const NormArgs& p, const RowTotals& totals, bool odd) {
+__device__ __forceinline__ RowFactors factors_of(const NormArgs& p, const RowTotals& totals) {
   RowFactors f;
+  const bool odd = totals.top == kInfinity;
   f.root = 1.0 / sqrt(totals.squares / p.width + p.eps);
   f.factor = totals.top > 0.0 && !odd ? 127.0 / totals.top : 0.0;
   f.scale = odd ? __uint_as_float(0x7fc00000u) : (totals.top > 0.0 ? (float)(totals.top * f.root / 127.0) : 0.0f);
@@ -189,9 +192,9 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS, STEPS && HELD > 1 ? 
       }
     }
   }
-  if constexpr (STEPS) squares += rest;
+  if constexpr (STEPS) top = rest == 0.0 ? top : kInfinity;
   const RowTotals totals = row_totals<THREADS, STEPS>(squares, top, shared);
-  const RowFactors f = factors_of(p, totals, !(totals.squares < __longlong_as_double(0x7ff0000000000000ll)));
+  const RowFactors f = factors_of(p, totals);
   int count = 0;
 #pragma unroll
   for (unsigned i = 0; i < HELD; ++i) {
@@ -258,9 +261,9 @@ __global__ __launch_bounds__(1024) void rms_norm_wide_kernel(NormArgs p) {
       rest = fma(t, 0.0, rest);
     }
   }
-  if constexpr (STEPS) squares += rest;
+  if constexpr (STEPS) top = rest == 0.0 ? top : kInfinity;
   const RowTotals totals = row_totals<1024, STEPS>(squares, top, shared);
-  const RowFactors f = factors_of(p, totals, !(totals.squares < __longlong_as_double(0x7ff0000000000000ll)));
+  const RowFactors f = factors_of(p, totals);
   int count = 0;
   for (unsigned at = threadIdx.x; at < p.width; at += 1024) {
     float h = x[at];
