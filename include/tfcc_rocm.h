@@ -602,11 +602,15 @@ int tfcc_rocm_cache_copy(void* stream, const tfcc_rocm_paged_cache* cache, const
  * workspace: tfcc_rocm_paged_attention_workspace() bytes, 16-byte aligned, of any contents, not in use by another call at the same time.
  * tokens * heads < 2^31, and no more workgroups than one launch takes: a chunk has one for every 16 rows (token, query head) of a
  * cache head, or part of 16, and 2^24 - 1 are the most.
- * Sums and weights are float32, whatever the cache's type.  A term of a product is right to 2^-23 of it, over a float32 cache with many rows to
+ * Sums and weights are float32, whatever the cache's type.  A term of a product is right to 2^-23 of it, over a float32 cache with many rows (below) to
  * 2^-21, but for parts of a row that lie 2^-30 below its largest value, which may be lost (F32, many rows: and below 2^-139; S8 and S4: where the scales are 2^-100 to 2^96 - where all of a row's values have scales below
  * 2^-(90 + n), 2^-(33 - n) of the largest product is lost).  Sums of weights times values are divided last: where those reach 2^128, they are
  * infinite.  Where rows of many see an infinity, a NaN or a number of 2^80 or more in a float32 cache, they and those beside them are worked out
- * twice, in up to four times the time.  out overlaps no input. */
+ * twice, in up to four times the time.  out overlaps no input.
+ * Many rows, of a float32 cache: pages of a multiple of 4 rows, 16 or more, heads of up to 64 values whose mean chunk has 64 rows (token, query head) of a cache head or
+ * more, or of up to 128 and 128 rows, and in all, as if every chunk were the mean one, rounded up, either 18000 rows - heads of up to 64: in 250 tiles of 128 rows or over 1000 keys - or 8192 over 2048
+ * keys (shaped scores, below: 1000).  The keys are max_length, with a window at most its rows + 32 + those of a tile (128, or 256).  Calls of fewer rows each stay with the float32 operations.
+ * Their workspace holds up to eight partial results [tokens, heads, size + 2] in float32. */
 typedef struct tfcc_rocm_paged_attention_desc {
   tfcc_rocm_paged_cache cache;
   const float* q;

@@ -1,6 +1,8 @@
 // Attention over a paged cache: the calls, how they are dealt out, and the launch that joins pieces of the keys.
 #include "paged_attention.hpp"
 
+#include <algorithm>
+
 namespace tfcc_rocm {
 namespace {
 
@@ -142,16 +144,16 @@ unsigned chunk_rows(const tfcc_rocm_paged_cache& c) {
   return wide_reads(c) ? 128 : 0;
 }
 
-PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d) {
+PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d, bool shaped) {
   return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, chunk_rows(d.cache),
-                              d.cache.type == TFCC_ROCM_F32, d.cache.type == TFCC_ROCM_S4);
+                              d.cache.type == TFCC_ROCM_F32, d.cache.type == TFCC_ROCM_S4, shaped ? kLongKeysShaped : kLongKeysPlain);
 }
 
 // Checks a call and deals it out; one without tokens or sequences has nothing to deal out.
-int plan_call(const tfcc_rocm_paged_attention_desc& d, PagedAttentionPlan& plan) {
+int plan_call(const tfcc_rocm_paged_attention_desc& d, bool shaped, PagedAttentionPlan& plan) {
   if (int e = check_attention(d)) return e;
   if (d.tokens == 0 || d.batch == 0) return TFCC_ROCM_OK;
-  plan = plan_of(d);
+  plan = plan_of(d, shaped);
   // a launch takes 2^32 - 1 threads; pieces, whose join has a workgroup for each row, are made of fewer rows than that is for
   const uint64_t groups = (uint64_t)plan.tiles * plan.splits * d.cache.heads;
   TFCC_REQUIRE(groups * plan.waves * 64 <= 0xffffffffu && (plan.splits == 1 || (uint64_t)d.tokens * d.heads * kThreads <= 0xffffffffu),
@@ -165,7 +167,7 @@ size_t workspace_of(const tfcc_rocm_paged_attention_desc& d, const PagedAttentio
 
 int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_rocm_attention_scores* scores) {
   PagedAttentionPlan plan;
-  if (int e = plan_call(d, plan)) return e;
+  if (int e = plan_call(d, scores != nullptr, plan)) return e;
   if (d.tokens == 0 || d.batch == 0) return TFCC_ROCM_OK;
   TFCC_REQUIRE(d.q && d.out && d.starts && d.lengths && (d.table || d.table_width == 0), "paged_attention: null argument");
   const size_t needs = workspace_of(d, plan);
@@ -235,9 +237,14 @@ using namespace tfcc_rocm;
 extern "C" {
 
 size_t tfcc_rocm_paged_attention_workspace(const tfcc_rocm_paged_attention_desc* desc) {
-  PagedAttentionPlan plan;
-  if (desc == nullptr || plan_call(*desc, plan) != TFCC_ROCM_OK || desc->tokens == 0 || desc->batch == 0) return 0;
-  return workspace_of(*desc, plan);
+  if (desc == nullptr) return 0;
+  size_t needs = 0;
+  for (const bool shaped : {false, true}) {  // one workspace is for both calls
+    PagedAttentionPlan plan;
+    if (plan_call(*desc, shaped, plan) != TFCC_ROCM_OK || desc->tokens == 0 || desc->batch == 0) return 0;
+    needs = std::max(needs, workspace_of(*desc, plan));
+  }
+  return needs;
 }
 
 int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_desc* desc) {
