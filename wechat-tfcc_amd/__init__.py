@@ -1139,6 +1139,7 @@ def _on_device(device, *tensors):
 
 
 _MOST = 0x7fffffff  # of a dimension or a count: the fields of a call have 32 bits
+_LEAST = 2.0 ** -149  # of float32's positive numbers
 
 
 def _heads_of(t, name):
@@ -1313,7 +1314,7 @@ def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window
     (int32 [batch]): cached tokens, the chunk's own among them; table: int32 [batch, pages].  max_length: an upper bound of lengths
     that the program knows, which the work is dealt out by.  Rows of out behind the last sequence are left as they were.
 
-    Shaped scores (tfcc_rocm_paged_attention_scores_f32): cap > 0 makes x = scale * q k^T cap * tanh(x / cap), slopes (float32 [heads])
+    Shaped scores (tfcc_rocm_paged_attention_scores_f32): cap > 0 makes x = scale * q k^T cap * tanh(x / cap) (one below float32's smallest number counts as that), slopes (float32 [heads])
     take slope * |distance of the positions| off it, and of sequence i all tokens see the first prefixes[i] cached ones (int32 [batch];
     causal, no window)."""
     if out is None:
@@ -1335,6 +1336,7 @@ def paged_attention(q, cache, table, starts, lengths, scale, causal=True, window
         raise InvalidArgumentError("invalid window")
     if not 0 <= cap <= 3.4028234e38:
         raise InvalidArgumentError("invalid cap")
+    cap = max(cap, _LEAST) if cap else 0.0
     slopes = None if slopes is None else _integers(slopes, "slopes", q.shape[1], (torch.float32,))
     prefixes = None if prefixes is None else _integers(prefixes, "prefixes", batch, (torch.int32,))
     if prefixes is not None and (window or not causal):

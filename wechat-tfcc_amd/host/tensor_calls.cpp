@@ -12,6 +12,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <limits>
+
 #include "tfcc_rocm.h"
 
 namespace {
@@ -544,7 +547,10 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t batch = table->size(0);
   if (lengths->dim() != 1 || lengths->size(0) != batch || starts->dim() != 1 || starts->size(0) != batch + 1) return none();
   if (!fits(q->size(0)) || !fits(q->size(1)) || q->size(2) != d.cache.size || !fits(batch) || !fits(table->size(1))) return none();
-  tfcc_rocm_attention_scores scores{static_cast<float>(PyFloat_AS_DOUBLE(args[9])), nullptr, nullptr};
+  const double cap = PyFloat_AS_DOUBLE(args[9]);
+  if (!(cap >= 0)) return none();
+  // (one below float32's smallest number is that: rounded to 0 it would be none)
+  tfcc_rocm_attention_scores scores{static_cast<float>(cap > 0 ? std::max<double>(cap, std::numeric_limits<float>::denorm_min()) : 0), nullptr, nullptr};
   if (args[10] != Py_None) {
     const Tensor* slopes = plain(args[10], at::kFloat, here.device);
     if (!slopes || slopes->dim() != 1 || slopes->size(0) != q->size(1)) return none();
