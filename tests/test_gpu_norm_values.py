@@ -49,3 +49,14 @@ def test_out_beside_steps_of_rows_that_are_not_finite(pkg, T, rows, width, weigh
     if not bad.all():
         t = t[~bad][:2]
         assert np.array_equal(steps[~bad][:2], 128 + R.norm_steps(t, np.abs(t).max(-1, keepdims=True)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [1e-46, 1e-60, 5e-324, 2.0 ** -150, -1e-60])
+def test_an_eps_that_float32_does_not_hold(pkg, T, eps):
+    """Rounded to float32 it would be 0, and a row of zeros 0 / 0."""
+    x, w = T.t(np.zeros((2, 8), np.float32)), T.t(np.ones(8, np.float32))
+    for call in (pkg.rms_norm, pkg.rms_norm_quantized):
+        with pytest.raises(pkg.InvalidArgumentError):
+            call(x, w, eps)
+    assert (T.n(pkg.rms_norm(x, w, 2.0 ** -149)[0]) == 0).all() and np.isnan(T.n(pkg.rms_norm(x, w, 0.0)[0])).all()

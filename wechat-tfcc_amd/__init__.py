@@ -1417,7 +1417,7 @@ def _norm(x, weight, eps, residual, quantized):
     weight = weight.contiguous()
     if residual is not None and residual.shape != x.shape:
         raise InvalidArgumentError("invalid residual")
-    if not 0 <= eps <= 3.4028234e38:
+    if not 0 <= eps <= 3.4028234e38 or 0 < eps <= _LEAST / 2:  # (such a one would be rounded to 0)
         raise InvalidArgumentError("invalid eps")
     added = None if residual is None else _rows(residual, "residual")
     d = RmsNormDesc()
@@ -1443,7 +1443,8 @@ def _norm(x, weight, eps, residual, quantized):
 
 def rms_norm(x, weight, eps, residual=None):
     """x [..., width], the residual added first where there is one, divided by the root of its rows' mean squares (and eps) and multiplied
-    by weight [width]: tfcc_rocm_rms_norm_f32.  Returns (result, x + residual or None)."""
+    by weight [width]: tfcc_rocm_rms_norm_f32.  eps is rounded to float32; a positive one that is 0 there is refused.  Returns (result,
+    x + residual or None)."""
     done = _native().rms_norm(x, weight, eps, residual, False)
     return _norm(x, weight, eps, residual, False) if done is None else done
 

@@ -634,6 +634,8 @@ PyObject* sample(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   if (n != 5 || !PyFloat_CheckExact(args[2]) || !PyBool_Check(args[4])) return none();
+  const double eps = PyFloat_AS_DOUBLE(args[2]);
+  if (eps != 0 && !(static_cast<float>(eps) > 0)) return none();
   Here here(args[0]);
   const Tensor *x = plain(args[0], at::kFloat, here.device), *weight = plain(args[1], at::kFloat, here.device);
   const Tensor* residual = args[3] == Py_None ? nullptr : plain(args[3], at::kFloat, here.device);
@@ -649,7 +651,7 @@ PyObject* rms_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   d.sum = residual ? data<float>(sum) : nullptr;
   d.rows = static_cast<unsigned>(rows);
   d.width = static_cast<unsigned>(width);
-  d.eps = static_cast<float>(PyFloat_AS_DOUBLE(args[2]));
+  d.eps = static_cast<float>(eps);
   d.x_row_stride = d.residual_row_stride = d.sum_row_stride = d.out_row_stride = d.steps_row_stride = static_cast<uint64_t>(width);
   const bool quantized = args[4] == Py_True;
   out = empty(x->sizes(), quantized ? at::kByte : at::kFloat, here.device);
