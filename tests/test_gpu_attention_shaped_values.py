@@ -1,4 +1,4 @@
-"""Attention with shaped scores at the ends of what its arguments may hold: caps below float32's smallest number."""
+"""Attention with shaped scores at the ends of what its arguments may hold: caps below float32's smallest number, slopes next to its largest."""
 import numpy as np
 import pytest
 
@@ -28,3 +28,14 @@ def test_caps_below_zero_are_refused_however_small(pkg, T):
             with pytest.raises(pkg.InvalidArgumentError):
                 m.run(T, out=out, cap=cap)
     assert np.array_equal(T.n(m.run(T, cap=-0.0)), T.n(m.run(T)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["s4", "s8", "f32"])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_slopes_next_to_the_largest_number(pkg, T, kind, cap):
+    """A slope of 2.4e38 and more is finite, though it is not in the units of log2: the key at distance 0 has a bias of 0 and is all there is."""
+    m = Made(pkg, kind, [300, 270, 40], [258, 3, 40], 4, 2, 64, 16, 3)
+    kw = m.shaped({}, cap=cap)
+    kw["slopes"] = np.array([3.4028234e38, 2.4e38, 2.3e38, 1e37], np.float32)
+    m.check(T, **kw)

@@ -254,6 +254,7 @@ struct ScoreShape {
     unit = biased ? 1.0f : cap > 0.0f ? cap : factor_of_row;
     if (biased && t.row_token >= 0) {
       slope = p.slopes[head * p.group.d + t.row_head] * 1.44269504088896341f;
+      if (fabsf(slope) == INFINITY) slope = copysignf(3.4028234e38f, slope);  // times a distance of 0 it stays 0
       position = t.row_position < t.row_high - 1 ? t.row_position : t.row_high - 1;
       position = position > 0 ? position : 0;
     }
