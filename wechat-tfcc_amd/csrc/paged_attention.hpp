@@ -27,6 +27,7 @@
 #include "lds_dma.hpp"
 #include "paged_attention_plan.hpp"
 #include "paged_cache.hpp"
+#include "score_tanh.hpp"
 
 namespace tfcc_rocm {
 
@@ -233,8 +234,7 @@ __device__ __forceinline__ int bound_of(float v) {
 
 // A row's scores with a cap and a bias that depends on distance.  In the units of log2, as all scores here.
 //
-// tanh to about float32's last place, of the result and not of 1: below 0.55, x + x^3 P(x^2) with P of degree 4 fitted for the smallest relative error (2^-29), above,
-// 1 - 2 / (2^(2 log2(e) x) + 1).  Most scores are far below their cap: where those of a whole wavefront are, the second is passed over.  A score as
+// tanh (score_tanh.hpp) has two forms, and most scores are far below their cap: where those of a whole wavefront are, the second is passed over.  A score as
 // it comes (`raw`) takes the factor of its row and the cap's inverse in one, and leaves in units of `unit`, the cap where nothing is added to it: a
 // cap costs nine operations, a bias two (int8, 32 sequences of up to 6000 with a window of 4096, 8 heads of 256, at the rate of HBM: 97 us with a cap, 92 without; 4 chunks of 1024
 // over 4096 in 4 bits, bound by operations: 385 us plain, 503 with a cap, 415 with slopes).
@@ -269,19 +269,14 @@ struct ScoreShape {
         s[i] *= factor;
         most = fmaxf(most, fabsf(s[i]));
       }
-      const bool large = __any(!(most < 0.55f));
+      const bool large = __any(!(most < kTanhNear));
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float x = s[i], y = x * x;
-        float r = -0.00627424f;
-        r = fmaf(r, y, 0.02107168f);
-        r = fmaf(r, y, -0.05385231f);
-        r = fmaf(r, y, 0.13332586f);
-        r = fmaf(r, y, -0.33333318f);
-        r = fmaf(x * y, r, x);
+        const float x = s[i];
+        float r = tanh_near(x);
         if (large) {
-          const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * 2.88539008177792681f) + 1.0f), 1.0f);
-          r = fabsf(x) < 0.55f ? r : far;
+          const float far = tanh_far(x, [](float v) { return __builtin_amdgcn_exp2f(v); }, [](float v) { return __builtin_amdgcn_rcpf(v); });
+          r = fabsf(x) < kTanhNear ? r : far;
         }
         s[i] = r;
       }
