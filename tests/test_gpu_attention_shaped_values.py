@@ -204,3 +204,26 @@ def test_far_numbers_between_replays_of_shaped_scores(pkg, T, case):
             if value != value:
                 rows = eager[:chunks[0], :group, 3].isnan().all(-1)
                 assert int(rows.sum()) == (chunks[0] if prefix > at else 3)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["s4", "s8"])
+@pytest.mark.parametrize("lengths,chunks,heads,kv,page", [([60], [2], 4, 2, 16), ([90], [1], 4, 2, 32), ([70], [1], 4, 2, 24), ([30], [2], 4, 2, 8), ([260, 270], [260, 270], 128, 64, 256)])
+def test_pages_more_than_32_bits_of_bytes_apart(pkg, T, kind, lengths, chunks, heads, kv, page):
+    """Every page but the first starts behind 2^32 bytes: rings for pages of each kind, keys one by one, wide tiles."""
+    import torch
+    m = Made(pkg, kind, lengths, chunks, heads, kv, 128, page, 6, spare=0)
+    shaped = m.shaped({}, cap=5.0, slopes=True, prefixes=[7] * len(lengths))
+    on = {k: T.t(v) if isinstance(v, np.ndarray) else v for k, v in shaped.items()}
+    want = [T.n(m.run(T)), T.n(m.run(T, **on))]
+    far = (1 << 32) + 4096
+    assert m.table[0, 0] > 0 or m.table[0, 1] > 0
+    cache = []
+    for t in m.on(T):
+        if t.dim() == 4:
+            memory = torch.empty((far * (t.shape[0] - 1) + t[0].numel(),), dtype=t.dtype, device="cuda")
+            v = torch.as_strided(memory, t.shape, (far, *t.stride()[1:]))
+            v.copy_(t)
+            t = v
+        cache.append(t)
+    assert np.array_equal(T.n(m.run(T, tuple(cache))), want[0]) and np.array_equal(T.n(m.run(T, tuple(cache), **on)), want[1])
