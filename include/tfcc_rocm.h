@@ -608,8 +608,8 @@ int tfcc_rocm_cache_copy(void* stream, const tfcc_rocm_paged_cache* cache, const
  * infinite.  Where rows of many see an infinity, a NaN or a number of 2^80 or more in a float32 cache, they and those beside them are worked out
  * twice, in up to four times the time.  out overlaps no input.
  * Many rows, of a float32 cache: pages of a multiple of 4 rows, 16 or more, heads of up to 64 values whose mean chunk has 64 rows (token, query head) of a cache head or
- * more, or of up to 128 and 128 rows, and in all, as if every chunk were the mean one, rounded up, either 18000 rows - heads of up to 64: in 250 tiles of 128 rows or over 1000 keys - or 8192 over 2048
- * keys (shaped scores, below: 1000).  The keys are max_length, with a window at most its rows + 32 + those of a tile (128, or 256).  Calls of fewer rows each stay with the float32 operations.
+ * more, or of up to 128 and 128 rows, and in all, as if every chunk were the mean one, rounded up, either 18000 rows or 8192 over 2048 keys (shaped scores, below: 8192 over 1000 keys or 18000, heads
+ * of up to 64 in 250 tiles of 128 rows).  The keys are max_length, with a window at most its rows + 32 + those of a tile (128, or 256).  Calls of fewer rows each stay with the float32 operations.
  * Their workspace holds up to eight partial results [tokens, heads, size + 2] in float32. */
 typedef struct tfcc_rocm_paged_attention_desc {
   tfcc_rocm_paged_cache cache;

@@ -17,7 +17,7 @@ static int failures = 0;
   } while (0)
 
 static unsigned rows(bool shaped, unsigned tokens, unsigned batch, unsigned group, unsigned heads, unsigned size, unsigned most) {
-  return paged_attention_plan(tokens, batch, group, heads, size, most, 1, 0, size <= 64 ? 128 : 256, true, false, shaped ? kLongKeysShaped : kLongKeysPlain).rows;
+  return paged_attention_plan(tokens, batch, group, heads, size, most, 1, 0, size <= 64 ? 128 : 256, true, false, shaped).rows;
 }
 
 int main() {
@@ -27,11 +27,14 @@ int main() {
   EXPECT(rows(false, 700, 1, 1, 16, 64, 1500) == 16 && rows(true, 700, 1, 1, 16, 64, 1500) == 128);
   EXPECT(rows(false, 256, 1, 4, 8, 128, 2047) == 16 && rows(false, 256, 1, 4, 8, 128, 2048) == 256 && rows(false, 255, 1, 4, 8, 128, 2048) == 16);
   EXPECT(rows(true, 256, 1, 4, 8, 128, 999) == 16 && rows(true, 256, 1, 4, 8, 128, 1000) == 256 && rows(true, 255, 1, 4, 8, 128, 1000) == 16);
-  // 18000 rows: for both
+  // 18000 rows: for both, over 1000 keys
   for (const bool shaped : {false, true}) {
     EXPECT(rows(shaped, 563, 1, 4, 8, 128, 563) == 256 && rows(shaped, 562, 1, 4, 8, 128, 563) == 16);
     EXPECT(rows(shaped, 5 * 512, 5, 1, 12, 64, 1000) == 128 && rows(shaped, 5 * 512, 5, 1, 12, 64, 1024) == 128);
   }
+  // plain ones of heads of 64 however few tiles and keys there are (12 heads of 64: 10 of 200 over 950 51 us, with tiles of 16 rows 89)
+  EXPECT(rows(false, 10 * 200, 10, 1, 12, 64, 950) == 128 && rows(false, 5 * 512, 5, 1, 12, 64, 850) == 128 && rows(false, 2 * 750, 2, 1, 12, 64, 750) == 128);
+  EXPECT(rows(false, 2 * 749, 2, 1, 12, 64, 750) == 16 && rows(false, 4 * 150, 4, 4, 8, 64, 999) == 128);
   if (failures == 0) std::printf("float cache plan: all passed\n");
   return failures != 0;
 }

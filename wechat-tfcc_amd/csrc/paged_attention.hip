@@ -146,7 +146,7 @@ unsigned chunk_rows(const tfcc_rocm_paged_cache& c) {
 
 PagedAttentionPlan plan_of(const tfcc_rocm_paged_attention_desc& d, bool shaped) {
   return paged_attention_plan(d.tokens, d.batch, d.heads / d.cache.heads, d.cache.heads, d.cache.size, most_keys(d), d.causal, d.window, chunk_rows(d.cache),
-                              d.cache.type == TFCC_ROCM_F32, d.cache.type == TFCC_ROCM_S4, shaped ? kLongKeysShaped : kLongKeysPlain);
+                              d.cache.type == TFCC_ROCM_F32, d.cache.type == TFCC_ROCM_S4, shaped);
 }
 
 // Checks a call and deals it out; one without tokens or sequences has nothing to deal out.

@@ -16,10 +16,6 @@ struct PagedAttentionPlan {
 constexpr unsigned kAttentionRows = 16;    // rows (a token's query heads of one cache head) of a tile
 constexpr unsigned kAttentionStep = 256;   // keys that eight wavefronts take of an int8 cache in one step
 constexpr unsigned kAttentionMostSplits = 256;
-// float32: from so many keys on chunks of 8192 to 17999 rows in all take wide tiles, whose products of pieces are right to 2^-21 of a term where the fp32 operations round to 2^-24, and lose
-// what lies 2^-30 below a row's largest value.  Plain scores keep float32's bits up to the contexts that cost several times as much with tiles of 16 rows (32 heads over 8 of 128: 256 over 4096
-// in eight pieces 84 us and 210); at shorter ones the time is what they cost (4 of 128 over 1500 170 us, wide 68).  With shaped scores, whose caps and biases are rounded to float32 besides, earlier.
-constexpr unsigned kLongKeysPlain = 2048, kLongKeysShaped = 1000;
 
 // A chunk of n tokens makes ceil(n * group / rows) tiles; how the tokens are spread over the sequences only the device knows.
 inline unsigned paged_attention_tiles(unsigned tokens, unsigned batch, unsigned group, unsigned rows) {
@@ -27,9 +23,9 @@ inline unsigned paged_attention_tiles(unsigned tokens, unsigned batch, unsigned 
   return (unsigned)(((uint64_t)tokens * group + (uint64_t)(rows - 1) * chunks) / rows);
 }
 
-// chunk_rows: of the tiles that chunks of many tokens may take, 128 or 256; 0: there are none.  halves: a cache of 4-bit integers.  long_keys: of a float32 cache, as above.
+// chunk_rows: of the tiles that chunks of many tokens may take, 128 or 256; 0: there are none.  halves: a cache of 4-bit integers.  shaped: with a cap, slopes or prefixes.
 inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, unsigned group, unsigned cache_heads, unsigned size, unsigned max_length,
-                                               int causal, unsigned window, unsigned chunk_rows, bool float_cache, bool halves = false, unsigned long_keys = kLongKeysShaped) {
+                                               int causal, unsigned window, unsigned chunk_rows, bool float_cache, bool halves = false, bool shaped = true) {
   PagedAttentionPlan p;
   // chunks of about the same number of tokens
   const uint64_t chunks = tokens < batch ? tokens : batch, mean = chunks == 0 ? 0 : (tokens + chunks - 1) / chunks;
@@ -55,11 +51,14 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
   } else if (chunk_rows > 0) {
     // float32, whose tiles of 16 rows run on slower matrix operations: earlier, and earlier still where long contexts can be cut into pieces
     // (32 heads over 8 of 128: 15 of 205 over 376, 16 heads over 2: 48 us, with tiles of 16 rows 94; 11 of 125 over 227: 35 and 45;
-    // one of 674, 24 heads over 4 of 96: 73 and 62; 4 of 128 over 1500 in four pieces 68 and 170; 12 heads of 64: 5 of 512 over 2000 in two pieces 99 and 185, over 1024 59 and 93;
-    // 2 of 512 over 1024 38 and 46, over 512 27 and 22).  Tiles of 128 rows, of which a CU takes two, want a workgroup for about every CU over short ones
-    // (8 of up to 300 over up to 700, 192 workgroups, 55 and 48; 12 of 300 over 1500, 288, 95 and 115).
+    // one of 674, 24 heads over 4 of 96: 73 and 62; one of 256 over 4096 in eight pieces 84 and 210; 4 of 128 over 1500 in four 68 and 162; 12 heads of 64: 5 of 512 over 2000 in two
+    // pieces 99 and 185, over 850 49 and 79; 10 of 200 over 950 51 and 89; 2 of 800 over 800 38 and 42, of up to 800 36 and 32; 2 of 512 over 1024 38 and 46, over 512 27 and 22).
+    // What they cost is bits: their products of pieces are right to 2^-21 of a term where the fp32 operations round to 2^-24, and lose what lies 2^-30 below a row's largest value.  So plain
+    // scores of fewer than 18000 rows keep the fp32 operations below 2048 keys; shaped ones, which are rounded besides, below 1000, where those of up to 64 values that do not make 250 tiles
+    // of 128 rows keep them as well.
     const uint64_t seen = keys_of(chunk_rows);
-    wide = 2 * mean * group >= chunk_rows && ((all >= 18000 && (chunk_rows > 128 || groups_of(chunk_rows) >= 250 || seen >= 1000)) || (all >= 8192 && seen >= long_keys));
+    const bool many = all >= 18000 && (!shaped || chunk_rows > 128 || groups_of(chunk_rows) >= 250);
+    wide = 2 * mean * group >= chunk_rows && (many || (all >= 8192 && seen >= (shaped ? 1000 : 2048)));
   }
   p.rows = wide ? chunk_rows : kAttentionRows;
   p.tiles = paged_attention_tiles(tokens, batch, group, p.rows);
