@@ -197,7 +197,7 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   a.pieces = Divisor::of(plan.splits);
   a.splits = plan.splits;
   a.split_keys = plan.split_keys;
-  if ((uint64_t)plan.tiles * plan.splits * d.cache.heads > (plan.rows == kAttentionRows ? 256 : 65536 / plan.rows)) {  // more workgroups than CUs, of wide tiles than run at once
+  if (attention_longest_first(plan, d.tokens, d.batch, a.max_length, a.window, d.cache.type == TFCC_ROCM_F32)) {
     int shift = 0;
     while (a.max_length >> shift > 16) ++shift;
     a.longest_first = shift + 1;
