@@ -1,4 +1,4 @@
-// When attention over a paged cache takes the longest sequences first (wechat-tfcc_amd/csrc/paged_attention_plan.hpp): both sides of each line.  No GPU.
+// When attention over a paged cache takes the longest sequences first, and which launch joins its pieces (wechat-tfcc_amd/csrc/paged_attention_plan.hpp): both sides of each line.  No GPU.
 #include <cstdio>
 #include <initializer_list>
 
@@ -34,6 +34,10 @@ int main() {
   EXPECT(first(FLOAT, 64, 64, 4, 8, 128, 257) && !first(FLOAT, 64, 64, 4, 8, 128, 256));
   EXPECT(first(FLOAT, 9000, 30, 1, 12, 64, 900) && !first(FLOAT, 9000, 30, 1, 12, 64, 256) && !first(FLOAT, 9000, 30, 1, 12, 64, 900, 450) && first(FLOAT, 9000, 30, 1, 12, 64, 901, 451));
   EXPECT(first(EIGHT, 16 * 500, 16, 4, 8, 128, 500) && !first(EIGHT, 16 * 250, 16, 4, 8, 128, 256));  // wide tiles
+  // joins
+  EXPECT(attention_joins_few(8, 1, 64) && attention_joins_few(8, 100000, 256) && !attention_joins_few(9, 1, 64));
+  EXPECT(!attention_joins_few(9, 512, 64) && attention_joins_few(9, 513, 64) && !attention_joins_few(16, 256, 128) && attention_joins_few(16, 257, 80) && !attention_joins_few(81, 16, 256));
+  EXPECT(!attention_joins_few(12, 128, 256) && attention_joins_few(12, 129, 256));
   if (failures == 0) std::printf("attention order: all passed\n");
   return failures != 0;
 }

@@ -1,4 +1,4 @@
-"""When attention over a paged cache takes the longest sequences first (tests/cpp/attention_order_tests.cpp), on the CPU."""
+"""When attention over a paged cache takes the longest sequences first, and which launch joins its pieces (tests/cpp/attention_order_tests.cpp), on the CPU."""
 import os
 import subprocess
 

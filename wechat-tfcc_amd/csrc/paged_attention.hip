@@ -69,7 +69,6 @@ __global__ __launch_bounds__(kThreads) void join_pieces_kernel(AttentionArgs p) 
 
 // Few pieces: LANES lanes to a row (at least a quarter of its values), which sum them one after the other.  HBM is its bound where there are many rows
 // (10 chunks of 512, 12 heads of 64, two pieces: 12 us, and 77 with a workgroup to a row).
-constexpr unsigned kFewPieces = 8;
 template <unsigned LANES>
 __global__ __launch_bounds__(kThreads) void join_few_kernel(AttentionArgs p) {
   const unsigned heads = p.cache.heads * p.group.d, size = p.cache.size, d = threadIdx.x % LANES * 4;
@@ -218,7 +217,7 @@ int attend(void* stream, const tfcc_rocm_paged_attention_desc& d, const tfcc_roc
   if (int e = check_launch("paged_attention")) return e;
   if (plan.splits > 1) {
     const unsigned rows = d.tokens * d.heads;
-    if (plan.splits > kFewPieces) {
+    if (!attention_joins_few(plan.splits, rows, a.cache.size)) {
       hipLaunchKernelGGL(join_pieces_kernel, dim3(rows, (a.cache.size + 63) / 64), dim3(kThreads), 0, s, a);
     } else {
       const unsigned lanes = a.cache.size <= 64 ? 16 : a.cache.size <= 128 ? 32 : 64, each = kThreads / lanes;
