@@ -35,6 +35,13 @@ int main() {
   // plain ones of heads of 64 however few tiles and keys there are (12 heads of 64: 10 of 200 over 950 51 us, with tiles of 16 rows 89)
   EXPECT(rows(false, 10 * 200, 10, 1, 12, 64, 950) == 128 && rows(false, 5 * 512, 5, 1, 12, 64, 850) == 128 && rows(false, 2 * 750, 2, 1, 12, 64, 750) == 128);
   EXPECT(rows(false, 2 * 749, 2, 1, 12, 64, 750) == 16 && rows(false, 4 * 150, 4, 4, 8, 64, 999) == 128);
+  // windows in two pieces of tiles of 256 rows, where these make no third round
+  const auto window = [](unsigned tokens, unsigned batch, unsigned group, unsigned heads) {
+    return paged_attention_plan(tokens, batch, group, heads, 128, 4000, 1, 512, 256, true, false, false).splits;
+  };
+  EXPECT(window(854, 14, 4, 8) == 1);   // 72 us, in two pieces 121
+  EXPECT(window(971, 4, 2, 16) == 1);   // 78 and 111
+  EXPECT(window(1024, 1, 4, 8) == 2 && window(2 * 512, 2, 4, 8) == 2);
   if (failures == 0) std::printf("float cache plan: all passed\n");
   return failures != 0;
 }
