@@ -33,6 +33,7 @@ int main() {
   }
   EXPECT(first(FLOAT, 64, 64, 4, 8, 128, 257) && !first(FLOAT, 64, 64, 4, 8, 128, 256));
   EXPECT(first(FLOAT, 9000, 30, 1, 12, 64, 900) && !first(FLOAT, 9000, 30, 1, 12, 64, 256) && !first(FLOAT, 9000, 30, 1, 12, 64, 900, 450) && first(FLOAT, 9000, 30, 1, 12, 64, 901, 451));
+  EXPECT(!first(FLOAT, 2 * 56, 2, 4, 4, 80, 5150) && !first(FLOAT, 8, 8, 1, 12, 96, 4588));  // 96 workgroups in three pieces each
   EXPECT(first(EIGHT, 16 * 500, 16, 4, 8, 128, 500) && !first(EIGHT, 16 * 250, 16, 4, 8, 128, 256));  // wide tiles
   // joins
   EXPECT(attention_joins_few(8, 1, 64) && attention_joins_few(8, 100000, 256) && !attention_joins_few(9, 1, 64));

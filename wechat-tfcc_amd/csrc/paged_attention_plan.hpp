@@ -121,10 +121,11 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
 // one that begins late costs is more than the microsecond that every workgroup spends on the order.  That is so from so many keys on (random calls of 8 and 4 bits and float32, geometric means of the
 // time without the order over that with it: single tokens over integers, ragged and uniform lengths, over 257 to 512 keys 0.97 and 0.95, over 513 to 1024 1.00 and 0.97, over 1025 to 2048 1.04 and
 // 0.98, over more 1.05 and 0.99; chunks over 129 to 256 keys 0.98 and 0.96, over 257 to 512 0.98 and 0.98, over 513 to 1024 1.01 and 1.00, over more 1.03 and 1.00; float32 and wide tiles over
-// up to 128 keys 1.00 and 0.96, over 129 to 256 1.01 and 0.98, over 257 to 512 1.03 and 1.01, over more 1.04 and 1.02), but not where a window of half the keys or less lets all rows see about as many (0.95 to 0.99 throughout).
+// up to 128 keys 1.00 and 0.96, over 129 to 256 1.01 and 0.98, over 257 to 512 1.03 and 1.01, over more 1.04 and 1.02), but not where a window of half the keys or less lets all rows see about as many (0.95 to
+// 0.99 throughout), nor in pieces (ragged ones 1.00, from 0.80 to 1.42, uniform ones 0.98 to 0.99, of wide tiles 0.99; 2 chunks of up to 75 over up to 5758, 16 heads over 4 of 80: 58 us in the batch's order, 93).
 inline bool attention_longest_first(const PagedAttentionPlan& p, unsigned tokens, unsigned batch, unsigned max_length, unsigned window, bool float_cache) {
   if (p.groups <= (p.rows == kAttentionRows ? 256 : 65536 / p.rows)) return false;
-  if (window > 0 && window <= max_length / 2) return false;
+  if (p.splits > 1 || (window > 0 && window <= max_length / 2)) return false;
   return max_length > (float_cache || p.rows != kAttentionRows ? 256u : tokens > batch ? 512u : 1024u);
 }
 
