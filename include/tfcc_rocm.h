@@ -634,8 +634,8 @@ int tfcc_rocm_paged_attention_f32(void* stream, const tfcc_rocm_paged_attention_
  *   x = scale * q k^T;  with a cap > 0 x = cap * tanh(x / cap);  with slopes x -= slopes[head] * |position of the token - position of the key|
  * A sequence's i first prefixes[i] tokens (of those that are cached) are seen by all tokens of its chunk, the later ones of the prefix by the
  * earlier too: a token sees the keys up to its own position and those of the prefix.  A prefix wants causal and no window.  A cap is finite, one of
- * 2^100 or more is none, and scores whose largest |q| * scale / cap lies below 2^-110 count as 0; slopes are finite, of any sign, and the bias is formed in float32.  Scores that overflow are those of an infinity: cap or -cap.  All three
- * unset: the call above. */
+ * 2^100 or more is none, and scores whose largest |q| * scale / cap lies below 2^-110 count as 0; slopes are finite, of any sign, and the bias is formed in float32 and infinite where it overflows.  Scores that overflow are those of an infinity: cap or
+ * -cap (over a float32 cache NaN where terms of both signs overflow, or a query times scale does that meets a 0).  All three unset: the call above. */
 typedef struct tfcc_rocm_attention_scores {
   float cap;               /* 0: none */
   const float* slopes;     /* [heads] or NULL */

@@ -237,7 +237,7 @@ __device__ __forceinline__ int bound_of(float v) {
 // tanh (score_tanh.hpp) has two forms, and most scores are far below their cap: where those of a whole wavefront are, the second is passed over.  A score as
 // it comes (`raw`) takes the factor of its row and the cap's inverse in one, and leaves in units of `unit`, the cap where nothing is added to it: a
 // cap costs nine operations, a bias two (int8, 32 sequences of up to 6000 with a window of 4096, 8 heads of 256, at the rate of HBM: 97 us with a cap, 92 without; 4 chunks of 1024
-// over 4096 in 4 bits, bound by operations: 385 us plain, 503 with a cap, 415 with slopes).
+// over 4096 in 4 bits: 380 us plain, 500 with a cap, 417 with slopes).
 // The bias is slope * distance.  A row's softmax does not change with what all its scores have in common, so a position behind the last key
 // that the row may see counts as that key's, and one before the first as the first's: differences are whole numbers, exact up to 2^24.
 struct ScoreShape {
@@ -658,7 +658,7 @@ struct ScaledRows : ScaledLayout<TYPE, BLOCKS> {
 // of 16; WITHIN: pages of a multiple of 16 rows, so that a half lies in one, or of 32 for a whole step (4 bits), else (0) a half in up to two, and so where
 // rows are no multiples of 16 bytes (-1, 4 bits), which come four bytes to a lane.  8 bits, 32 sequences of up to 4096, 186 MB: 46 us, 4.1 TB/s, pages of 24 rows 49.
 // Bound: HBM, which wants more on its way than registers can take: a wavefront copies the rows of its next steps straight into LDS, a ring of kStages of its own
-// (no barriers), and reads a step from there when it is due.  4 bits: as much by the vector unit, whose operations take 57 % of the time (64 sequences of 1024 to 4096,
+// (no barriers), and reads a step from there when it is due.  4 bits: by the vector unit besides, which is active 42 to 45 % of the time, the matrix cores 16 % (64 sequences of 1024 to 4096,
 // 8 heads of 128, 197 MB: 48 to 51 us, 3.9 to 4.1 TB/s; 32 of 16384, 571 MB: 117 to 130 us, 4.4 to 4.9 TB/s).
 template <int TYPE, int BLOCKS, int WAVES, bool NARROW>
 struct ScaledRing {
@@ -915,9 +915,10 @@ __global__ __launch_bounds__(WAVES * 64, TYPE == TFCC_ROCM_S4 ? (BLOCKS == 1 ? 4
   rows.template finish<WAVES>(shared.joining, p, t, head, split, g);
 }
 
-// Chunks of many tokens, int8 as above: a workgroup takes 128 rows, a wavefront 32 of them, and all go over the same keys, 32 in a step.  Bound: the
-// matrix cores and, with as much to do, the vector unit (4 chunks of 1024 over 4096, 32 heads over 8 of 128: int8 377 us, matrix operations and LDS
-// reads alone 283; 4 bits 385; float32 589, with tiles of 16 rows on the fp32 matrix operations 1930).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
+// Chunks of many tokens, int8 as above: a workgroup takes 128 rows, a wavefront 32 of them, and all go over the same keys, 32 in a step.  Bound: the waits of steps whose wavefronts
+// take turns with matrix cores and vector unit; neither is full (4 chunks of 1024 over 4096, 32 heads over 8 of 128: int8 377 us, matrix operations and LDS
+// reads alone 283; 4 bits 380; matrix cores active 34 to 35 % of the time, the vector unit 37 to 41 %, 1.5 wavefronts to a SIMD where two fit, of whose cycles 30 to 39 % are waits; with a cap 57 % of the
+// vector unit; float32 589, with tiles of 16 rows on the fp32 matrix operations 1930).  So the keys and values of a step are turned into fp16 once for all wavefronts, in the
 // order in which the matrix cores take them, into one of two LDS buffers while the other is worked on; the next step's rows
 // are on their way to registers meanwhile.  Products of 32 x 32 as above, with
 //   S^T: lane l holds row l % 32 and keys 8 a + 4 (l / 32) + i in [4 a + i]

@@ -84,7 +84,7 @@ inline PagedAttentionPlan paged_attention_plan(unsigned tokens, unsigned batch, 
     uint64_t fit = groups == 0 ? 1 : 256 * 256 / chunk_rows / groups;
     // One more where that leaves many places free: of two or three pieces the tiles that see few keys, or are not there, make room for the others' (12 heads of 64, two and
     // one: 6 of up to 517 over up to 1201 67 us and 82, 3 of 1000 over 6000 401 and 471; three and two: one prompt of 1900 67 and 85, 3 of up to 600 over up to 2000 72 and 95,
-    // but 5 of up to 512 over up to 1024, pieces of 350, 64 and 56, 6 of up to 517 over up to 1201 with 16 heads, 384 workgroups, 98 and 86; six and five: one of 1024 over 4096 104 and 82; tiles of 256 rows, 20 of 64 over 1000, 144 and 120).
+    // but 5 of up to 512 over up to 1024, pieces of 350, 64 and 56; next to the line at 320 workgroups, chunks of one length over 1201: 300 85 and 91, 336 95 and 91, 360 96 and 91, 384 over 3000 207 and 204; six and five: one of 1024 over 4096 104 and 82; tiles of 256 rows, 20 of 64 over 1000, 144 and 120).
     if (chunk_rows == 128 && ((fit == 1 && groups <= 320) || (fit == 2 && groups <= 192)) && keys >= 512 * (fit + 1)) ++fit;
     // Of tiles of 256 rows a CU takes one, so a third round outweighs what two pieces of a window give: where ragged chunks, of which each makes half a tile more than its rows fill, would need one (window of 512,
     // 32 heads over 8 of 128: 14 of up to 91 over up to 4817 72 us, in two pieces 121; 32 over 16, 4 of up to 344 over up to 1800 78 and 111; with less to do in two pieces 0.92 to 0.95 of the time).
