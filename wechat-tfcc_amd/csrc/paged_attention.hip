@@ -139,7 +139,7 @@ bool wide_reads(const tfcc_rocm_paged_cache& c) {
 unsigned chunk_rows(const tfcc_rocm_paged_cache& c) {
   if (c.page_size < 16 || c.page_size % 4 != 0) return 0;
   if (c.type == TFCC_ROCM_F32) return c.size <= 64 ? 128 : c.size <= 128 ? 256 : 0;
-  if (c.type == TFCC_ROCM_S4) return wide_reads(c) && c.size > 64 && c.size <= 128 ? 128 : 0;  // others stay with 16 rows (4 chunks of 1024 over 4096, 12 heads of 64: 114 us, with 128 rows 208)
+  if (c.type == TFCC_ROCM_S4) return wide_reads(c) && c.size > 64 && c.size <= 128 ? 128 : 0;  // others stay with 16 rows (4 chunks of 1024 over 4096, 12 heads of 64: 114 us, with 128 rows 208; 16 heads over 8 of 256 554, int8 with 128 rows 826)
   return wide_reads(c) ? 128 : 0;
 }
 
